@@ -14,7 +14,7 @@ for o in ttts_amd/csrc/build/*.o; do
 done
 for f in "$@"; do
   git show $REV:ttts_amd/csrc/$f > $T/$f
-  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -munsafe-fp-atomics -fPIC -Iinclude -Ittts_amd/csrc -c $T/$f -o $T/${f%.hip}.o
+  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -munsafe-fp-atomics -Xclang -target-feature -Xclang -packed-fp32-ops -fPIC -Iinclude -Ittts_amd/csrc -c $T/$f -o $T/${f%.hip}.o
   OBJS="$OBJS $T/${f%.hip}.o"
 done
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o ttts_amd/libttts_hip_alt.so $OBJS

@@ -9,6 +9,6 @@ OBJS=""
 for o in ttts_amd/csrc/build/*.o; do
   [ "$(basename $o .o).hip" == "$F" ] || OBJS="$OBJS $o"
 done
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -munsafe-fp-atomics -fPIC -Iinclude -Ittts_amd/csrc "$@" -c ttts_amd/csrc/$F -o $T/x.o
+/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -munsafe-fp-atomics -Xclang -target-feature -Xclang -packed-fp32-ops -fPIC -Iinclude -Ittts_amd/csrc "$@" -c ttts_amd/csrc/$F -o $T/x.o
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o $OUT $OBJS $T/x.o
 ls -la $OUT

@@ -5,7 +5,7 @@ export TMPDIR=/tmp
 O=gpurun_out/r3c
 mkdir -p $O
 cp ttts_amd/libttts_hip.so /tmp/lib_default.so
-FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -munsafe-fp-atomics -fPIC -Wno-unused-variable -Iinclude"
+FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -munsafe-fp-atomics -Xclang -target-feature -Xclang -packed-fp32-ops -fPIC -Wno-unused-variable -Iinclude"
 swap() { cp $1 ttts_amd/libttts_hip.so; touch ttts_amd/csrc/build/*.o; sleep 0.1; touch ttts_amd/libttts_hip.so; }
 timeout 200 python tools/vqvae_bench.py 32 6 1 > $O/vq_default.log 2>&1; tail -2 $O/vq_default.log
 timeout 100 python tools/hbm_bench.py > $O/hbm_default.log 2>&1; grep -i "vq_nearest" $O/hbm_default.log | head -3

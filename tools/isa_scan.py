@@ -71,7 +71,7 @@ def main():
     trace = args[args.index("--trace") + 1] if "--trace" in args else None
     with tempfile.TemporaryDirectory() as td:
         out = os.path.join(td, "k.s")
-        subprocess.run([HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-munsafe-fp-atomics", "-I" + os.path.join(ROOT, "include"),
+        subprocess.run([HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-munsafe-fp-atomics -Xclang -target-feature -Xclang -packed-fp32-ops", "-I" + os.path.join(ROOT, "include"),
                         "-I" + os.path.join(ROOT, "ttts_amd", "csrc"), "--cuda-device-only", "-S", "-o", out, src] + defs,
                        check=True, stderr=subprocess.DEVNULL)
         asm = open(out).read()

@@ -11,7 +11,7 @@ mkdir -p $B
 rm -f $B/attn_*
 T=$(mktemp -d)
 trap 'rm -rf "$T"' EXIT
-FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -munsafe-fp-atomics -fPIC -Iinclude -Ittts_amd/csrc"
+FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -munsafe-fp-atomics -Xclang -target-feature -Xclang -packed-fp32-ops -fPIC -Iinclude -Ittts_amd/csrc"
 DH64="-fno-honor-nans -fno-slp-vectorize"      # ttts_amd/lib.py EXTRA_FLAGS["attn_dh64.hip"]
 lib() {  # name, source dir, flags for attn_dh64.hip
   local name=$1 src=$2; shift 2

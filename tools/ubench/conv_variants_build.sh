@@ -10,7 +10,7 @@ mkdir -p $B
 rm -f $B/conv_*
 T=$(mktemp -d)
 trap 'rm -rf "$T"' EXIT
-FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -munsafe-fp-atomics -fPIC -Iinclude -Ittts_amd/csrc"
+FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -munsafe-fp-atomics -Xclang -target-feature -Xclang -packed-fp32-ops -fPIC -Iinclude -Ittts_amd/csrc"
 SRC="conv.hip conv_mfma.hip conv_grouped.hip conv_thin.hip"
 lib() {  # name, source dir, extra flags
   local name=$1 src=$2; shift 2

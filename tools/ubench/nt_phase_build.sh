@@ -7,7 +7,7 @@ cd "$(dirname "$0")/../.."
 B=tools/ubench/bin
 mkdir -p $B
 rm -f $B/nt_*
-FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -munsafe-fp-atomics -fPIC -Iinclude -Ittts_amd/csrc"
+FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -munsafe-fp-atomics -Xclang -target-feature -Xclang -packed-fp32-ops -fPIC -Iinclude -Ittts_amd/csrc"
 build() {  # name, -D flags
   local name=$1; shift
   /opt/rocm/bin/hipcc $FLAGS "$@" -shared -o $B/nt_$name.so ttts_amd/csrc/gemm.hip ttts_amd/csrc/lib.hip &

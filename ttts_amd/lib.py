@@ -16,7 +16,10 @@ BUILD = os.path.join(CSRC, "build")
 SO_PATH = os.environ.get("TTTS_LIB") or os.path.join(HERE, "libttts_hip.so")   # TTTS_LIB: an alternate build of the same ABI (same-box A/B runs: tools/gpu_ab_lib.sh)
 SOURCES = ["lib.hip", "elementwise.hip", "gemm.hip", "attn.hip", "attn_dh64.hip", "vq.hip", "stft.hip", "conv.hip", "conv_mfma.hip", "conv_thin.hip", "conv_grouped.hip", "losses.hip", "vqvae_ops.hip", "attn_f32.hip", "attn_cross.hip", "peq.hip", "decode.hip", "diffusion_ops.hip", "fp8_gemm.hip", "attn_relpos.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-munsafe-fp-atomics", "-fPIC", "-Wall", "-Wno-unused-variable"]
+# No packed fp32 instructions (v_pk_add / mul / fma_f32): some of their forms have given wrong results on this hardware now and then.
+# hipcc -O3 forms them from ordinary float code by itself; the host pass does not know the feature and says so (harmless).
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-munsafe-fp-atomics", "-fPIC", "-Wall", "-Wno-unused-variable"] + NO_PACKED_FP32
 
 # per-file additions (reasons in the file headers)
 EXTRA_FLAGS = {"attn_dh64.hip": ["-fno-honor-nans", "-fno-slp-vectorize"]}

@@ -272,16 +272,16 @@ def _own_logprob(s):
     if s["top"]:
         out += [r.top_logp, r.top_idx]
     if s["train"]:
-        out.append(ops.token_logprobs_bwd(s["logits"], s["tokens"], r.lse, r.entropy, s["g_logp"], s["g_entropy"], C=s["classes"],
+        out.append(ops.token_logprobs_bwd(s["logits"], s["tokens"], r.stats, r.entropy, s["g_logp"], s["g_entropy"], C=s["classes"],
                                           temperature=s["temperature"]))
     return out
 
 
 def _own_distill(s):
     from ttts_amd import ops
-    loss, lse, lse_rest = ops.distill_fwd(s["logits"], s["teacher_idx"], s["teacher_logp"], C=s["classes"],
-                                          temperature=s["temperature"], tail=s["tail"])
-    return [loss, ops.distill_bwd(s["logits"], s["teacher_idx"], s["teacher_logp"], lse, lse_rest, s["g_loss"], C=s["classes"],
+    loss, stats = ops.distill_fwd(s["logits"], s["teacher_idx"], s["teacher_logp"], C=s["classes"], temperature=s["temperature"],
+                                  tail=s["tail"])
+    return [loss, ops.distill_bwd(s["logits"], s["teacher_idx"], s["teacher_logp"], stats, s["g_loss"], C=s["classes"],
                                   temperature=s["temperature"], tail=s["tail"])]
 
 

@@ -421,6 +421,74 @@ int ttts_diffusion_loss_bwd_f32(const float* model_out, const float* x_start, co
                                 const int64_t* t, const float* table, const float* gout, float* d_model_out, int32_t B,
                                 int32_t C, int32_t T, void* stream);
 
+/* ---- scoring of given tokens and distillation on a teacher's alternatives ------------------------------------------
+ * Beside ttts_ce_fwd_bf16 (the mean loss alone) and ttts_sample_logits_f32 (the drawn token alone): what a token was worth, what
+ * else was likely, and a student's loss on that.  logits [R, ldl] of `dtype`, C classes per row (columns C .. ldl - 1 are never
+ * looked at), any row pitch >= C and any alignment of the type (16-byte aligned rows are read 16 bytes at a time);
+ * y = logits / temperature; sums and statistics are fp32.  A class at -inf has no probability and is no alternative.
+ * Rows: one whose classes are all -inf has no distribution (below); one that holds a NaN or +inf gets NaN. */
+enum { TTTS_DTYPE_F32 = 0, TTTS_DTYPE_BF16 = 1, TTTS_DTYPE_F16 = 2 };
+#define TTTS_SCORE_MAX_CLASSES 1048576
+#define TTTS_SCORE_MAX_TOP 64
+#define TTTS_DISTILL_MAX_K 128
+/* fwd: logp[r] = log softmax(y)[tokens[r]] (0 where tokens[r] is outside [0, C): the row has no token); entropy[r] = -sum p log p;
+ *   stats f32 [R, 2] = (max of the row's logits, log sum e^(y - max / temperature)) for the backward -- their sum, the first over
+ *   the temperature, is the log-sum-exp; top_logp f32 / top_idx int64 [R, top_k]: the top_k <= TTTS_SCORE_MAX_TOP best classes, best
+ *   first, equal logits by ascending class (top_k 0: not written, may be NULL); where a row has fewer, -inf and -1.
+ *   All classes at -inf: logp -inf (0 without a token), entropy 0, no alternatives.  NaN rows: every float NaN, every index -1.
+ * workspace: ttts_token_logprobs_workspace_bytes (16-byte aligned; may be 0 -> NULL), the call's own until it has run. */
+int64_t ttts_token_logprobs_workspace_bytes(int32_t R, int32_t C, int32_t top_k);
+int ttts_token_logprobs_fwd(const void* logits, int32_t dtype, int64_t ldl, const int64_t* tokens, float* logp, float* entropy,
+                            float* stats, float* top_logp, int64_t* top_idx, int32_t R, int32_t C, int32_t top_k,
+                            float temperature, void* workspace, int64_t workspace_bytes, void* stream);
+/* bwd: dlogits [R, ldd] of the logits' type = [g_logp (1[class = token] - p) - g_entropy p (log p + entropy)] / temperature, from the
+ *   forward's stats and entropy; g_logp / g_entropy f32 [R] (g_entropy may be NULL); rows without a token ignore g_logp.  Columns
+ *   C .. Cd - 1 are written as zeros (C <= Cd <= ldd).  dlogits may be the logits' own buffer (same pitch).  A row whose classes are
+ *   all -inf gets zeros. */
+int ttts_token_logprobs_bwd(const void* logits, int32_t dtype, int64_t ldl, const int64_t* tokens, const float* stats,
+                            const float* entropy, const float* g_logp, const float* g_entropy, void* dlogits, int64_t ldd,
+                            int32_t R, int32_t C, int32_t Cd, float temperature, void* stream);
+/* Distillation: teacher_idx int64 / teacher_logp f32 [R, K], K <= TTTS_DISTILL_MAX_K; an index outside [0, C) is an empty entry (its
+ *   value is not looked at).  With q = softmax(y) the student's,
+ *   tail 0: p = softmax(teacher_logp / temperature) over the row's entries;  row_loss = sum p (log p - log q[idx])
+ *   tail 1: p = exp(teacher_logp) as given (log-probabilities of the teacher's whole softmax, at the same temperature),
+ *           left = max(0, 1 - sum p);  row_loss += left (log left - log q_rest), q_rest = the student's mass on the classes that
+ *           the list does not name (summed as such, not as 1 - the rest).  Without such a class the term is left out.
+ *   A class named twice counts with both of its p.  A row without entries has loss 0 with tail 0; a row whose student classes are
+ *   all -inf has loss 0 and no gradient.  stats f32 [R, 3] for the backward: (max, log Z, log Z of the classes not named).
+ * bwd: dlogits = g_loss[r] d row_loss / d logits:  g / temperature [q (sum p + left) - p - left q / q_rest (classes not named)];
+ *   written over Cd columns as above, or with accumulate 1 added to what is there (columns 0 .. C - 1, one rounding of the sum). */
+int64_t ttts_distill_workspace_bytes(int32_t R, int32_t C);
+int ttts_distill_fwd(const void* logits, int32_t dtype, int64_t ldl, const int64_t* teacher_idx, const float* teacher_logp,
+                     float* row_loss, float* stats, int32_t R, int32_t C, int32_t K, float temperature, int32_t tail,
+                     void* workspace, int64_t workspace_bytes, void* stream);
+int ttts_distill_bwd(const void* logits, int32_t dtype, int64_t ldl, const int64_t* teacher_idx, const float* teacher_logp,
+                     const float* stats, const float* g_loss, void* dlogits, int64_t ldd, int32_t R, int32_t C, int32_t Cd,
+                     int32_t K, float temperature, int32_t tail, int32_t accumulate, void* stream);
+
+/* ---- paged key / value cache and the attention of one new token that reads it ---------------------------------------
+ * Beside ttts_kv_cache_fill_bf16 / ttts_attn_decode_bf16 (one block per sequence, all of one length): sequences of any length share
+ * pages.  k_pages / v_pages [P, Hkv, page, head_dim] of bf16 or fp16, contiguous, page a power of two 16 .. 1024, head_dim in
+ * {32, 64, 128}.  What comes from device memory is checked there and never reaches outside the cache.
+ *  ttts_kv_page_write: row n of k / v [N, Hkv, head_dim] (strides in elements, multiples of 8; 16-byte aligned) -> position
+ *    slots[n] % page of page slots[n] / page.  A slot outside [0, P page) writes nothing (padding rows: -1).  The slots of one call
+ *    differ; where two rows name the same one, its 16-byte pieces are one row's or the other's.
+ *  ttts_attn_paged_decode: q [M, H, head_dim] (strides as above), heads h H/Hkv .. share key / value head h; block_table
+ *    int32 [M, width] (row pitch table_stride): pages of sequence m in order; seq_lens int32 [M]: its keys, the new token's among
+ *    them (write it first).  out [M, H, head_dim] = softmax(scale q K^T) V over keys 0 .. seq_lens[m] - 1, lse f32 [M, H] =
+ *    log sum exp(scaled scores).  A length beyond width * page ends there; keys of a table entry outside [0, P) are left out;
+ *    without keys (length <= 0) out is 0 and lse -inf.  fp32 softmax and sums; the weights are rounded to the cache's type for the
+ *    product with V.  workspace: ttts_attn_paged_decode_workspace_bytes (16-byte aligned), the call's own until it has run. */
+int ttts_kv_page_write(const void* k, const void* v, int64_t k_stride_n, int64_t k_stride_h, int64_t v_stride_n,
+                       int64_t v_stride_h, void* k_pages, void* v_pages, const int64_t* slots, int32_t dtype, int32_t N,
+                       int32_t Hkv, int32_t head_dim, int32_t page, int32_t P, void* stream);
+int64_t ttts_attn_paged_decode_workspace_bytes(int32_t M, int32_t H, int32_t Hkv, int32_t head_dim, int32_t page, int32_t width);
+int ttts_attn_paged_decode(const void* q, int64_t q_stride_m, int64_t q_stride_h, const void* k_pages, const void* v_pages,
+                           const int32_t* block_table, int64_t table_stride, const int32_t* seq_lens, void* out,
+                           int64_t o_stride_m, int64_t o_stride_h, float* lse, int32_t dtype, int32_t M, int32_t H, int32_t Hkv,
+                           int32_t head_dim, int32_t page, int32_t P, int32_t width, float scale, void* workspace,
+                           int64_t workspace_bytes, void* stream);
+
 /* ---- autoregressive decoding of the GPT --------------------------------------------------------
  * Replaces: GPT2InferenceModel.forward with a KV cache (ttts/gpt/model.py:34-184), inference_speech (:533-562) and the
  * sample loop + logits processors of transformers' GenerationMixin it calls (RepetitionPenaltyLogitsProcessor,

@@ -1,0 +1,429 @@
+"""Token log-probabilities with entropy and alternatives, and distillation on a teacher's alternatives (csrc/scoring.hip), against
+their definitions in 64 bits.  Tolerances are error bounds of fp32 arithmetic (U = 2^-24, half a step of a value near one):
+ * a row's log Z: its terms are each off by a few U (the exponential is good to one step), and a sum of C of them, taken in
+   parts of at most C / 64 by one lane, by at most (C / 64 + 32) U of itself;
+ * log p = (x - m) / T - log Z: two more roundings of the size of |log p|, and of |(x - m) / T| <= |log p|.
+Outputs of 16 bits add half a step of their type, torch.finfo(t).eps / 2 of the value (and of its smallest step near zero)."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+LOWEST = {torch.float32: -3.4e38, torch.bfloat16: -3.3e38, torch.float16: -65504.0}
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _logits(R, C, pitch, dtype, seed, offset=0, std=3.0):
+    """[R, pitch] rows on the GPU, `offset` elements into their allocation; the columns from C on hold NaN."""
+    buf = torch.full((offset + R * pitch,), math.nan, dtype=dtype, device="cuda")
+    x = buf[offset:].view(R, pitch)
+    x[:, :C] = (torch.randn(R, C, generator=_gen(seed)) * std).to(dtype).cuda()
+    return x
+
+
+def _inside(got, ref, bound, what):
+    got, ref = got.double().cpu(), ref.cpu()
+    bound = torch.as_tensor(bound, dtype=torch.float64).cpu().expand_as(ref)
+    assert torch.equal(torch.isnan(got), torch.isnan(ref)), what
+    inf = torch.isinf(ref)
+    assert torch.equal(got[inf], ref[inf]), what
+    fine = torch.isfinite(ref)
+    off = (got - ref).abs()[fine] - bound[fine]
+    assert off.numel() == 0 or off.max().item() <= 0, "%s: over its bound by %.3g" % (what, off.max().item())
+
+
+def _half_step(ref, dtype):
+    f = torch.finfo(dtype)
+    return f.eps / 2 * ref.abs() + f.tiny * f.eps
+
+
+def _ref_logprobs(x, tokens, C, top_k, T):
+    """logp, entropy, top_logp, top_idx, y in 64 bits (rows with a distribution)."""
+    x = x[:, :C].double().cpu()
+    tokens = tokens.cpu()
+    y = torch.log_softmax(x / T, dim=1)
+    given = (tokens >= 0) & (tokens < C)
+    logp = torch.where(given, y.gather(1, tokens.clamp(0, C - 1)[:, None])[:, 0], 0.0)
+    ent = torch.special.entr(y.exp()).sum(dim=1)
+    k = min(top_k, C)
+    v, i = torch.sort(x, dim=1, descending=True, stable=True)
+    v, i = v[:, :k], i[:, :k]
+    tl = torch.where(v > -math.inf, y.gather(1, i), -math.inf)
+    ti = torch.where(v > -math.inf, i, -1)
+    pad = top_k - k
+    return logp, ent, torch.nn.functional.pad(tl, (0, pad), value=-math.inf), torch.nn.functional.pad(ti, (0, pad), value=-1), y, given
+
+
+def _r(C):
+    return (C / 64 + 32) * U
+
+
+SHAPES = [(1, 1, 1, 0), (3, 2, 2, 0), (5, 9, 16, 0), (8, 1026, 1088, 0), (130, 1026, 1026, 0), (7, 515, 515, 1), (33, 2048, 2048, 0),
+          (9, 2049, 2056, 0), (6, 8194, 8256, 0), (4, 8195, 8195, 3), (3, 32768, 32768, 0), (2, 32801, 32808, 0), (2, 100003, 100003, 1),
+          (1, 300007, 300008, 0)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("R,C,pitch,offset", SHAPES)
+@pytest.mark.parametrize("top_k,T", [(0, 1.0), (5, 0.7), (64, 2.0)])
+def test_token_logprobs(R, C, pitch, offset, dtype, top_k, T):
+    from ttts_amd import ops
+    x = _logits(R, C, pitch, dtype, R + C, offset)
+    tokens = torch.randint(0, C, (R,), generator=_gen(C)).cuda()
+    tokens[R // 2] = -1 if R % 2 else C
+    r = ops.token_logprobs_fwd(x, tokens, C=C, top_k=top_k, temperature=T)
+    logp, ent, tl, ti, y, given = _ref_logprobs(x, tokens, C, top_k, T)
+    _inside(r.logp, logp, _r(C) + 4 * U * logp.abs(), "logp")
+    # entropy = log Z - sum e t / Z: a second sum of that kind, of terms whose sum is entropy - log Z
+    span = (ent.abs() + (y.max(dim=1).values).abs() + 1)
+    _inside(r.entropy, ent, 3 * _r(C) * span, "entropy")
+    if top_k:
+        assert torch.equal(r.top_idx.cpu(), ti)
+        _inside(r.top_logp, tl, _r(C) + 4 * U * tl.abs().nan_to_num(posinf=0.0), "top_logp")
+    else:
+        assert r.top_idx is None and r.top_logp is None
+    lse = torch.logsumexp(x[:, :C].double().cpu() / T, dim=1)
+    s = r.stats.double().cpu()
+    _inside(s[:, 0] / T + s[:, 1], lse, _r(C) + 4 * U * s[:, 1].abs(), "log-sum-exp")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("R,C,pitch,offset", [s for s in SHAPES if s[1] < 200000])
+@pytest.mark.parametrize("T,with_entropy", [(1.0, True), (0.7, False), (2.0, True)])
+def test_token_logprobs_gradient(R, C, pitch, offset, dtype, T, with_entropy):
+    from ttts_amd import ops
+    x = _logits(R, C, pitch, dtype, 7 * R + C, offset)
+    tokens = torch.randint(0, C, (R,), generator=_gen(C + 1)).cuda()
+    tokens[R // 2] = -5 if R % 2 else C + 3
+    g_l, g_h = torch.randn(R, generator=_gen(5)), torch.randn(R, generator=_gen(6))
+    r = ops.token_logprobs_fwd(x, tokens, C=C, temperature=T)
+    d = ops.token_logprobs_bwd(x, tokens, r.stats, r.entropy, g_l.cuda(), g_h.cuda() if with_entropy else None, C=C, temperature=T)
+    leaf = x[:, :C].double().cpu().requires_grad_(True)
+    y = torch.log_softmax(leaf / T, dim=1)
+    tok = tokens.cpu()
+    given = (tok >= 0) & (tok < C)
+    total = (y.gather(1, tok.clamp(0, C - 1)[:, None])[:, 0] * g_l.double() * given).sum()
+    if with_entropy:
+        total = total - ((y.exp() * y).sum(dim=1) * g_h.double()).sum()
+    ref, = torch.autograd.grad(total, leaf)
+    y = y.detach()
+    p = y.exp()
+    ent = torch.special.entr(p).sum(dim=1)
+    gl, gh = (g_l.double().abs() * given)[:, None], (g_h.double().abs() * with_entropy)[:, None]
+    # p is off by (_r(C) + 4 U |y|) of itself, y + H by that and three steps of the larger
+    size = (gl * p + gh * p * (y.abs() + ent[:, None] + 1)) / T
+    bound = size * (4 * _r(C) + 8 * U * (y.abs() + 1)) + 4 * U * gl / T + _half_step(ref, dtype) + 1e-37
+    _inside(d[:, :C], ref, bound, "dlogits")
+    assert d.dtype == dtype and d.shape == x.shape and not d[:, C:].any()
+    # in the logits' own place
+    x2 = x.clone() if offset == 0 else x
+    d2 = ops.token_logprobs_bwd(x2, tokens, r.stats, r.entropy, g_l.cuda(), g_h.cuda() if with_entropy else None, C=C, temperature=T, dlogits=x2)
+    assert d2 is x2 and torch.equal(d2, d)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("C", [70, 1026, 8195, 40000])
+def test_token_logprobs_special_rows(dtype, C):
+    """Rows whose mask leaves nothing or little, the type's lowest value, infinities, NaN, constant rows, zeros of both signs."""
+    from ttts_amd import ops
+    x = _logits(12, C, C, dtype, 3)
+    x[0] = -math.inf                                       # nothing left
+    x[1] = LOWEST[dtype]                                   # a mask of the lowest value on everything: uniform
+    x[2] = -math.inf; x[2, C // 2] = 1.5                   # one class left
+    x[3] = -math.inf; x[3, 1::2] = x[4, 1::2]              # half the classes
+    x[5, C // 3] = math.nan
+    x[6, C // 3] = math.inf
+    x[7] = 0.25                                            # constant: alternatives in the order of the classes
+    x[8] = -0.0; x[8, 5::3] = 0.0                          # zeros of both signs are equal
+    x[9] = LOWEST[dtype]; x[9, 3] = 2.0; x[9, C - 1] = 2.0 # the lowest value beside ordinary ones
+    x[10, : C // 2] = x[10, 0]                             # one value in half of the row
+    x[11] = -math.inf; x[11, 0] = math.nan
+    tokens = torch.arange(12).remainder(C).cuda()
+    tokens[2] = C // 2; tokens[9] = C - 1; tokens[1] = C - 1
+    k = 20
+    r = ops.token_logprobs_fwd(x, tokens, top_k=k)
+    keep = torch.tensor([i for i in range(12) if i not in (0, 5, 6, 11)])
+    logp, ent, tl, ti, y, _ = _ref_logprobs(x[keep.cuda()], tokens[keep.cuda()], C, k, 1.0)
+    span = ent.abs() + y.max(dim=1).values.abs() + 1
+    _inside(r.logp.cpu()[keep], logp, _r(C) + 4 * U * logp.abs().nan_to_num(posinf=0.0), "logp")
+    _inside(r.entropy.cpu()[keep], ent, 3 * _r(C) * span, "entropy")
+    assert torch.equal(r.top_idx.cpu()[keep], ti)
+    _inside(r.top_logp.cpu()[keep], tl, _r(C) + 4 * U * tl.abs().nan_to_num(posinf=0.0), "top_logp")
+    assert r.logp[0].item() == -math.inf and r.entropy[0].item() == 0.0 and (r.top_idx[0] == -1).all() and (r.top_logp[0] == -math.inf).all()
+    for i in (5, 6, 11):
+        assert torch.isnan(r.logp[i]) and torch.isnan(r.entropy[i]) and torch.isnan(r.top_logp[i]).all() and (r.top_idx[i] == -1).all(), i
+    ones = torch.ones(12, device="cuda")
+    d = ops.token_logprobs_bwd(x, tokens, r.stats, r.entropy, ones, ones)
+    assert not d[0].any() and torch.isnan(d[5]).any() and torch.isnan(d[6]).any()
+    leaf = x[keep.cuda()].double().cpu()
+    p = y.exp()
+    ref = -p - torch.where(p > 0, p * (y.clamp(min=-1e4) + ent[:, None]), 0.0)
+    ref[torch.arange(len(keep)), tokens.cpu()[keep]] += 1.0
+    size = p * (y.abs().nan_to_num(posinf=0.0).clamp(max=1e4) + ent[:, None] + 2)
+    assert torch.isfinite(leaf.exp()).any()
+    _inside(d.cpu()[keep], ref, size * (4 * _r(C) + 8 * U * 100) + 4 * U + _half_step(ref, dtype), "dlogits")
+
+
+def test_logits_far_from_zero():
+    """The statistics hand the maximum and log Z on apart: rows around 4096 lose nothing of their gradient."""
+    from ttts_amd import ops
+    x = _logits(16, 1000, 1000, torch.float32, 1)
+    far = x + 4096.0                                      # rounds x: the reference takes the rounded one
+    tokens = torch.arange(16, device="cuda")
+    one = torch.ones(16, device="cuda")
+    r = ops.token_logprobs_fwd(far, tokens, top_k=3)
+    d = ops.token_logprobs_bwd(far, tokens, r.stats, r.entropy, one)
+    y = torch.log_softmax(far.double().cpu(), dim=1)
+    ref = -y.exp()
+    ref[torch.arange(16), torch.arange(16)] += 1
+    _inside(d, ref, y.exp() * (4 * _r(1000) + 8 * U * (y.abs() + 1)) + 4 * U, "dlogits")
+
+
+def _ref_distill(x, idx, t, C, T, tail):
+    """(row_loss, p, listed, left, q_rest, y) in 64 bits; x leaf of [R, C] doubles."""
+    y = torch.log_softmax(x / T, dim=1)
+    there = (idx >= 0) & (idx < C)
+    at = idx.clamp(0, C - 1)
+    t = t.double()
+    if tail:
+        lp = t
+        p = torch.where(there, t.exp(), 0.0)
+    else:
+        lp = torch.log_softmax((t / T).masked_fill(~there, -math.inf), dim=1).nan_to_num(nan=-math.inf)
+        p = lp.exp()
+    term = torch.where(p > 0, p * (torch.where(p > 0, lp, 0.0) - y.gather(1, at)), 0.0)
+    loss = term.sum(dim=1)
+    listed = torch.zeros(x.shape, dtype=torch.float64).scatter_add_(1, at, there.double()) > 0
+    left = (1 - p.sum(dim=1)).clamp(min=0) if tail else torch.zeros(len(x), dtype=torch.float64)
+    some = ((~listed) & (x.detach() > -math.inf)).any(dim=1)
+    rest = torch.logsumexp(y.masked_fill(listed, -math.inf), dim=1)
+    held = some & (left > 0)
+    safe = torch.where(held, left, 1.0)
+    loss = loss + torch.where(held, left * (safe.log() - torch.where(held, rest, 0.0)), 0.0)
+    return loss, p, listed, torch.where(held, left, 0.0), rest, y
+
+
+def _teacher(R, C, K, T, tail, seed, empty=0.1, repeat=False):
+    g = _gen(seed)
+    idx = torch.stack([torch.randperm(C, generator=g)[:K] if K <= C else torch.randint(0, C, (K,), generator=g) for _ in range(R)])
+    t = torch.randn(R, K, generator=g) * 2
+    if tail:
+        t = torch.log_softmax(torch.cat([t, torch.full((R, 1), 1.0)], dim=1), dim=1)[:, :K].contiguous()
+    gone = torch.rand(R, K, generator=g) < empty
+    idx = torch.where(gone, torch.where(torch.rand(R, K, generator=g) < 0.5, -1, C + 2), idx)
+    t = torch.where(gone, math.nan, t)                    # the value of an empty entry is not looked at
+    if repeat and K >= 4:
+        idx[:, K // 2] = idx[:, 0]; idx[:, K - 1] = idx[:, 0]
+        for c in (K // 2, K - 1):
+            t[:, c] = torch.where(idx[:, 0] == idx[:, c], torch.where(torch.isnan(t[:, 0]), t[:, 0], t[:, 0] - 1.0), t[:, c])
+    return idx, t
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("R,C,pitch,offset", [s for s in SHAPES if s[1] < 200000])
+@pytest.mark.parametrize("K,T,tail,repeat", [(1, 1.0, False, False), (20, 2.0, False, True), (64, 1.0, True, False), (128, 0.7, True, True)])
+def test_distill(R, C, pitch, offset, dtype, K, T, tail, repeat):
+    from ttts_amd import ops
+    x = _logits(R, C, pitch, dtype, 11 * R + C, offset)
+    repeat = repeat or K > C
+    idx, t = _teacher(R, C, K, T, tail, C + K, repeat=repeat)
+    g = torch.randn(R, generator=_gen(9))
+    loss, stats = ops.distill_fwd(x, idx.cuda(), t.cuda(), C=C, temperature=T, tail=tail)
+    d = ops.distill_bwd(x, idx.cuda(), t.cuda(), stats, g.cuda(), C=C, temperature=T, tail=tail)
+    leaf = x[:, :C].double().cpu().requires_grad_(True)
+    tz = torch.where((idx >= 0) & (idx < C), t, 0.0)
+    ref, p, listed, left, rest, y = _ref_distill(leaf, idx, tz, C, T, tail)
+    grad, = torch.autograd.grad((ref * g.double()).sum(), leaf)
+    ref, y, rest = ref.detach(), y.detach(), rest.detach()
+    q = y.exp()
+    at = idx.clamp(0, C - 1)
+    mass = p.sum(dim=1)
+    # every p is off by a few U of itself and of its exponent, log q as log p above; what is left of the mass by K / 2 + 4 steps of the sum
+    logs = torch.where(p > 0, p * (torch.where(p > 0, p, 1.0).log().abs() + y.gather(1, at).abs()), 0.0).sum(dim=1)
+    l_off = (K / 2 + 8) * U * (1 + mass)
+    r_log = torch.where(left > 0, torch.where(left > 0, left, 1.0).log().abs() + rest.nan_to_num(neginf=0.0).abs() + 1, 0.0)
+    # the relative error of q_rest / q_listed is that of two sums
+    bound = (_r(C) + 16 * U) * (mass + logs + left * (1 + rest.nan_to_num(neginf=0.0).abs())) + (K + 8) * U * logs + l_off * r_log * tail + 8 * U
+    _inside(loss, ref, bound, "row_loss")
+    target = torch.zeros(R, C, dtype=torch.float64).scatter_add_(1, at, p)
+    r = torch.where(listed, 0.0, (y - rest[:, None]).exp().nan_to_num(nan=0.0, posinf=0.0))
+    size = q * (mass + left)[:, None] + target + left[:, None] * r
+    l_err = (l_off * tail)[:, None] * (q + r) * (left > 0)[:, None]
+    gb = g.double().abs()[:, None] / T
+    bound = gb * (size * (4 * _r(C) + (K + 16) * U + 8 * U * (y.abs() + 1)) + 2 * l_err + 4 * U * size) + _half_step(grad, dtype) + 1e-37
+    _inside(d[:, :C], grad, bound, "dlogits")
+    assert not d[:, C:].any()
+    # added to what is there, in one rounding; the columns from C on stay
+    base = torch.randn(x.shape, generator=_gen(4)).to(dtype).cuda()
+    acc = ops.distill_bwd(x, idx.cuda(), t.cuda(), stats, g.cuda(), C=C, temperature=T, tail=tail, dlogits=base.clone(), accumulate=True)
+    want = base[:, :C].double().cpu() + grad
+    _inside(acc[:, :C], want, bound + _half_step(want, dtype) + 2 * U * want.abs(), "accumulated dlogits")
+    assert torch.equal(acc[:, C:], base[:, C:])
+
+
+@pytest.mark.parametrize("C", [40, 1026, 40000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_distill_special_rows(C, dtype):
+    from ttts_amd import ops
+    K = 16
+    x = _logits(9, C, C, dtype, 2)
+    idx, t = _teacher(9, C, K, 1.0, True, 1, empty=0.0)
+    x[0] = -math.inf                                       # the student's mask leaves nothing
+    x[1] = LOWEST[dtype]                                   # uniform
+    idx[2] = -1                                            # no entries: tail mode compares the whole mass with the whole
+    x[3] = -math.inf; x[3].scatter_(0, idx[3].cuda(), torch.linspace(-1, 1, K).to(dtype).cuda())   # every class left is named
+    x[4, idx[4, 3]] = -math.inf                            # the teacher wants a class that the student forbids
+    t[5] = -math.inf; t[5, 2] = 0.0                        # all mass on one class
+    x[6, 3] = math.nan
+    t[7, 4] = -math.inf
+    for tail in (False, True):
+        loss, stats = ops.distill_fwd(x, idx.cuda(), t.cuda(), tail=tail)
+        d = ops.distill_bwd(x, idx.cuda(), t.cuda(), stats, torch.ones(9, device="cuda"), tail=tail)
+        keep = torch.tensor([1, 2, 3, 5, 7, 8])
+        leaf = x[keep.cuda()].double().cpu().requires_grad_(True)
+        ref, p, listed, left, rest, y = _ref_distill(leaf, idx[keep], t[keep], C, 1.0, tail)
+        _inside(loss.cpu()[keep], ref.detach(), 1e-5 * (1 + ref.detach().abs()), "row_loss")   # 1e-5 = 168 U: C / 64 of 40000 is 625 parts, most of them empty lanes' 20
+        q = y.detach().exp()
+        target = torch.zeros(len(keep), C, dtype=torch.float64).scatter_add_(1, idx[keep].clamp(min=0), p)
+        r = torch.where(listed, 0.0, (y.detach() - rest.detach()[:, None]).exp().nan_to_num(0.0))
+        grad = q * (p.sum(dim=1) + left)[:, None] - target - left[:, None] * r
+        size = q + target + left[:, None] * r
+        _inside(d.cpu()[keep], grad, size * 4e-5 + 40 * U + _half_step(grad, dtype), "dlogits")
+        assert loss[0].item() == 0.0 and not d[0].any()
+        assert loss[4].item() == math.inf and torch.isfinite(d[4]).all()
+        assert torch.isnan(loss[6]) and torch.isnan(d[6]).any()
+        if not tail:
+            assert loss[2].item() == 0.0 and not d[2].any()
+
+
+def test_gradients_agree_with_differences():
+    """(f(x + h v) - f(x - h v)) / 2h of the kernels' own forward against <gradient, v>, |v| <= 1 per class: the cubic term is at most
+    h^2 / 6 times a third cumulant (<= 8 / 6^(3/2) < 1) and the sums are good to 2 B / 2h with B the forward's bound."""
+    from ttts_amd import ops
+    R, C, h, K = 6, 1500, 2.0 ** -5, 24
+    x = _logits(R, C, C, torch.float32, 21, std=1.0)
+    v = torch.rand(R, C, generator=_gen(3)).cuda() * 2 - 1
+    tokens = torch.randint(0, C, (R,), generator=_gen(4)).cuda()
+    one = torch.ones(R, device="cuda")
+    B = _r(C) * 12 + 4 * U * 12
+    tol = B / h + h * h / 6 * 12
+    fwd = lambda z: ops.token_logprobs_fwd(z, tokens)  # noqa: E731
+    r = fwd(x)
+    up, down = fwd(x + h * v), fwd(x - h * v)
+    for name, gl, gh in (("logp", one, None), ("entropy", 0 * one, one)):
+        d = ops.token_logprobs_bwd(x, tokens, r.stats, r.entropy, gl, gh)
+        num = (getattr(up, name) - getattr(down, name)).double() / (2 * h)
+        assert ((d.double() * v.double()).sum(dim=1) - num).abs().max().item() <= tol, name
+    for tail in (False, True):
+        idx, t = (z.cuda() for z in _teacher(R, C, K, 1.0, tail, 5, empty=0.0))
+        _, stats = ops.distill_fwd(x, idx, t, tail=tail)
+        d = ops.distill_bwd(x, idx, t, stats, one, tail=tail)
+        num = (ops.distill_fwd(x + h * v, idx, t, tail=tail)[0] - ops.distill_fwd(x - h * v, idx, t, tail=tail)[0]).double() / (2 * h)
+        assert ((d.double() * v.double()).sum(dim=1) - num).abs().max().item() <= tol, tail
+
+
+def test_no_rows_and_many_rows():
+    from ttts_amd import ops
+    e = torch.empty(0, 100, device="cuda")
+    none = torch.empty(0, dtype=torch.int64, device="cuda")
+    r = ops.token_logprobs_fwd(e, none, top_k=4)
+    assert r.logp.shape == (0,) and r.top_idx.shape == (0, 4)
+    assert ops.token_logprobs_bwd(e, none, r.stats, r.entropy, r.logp).shape == (0, 100)
+    i, t = torch.empty(0, 3, dtype=torch.int64, device="cuda"), torch.empty(0, 3, device="cuda")
+    loss, stats = ops.distill_fwd(e, i, t)
+    assert loss.shape == (0,) and ops.distill_bwd(e, i, t, stats, loss).shape == (0, 100)
+    # more rows than a 16-bit grid dimension
+    R = 70001
+    x = _logits(R, 4, 8, torch.float16, 1)
+    tok = torch.randint(0, 4, (R,), generator=_gen(2)).cuda()
+    r = ops.token_logprobs_fwd(x, tok, C=4, top_k=2)
+    logp, ent, tl, ti, _, _ = _ref_logprobs(x, tok, 4, 2, 1.0)
+    _inside(r.logp, logp, _r(4) + 4 * U * logp.abs(), "logp")
+    assert torch.equal(r.top_idx.cpu(), ti)
+
+
+def test_offsets_past_32_bits():
+    """The last rows of a logits tensor of more than 2^31 elements (two-byte classes: 4.3 GB)."""
+    from ttts_amd import ops
+    R, C = 2200, 1000003
+    x = torch.zeros(R, C, dtype=torch.float16, device="cuda")
+    x[-2:] = (torch.randn(2, C, generator=_gen(8)) * 2).half().cuda()
+    tokens = torch.zeros(R, dtype=torch.int64, device="cuda"); tokens[-1] = C - 1
+    r = ops.token_logprobs_fwd(x, tokens, top_k=3)
+    logp, ent, tl, ti, y, _ = _ref_logprobs(x[-2:], tokens[-2:], C, 3, 1.0)
+    _inside(r.logp[-2:], logp, _r(C) + 4 * U * logp.abs(), "logp")
+    assert torch.equal(r.top_idx[-2:].cpu(), ti)
+    assert abs(r.logp[0].item() + math.log(C)) < _r(C) and r.top_idx[0].tolist() == [0, 1, 2]
+    d = ops.token_logprobs_bwd(x, tokens, r.stats, r.entropy, torch.ones(R, device="cuda"), dlogits=x)
+    ref = -y.exp()
+    ref[0, 0] += 1; ref[1, C - 1] += 1
+    _inside(d[-2:], ref, y.exp() * (4 * _r(C) + 200 * U) + 4 * U + _half_step(ref, torch.float16), "dlogits")
+
+
+def test_streams_and_graphs():
+    """On a side stream, and captured: every replay, with other work between them, gives what the eager calls give."""
+    from ttts_amd import ops
+    R, C, K = 40, 40000, 12                                # rows of several segments: the calls that use a workspace
+    xs = [_logits(R, C, C, torch.bfloat16, s) for s in range(3)]
+    tokens = torch.randint(0, C, (R,), generator=_gen(1)).cuda()
+    idx, t = (z.cuda() for z in _teacher(R, C, K, 1.0, True, 5))
+    one = torch.ones(R, device="cuda")
+
+    def step(x):
+        r = ops.token_logprobs_fwd(x, tokens, top_k=8)
+        d = ops.token_logprobs_bwd(x, tokens, r.stats, r.entropy, one, one)
+        loss, stats = ops.distill_fwd(x, idx, t, tail=True)
+        return list(r) + [d, loss, stats, ops.distill_bwd(x, idx, t, stats, one, tail=True)]
+    want = [step(x) for x in xs]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step(xs[0])
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want[0]))
+    static = [xs[0].clone(), xs[0].clone()]
+    graphs, outs = [], []
+    for s in static:                                       # two graphs alive at once
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step(s))
+        graphs.append(g)
+    for n in range(4):
+        for j in (0, 1):
+            static[j].copy_(xs[(n + j) % 3])
+        graphs[0].replay(); graphs[1].replay()
+        step(xs[2])
+        torch.cuda.synchronize()
+        for j in (0, 1):
+            assert all(torch.equal(a, b) for a, b in zip(outs[j], want[(n + j) % 3])), (n, j)
+
+
+def test_refusals_on_the_gpu():
+    from ttts_amd import ops
+    from ttts_amd.lib import TttsError
+    x = torch.zeros(4, 16, device="cuda")
+    tok = torch.zeros(4, dtype=torch.int64, device="cuda")
+    idx, t = torch.zeros(4, 3, dtype=torch.int64, device="cuda"), torch.zeros(4, 3, device="cuda")
+    bad = [lambda: ops.token_logprobs_fwd(x.double(), tok), lambda: ops.token_logprobs_fwd(x, tok[:3]), lambda: ops.token_logprobs_fwd(x, tok.int()),
+           lambda: ops.token_logprobs_fwd(x, tok, C=17), lambda: ops.token_logprobs_fwd(x, tok, C=0), lambda: ops.token_logprobs_fwd(x, tok, top_k=65),
+           lambda: ops.token_logprobs_fwd(x, tok, top_k=-1), lambda: ops.token_logprobs_fwd(x, tok, temperature=0.0),
+           lambda: ops.token_logprobs_fwd(x, tok, temperature=math.nan), lambda: ops.token_logprobs_fwd(x.t(), tok),
+           lambda: ops.token_logprobs_fwd(x[:1].expand(4, 16), tok), lambda: ops.token_logprobs_fwd(x, tok.cpu()), lambda: ops.token_logprobs_fwd(x.cpu(), tok),
+           lambda: ops.distill_fwd(x, idx, t[:, :2]), lambda: ops.distill_fwd(x, idx, t.double()), lambda: ops.distill_fwd(x, idx[:, 0], t),
+           lambda: ops.distill_fwd(x, torch.zeros(4, 129, dtype=torch.int64, device="cuda"), torch.zeros(4, 129, device="cuda")),
+           lambda: ops.distill_fwd(x, idx[:, :0], t[:, :0]), lambda: ops.distill_fwd(x, idx, t, temperature=-1.0)]
+    s2, s3, v = torch.zeros(4, 2, device="cuda"), torch.zeros(4, 3, device="cuda"), torch.zeros(4, device="cuda")
+    bad += [lambda: ops.token_logprobs_bwd(x, tok, s3, v, v), lambda: ops.token_logprobs_bwd(x, tok, s2, v, v[:2]),
+            lambda: ops.token_logprobs_bwd(x, tok, s2, v, v, dlogits=x.half()), lambda: ops.token_logprobs_bwd(x, tok, s2, v, v, dlogits=x[:, :8]),
+            lambda: ops.distill_bwd(x, idx, t, s2, v), lambda: ops.distill_bwd(x, idx, t, s3, v, accumulate=True),
+            lambda: ops.distill_bwd(x, idx, t, s3, v, accumulate=True, dlogits=x)]
+    for n, f in enumerate(bad):
+        with pytest.raises(TttsError):
+            f()
+            pytest.fail("refusal %d did not come" % n)

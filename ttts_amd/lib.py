@@ -14,7 +14,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(CSRC, "build")
 SO_PATH = os.environ.get("TTTS_LIB") or os.path.join(HERE, "libttts_hip.so")   # TTTS_LIB: an alternate build of the same ABI (same-box A/B runs: tools/gpu_ab_lib.sh)
-SOURCES = ["lib.hip", "elementwise.hip", "gemm.hip", "attn.hip", "attn_dh64.hip", "vq.hip", "stft.hip", "conv.hip", "conv_mfma.hip", "conv_thin.hip", "conv_grouped.hip", "losses.hip", "vqvae_ops.hip", "attn_f32.hip", "attn_cross.hip", "peq.hip", "decode.hip", "diffusion_ops.hip", "fp8_gemm.hip", "attn_relpos.hip"]
+SOURCES = ["lib.hip", "elementwise.hip", "gemm.hip", "attn.hip", "attn_dh64.hip", "vq.hip", "stft.hip", "conv.hip", "conv_mfma.hip", "conv_thin.hip", "conv_grouped.hip", "losses.hip", "vqvae_ops.hip", "attn_f32.hip", "attn_cross.hip", "peq.hip", "decode.hip", "diffusion_ops.hip", "fp8_gemm.hip", "attn_relpos.hip", "scoring.hip", "paged.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # No packed fp32 instructions (v_pk_add / mul / fma_f32): some of their forms have given wrong results on this hardware now and then.
 # hipcc -O3 forms them from ordinary float code by itself; the host pass does not know the feature and says so (harmless).
@@ -25,6 +25,8 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-munsafe-fp-atomics", "-
 EXTRA_FLAGS = {"attn_dh64.hip": ["-fno-honor-nans", "-fno-slp-vectorize"]}
 
 TTTS_OK = 0
+DTYPE_F32, DTYPE_BF16, DTYPE_F16 = range(3)
+SCORE_MAX_CLASSES, SCORE_MAX_TOP, DISTILL_MAX_K = 1 << 20, 64, 128
 EPI_STORE_BF16, EPI_GELU_BF16, EPI_RESID_ADD_F32, EPI_DGELU_BF16, EPI_STORE_F32 = range(5)
 
 
@@ -191,6 +193,16 @@ SIGNATURES = {
     "ttts_diffusion_loss_workspace_bytes": (_I64, [_I32]),
     "ttts_diffusion_loss_fwd_f32": (_I32, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _P]),
     "ttts_diffusion_loss_bwd_f32": (_I32, [_P, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _P]),
+    "ttts_token_logprobs_workspace_bytes": (_I64, [_I32, _I32, _I32]),
+    "ttts_token_logprobs_fwd": (_I32, [_P, _I32, _I64, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _F, _P, _I64, _P]),
+    "ttts_token_logprobs_bwd": (_I32, [_P, _I32, _I64, _P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _F, _P]),
+    "ttts_distill_workspace_bytes": (_I64, [_I32, _I32]),
+    "ttts_distill_fwd": (_I32, [_P, _I32, _I64, _P, _P, _P, _P, _I32, _I32, _I32, _F, _I32, _P, _I64, _P]),
+    "ttts_distill_bwd": (_I32, [_P, _I32, _I64, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _F, _I32, _I32, _P]),
+    "ttts_kv_page_write": (_I32, [_P, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _P]),
+    "ttts_attn_paged_decode_workspace_bytes": (_I64, [_I32, _I32, _I32, _I32, _I32, _I32]),
+    "ttts_attn_paged_decode": (_I32, [_P, _I64, _I64, _P, _P, _P, _I64, _P, _P, _I64, _I64, _P, _I32, _I32, _I32, _I32, _I32, _I32,
+                                      _I32, _I32, _F, _P, _I64, _P]),
     "ttts_linear_decode_bf16": (_I32, [_P, _I64, _I32, _P, _P, _P, _P, _P, _I64, _P, _P, _I64, _P, _I32, _I32, _I32, _I32, _P]),
     "ttts_decode_embed_f32": (_I32, [_P, _P, _P, _P, _I32, _P, _I32, _I32, _I32, _I32, _P]),
     "ttts_kv_cache_fill_bf16": (_I32, [_P, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _P]),

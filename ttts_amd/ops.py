@@ -2,6 +2,8 @@
 the current HIP stream and (elsewhere) torch.distributed.  Every function requires tensors on a ROCm device and
 raises `TttsError` on any failure -- there is no eager / CPU fallback.
 """
+import collections
+import contextlib
 import ctypes
 
 import numpy as np
@@ -14,7 +16,8 @@ from .lib import (EPI_DGELU_BF16, EPI_GELU_BF16, EPI_RESID_ADD_F32, EPI_STORE_BF
 
 __all__ = ["gemm_nt", "gemm_tn_accum", "colsum_accum", "attn_fwd", "attn_bwd", "layernorm_fwd", "layernorm_bwd",
            "embed_fwd", "embed_bwd", "ce_fwd", "ce_bwd", "gradnorm", "adamw", "adamw_schedule", "vq_nearest",
-           "vq_commit", "vq_ema_update", "stft_mag", "mel_log", "CastPlan", "TransposePlan", "ColsumPlan", "LnFinalizePlan", "TnPlan", "probe_layout", "device_info"]
+           "vq_commit", "vq_ema_update", "stft_mag", "mel_log", "CastPlan", "TransposePlan", "ColsumPlan", "LnFinalizePlan", "TnPlan", "probe_layout", "device_info",
+           "token_logprobs_fwd", "token_logprobs_bwd", "distill_fwd", "distill_bwd", "kv_page_write", "attn_paged_decode"]
 
 
 def _raw_stream(index=None):
@@ -882,6 +885,206 @@ def sample_logits(logits, ctr, tokens, finished, V, history=None, hist_base=0, o
 def decode_advance(ctr, finished):
     _req(ctr, torch.int32, "ctr"); _req(finished, torch.uint8, "finished")
     check(_l.get().ttts_decode_advance(_p(ctr), _p(finished), finished.shape[0], _stream()), "decode_advance")
+
+
+# ---- scoring of given tokens, distillation on a teacher's alternatives (csrc/scoring.hip) -------------------------------
+_DTYPE_CODES = {torch.float32: _l.DTYPE_F32, torch.bfloat16: _l.DTYPE_BF16, torch.float16: _l.DTYPE_F16}
+
+
+def _on(what, *named):
+    """All of the (tensor, name) pairs live on one GPU: a context that makes it the current device, so that the launch goes to torch's
+    current stream of THAT device.  Raises for a CPU tensor or two devices."""
+    dev = None
+    for t, name in named:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise TttsError("%s: %s must live on the GPU (no CPU fallback in ttts_amd)" % (what, name))
+        if dev is not None and t.device != dev:
+            raise TttsError("%s: %s is on %s, the others on %s" % (what, name, t.device, dev))
+        dev = t.device
+    return contextlib.nullcontext() if dev.index == torch._C._cuda_getDevice() else torch.cuda.device(dev)
+
+
+def _rows(t, what, name):
+    """(row pitch, rows, columns) of a 2-D tensor with contiguous rows that do not overlap."""
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        raise TttsError("%s: %s must be 2-D with contiguous rows, got shape %s strides %s" % (what, name, tuple(t.shape), t.stride()))
+    return (t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])), t.shape[0], t.shape[1]
+
+
+def _vec(t, dtype, shape, what, name):
+    if t is not None and (t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous()):
+        raise TttsError("%s: %s must be a contiguous %s tensor of shape %s, got %s %s" % (what, name, dtype, tuple(shape), t.dtype, tuple(t.shape)))
+
+
+def _logits(logits, C, what):
+    code = _DTYPE_CODES.get(logits.dtype)
+    if code is None:
+        raise TttsError("%s: logits must be float32, bfloat16 or float16, got %s" % (what, logits.dtype))
+    ld, R, cols = _rows(logits, what, "logits")
+    C = cols if C is None else int(C)
+    if not 0 < C <= cols:
+        raise TttsError("%s: C = %d classes of %d columns" % (what, C, cols))
+    return code, ld, R, C
+
+
+def _grad_rows(dlogits, logits, what):
+    if dlogits is None:
+        dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    if dlogits.dtype != logits.dtype or dlogits.shape != logits.shape:
+        raise TttsError("%s: dlogits must have the type and the shape of logits" % what)
+    ldd, _, _ = _rows(dlogits, what, "dlogits")
+    if dlogits.data_ptr() == logits.data_ptr() and logits.shape[0] > 1 and ldd != logits.stride(0):
+        raise TttsError("%s: dlogits in the logits' place needs their row pitch" % what)
+    return dlogits, ldd
+
+
+def _workspace(nbytes, device):
+    """Scratch of one call: allocated on the current stream (a captured call gets it from its graph's own pool)."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None
+
+
+TokenLogprobs = collections.namedtuple("TokenLogprobs", ["logp", "entropy", "top_logp", "top_idx", "stats"])
+
+
+def token_logprobs_fwd(logits, tokens, C=None, top_k=0, temperature=1.0):
+    """Log-probabilities of given tokens under softmax(logits / temperature), the rows' entropies and the top_k <= 64 best classes.
+    logits f32 / bf16 / f16 [R, >= C] (rows may have a pitch; columns from C on are not looked at), tokens int64 [R] (outside [0, C): no
+    token, logp 0).  Returns TokenLogprobs(logp f32 [R], entropy f32 [R], top_logp f32 [R, top_k] | None, top_idx int64 [R, top_k] |
+    None, stats f32 [R, 2] for the backward).  Alternatives: best first, equal logits by ascending class; -inf / -1 where a row has
+    fewer classes above -inf.  Rows of -inf only and rows with NaN: include/ttts_hip.h."""
+    what = "token_logprobs_fwd"
+    code, ld, R, C = _logits(logits, C, what)
+    _vec(tokens, torch.int64, (R,), what, "tokens")
+    k = int(top_k)
+    with _on(what, (logits, "logits"), (tokens, "tokens")):
+        f = lambda *shape, dt=torch.float32: torch.empty(shape, dtype=dt, device=logits.device)  # noqa: E731
+        r = TokenLogprobs(f(R), f(R), f(R, k) if k > 0 else None, f(R, k, dt=torch.int64) if k > 0 else None, f(R, 2))
+        n = _l.get().ttts_token_logprobs_workspace_bytes(R, C, k)
+        ws = _workspace(n, logits.device)
+        check(_l.get().ttts_token_logprobs_fwd(_p(logits), code, ld, _p(tokens), _p(r.logp), _p(r.entropy), _p(r.stats), _p(r.top_logp),
+                                               _p(r.top_idx), R, C, k, float(temperature), _p(ws), n, _stream()), what)
+    return r
+
+
+def token_logprobs_bwd(logits, tokens, stats, entropy, g_logp, g_entropy=None, C=None, temperature=1.0, dlogits=None):
+    """Gradient of token_logprobs_fwd's logp and entropy to the logits: dlogits (new, or the given tensor; `logits` itself is allowed)
+    of the logits' type and shape, columns from C on zero.  g_logp / g_entropy f32 [R]."""
+    what = "token_logprobs_bwd"
+    code, ld, R, C = _logits(logits, C, what)
+    _vec(tokens, torch.int64, (R,), what, "tokens"); _vec(stats, torch.float32, (R, 2), what, "stats")
+    for t, name in ((entropy, "entropy"), (g_logp, "g_logp"), (g_entropy, "g_entropy")):
+        _vec(t, torch.float32, (R,), what, name)
+    with _on(what, (logits, "logits"), (tokens, "tokens"), (stats, "stats"), (entropy, "entropy"), (g_logp, "g_logp"),
+             (g_entropy, "g_entropy"), (dlogits, "dlogits")):
+        dlogits, ldd = _grad_rows(dlogits, logits, what)
+        check(_l.get().ttts_token_logprobs_bwd(_p(logits), code, ld, _p(tokens), _p(stats), _p(entropy), _p(g_logp), _p(g_entropy),
+                                               _p(dlogits), ldd, R, C, logits.shape[1], float(temperature), _stream()), what)
+    return dlogits
+
+
+def distill_fwd(logits, teacher_idx, teacher_logp, C=None, temperature=1.0, tail=False):
+    """KL(teacher's listed classes || softmax(logits / temperature)) per row.  teacher_idx int64 / teacher_logp f32 [R, K], K <= 128
+    (an index outside [0, C): an empty entry).  tail False: teacher_logp / temperature is normalised over the row's entries; tail
+    True: they are log-probabilities at that temperature, and the mass that they leave out is compared with the student's on all
+    other classes.  Returns (row_loss f32 [R], stats f32 [R, 3] for the backward)."""
+    what = "distill_fwd"
+    code, ld, R, C = _logits(logits, C, what)
+    K = _teacher(teacher_idx, teacher_logp, R, what)
+    with _on(what, (logits, "logits"), (teacher_idx, "teacher_idx"), (teacher_logp, "teacher_logp")):
+        loss = torch.empty(R, dtype=torch.float32, device=logits.device)
+        stats = torch.empty(R, 3, dtype=torch.float32, device=logits.device)
+        n = _l.get().ttts_distill_workspace_bytes(R, C)
+        ws = _workspace(n, logits.device)
+        check(_l.get().ttts_distill_fwd(_p(logits), code, ld, _p(teacher_idx), _p(teacher_logp), _p(loss), _p(stats), R, C, K,
+                                        float(temperature), int(bool(tail)), _p(ws), n, _stream()), what)
+    return loss, stats
+
+
+def _teacher(idx, logp, R, what):
+    if idx.dim() != 2:
+        raise TttsError("%s: teacher_idx must be [rows, entries], got %s" % (what, tuple(idx.shape)))
+    _vec(idx, torch.int64, (R, idx.shape[1]), what, "teacher_idx"); _vec(logp, torch.float32, (R, idx.shape[1]), what, "teacher_logp")
+    return idx.shape[1]
+
+
+def distill_bwd(logits, teacher_idx, teacher_logp, stats, g_loss, C=None, temperature=1.0, tail=False, dlogits=None, accumulate=False):
+    """Gradient of distill_fwd's row losses to the logits, weighted by g_loss f32 [R]: dlogits (new, or the given tensor; `logits`
+    itself is allowed) of the logits' type and shape, columns from C on zero.  accumulate: added to the given dlogits instead
+    (columns from C on stay)."""
+    what = "distill_bwd"
+    code, ld, R, C = _logits(logits, C, what)
+    K = _teacher(teacher_idx, teacher_logp, R, what)
+    _vec(stats, torch.float32, (R, 3), what, "stats"); _vec(g_loss, torch.float32, (R,), what, "g_loss")
+    if accumulate and (dlogits is None or dlogits.data_ptr() == logits.data_ptr()):
+        raise TttsError("%s: accumulate needs a dlogits of its own" % what)
+    with _on(what, (logits, "logits"), (teacher_idx, "teacher_idx"), (teacher_logp, "teacher_logp"), (stats, "stats"), (g_loss, "g_loss"),
+             (dlogits, "dlogits")):
+        dlogits, ldd = _grad_rows(dlogits, logits, what)
+        check(_l.get().ttts_distill_bwd(_p(logits), code, ld, _p(teacher_idx), _p(teacher_logp), _p(stats), _p(g_loss), _p(dlogits), ldd, R, C,
+                                        logits.shape[1], K, float(temperature), int(bool(tail)), int(bool(accumulate)), _stream()), what)
+    return dlogits
+
+
+# ---- paged key / value cache (csrc/paged.hip) -----------------------------------------------------------------------------
+def _pages(k_pages, v_pages, what):
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or not (k_pages.is_contiguous() and v_pages.is_contiguous()):
+        raise TttsError("%s: k_pages / v_pages must be contiguous [pages, heads, page size, head_dim] tensors of one shape" % what)
+    if k_pages.dtype not in (torch.bfloat16, torch.float16) or v_pages.dtype != k_pages.dtype:
+        raise TttsError("%s: the cache must be bfloat16 or float16, got %s / %s" % (what, k_pages.dtype, v_pages.dtype))
+    return _DTYPE_CODES[k_pages.dtype]
+
+
+def _heads(t, dtype, shape, what, name):
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or t.stride(2) != 1:
+        raise TttsError("%s: %s must be a %s tensor of shape %s with contiguous heads, got %s %s strides %s"
+                        % (what, name, dtype, tuple(shape), t.dtype, tuple(t.shape), t.stride()))
+
+
+def kv_page_write(k, v, k_pages, v_pages, slots):
+    """Keys and values of new tokens enter a paged cache: row n of k / v [N, heads, head_dim] (views with strides of multiples of 8, as the
+    parts of a packed projection) goes to position slots[n] % page of page slots[n] // page of k_pages / v_pages [pages, heads, page
+    size, head_dim], bf16 or fp16.  slots int64 [N]; one outside the cache (-1: a padding row) writes nothing.  The slots of a call
+    differ from each other."""
+    what = "kv_page_write"
+    code = _pages(k_pages, v_pages, what)
+    P, H, page, dh = k_pages.shape
+    N = slots.shape[0] if slots.dim() == 1 else -1
+    _vec(slots, torch.int64, (N,), what, "slots")
+    _heads(k, k_pages.dtype, (N, H, dh), what, "k"); _heads(v, k_pages.dtype, (N, H, dh), what, "v")
+    with _on(what, (k, "k"), (v, "v"), (k_pages, "k_pages"), (v_pages, "v_pages"), (slots, "slots")):
+        check(_l.get().ttts_kv_page_write(_p(k), _p(v), k.stride(0), k.stride(1), v.stride(0), v.stride(1), _p(k_pages), _p(v_pages),
+                                          _p(slots), code, N, H, dh, page, P, _stream()), what)
+
+
+def attn_paged_decode(q, k_pages, v_pages, block_table, seq_lens, scale, out=None):
+    """Attention of one new token per sequence over a paged cache: q [M, H, head_dim] (a view with strides of multiples of 8), H a multiple
+    of the cache's heads (shared by neighbours); block_table int32 [M, width]: a sequence's pages in order; seq_lens int32 [M]: its
+    keys, the new token's among them.  Returns (out [M, H, head_dim] of q's type, lse f32 [M, H]).  A sequence without keys gets 0 and
+    -inf; keys of a table entry outside the cache are left out.  A slice block_table[:, :n] bounds the lengths to n pages."""
+    what = "attn_paged_decode"
+    code = _pages(k_pages, v_pages, what)
+    P, Hkv, page, dh = k_pages.shape
+    if q.dim() != 3 or block_table.dim() != 2 or block_table.dtype != torch.int32:
+        raise TttsError("%s: q must be [M, H, head_dim], block_table int32 [M, width]" % what)
+    M, H = q.shape[:2]
+    _heads(q, k_pages.dtype, (M, H, dh), what, "q"); _vec(seq_lens, torch.int32, (M,), what, "seq_lens")
+    ts, tm, width = _rows(block_table, what, "block_table")
+    if tm != M:
+        raise TttsError("%s: block_table has %d rows for %d sequences" % (what, tm, M))
+    if out is not None:
+        _heads(out, q.dtype, (M, H, dh), what, "out")
+    with _on(what, (q, "q"), (k_pages, "k_pages"), (v_pages, "v_pages"), (block_table, "block_table"), (seq_lens, "seq_lens"), (out, "out")):
+        if out is None:
+            out = torch.empty(M, H, dh, dtype=q.dtype, device=q.device)
+        lse = torch.empty(M, H, dtype=torch.float32, device=q.device)
+        n = _l.get().ttts_attn_paged_decode_workspace_bytes(M, H, Hkv, dh, page, width)
+        ws = _workspace(n, q.device)
+        check(_l.get().ttts_attn_paged_decode(_p(q), q.stride(0), q.stride(1), _p(k_pages), _p(v_pages), _p(block_table), ts, _p(seq_lens),
+                                              _p(out), out.stride(0), out.stride(1), _p(lse), code, M, H, Hkv, dh, page, P, width,
+                                              float(scale), _p(ws), n, _stream()), what)
+    return out, lse
 
 
 PEQ_PEAK, PEQ_LOW_SHELF, PEQ_HIGH_SHELF = 0, 1, 2

@@ -29,70 +29,247 @@ __global__ __launch_bounds__(256) void kv_page_write_kernel(const uint4* __restr
 struct PagedParams {
   const void *q, *kp, *vp;
   void* out;
-  float* lse;
+  float *lse, *part_o, *part_ml;          // partial results of split sequences: [M, H, chunks, DH] and [M, H, chunks][2]
   const int32_t *table, *lens;
   int64_t qs_m, qs_h, os_m, os_h, ts_m;   // strides in elements
-  int M, H, Hkv, page, P, width;          // width: pages of a table row
+  int H, Hkv, group, tiles, page_shift, P, width, chunk, chunks;   // tiles: 16-row tiles of a head group; width: pages of a table row
   float scale_log2;
 };
 
+template <typename T> struct Frag;
+template <> struct Frag<bf16> {
+  static __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Frag<_Float16> {
+  static __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+// maximum / sum over the four lanes that hold one column (lane & 15): rows of 16 lanes, then halves, exchanged by register swaps
+template <typename F>
+__device__ __forceinline__ float over_rows(float x, F op) {
+  const unsigned u = __builtin_bit_cast(unsigned, x);
+  const auto h = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const unsigned h0 = h[0], h1 = h[1];   // (scalars of their own: a bit_cast of a vector's element reads element 0)
+  const unsigned v = __builtin_bit_cast(unsigned, op(__builtin_bit_cast(float, h0), __builtin_bit_cast(float, h1)));
+  const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  const unsigned r0 = r[0], r1 = r[1];
+  return op(__builtin_bit_cast(float, r0), __builtin_bit_cast(float, r1));
+}
+
+// One workgroup = one chunk of keys of one (sequence, key / value head, 16 query rows); its waves take the chunk's 32-key tiles in turn,
+// each with a running maximum, sum and accumulator of its own, joined through LDS at the end.
+// A tile never touches LDS: both products are 16x16x32 MFMAs with the operand layout row = lane & 15, k = 8 (lane >> 4) ..+7,
+//   S[key][q]   = K Q^T   two products of 16 keys: lane (g = lane >> 4) gets the scores of keys 16 t + 4 g + r of query lane & 15;
+//   O^T[d][q]  += V^T P   the k index is a key in ANY order that both operands share: with k = 8 g + 4 t + r <-> key 16 t + 4 g + r the
+//                         weights are the B operand where they are, and a lane loads V rows 16 t + 4 g + r, DH / 16 neighbouring
+//                         columns each, which it re-pairs across rows in registers (product r of DH / 16 has rows d = (DH / 16) m + r).
+// The next tile's loads are in flight under this one's products, the table entries another tile ahead.  The queries of a shared
+// head fill rows of the products that are there anyway, so a cached key is read once for up to 16 of them.
+constexpr int PAGED_WAVES = 8;
 template <typename T, int DH>
-__global__ __launch_bounds__(256) void attn_paged_decode_kernel(PagedParams p) {
-  constexpr int LPK = DH / 8, KPW = 64 / LPK;
+__global__ __launch_bounds__(PAGED_WAVES * 64) void attn_paged_decode_kernel(PagedParams p) {
+  constexpr int NW = PAGED_WAVES, W = DH / 16, KC = DH / 32;
   typedef T T8 __attribute__((ext_vector_type(8)));
-  __shared__ float sm_acc[4][DH];
-  __shared__ float sm_ml[4][2];
-  const int h = blockIdx.x, m = blockIdx.y, hk = h / (p.H / p.Hkv);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane % LPK, grp = lane / LPK;
-  const int len = min(p.lens[m], (int)min((int64_t)p.width * p.page, (int64_t)0x7fffffff));
-  const T8 qv = *reinterpret_cast<const T8*>((const T*)p.q + m * p.qs_m + h * p.qs_h + sub * 8);
-  float mx = -3.0e38f, l = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int k0 = wave * KPW; k0 < len; k0 += 4 * KPW) {
-    const int key = k0 + grp;
-    if (key >= len) continue;
-    const int pg = p.table[m * p.ts_m + key / p.page];
-    if (pg < 0 || pg >= p.P) continue;
-    const int64_t at = (((int64_t)pg * p.Hkv + hk) * p.page + key % p.page) * DH + sub * 8;
-    const T8 kv = *reinterpret_cast<const T8*>((const T*)p.kp + at), vv = *reinterpret_cast<const T8*>((const T*)p.vp + at);
-    float s = 0.f;
+  typedef T TW __attribute__((ext_vector_type(W)));
+  extern __shared__ __attribute__((aligned(16))) float paged_lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
+  int id = blockIdx.x;
+  const int hk = id % p.Hkv; id /= p.Hkv;
+  const int tile = id % p.tiles; id /= p.tiles;
+  const int chunk = id % p.chunks;
+  const int64_t m = id / p.chunks;
+  const int len = min(p.lens[m], p.width << p.page_shift);
+  const int c0 = chunk * p.chunk, c1 = min(len, c0 + p.chunk);
+  if (c0 >= len && !(chunk == 0 && p.chunks == 1)) return;   // (the join looks at no chunk behind the sequence's end)
+  const int rows = min(16, p.group - tile * 16);
+  const int h0 = hk * p.group + tile * 16;
+  T8 qf[KC];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s = fmaf((float)qv[e], (float)kv[e], s);
-#pragma unroll
-    for (int o = 1; o < LPK; o <<= 1) s += __shfl_xor(s, o, 64);
-    s *= p.scale_log2;
-    const float mn = fmaxf(mx, s), a = __builtin_amdgcn_exp2f(mx - mn), e = __builtin_amdgcn_exp2f(s - mn);
-    l = l * a + e;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] = acc[j] * a + e * (float)vv[j];
-    mx = mn;
+  for (int c = 0; c < KC; ++c) {
+    qf[c] = T8{};
+    if (col < rows) qf[c] = *reinterpret_cast<const T8*>((const T*)p.q + m * p.qs_m + (int64_t)(h0 + col) * p.qs_h + 32 * c + 8 * g);
   }
+  float mx = -3.0e38f, l = 0.f;
+  f32x4 acc[W];
 #pragma unroll
-  for (int o = LPK; o < 64; o <<= 1) {
-    const float m2 = __shfl_xor(mx, o, 64), l2 = __shfl_xor(l, o, 64), mn = fmaxf(mx, m2);
-    const float a = __builtin_amdgcn_exp2f(mx - mn), b = __builtin_amdgcn_exp2f(m2 - mn);
-    l = l * a + l2 * b;
+  for (int r = 0; r < W; ++r) acc[r] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  struct Tile { T8 k[2][KC]; TW v[8]; int ok[2]; };
+  const int32_t* tab = p.table + m * p.ts_m;
+  const int last = max((c1 - 1) >> p.page_shift, 0);
+  auto entry = [&](int key) { return tab[min(key >> p.page_shift, last)]; };   // (never past the chunk's own pages)
+  auto load = [&](Tile& t, int key0, int e0, int e1) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] = acc[j] * a + __shfl_xor(acc[j], o, 64) * b;
-    mx = mn;
+    for (int h = 0; h < 2; ++h) {
+      const int e = h ? e1 : e0, key = key0 + 16 * h;
+      t.ok[h] = key < c1 && e >= 0 && e < p.P;
+      const int off = key & ((1 << p.page_shift) - 1);
+      const int64_t base = ((((int64_t)(t.ok[h] ? e : 0) * p.Hkv + hk) << p.page_shift) + off) * DH;
+      const T* kb = (const T*)p.kp + base + col * DH + 8 * g;
+      const T* vb = (const T*)p.vp + base + 4 * g * DH + col * W;
+#pragma unroll
+      for (int c = 0; c < KC; ++c) t.k[h][c] = *reinterpret_cast<const T8*>(kb + 32 * c);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) t.v[4 * h + r] = *reinterpret_cast<const TW*>(vb + r * DH);
+    }
+  };
+  auto attend = [&](Tile& t, int key0) {
+    float s[8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      f32x4 d = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < KC; ++c) d = Frag<T>::mfma(t.k[h][c], qf[c], d);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[4 * h + r] = d[r] * p.scale_log2;
+    }
+    if (!(t.ok[0] && t.ok[1] && key0 + 32 <= c1)) {   // keys behind the end, or of no page: whatever the memory holds there
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const bool in = t.ok[j >> 2] && key0 + 16 * (j >> 2) + 4 * g + (j & 3) < c1;
+        s[j] = in ? s[j] : -INFINITY;
+        t.v[j] = in ? t.v[j] : TW{};
+      }
+    }
+    float mt = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+    mt = over_rows(mt, [](float a, float b) { return fmaxf(a, b); });
+    if (__any(mt > mx)) {
+      const float mn = fmaxf(mx, mt), a = __builtin_amdgcn_exp2f(mx - mn);
+      l *= a;
+#pragma unroll
+      for (int r = 0; r < W; ++r) acc[r] *= a;
+      mx = mn;
+    }
+    T8 pf;                       // the weights enter the product in the cache's type; their sum is of the unrounded ones
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float e = __builtin_amdgcn_exp2f(s[j] - mx);
+      l += e;
+      pf[j] = (T)e;
+    }
+#pragma unroll
+    for (int r = 0; r < W; ++r) {
+      T8 a;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) a[j] = t.v[j][r];
+      acc[r] = Frag<T>::mfma(a, pf, acc[r]);
+    }
+  };
+  constexpr int STEP = 32 * NW;
+  int key = c0 + 32 * wave;
+  if (key < c1) {
+    Tile ta, tb;
+    load(ta, key, entry(key), entry(key + 16));
+    int e0 = entry(key + STEP), e1 = entry(key + STEP + 16);
+    for (;;) {
+      if (key + STEP < c1) {
+        load(tb, key + STEP, e0, e1);
+        e0 = entry(key + 2 * STEP); e1 = entry(key + 2 * STEP + 16);
+      }
+      attend(ta, key);
+      key += STEP;
+      if (key >= c1) break;
+      if (key + STEP < c1) {
+        load(ta, key + STEP, e0, e1);
+        e0 = entry(key + 2 * STEP); e1 = entry(key + 2 * STEP + 16);
+      }
+      attend(tb, key);
+      key += STEP;
+      if (key >= c1) break;
+    }
   }
-  if (grp == 0) {
+  l = over_rows(l, [](float a, float b) { return a + b; });
+  // ---- join the waves
+  float* sm_o = paged_lds;                       // [NW][rows][DH]
+  float* sm_ml = paged_lds + NW * rows * DH;     // [NW][rows][2]
+  if (col < rows) {
+    float* o = sm_o + (wave * rows + col) * DH + 4 * g * W;   // acc[r][i] is d = (4 g + i) W + r
 #pragma unroll
-    for (int j = 0; j < 8; ++j) sm_acc[wave][sub * 8 + j] = acc[j];
-    if (sub == 0) { sm_ml[wave][0] = mx; sm_ml[wave][1] = l; }
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int r = 0; r < W; ++r) o[i * W + r] = acc[r][i];
+    if (g == 0) { sm_ml[(wave * rows + col) * 2] = mx; sm_ml[(wave * rows + col) * 2 + 1] = l; }
   }
   __syncthreads();
-  if (threadIdx.x < DH) {
-    const float M = fmaxf(fmaxf(sm_ml[0][0], sm_ml[1][0]), fmaxf(sm_ml[2][0], sm_ml[3][0]));
+  for (int e = threadIdx.x; e < rows * DH; e += NW * 64) {
+    const int r = e / DH, d = e % DH;
+    float M = sm_ml[r * 2];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) M = fmaxf(M, sm_ml[(w * rows + r) * 2]);
     float L = 0.f, o = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float a = __builtin_amdgcn_exp2f(sm_ml[w][0] - M);
-      L += sm_ml[w][1] * a;
-      o += sm_acc[w][threadIdx.x] * a;
+    for (int w = 0; w < NW; ++w) {
+      const float a = __builtin_amdgcn_exp2f(sm_ml[(w * rows + r) * 2] - M);
+      L += sm_ml[(w * rows + r) * 2 + 1] * a;
+      o += sm_o[(w * rows + r) * DH + d] * a;
     }
-    ((T*)p.out)[m * p.os_m + h * p.os_h + threadIdx.x] = (T)(L == 0.f ? 0.f : o / L);
-    if (threadIdx.x == 0) p.lse[(int64_t)m * p.H + h] = L == 0.f ? -INFINITY : (M + __log2f(L)) * 0.6931471805599453f;
+    const int64_t mh = m * p.H + h0 + r;
+    if (p.chunks == 1) {
+      ((T*)p.out)[m * p.os_m + (int64_t)(h0 + r) * p.os_h + d] = (T)(L == 0.f ? 0.f : o / L);
+      if (d == 0) p.lse[mh] = L == 0.f ? -INFINITY : (M + __log2f(L)) * 0.6931471805599453f;
+    } else {
+      p.part_o[(mh * p.chunks + chunk) * DH + d] = o;
+      if (d == 0) { p.part_ml[(mh * p.chunks + chunk) * 2] = M; p.part_ml[(mh * p.chunks + chunk) * 2 + 1] = L; }
+    }
   }
+}
+
+// the chunks of a split sequence: one workgroup per (sequence, query head), DH / 4 lanes per chunk
+template <typename T, int DH>
+__global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedParams p) {
+  constexpr int LPC = DH / 4, G = 256 / LPC;
+  __shared__ float4 sm_o[G][LPC];
+  __shared__ float sm_ml[G][2];
+  const int64_t mh = blockIdx.x, m = mh / p.H;
+  const int sub = threadIdx.x % LPC, grp = threadIdx.x / LPC;
+  const int len = min(p.lens[m], p.width << p.page_shift);
+  const int n = len > 0 ? (len + p.chunk - 1) / p.chunk : 0;
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + mh * p.chunks;
+  const float4* po = reinterpret_cast<const float4*>(p.part_o) + mh * p.chunks * LPC + sub;
+  float M = -3.0e38f, L = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int c = grp; c < n; c += G) {
+    const float2 s = ml[c];
+    const float4 v = po[(int64_t)c * LPC];
+    const float mn = fmaxf(M, s.x), a = __builtin_amdgcn_exp2f(M - mn), b = __builtin_amdgcn_exp2f(s.x - mn);
+    L = L * a + s.y * b;
+    o.x = o.x * a + v.x * b; o.y = o.y * a + v.y * b; o.z = o.z * a + v.z * b; o.w = o.w * a + v.w * b;
+    M = mn;
+  }
+  sm_o[grp][sub] = o;
+  if (sub == 0) { sm_ml[grp][0] = M; sm_ml[grp][1] = L; }
+  __syncthreads();
+  if (threadIdx.x < DH) {
+    const int d = threadIdx.x;
+    M = sm_ml[0][0];
+#pragma unroll
+    for (int i = 1; i < G; ++i) M = fmaxf(M, sm_ml[i][0]);
+    float x = 0.f;
+    L = 0.f;
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      const float a = __builtin_amdgcn_exp2f(sm_ml[i][0] - M);
+      L += sm_ml[i][1] * a;
+      x += reinterpret_cast<const float*>(sm_o[i])[d] * a;
+    }
+    ((T*)p.out)[m * p.os_m + (mh % p.H) * p.os_h + d] = (T)(L == 0.f ? 0.f : x / L);
+    if (d == 0) p.lse[mh] = L == 0.f ? -INFINITY : (M + __log2f(L)) * 0.6931471805599453f;
+  }
+}
+
+#ifndef PAGED_TARGET
+#define PAGED_TARGET 2048
+#endif
+#ifndef PAGED_MIN_CHUNK
+#define PAGED_MIN_CHUNK 512
+#endif
+// How a sequence of up to `longest` keys is split: enough workgroups to fill the card, but no chunk under what pays for its join.
+static void paged_split(int64_t units, int64_t longest, int& chunk, int& chunks) {
+  int64_t n = cdiv(PAGED_TARGET, units);
+  n = n < cdiv(longest, PAGED_MIN_CHUNK) ? n : cdiv(longest, PAGED_MIN_CHUNK);
+  const int64_t c = cdiv(cdiv(longest, n), 32 * PAGED_WAVES) * 32 * PAGED_WAVES;
+  chunk = (int)(c < 0x40000000 ? c : 0x40000000);
+  chunks = (int)cdiv(longest, chunk);
 }
 
 }  // namespace ttts
@@ -126,16 +303,28 @@ extern "C" int ttts_kv_page_write(const void* k, const void* v, int64_t k_stride
   return check_launch("kv_page_write");
 }
 
+static int64_t paged_tiles(int32_t H, int32_t Hkv) { return cdiv(H / Hkv, 16); }
+// bytes of the partial results; 0 where no sequence is split
+static int64_t paged_bytes(int64_t M, int64_t H, int dh, int chunks) { return chunks > 1 ? cdiv(M * H * chunks * (dh + 2) * 4, 16) * 16 : 0; }
+
 extern "C" int64_t ttts_attn_paged_decode_workspace_bytes(int32_t M, int32_t H, int32_t Hkv, int32_t head_dim, int32_t page, int32_t width) {
-  return 0;
+  if (M <= 0 || Hkv <= 0 || H < Hkv || head_dim <= 0 || page <= 0 || width <= 0) return 0;
+  int chunk, chunks;
+  paged_split(M * (int64_t)Hkv * paged_tiles(H, Hkv), (int64_t)width * page, chunk, chunks);
+  return paged_bytes(M, H, head_dim, chunks);
 }
 
-template <typename T>
-static void launch_paged(const PagedParams& p, int dh, hipStream_t st) {
-  const dim3 grid(p.H, p.M);
-  if (dh == 32) attn_paged_decode_kernel<T, 32><<<grid, 256, 0, st>>>(p);
-  else if (dh == 64) attn_paged_decode_kernel<T, 64><<<grid, 256, 0, st>>>(p);
-  else attn_paged_decode_kernel<T, 128><<<grid, 256, 0, st>>>(p);
+template <typename T, int DH>
+static int launch_paged(const PagedParams& p, int64_t grid, int64_t rows, hipStream_t st) {
+  static OnceFlag once;
+  const int lds = PAGED_WAVES * (p.group < 16 ? p.group : 16) * (DH + 2) * 4;
+  if (lds_opt_in(once, (const void*)attn_paged_decode_kernel<T, DH>, PAGED_WAVES * 16 * (DH + 2) * 4) != hipSuccess)
+    return fail(TTTS_EHIP, "attn_paged_decode: LDS opt-in failed");
+  attn_paged_decode_kernel<T, DH><<<(unsigned)grid, PAGED_WAVES * 64, lds, st>>>(p);
+  const int rc = check_launch("attn_paged_decode");
+  if (rc || p.chunks == 1) return rc;
+  attn_paged_join_kernel<T, DH><<<(unsigned)rows, 256, 0, st>>>(p);
+  return check_launch("attn_paged_decode join");
 }
 
 extern "C" int ttts_attn_paged_decode(const void* q, int64_t q_stride_m, int64_t q_stride_h, const void* k_pages, const void* v_pages,
@@ -143,18 +332,33 @@ extern "C" int ttts_attn_paged_decode(const void* q, int64_t q_stride_m, int64_t
                                       int64_t o_stride_m, int64_t o_stride_h, float* lse, int32_t dtype, int32_t M, int32_t H, int32_t Hkv,
                                       int32_t head_dim, int32_t page, int32_t P, int32_t width, float scale, void* workspace,
                                       int64_t workspace_bytes, void* stream) {
-  const int rc = check_pages("attn_paged_decode", dtype, Hkv, head_dim, page, P);
+  int rc = check_pages("attn_paged_decode", dtype, Hkv, head_dim, page, P);
   if (rc) return rc;
-  TTTS_REQUIRE(M >= 0 && M <= 65535 && H > 0 && H % Hkv == 0, "attn_paged_decode: need 0 <= M <= 65535 and H %% Hkv == 0 (M %d, H %d, Hkv %d)", M, H, Hkv);
-  TTTS_REQUIRE(width > 0 && table_stride >= width && (int64_t)width * page <= 0x7fffffff, "attn_paged_decode: bad block table");
-  TTTS_REQUIRE(scale == scale && scale - scale == 0.f, "attn_paged_decode: the scale must be finite");
+  TTTS_REQUIRE(M >= 0 && H > 0 && H % Hkv == 0, "attn_paged_decode: need M >= 0 and H %% Hkv == 0 (M %d, H %d, Hkv %d)", M, H, Hkv);
+  TTTS_REQUIRE(width > 0 && table_stride >= width && (int64_t)width * page <= 0x40000000,
+               "attn_paged_decode: bad block table (width %d, row pitch %lld, at most 2^30 keys)", width, (long long)table_stride);
+  TTTS_REQUIRE(scale - scale == 0.f, "attn_paged_decode: the scale must be finite");
   if (M == 0) return TTTS_OK;
   TTTS_REQUIRE(q && k_pages && v_pages && block_table && seq_lens && out && lse, "attn_paged_decode: null pointer");
   TTTS_REQUIRE(aligned16(q) && aligned16(k_pages) && aligned16(v_pages) && aligned16(out), "attn_paged_decode: 16-byte aligned bases are needed");
   TTTS_REQUIRE(((q_stride_m | q_stride_h | o_stride_m | o_stride_h) & 7) == 0, "attn_paged_decode: strides must be multiples of 8 elements");
-  PagedParams p{q, k_pages, v_pages, out, lse, block_table, seq_lens, q_stride_m, q_stride_h, o_stride_m, o_stride_h, table_stride,
-                M, H, Hkv, page, P, width, scale * 1.4426950408889634f};
-  if (dtype == TTTS_DTYPE_BF16) launch_paged<bf16>(p, head_dim, as_stream(stream));
-  else launch_paged<_Float16>(p, head_dim, as_stream(stream));
-  return check_launch("attn_paged_decode");
+  PagedParams p{};
+  p.q = q; p.kp = k_pages; p.vp = v_pages; p.out = out; p.lse = lse; p.table = block_table; p.lens = seq_lens;
+  p.qs_m = q_stride_m; p.qs_h = q_stride_h; p.os_m = o_stride_m; p.os_h = o_stride_h; p.ts_m = table_stride;
+  p.H = H; p.Hkv = Hkv; p.group = H / Hkv; p.tiles = (int)paged_tiles(H, Hkv); p.page_shift = __builtin_ctz(page); p.P = P; p.width = width;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  const int64_t units = M * (int64_t)Hkv * p.tiles;
+  paged_split(units, (int64_t)width * page, p.chunk, p.chunks);
+  const int64_t grid = units * p.chunks, rows = (int64_t)M * H, need = paged_bytes(M, H, head_dim, p.chunks);
+  TTTS_REQUIRE(grid <= 0x7fffffff && rows <= 0x7fffffff, "attn_paged_decode: more work than one launch holds (M %d, H %d)", M, H);
+  TTTS_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned16(workspace)),
+               "attn_paged_decode: needs a 16-byte aligned workspace of %lld bytes", (long long)need);
+  p.part_o = (float*)workspace;
+  p.part_ml = p.part_o + rows * p.chunks * head_dim;
+  hipStream_t st = as_stream(stream);
+  if (dtype == TTTS_DTYPE_BF16)
+    return head_dim == 32 ? launch_paged<bf16, 32>(p, grid, rows, st) : head_dim == 64 ? launch_paged<bf16, 64>(p, grid, rows, st)
+                                                                                       : launch_paged<bf16, 128>(p, grid, rows, st);
+  return head_dim == 32 ? launch_paged<_Float16, 32>(p, grid, rows, st) : head_dim == 64 ? launch_paged<_Float16, 64>(p, grid, rows, st)
+                                                                                         : launch_paged<_Float16, 128>(p, grid, rows, st);
 }

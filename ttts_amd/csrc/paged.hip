@@ -62,7 +62,8 @@ __device__ __forceinline__ float over_rows(float x, F op) {
 //   O^T[d][q]  += V^T P   the k index is a key in ANY order that both operands share: with k = 8 g + 4 t + r <-> key 16 t + 4 g + r the
 //                         weights are the B operand where they are, and a lane loads V rows 16 t + 4 g + r, DH / 16 neighbouring
 //                         columns each, which it re-pairs across rows in registers (product r of DH / 16 has rows d = (DH / 16) m + r).
-// The next tile's loads are in flight under this one's products, the table entries another tile ahead.  The queries of a shared
+// The next tile's keys are loaded as soon as this one's have been multiplied, its values after the second product (held twice over,
+// 209 instead of 145 registers at 128 columns, they were no faster), the table entries another tile ahead.  The queries of a shared
 // head fill rows of the products that are there anyway, so a cached key is read once for up to 16 of them.
 constexpr int PAGED_WAVES = 8;
 template <typename T, int DH>
@@ -93,88 +94,90 @@ __global__ __launch_bounds__(PAGED_WAVES * 64) void attn_paged_decode_kernel(Pag
 #pragma unroll
   for (int r = 0; r < W; ++r) acc[r] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  struct Tile { T8 k[2][KC]; TW v[8]; int ok[2]; };
   const int32_t* tab = p.table + m * p.ts_m;
   const int last = max((c1 - 1) >> p.page_shift, 0);
   auto entry = [&](int key) { return tab[min(key >> p.page_shift, last)]; };   // (never past the chunk's own pages)
-  auto load = [&](Tile& t, int key0, int e0, int e1) {
+  T8 kf[2][KC];
+  TW vf[8];
+  struct Place { int64_t base[2]; int ok[2]; };   // where a tile's two 16-key halves lie (a page holds whole halves), and whether they count
+  auto place = [&](int key0, int e0, int e1) {
+    Place w;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int e = h ? e1 : e0, key = key0 + 16 * h;
-      t.ok[h] = key < c1 && e >= 0 && e < p.P;
-      const int off = key & ((1 << p.page_shift) - 1);
-      const int64_t base = ((((int64_t)(t.ok[h] ? e : 0) * p.Hkv + hk) << p.page_shift) + off) * DH;
-      const T* kb = (const T*)p.kp + base + col * DH + 8 * g;
-      const T* vb = (const T*)p.vp + base + 4 * g * DH + col * W;
-#pragma unroll
-      for (int c = 0; c < KC; ++c) t.k[h][c] = *reinterpret_cast<const T8*>(kb + 32 * c);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) t.v[4 * h + r] = *reinterpret_cast<const TW*>(vb + r * DH);
+      w.ok[h] = key < c1 && e >= 0 && e < p.P;
+      w.base[h] = ((((int64_t)(w.ok[h] ? e : 0) * p.Hkv + hk) << p.page_shift) + (key & ((1 << p.page_shift) - 1))) * DH;
     }
+    return w;
   };
-  auto attend = [&](Tile& t, int key0) {
-    float s[8];
+  auto load_k = [&](const Place& w) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      f32x4 d = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int c = 0; c < KC; ++c) d = Frag<T>::mfma(t.k[h][c], qf[c], d);
+      for (int c = 0; c < KC; ++c) kf[h][c] = *reinterpret_cast<const T8*>((const T*)p.kp + w.base[h] + col * DH + 8 * g + 32 * c);
+  };
+  auto load_v = [&](const Place& w) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) s[4 * h + r] = d[r] * p.scale_log2;
-    }
-    if (!(t.ok[0] && t.ok[1] && key0 + 32 <= c1)) {   // keys behind the end, or of no page: whatever the memory holds there
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const bool in = t.ok[j >> 2] && key0 + 16 * (j >> 2) + 4 * g + (j & 3) < c1;
-        s[j] = in ? s[j] : -INFINITY;
-        t.v[j] = in ? t.v[j] : TW{};
-      }
-    }
-    float mt = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
-    mt = over_rows(mt, [](float a, float b) { return fmaxf(a, b); });
-    if (__any(mt > mx)) {
-      const float mn = fmaxf(mx, mt), a = __builtin_amdgcn_exp2f(mx - mn);
-      l *= a;
-#pragma unroll
-      for (int r = 0; r < W; ++r) acc[r] *= a;
-      mx = mn;
-    }
-    T8 pf;                       // the weights enter the product in the cache's type; their sum is of the unrounded ones
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float e = __builtin_amdgcn_exp2f(s[j] - mx);
-      l += e;
-      pf[j] = (T)e;
-    }
-#pragma unroll
-    for (int r = 0; r < W; ++r) {
-      T8 a;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) a[j] = t.v[j][r];
-      acc[r] = Frag<T>::mfma(a, pf, acc[r]);
-    }
+    for (int j = 0; j < 8; ++j)
+      vf[j] = *reinterpret_cast<const TW*>((const T*)p.vp + w.base[j >> 2] + (4 * g + (j & 3)) * DH + col * W);
   };
   constexpr int STEP = 32 * NW;
   int key = c0 + 32 * wave;
   if (key < c1) {
-    Tile ta, tb;
-    load(ta, key, entry(key), entry(key + 16));
+    Place cur = place(key, entry(key), entry(key + 16));
+    load_k(cur);
+    load_v(cur);
     int e0 = entry(key + STEP), e1 = entry(key + STEP + 16);
-    for (;;) {
-      if (key + STEP < c1) {
-        load(tb, key + STEP, e0, e1);
+    for (; key < c1; key += STEP) {
+      const bool more = key + STEP < c1;
+      float s[8];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        f32x4 d = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < KC; ++c) d = Frag<T>::mfma(kf[h][c], qf[c], d);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[4 * h + r] = d[r] * p.scale_log2;
+      }
+      Place next = cur;
+      if (more) {
+        next = place(key + STEP, e0, e1);
+        load_k(next);
         e0 = entry(key + 2 * STEP); e1 = entry(key + 2 * STEP + 16);
       }
-      attend(ta, key);
-      key += STEP;
-      if (key >= c1) break;
-      if (key + STEP < c1) {
-        load(ta, key + STEP, e0, e1);
-        e0 = entry(key + 2 * STEP); e1 = entry(key + 2 * STEP + 16);
+      if (!(cur.ok[0] && cur.ok[1] && key + 32 <= c1)) {   // keys behind the end, or of no page: whatever the memory holds there
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const bool in = cur.ok[j >> 2] && key + 16 * (j >> 2) + 4 * g + (j & 3) < c1;
+          s[j] = in ? s[j] : -INFINITY;
+          vf[j] = in ? vf[j] : TW{};
+        }
       }
-      attend(tb, key);
-      key += STEP;
-      if (key >= c1) break;
+      float mt = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+      mt = over_rows(mt, [](float a, float b) { return fmaxf(a, b); });
+      if (__any(mt > mx)) {
+        const float mn = fmaxf(mx, mt), a = __builtin_amdgcn_exp2f(mx - mn);
+        l *= a;
+#pragma unroll
+        for (int r = 0; r < W; ++r) acc[r] *= a;
+        mx = mn;
+      }
+      T8 pf;                       // the weights enter the product in the cache's type; their sum is of the unrounded ones
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float e = __builtin_amdgcn_exp2f(s[j] - mx);
+        l += e;
+        pf[j] = (T)e;
+      }
+#pragma unroll
+      for (int r = 0; r < W; ++r) {
+        T8 a;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) a[j] = vf[j][r];
+        acc[r] = Frag<T>::mfma(a, pf, acc[r]);
+      }
+      if (more) load_v(next);
+      cur = next;
     }
   }
   l = over_rows(l, [](float a, float b) { return a + b; });
@@ -213,63 +216,77 @@ __global__ __launch_bounds__(PAGED_WAVES * 64) void attn_paged_decode_kernel(Pag
   }
 }
 
-// the chunks of a split sequence: one workgroup per (sequence, query head), DH / 4 lanes per chunk
+// the chunks of a split sequence: one workgroup per (sequence, query head).  First every chunk's weight 2^(m - M), a chunk per thread, then
+// DH / 4 lanes per chunk add up the weighted parts: two rounds of independent loads, whatever the number of chunks (<= PAGED_MAX_CHUNKS).
+constexpr int PAGED_MAX_CHUNKS = 2048;
 template <typename T, int DH>
 __global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedParams p) {
   constexpr int LPC = DH / 4, G = 256 / LPC;
+  __shared__ float sm_w[PAGED_MAX_CHUNKS];
   __shared__ float4 sm_o[G][LPC];
-  __shared__ float sm_ml[G][2];
+  __shared__ float sm_r[2][4];
   const int64_t mh = blockIdx.x, m = mh / p.H;
-  const int sub = threadIdx.x % LPC, grp = threadIdx.x / LPC;
+  const int tid = threadIdx.x, sub = tid % LPC, grp = tid / LPC;
   const int len = min(p.lens[m], p.width << p.page_shift);
   const int n = len > 0 ? (len + p.chunk - 1) / p.chunk : 0;
   const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + mh * p.chunks;
   const float4* po = reinterpret_cast<const float4*>(p.part_o) + mh * p.chunks * LPC + sub;
-  float M = -3.0e38f, L = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int c = grp; c < n; c += G) {
+  float M = -3.0e38f;
+  for (int c = tid; c < n; c += 256) M = fmaxf(M, ml[c].x);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+  if ((tid & 63) == 0) sm_r[0][tid >> 6] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(sm_r[0][0], sm_r[0][1]), fmaxf(sm_r[0][2], sm_r[0][3]));
+  float L = 0.f;
+  for (int c = tid; c < n; c += 256) {
     const float2 s = ml[c];
+    const float w = __builtin_amdgcn_exp2f(s.x - M);
+    sm_w[c] = w;
+    L += s.y * w;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) L += __shfl_xor(L, o, 64);
+  if ((tid & 63) == 0) sm_r[1][tid >> 6] = L;
+  __syncthreads();
+  L = (sm_r[1][0] + sm_r[1][1]) + (sm_r[1][2] + sm_r[1][3]);
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int c = grp; c < n; c += G) {
     const float4 v = po[(int64_t)c * LPC];
-    const float mn = fmaxf(M, s.x), a = __builtin_amdgcn_exp2f(M - mn), b = __builtin_amdgcn_exp2f(s.x - mn);
-    L = L * a + s.y * b;
-    o.x = o.x * a + v.x * b; o.y = o.y * a + v.y * b; o.z = o.z * a + v.z * b; o.w = o.w * a + v.w * b;
-    M = mn;
+    const float w = sm_w[c];
+    o.x = fmaf(v.x, w, o.x); o.y = fmaf(v.y, w, o.y); o.z = fmaf(v.z, w, o.z); o.w = fmaf(v.w, w, o.w);
   }
   sm_o[grp][sub] = o;
-  if (sub == 0) { sm_ml[grp][0] = M; sm_ml[grp][1] = L; }
   __syncthreads();
-  if (threadIdx.x < DH) {
-    const int d = threadIdx.x;
-    M = sm_ml[0][0];
-#pragma unroll
-    for (int i = 1; i < G; ++i) M = fmaxf(M, sm_ml[i][0]);
+  if (tid < DH) {
     float x = 0.f;
-    L = 0.f;
 #pragma unroll
-    for (int i = 0; i < G; ++i) {
-      const float a = __builtin_amdgcn_exp2f(sm_ml[i][0] - M);
-      L += sm_ml[i][1] * a;
-      x += reinterpret_cast<const float*>(sm_o[i])[d] * a;
-    }
-    ((T*)p.out)[m * p.os_m + (mh % p.H) * p.os_h + d] = (T)(L == 0.f ? 0.f : x / L);
-    if (d == 0) p.lse[mh] = L == 0.f ? -INFINITY : (M + __log2f(L)) * 0.6931471805599453f;
+    for (int i = 0; i < G; ++i) x += reinterpret_cast<const float*>(sm_o[i])[tid];
+    ((T*)p.out)[m * p.os_m + (mh % p.H) * p.os_h + tid] = (T)(L == 0.f ? 0.f : x / L);
+    if (tid == 0) p.lse[mh] = L == 0.f ? -INFINITY : (M + __log2f(L)) * 0.6931471805599453f;
   }
 }
 
-#ifndef PAGED_TARGET
-#define PAGED_TARGET 2048
-#endif
-#ifndef PAGED_MIN_CHUNK
-#define PAGED_MIN_CHUNK 512
-#endif
-// How a sequence of up to `longest` keys is split: enough workgroups to fill the card, but no chunk under what pays for its join.
+// How sequences of up to `longest` keys (what the table holds; their lengths stay on the device) are split into chunks, one workgroup each:
+//  * not at all up to 768 keys (three tiles a wave): 613 keys of one sequence, 8 heads of 64: 6.0 us; split 6.4 - 7.0, two launches.
+//  * into 256 keys, one tile a wave, while that gives the card's 256 CUs one workgroup each at most: 2404 keys of one sequence
+//    6.9 us, against 10.8 in chunks of 1024; more workgroups than CUs cost more than they give (20000 keys: 12.2 us, 14.2 with 512).
+//  * beyond that into 1024 keys or more, about 1024 workgroups (4 sequences of 130000 keys: 178 us, 188 with 2048), or about 2048
+//    where a sequence gets few chunks, which a ragged batch fills unevenly (96 sequences up to 4096: 150 us, 173 with 1024).
 static void paged_split(int64_t units, int64_t longest, int& chunk, int& chunks) {
-  int64_t n = cdiv(PAGED_TARGET, units);
-  n = n < cdiv(longest, PAGED_MIN_CHUNK) ? n : cdiv(longest, PAGED_MIN_CHUNK);
+  auto least = [](int64_t a, int64_t b) { return a < b ? a : b; };
+  int64_t n = 1;
+  if (longest > 768) {
+    int64_t wide = cdiv(1024, units);
+    if (wide < 8) wide = cdiv(2048, units);
+    n = least(cdiv(longest, 1024), wide);
+    const int64_t fine = least(cdiv(longest, 256), 256 / units);
+    n = n > fine ? n : fine;
+  }
   const int64_t c = cdiv(cdiv(longest, n), 32 * PAGED_WAVES) * 32 * PAGED_WAVES;
-  chunk = (int)(c < 0x40000000 ? c : 0x40000000);
-  chunks = (int)cdiv(longest, chunk);
+  chunk = (int)c;
+  chunks = (int)cdiv(longest, c);
 }
 
 }  // namespace ttts

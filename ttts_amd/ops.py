@@ -891,30 +891,35 @@ def decode_advance(ctr, finished):
 _DTYPE_CODES = {torch.float32: _l.DTYPE_F32, torch.bfloat16: _l.DTYPE_BF16, torch.float16: _l.DTYPE_F16}
 
 
-def _on(what, *named):
-    """All of the (tensor, name) pairs live on one GPU: a context that makes it the current device, so that the launch goes to torch's
+_NO_GUARD = contextlib.nullcontext()
+
+
+def _on(what, *tensors):
+    """All of the tensors (None: left out) live on one GPU: a context that makes it the current device, so that the launch goes to torch's
     current stream of THAT device.  Raises for a CPU tensor or two devices."""
-    dev = None
-    for t, name in named:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise TttsError("%s: %s must live on the GPU (no CPU fallback in ttts_amd)" % (what, name))
-        if dev is not None and t.device != dev:
-            raise TttsError("%s: %s is on %s, the others on %s" % (what, name, t.device, dev))
-        dev = t.device
-    return contextlib.nullcontext() if dev.index == torch._C._cuda_getDevice() else torch.cuda.device(dev)
+    index = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and (index < 0 or t.get_device() != index):
+            raise TttsError("%s: every tensor must live on the GPU, all on the same one (no CPU fallback in ttts_amd); got %s"
+                            % (what, ", ".join(sorted({str(x.device) for x in tensors if x is not None}))))
+    return _NO_GUARD if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
+
+
+def _a(t):
+    """A tensor's address as a plain int (ctypes turns it into the pointer: an object less per argument than `_p`)."""
+    return None if t is None else t.data_ptr()
 
 
 def _rows(t, what, name):
     """(row pitch, rows, columns) of a 2-D tensor with contiguous rows that do not overlap."""
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-        raise TttsError("%s: %s must be 2-D with contiguous rows, got shape %s strides %s" % (what, name, tuple(t.shape), t.stride()))
-    return (t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])), t.shape[0], t.shape[1]
+    shape, strides = t.shape, t.stride()
+    if len(shape) != 2 or (strides[1] != 1 and shape[1] > 1) or (strides[0] < shape[1] and shape[0] > 1):
+        raise TttsError("%s: %s must be 2-D with contiguous rows, got shape %s strides %s" % (what, name, tuple(shape), strides))
+    return (strides[0] if shape[0] > 1 else max(strides[0], shape[1])), shape[0], shape[1]
 
 
 def _vec(t, dtype, shape, what, name):
-    if t is not None and (t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous()):
+    if t is not None and (t.dtype != dtype or t.shape != shape or not t.is_contiguous()):
         raise TttsError("%s: %s must be a contiguous %s tensor of shape %s, got %s %s" % (what, name, dtype, tuple(shape), t.dtype, tuple(t.shape)))
 
 
@@ -958,13 +963,13 @@ def token_logprobs_fwd(logits, tokens, C=None, top_k=0, temperature=1.0):
     code, ld, R, C = _logits(logits, C, what)
     _vec(tokens, torch.int64, (R,), what, "tokens")
     k = int(top_k)
-    with _on(what, (logits, "logits"), (tokens, "tokens")):
+    with _on(what, logits, tokens):
         f = lambda *shape, dt=torch.float32: torch.empty(shape, dtype=dt, device=logits.device)  # noqa: E731
         r = TokenLogprobs(f(R), f(R), f(R, k) if k > 0 else None, f(R, k, dt=torch.int64) if k > 0 else None, f(R, 2))
         n = _l.get().ttts_token_logprobs_workspace_bytes(R, C, k)
         ws = _workspace(n, logits.device)
-        check(_l.get().ttts_token_logprobs_fwd(_p(logits), code, ld, _p(tokens), _p(r.logp), _p(r.entropy), _p(r.stats), _p(r.top_logp),
-                                               _p(r.top_idx), R, C, k, float(temperature), _p(ws), n, _stream()), what)
+        check(_l.get().ttts_token_logprobs_fwd(_a(logits), code, ld, _a(tokens), _a(r.logp), _a(r.entropy), _a(r.stats), _a(r.top_logp),
+                                               _a(r.top_idx), R, C, k, float(temperature), _a(ws), n, _raw_stream()), what)
     return r
 
 
@@ -976,11 +981,10 @@ def token_logprobs_bwd(logits, tokens, stats, entropy, g_logp, g_entropy=None, C
     _vec(tokens, torch.int64, (R,), what, "tokens"); _vec(stats, torch.float32, (R, 2), what, "stats")
     for t, name in ((entropy, "entropy"), (g_logp, "g_logp"), (g_entropy, "g_entropy")):
         _vec(t, torch.float32, (R,), what, name)
-    with _on(what, (logits, "logits"), (tokens, "tokens"), (stats, "stats"), (entropy, "entropy"), (g_logp, "g_logp"),
-             (g_entropy, "g_entropy"), (dlogits, "dlogits")):
+    with _on(what, logits, tokens, stats, entropy, g_logp, g_entropy, dlogits):
         dlogits, ldd = _grad_rows(dlogits, logits, what)
-        check(_l.get().ttts_token_logprobs_bwd(_p(logits), code, ld, _p(tokens), _p(stats), _p(entropy), _p(g_logp), _p(g_entropy),
-                                               _p(dlogits), ldd, R, C, logits.shape[1], float(temperature), _stream()), what)
+        check(_l.get().ttts_token_logprobs_bwd(_a(logits), code, ld, _a(tokens), _a(stats), _a(entropy), _a(g_logp), _a(g_entropy),
+                                               _a(dlogits), ldd, R, C, logits.shape[1], float(temperature), _raw_stream()), what)
     return dlogits
 
 
@@ -992,13 +996,13 @@ def distill_fwd(logits, teacher_idx, teacher_logp, C=None, temperature=1.0, tail
     what = "distill_fwd"
     code, ld, R, C = _logits(logits, C, what)
     K = _teacher(teacher_idx, teacher_logp, R, what)
-    with _on(what, (logits, "logits"), (teacher_idx, "teacher_idx"), (teacher_logp, "teacher_logp")):
+    with _on(what, logits, teacher_idx, teacher_logp):
         loss = torch.empty(R, dtype=torch.float32, device=logits.device)
         stats = torch.empty(R, 3, dtype=torch.float32, device=logits.device)
         n = _l.get().ttts_distill_workspace_bytes(R, C)
         ws = _workspace(n, logits.device)
-        check(_l.get().ttts_distill_fwd(_p(logits), code, ld, _p(teacher_idx), _p(teacher_logp), _p(loss), _p(stats), R, C, K,
-                                        float(temperature), int(bool(tail)), _p(ws), n, _stream()), what)
+        check(_l.get().ttts_distill_fwd(_a(logits), code, ld, _a(teacher_idx), _a(teacher_logp), _a(loss), _a(stats), R, C, K,
+                                        float(temperature), int(bool(tail)), _a(ws), n, _raw_stream()), what)
     return loss, stats
 
 
@@ -1019,11 +1023,10 @@ def distill_bwd(logits, teacher_idx, teacher_logp, stats, g_loss, C=None, temper
     _vec(stats, torch.float32, (R, 3), what, "stats"); _vec(g_loss, torch.float32, (R,), what, "g_loss")
     if accumulate and (dlogits is None or dlogits.data_ptr() == logits.data_ptr()):
         raise TttsError("%s: accumulate needs a dlogits of its own" % what)
-    with _on(what, (logits, "logits"), (teacher_idx, "teacher_idx"), (teacher_logp, "teacher_logp"), (stats, "stats"), (g_loss, "g_loss"),
-             (dlogits, "dlogits")):
+    with _on(what, logits, teacher_idx, teacher_logp, stats, g_loss, dlogits):
         dlogits, ldd = _grad_rows(dlogits, logits, what)
-        check(_l.get().ttts_distill_bwd(_p(logits), code, ld, _p(teacher_idx), _p(teacher_logp), _p(stats), _p(g_loss), _p(dlogits), ldd, R, C,
-                                        logits.shape[1], K, float(temperature), int(bool(tail)), int(bool(accumulate)), _stream()), what)
+        check(_l.get().ttts_distill_bwd(_a(logits), code, ld, _a(teacher_idx), _a(teacher_logp), _a(stats), _a(g_loss), _a(dlogits), ldd, R, C,
+                                        logits.shape[1], K, float(temperature), int(bool(tail)), int(bool(accumulate)), _raw_stream()), what)
     return dlogits
 
 
@@ -1037,9 +1040,12 @@ def _pages(k_pages, v_pages, what):
 
 
 def _heads(t, dtype, shape, what, name):
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or t.stride(2) != 1:
+    """Strides of rows and heads of a [rows, heads, head_dim] view with contiguous heads."""
+    strides = t.stride()
+    if t.shape != shape or t.dtype != dtype or strides[2] != 1:
         raise TttsError("%s: %s must be a %s tensor of shape %s with contiguous heads, got %s %s strides %s"
-                        % (what, name, dtype, tuple(shape), t.dtype, tuple(t.shape), t.stride()))
+                        % (what, name, dtype, tuple(shape), t.dtype, tuple(t.shape), strides))
+    return strides[0], strides[1]
 
 
 def kv_page_write(k, v, k_pages, v_pages, slots):
@@ -1052,10 +1058,11 @@ def kv_page_write(k, v, k_pages, v_pages, slots):
     P, H, page, dh = k_pages.shape
     N = slots.shape[0] if slots.dim() == 1 else -1
     _vec(slots, torch.int64, (N,), what, "slots")
-    _heads(k, k_pages.dtype, (N, H, dh), what, "k"); _heads(v, k_pages.dtype, (N, H, dh), what, "v")
-    with _on(what, (k, "k"), (v, "v"), (k_pages, "k_pages"), (v_pages, "v_pages"), (slots, "slots")):
-        check(_l.get().ttts_kv_page_write(_p(k), _p(v), k.stride(0), k.stride(1), v.stride(0), v.stride(1), _p(k_pages), _p(v_pages),
-                                          _p(slots), code, N, H, dh, page, P, _stream()), what)
+    ksn, ksh = _heads(k, k_pages.dtype, (N, H, dh), what, "k")
+    vsn, vsh = _heads(v, k_pages.dtype, (N, H, dh), what, "v")
+    with _on(what, k, v, k_pages, v_pages, slots):
+        check(_l.get().ttts_kv_page_write(_a(k), _a(v), ksn, ksh, vsn, vsh, _a(k_pages), _a(v_pages),
+                                          _a(slots), code, N, H, dh, page, P, _raw_stream()), what)
 
 
 def attn_paged_decode(q, k_pages, v_pages, block_table, seq_lens, scale, out=None):
@@ -1069,21 +1076,21 @@ def attn_paged_decode(q, k_pages, v_pages, block_table, seq_lens, scale, out=Non
     if q.dim() != 3 or block_table.dim() != 2 or block_table.dtype != torch.int32:
         raise TttsError("%s: q must be [M, H, head_dim], block_table int32 [M, width]" % what)
     M, H = q.shape[:2]
-    _heads(q, k_pages.dtype, (M, H, dh), what, "q"); _vec(seq_lens, torch.int32, (M,), what, "seq_lens")
+    qsm, qsh = _heads(q, k_pages.dtype, (M, H, dh), what, "q")
+    _vec(seq_lens, torch.int32, (M,), what, "seq_lens")
     ts, tm, width = _rows(block_table, what, "block_table")
     if tm != M:
         raise TttsError("%s: block_table has %d rows for %d sequences" % (what, tm, M))
-    if out is not None:
-        _heads(out, q.dtype, (M, H, dh), what, "out")
-    with _on(what, (q, "q"), (k_pages, "k_pages"), (v_pages, "v_pages"), (block_table, "block_table"), (seq_lens, "seq_lens"), (out, "out")):
+    with _on(what, q, k_pages, v_pages, block_table, seq_lens, out):
         if out is None:
             out = torch.empty(M, H, dh, dtype=q.dtype, device=q.device)
+        osm, osh = _heads(out, q.dtype, (M, H, dh), what, "out")
         lse = torch.empty(M, H, dtype=torch.float32, device=q.device)
         n = _l.get().ttts_attn_paged_decode_workspace_bytes(M, H, Hkv, dh, page, width)
         ws = _workspace(n, q.device)
-        check(_l.get().ttts_attn_paged_decode(_p(q), q.stride(0), q.stride(1), _p(k_pages), _p(v_pages), _p(block_table), ts, _p(seq_lens),
-                                              _p(out), out.stride(0), out.stride(1), _p(lse), code, M, H, Hkv, dh, page, P, width,
-                                              float(scale), _p(ws), n, _stream()), what)
+        check(_l.get().ttts_attn_paged_decode(_a(q), qsm, qsh, _a(k_pages), _a(v_pages), _a(block_table), ts, _a(seq_lens),
+                                              _a(out), osm, osh, _a(lse), code, M, H, Hkv, dh, page, P, width,
+                                              float(scale), _a(ws), n, _raw_stream()), what)
     return out, lse
 
 

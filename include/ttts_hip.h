@@ -424,7 +424,7 @@ int ttts_diffusion_loss_bwd_f32(const float* model_out, const float* x_start, co
 /* ---- scoring of given tokens and distillation on a teacher's alternatives ------------------------------------------
  * Beside ttts_ce_fwd_bf16 (the mean loss alone) and ttts_sample_logits_f32 (the drawn token alone): what a token was worth, what
  * else was likely, and a student's loss on that.  logits [R, ldl] of `dtype`, C classes per row (columns C .. ldl - 1 are never
- * looked at), any row pitch >= C and any alignment of the type (16-byte aligned rows are read 16 bytes at a time);
+ * looked at), any row pitch >= C, aligned to the type only;
  * y = logits / temperature; sums and statistics are fp32.  A class at -inf has no probability and is no alternative.
  * Rows: one whose classes are all -inf has no distribution (below); one that holds a NaN or +inf gets NaN. */
 enum { TTTS_DTYPE_F32 = 0, TTTS_DTYPE_BF16 = 1, TTTS_DTYPE_F16 = 2 };
@@ -455,7 +455,7 @@ int ttts_token_logprobs_bwd(const void* logits, int32_t dtype, int64_t ldl, cons
  *           left = max(0, 1 - sum p);  row_loss += left (log left - log q_rest), q_rest = the student's mass on the classes that
  *           the list does not name (summed as such, not as 1 - the rest).  Without such a class the term is left out.
  *   A class named twice counts with both of its p.  A row without entries has loss 0 with tail 0; a row whose student classes are
- *   all -inf has loss 0 and no gradient.  stats f32 [R, 3] for the backward: (max, log Z, log Z of the classes not named).
+ *   all -inf has loss 0 and no gradient.  stats f32 [R, 3] for the backward: (max, log Z, Z of the named classes over Z of the others).
  * bwd: dlogits = g_loss[r] d row_loss / d logits:  g / temperature [q (sum p + left) - p - left q / q_rest (classes not named)];
  *   written over Cd columns as above, or with accumulate 1 added to what is there (columns 0 .. C - 1, one rounding of the sum). */
 int64_t ttts_distill_workspace_bytes(int32_t R, int32_t C);

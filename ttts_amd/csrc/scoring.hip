@@ -2,243 +2,710 @@
 //   token_logprobs : y = x / T, log p of the given token, entropy, the k best classes with their log p; and the gradient
 //   distill        : KL(teacher's listed classes || student), optionally with the mass that the list leaves out; and the gradient
 // All sums, maxima and statistics are fp32 whatever the logits' type; a row's maximum m and log Z = log sum e^((x - m) / T) are
-// handed to the gradient APART: one log-sum-exp would round log Z to the maximum's step.
+// handed to the gradient APART: one log-sum-exp would round log Z to the maximum's step.  Bound by HBM: the logits once (twice and a
+// write with the gradient).
 #include <math.h>
 
 #include "common.hpp"
 
 namespace ttts {
 
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f, FMAX = 3.402823466e38f;
 
-template <typename T>
-struct Row {   // one row of logits as fp32
-  const T* p;
-  __device__ __forceinline__ float operator[](int64_t c) const { return (float)p[c]; }
+// ---- one wave = up to 2048 columns of a row, held in registers as fp32 -------------------------------------------------
+// A row is read ONCE: maximum, sums, and the alternatives all come from the registers.  Rows up to 2048 columns take one wave, up to 32768
+// one workgroup of up to 16 waves that meet once in LDS, longer ones several workgroups (segments) and a second kernel that
+// joins their results.  Aligned rows: a lane holds 8 neighbouring columns per load; others: single columns, neighbouring lanes.
+constexpr int NV = 4, WAVE_COLS = NV * 512, MAX_WAVES = 16, SEG_COLS = WAVE_COLS * MAX_WAVES;
+
+struct Split {   // columns of a row -> segments (workgroups) -> waves
+  int seg, nseg, waves, wave_cols;
 };
-
-constexpr int ROW_T = 256;
-template <typename F>
-__device__ __forceinline__ float block_reduce(float v, F op, float* sh) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = op(v, __shfl_xor(v, o, 64));
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
-  __syncthreads();
-  return op(op(sh[0], sh[1]), op(sh[2], sh[3]));
+static Split split_row(int C) {
+  Split s;
+  s.nseg = (int)cdiv(C, SEG_COLS);
+  s.seg = (int)cdiv(cdiv(C, s.nseg), 8) * 8;
+  s.nseg = (int)cdiv(C, s.seg);
+  s.waves = (int)cdiv(s.seg, WAVE_COLS);
+  s.wave_cols = (int)cdiv(cdiv(s.seg, s.waves), 8) * 8;
+  return s;
 }
-__device__ __forceinline__ float add_f(float a, float b) { return a + b; }
-__device__ __forceinline__ float max_f(float a, float b) { return fmaxf(a, b); }
 
-// (value, class) order of the alternatives: larger value first, lower class first among equals
-__device__ __forceinline__ bool before(float va, int ia, float vb, int ib) { return va > vb || (va == vb && ia < ib); }
+template <typename T> __device__ __forceinline__ void load8(const T* p, int n, float (&v)[8]);   // n valid columns (1 .. 8) of an aligned 8
+template <> __device__ __forceinline__ void load8<bf16>(const bf16* p, int n, float (&v)[8]) {
+  const bf16x8 r = *reinterpret_cast<const bf16x8*>(p);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = j < n ? (float)r[j] : -INFINITY;
+}
+template <> __device__ __forceinline__ void load8<_Float16>(const _Float16* p, int n, float (&v)[8]) {
+  const f16x8 r = *reinterpret_cast<const f16x8*>(p);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = j < n ? (float)r[j] : -INFINITY;
+}
+template <> __device__ __forceinline__ void load8<float>(const float* p, int n, float (&v)[8]) {
+  const float4 a = *reinterpret_cast<const float4*>(p);
+  float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (n > 4) b = *reinterpret_cast<const float4*>(p + 4);   // (the pitch is a multiple of 4 only)
+  const float r[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = j < n ? r[j] : -INFINITY;
+}
 
-// e = 2^((x - m) c), t = (x - m) c kept finite (a class at -inf, or at the type's lowest value, has e = 0: e t must be 0, not NaN).
-// m is never -inf here (>= -FLT_MAX), so -inf - m = -inf; NaN passes through e.
+// columns c0 .. cend - 1 of a row; columns outside are -inf.  Column of x[i][j]: wave_col(c0, i, j).
+template <bool VEC>
+__device__ __forceinline__ int wave_col(int c0, int i, int j, int lane) { return VEC ? c0 + i * 512 + lane * 8 + j : c0 + i * 512 + j * 64 + lane; }
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_wave(const T* row, int c0, int cend, int lane, float (&x)[NV][8]) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[i][j] = -INFINITY;
+    if (c0 + i * 512 < cend) {
+      if (VEC) {
+        const int c = c0 + i * 512 + lane * 8;
+        if (c < cend) load8<T>(row + c, cend - c, x[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int c = c0 + i * 512 + j * 64 + lane;
+          if (c < cend) x[i][j] = (float)row[c];
+        }
+      }
+    }
+  }
+}
+
+// e = 2^((x - m) c); t = (x - m) c kept finite (a class at -inf, or at the type's lowest value, has e = 0: e t must be 0, not NaN).
+// m is never -inf here (>= -FMAX), so -inf - m = -inf; NaN passes through e.  The difference comes first: lowest - lowest is 0.
 __device__ __forceinline__ float expo(float x, float m, float c, float& t) {
   t = (x - m) * c;
   const float e = __builtin_amdgcn_exp2f(t);
   t = fmaxf(t, -200.f);
   return e;
 }
+__device__ __forceinline__ void wave_fence() {   // LDS written by this wave's lanes is read by its other lanes
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
 
-template <typename T>
-__global__ __launch_bounds__(ROW_T) void token_logprobs_fwd_kernel(const T* __restrict__ logits, int64_t ldl,
-                                                                   const int64_t* __restrict__ tokens, float* __restrict__ logp,
-                                                                   float* __restrict__ entropy, float* __restrict__ stats,
-                                                                   float* __restrict__ top_logp, int64_t* __restrict__ top_idx, int C,
-                                                                   int top_k, float inv_t) {
-  __shared__ float sh[4];
-  __shared__ float shv[4];
-  __shared__ int shi[4];
-  const int64_t row = blockIdx.x;
-  const Row<T> x{logits + row * ldl};
-  const float c = inv_t * LOG2E;
-  float mx = -3.402823466e38f;
-  for (int i = threadIdx.x; i < C; i += ROW_T) mx = fmaxf(mx, x[i]);
-  mx = block_reduce(mx, max_f, sh);
-  float z = 0.f, s = 0.f;
-  for (int i = threadIdx.x; i < C; i += ROW_T) {
-    float t;
-    const float e = expo(x[i], mx, c, t);
-    z += e;
-    s = fmaf(e, t, s);
+// ---- the k best of a wave's columns ---------------------------------------------------------------------------------------
+// Order: larger value first, lower class first among equals.  A 64-bit key holds both: the value's bits in the order of the numbers
+// (zeros of both signs the same), and the class, inverted; key 0 is none.
+typedef unsigned long long u64;
+__device__ __forceinline__ uint32_t ord(float v) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, v + 0.f);
+  return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float unord(uint32_t u) { return __builtin_bit_cast(float, (u & 0x80000000u) ? u ^ 0x80000000u : ~u); }
+__device__ __forceinline__ u64 top_key(float v, int c) { return ((u64)ord(v) << 32) | (uint32_t)~c; }
+__device__ __forceinline__ int key_class(u64 k) { return (int)~(uint32_t)k; }
+constexpr uint32_t ORD_NONE = 0x007fffffu;   // ord(-inf)
+
+constexpr int TOP_CAND = 64 * 8 + 64;        // candidates a wave keeps; TOP_LDS: and its sorted list, in u64
+constexpr int TOP_LDS = TOP_CAND + 2 + TTTS_SCORE_MAX_TOP;
+__device__ __forceinline__ int lanes_below(u64 mask) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+}
+// A threshold first: the k-th largest of the 256 maxima of 8 columns each (vmax), found bit by bit with ballots, is at most the k-th
+// largest value, and what reaches it lies in few of those groups: about k + 10 % columns of ordinary rows.  These are ranked by
+// counting.  When values repeat (a constant row) any number of columns can reach it: then those above it are taken (under 64
+// groups of 8) and of those AT it the lowest classes, as many as are needed.
+template <bool VEC>
+__device__ __forceinline__ int wave_top(const float (&x)[NV][8], const float (&vmax)[NV], int c0, int cend, int k, int lane, u64* cand) {
+  u64* list = cand + TOP_CAND + 2;
+  uint32_t g[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) g[i] = ord(vmax[i]);
+  uint32_t t = 0;
+  for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
+    const uint32_t c = t | bit;
+    int cnt = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) cnt += __builtin_popcountll(__ballot(g[i] >= c));
+    if (cnt >= k) {
+      t = c;
+      if (cnt == k) break;
+    }
   }
-  z = block_reduce(z, add_f, sh);
-  s = block_reduce(s, add_f, sh);
-  const bool none = z == 0.f;          // every class at -inf
-  const float log2z = __log2f(z);
-  if (threadIdx.x == 0) {
-    const int64_t tok = tokens[row];
-    stats[2 * row] = none ? -INFINITY : mx;
-    stats[2 * row + 1] = none ? -INFINITY : log2z * LN2;
-    entropy[row] = none ? 0.f : (log2z - s / z) * LN2;
-    float lp = 0.f;
-    if (tok >= 0 && tok < C) lp = none ? -INFINITY : (x[tok] - mx) * inv_t - log2z * LN2;
-    logp[row] = lp;
-  }
-  float pv = INFINITY;
-  int pi = -1;
-  for (int k = 0; k < top_k; ++k) {
-    float bv = -INFINITY;
-    int bi = 0x7fffffff;
-    if (z == z)
-      for (int i = threadIdx.x; i < C; i += ROW_T) {
-        const float v = x[i];
-        if (v > -INFINITY && before(pv, pi, v, i) && before(v, i, bv, bi)) { bv = v; bi = i; }
+  const float thr = t <= ORD_NONE ? -FMAX : unord(t);
+  int n = 0;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (c0 + i * 512 >= cend) break;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const bool in = x[i][j] >= thr;
+      const u64 mask = __ballot(in);
+      if (mask) {
+        const int at = n + lanes_below(mask);
+        if (in && at < TOP_CAND) cand[at] = top_key(x[i][j], wave_col<VEC>(c0, i, j, lane));
+        n += __builtin_popcountll(mask);
       }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      const float v2 = __shfl_xor(bv, o, 64);
-      const int i2 = __shfl_xor(bi, o, 64);
-      if (before(v2, i2, bv, bi)) { bv = v2; bi = i2; }
     }
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) { shv[threadIdx.x >> 6] = bv; shi[threadIdx.x >> 6] = bi; }
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < 4; ++w)
-      if (before(shv[w], shi[w], bv, bi)) { bv = shv[w]; bi = shi[w]; }
-    const bool have = bi != 0x7fffffff;
-    if (threadIdx.x == 0) {
-      top_idx[row * top_k + k] = have ? bi : -1;
-      top_logp[row * top_k + k] = z != z ? z : (have ? (bv - mx) * inv_t - log2z * LN2 : -INFINITY);
-    }
-    pv = have ? bv : -INFINITY;
-    pi = bi;
   }
+  if (n > TOP_CAND) {
+    n = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const bool in = x[i][j] > thr;
+        const u64 mask = __ballot(in);
+        if (in) cand[n + lanes_below(mask)] = top_key(x[i][j], wave_col<VEC>(c0, i, j, lane));
+        n += __builtin_popcountll(mask);
+      }
+    const int end = max(n, k);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (VEC) {   // classes ascend with (lane, j)
+        int mine = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) mine += x[i][j] == thr;
+        int upto = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+          const int v = __shfl_up(upto, o, 64);
+          if (lane >= o) upto += v;
+        }
+        int at = n + upto - mine;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (x[i][j] == thr) {
+            if (at < end) cand[at] = top_key(x[i][j], wave_col<VEC>(c0, i, j, lane));
+            ++at;
+          }
+        n += __shfl(upto, 63, 64);
+      } else {     // classes ascend with (j, lane)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const bool in = x[i][j] == thr;
+          const u64 mask = __ballot(in);
+          const int at = n + lanes_below(mask);
+          if (in && at < end) cand[at] = top_key(x[i][j], wave_col<VEC>(c0, i, j, lane));
+          n += __builtin_popcountll(mask);
+        }
+      }
+      n = min(n, end);
+    }
+  }
+  if (lane < 2) cand[n + lane] = 0;
+  if (lane < k) list[lane] = 0;
+  wave_fence();
+  for (int s = 0; s < n; s += 64) {
+    const u64 key = s + lane < n ? cand[s + lane] : 0;
+    int r = 0;
+    for (int j = 0; j < n; j += 2) r += (cand[j] > key) + (cand[j + 1] > key);
+    if (s + lane < n && r < k) list[r] = key;
+  }
+  wave_fence();
+  return min(n, k);
+}
+// place of list w's entry r among `lists` sorted lists of k (stride in u64): its own, and in each other one those above it
+__device__ __forceinline__ int merged_rank(const u64* base, int stride, int lists, int w, int r, int k, u64 key) {
+  int rank = r;
+  for (int o = 0; o < lists; ++o) {
+    if (o == w) continue;
+    const u64* l = base + o * stride;
+    int lo = 0, hi = k;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (l[mid] > key) lo = mid + 1; else hi = mid;
+    }
+    rank += lo;
+    if (rank >= k) break;
+  }
+  return rank;
 }
 
-template <typename T>
-__global__ __launch_bounds__(ROW_T) void token_logprobs_bwd_kernel(const T* __restrict__ logits, int64_t ldl,
-                                                                   const int64_t* __restrict__ tokens, const float* __restrict__ stats,
-                                                                   const float* __restrict__ entropy, const float* __restrict__ g_logp,
-                                                                   const float* __restrict__ g_entropy, T* __restrict__ dlogits,
-                                                                   int64_t ldd, int C, int Cd, float inv_t) {
-  const int64_t row = blockIdx.x;
-  const Row<T> x{logits + row * ldl};
-  const float mx = stats[2 * row], logz = stats[2 * row + 1], H = entropy[row];
-  const int64_t tok = tokens[row];
-  const bool given = tok >= 0 && tok < C;
-  const float gl = given ? g_logp[row] : 0.f, gh = g_entropy ? g_entropy[row] : 0.f;
-  for (int i = threadIdx.x; i < Cd; i += ROW_T) {
-    float d = 0.f;
-    if (i < C && mx != -INFINITY) {
-      const float y = (x[i] - mx) * inv_t - logz;
-      const float p = __builtin_amdgcn_exp2f(y * LOG2E);
-      d = -gl * p - (p == 0.f ? 0.f : gh * p * (y + H));
-      if (given && i == tok) d += gl;
-      d *= inv_t;
-    }
-    dlogits[row * ldd + i] = (T)d;
-  }
+struct RowSums { float m, z, s; };   // maximum, sum e, sum e t (t in bits, from the maximum)
+__device__ __forceinline__ void add_sums(RowSums& a, float m, float z, float s, float M, float c) {   // a's maximum is M already
+  const float d = fmaxf((m - M) * c, -200.f), f = __builtin_amdgcn_exp2f(d);
+  a.z += z * f;
+  a.s += f * (s + z * d);
 }
 
-// the teacher's list of one row in LDS: class (or -1), p and log p
-struct Listed {
-  int idx[TTTS_DISTILL_MAX_K];
-  float p[TTTS_DISTILL_MAX_K], logp[TTTS_DISTILL_MAX_K];
+struct ScoreParams {
+  const void* logits; int64_t ldl;
+  const int64_t* tokens;
+  float *logp, *entropy, *stats, *top_logp;
+  int64_t* top_idx;
+  float4* part;      // [R, nseg] (m, z, s, -) of the segments of a long row, and their sorted keys [R, nseg, k]
+  u64* part_key;
+  int R, C, k;
+  float inv_t;
+  Split sp;
 };
-__device__ __forceinline__ void load_listed(Listed& L, const int64_t* idx, const float* tl, int K, int C, float inv_t, int tail, float& mass,
-                                            float* sh) {
-  const int j = threadIdx.x;
-  int id = -1;
-  float t = -INFINITY;
-  if (j < K) {
-    const int64_t i = idx[j];
-    if (i >= 0 && i < C) { id = (int)i; t = tl[j]; }
+
+__device__ __forceinline__ void write_row(const ScoreParams& p, int64_t row, const RowSums& a, bool given, float xt) {
+  const bool none = a.z == 0.f;   // every class at -inf
+  const float log2z = __builtin_amdgcn_logf(a.z);
+  p.stats[2 * row] = none ? -INFINITY : a.m;
+  p.stats[2 * row + 1] = none ? -INFINITY : log2z * LN2;
+  p.entropy[row] = none ? 0.f : (log2z - a.s / a.z) * LN2;
+  p.logp[row] = !given ? 0.f : none ? -INFINITY : (xt - a.m) * p.inv_t - log2z * LN2;
+}
+__device__ __forceinline__ void write_top(const ScoreParams& p, int64_t row, int r, u64 key, const RowSums& a) {
+  const bool nan = a.z != a.z, have = key != 0 && !nan;
+  p.top_idx[row * p.k + r] = have ? key_class(key) : -1;
+  p.top_logp[row * p.k + r] = have ? (unord((uint32_t)(key >> 32)) - a.m) * p.inv_t - __builtin_amdgcn_logf(a.z) * LN2 : nan ? a.z : -INFINITY;
+}
+
+// MULTI false: a wave per row, four rows a workgroup, no barrier.  MULTI: a workgroup per segment of a row.
+template <typename T, bool VEC, bool MULTI>
+__global__ __launch_bounds__(MULTI ? 1024 : 256) void token_logprobs_fwd_kernel(ScoreParams p) {
+  extern __shared__ __attribute__((aligned(16))) u64 score_lds[];
+  __shared__ RowSums sm[MAX_WAVES];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t unit = MULTI ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
+  const int64_t row = MULTI ? blockIdx.x / (unsigned)p.sp.nseg : unit;
+  if (row >= p.R) return;
+  const int seg = MULTI ? (int)(blockIdx.x % (unsigned)p.sp.nseg) : 0;
+  const T* lr = (const T*)p.logits + row * p.ldl;
+  const int64_t tok = p.tokens[row];
+  const bool given = tok >= 0 && tok < p.C;
+  const float xt = given ? (float)lr[tok] : 0.f;      // (its latency runs beside the row's)
+  const int send = MULTI ? min(p.C, (seg + 1) * p.sp.seg) : p.C;
+  const int c0 = MULTI ? seg * p.sp.seg + wave * p.sp.wave_cols : 0, cend = MULTI ? min(send, c0 + p.sp.wave_cols) : p.C;
+  const float c = p.inv_t * LOG2E;
+  float x[NV][8], vmax[NV];
+  load_wave<T, VEC>(lr, c0, cend, lane, x);
+  float m = -FMAX;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    vmax[i] = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) vmax[i] = fmaxf(vmax[i], x[i][j]);
+    m = fmaxf(m, vmax[i]);
   }
-  float p, lp;
-  if (tail) {
-    lp = t;
-    p = id >= 0 ? __expf(t) : 0.f;
-  } else {
-    const float m = fmaxf(block_reduce(t, max_f, sh), -3.402823466e38f);
-    const float u = (t - m) * inv_t;
-    const float e = id >= 0 ? __expf(u) : 0.f;
-    const float z = block_reduce(e, add_f, sh);
-    p = z > 0.f ? e / z : (z == 0.f ? 0.f : z);
-    lp = u - __logf(z);
+  RowSums a;
+  a.m = wave_max(m);
+  a.z = a.s = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (c0 + i * 512 < cend)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float t;
+        const float e = expo(x[i][j], a.m, c, t);
+        a.z += e;
+        a.s = fmaf(e, t, a.s);
+      }
+  a.z = wave_sum(a.z);
+  a.s = wave_sum(a.s);
+  u64* cand = score_lds + (p.k ? wave * TOP_LDS : 0);
+  u64* list = cand + TOP_CAND + 2;
+  if (p.k) wave_top<VEC>(x, vmax, c0, cend, p.k, lane, cand);
+  if (!MULTI) {
+    if (lane == 0) write_row(p, row, a, given, xt);
+    if (lane < p.k) write_top(p, row, lane, list[lane], a);
+    return;
   }
-  if (j < K) { L.idx[j] = id; L.p[j] = p; L.logp[j] = lp; }
-  mass = block_reduce(p, add_f, sh);
+  if (lane == 0) sm[wave] = a;
   __syncthreads();
-}
-
-template <typename T>
-__global__ __launch_bounds__(ROW_T) void distill_fwd_kernel(const T* __restrict__ logits, int64_t ldl, const int64_t* __restrict__ tidx,
-                                                            const float* __restrict__ tlogp, float* __restrict__ row_loss,
-                                                            float* __restrict__ stats, int C, int K, float inv_t, int tail) {
-  __shared__ float sh[4];
-  __shared__ Listed L;
-  const int64_t row = blockIdx.x;
-  const Row<T> x{logits + row * ldl};
-  const float c = inv_t * LOG2E;
-  float mass;
-  load_listed(L, tidx + row * K, tlogp + row * K, K, C, inv_t, tail, mass, sh);
-  float mx = -3.402823466e38f;
-  for (int i = threadIdx.x; i < C; i += ROW_T) mx = fmaxf(mx, x[i]);
-  mx = block_reduce(mx, max_f, sh);
-  float zl = 0.f, zr = 0.f;
-  for (int i = threadIdx.x; i < C; i += ROW_T) {
-    float t;
-    const float e = expo(x[i], mx, c, t);
-    bool hit = false;
-    for (int j = 0; j < K; ++j) hit |= L.idx[j] == i;
-    if (hit) zl += e; else zr += e;
-  }
-  zl = block_reduce(zl, add_f, sh);
-  zr = block_reduce(zr, add_f, sh);
-  const float z = zl + zr;
-  const bool none = z == 0.f;
-  const float logz = __logf(z);
-  float loss = 0.f;
-  if ((int)threadIdx.x < K && L.idx[threadIdx.x] >= 0) {
-    const float p = L.p[threadIdx.x];
-    const float logq = (x[L.idx[threadIdx.x]] - mx) * inv_t - logz;
-    loss = p == 0.f ? 0.f : p * (L.logp[threadIdx.x] - logq);
-  }
-  loss = block_reduce(loss, add_f, sh);
+  const int nw = p.sp.waves;
+  RowSums b = {sm[0].m, 0.f, 0.f};
+  for (int w = 1; w < nw; ++w) b.m = fmaxf(b.m, sm[w].m);
+  for (int w = 0; w < nw; ++w) add_sums(b, sm[w].m, sm[w].z, sm[w].s, b.m, c);
+  const bool whole = p.sp.nseg == 1;
   if (threadIdx.x == 0) {
-    const float left = 1.f - mass;
-    if (tail && left > 0.f && zr > 0.f) loss += left * (log1pf(-mass) + log1pf(zl / zr));
-    row_loss[row] = none ? 0.f : loss;
-    stats[3 * row] = none ? -INFINITY : mx;
-    stats[3 * row + 1] = none ? -INFINITY : logz;
-    stats[3 * row + 2] = none ? -INFINITY : __logf(zr);
+    if (whole) write_row(p, row, b, given, xt);
+    else p.part[unit] = make_float4(b.m, b.z, b.s, 0.f);
+  }
+  if (p.k) {   // one entry of a wave's list per lane; places behind the last entry of all lists stay empty
+    u64* lists = score_lds + TOP_CAND + 2;
+    int have = 0;
+    for (int w = 0; w < nw; ++w) have += __builtin_popcountll(__ballot(lane < p.k && lists[w * TOP_LDS + lane] != 0));
+    const u64 key = lane < p.k ? list[lane] : 0;
+    if (key) {
+      const int r = merged_rank(lists, TOP_LDS, nw, wave, lane, p.k, key);
+      if (r < p.k) {
+        if (whole) write_top(p, row, r, key, b);
+        else p.part_key[unit * p.k + r] = key;
+      }
+    }
+    if (wave == 0 && lane >= have && lane < p.k) {
+      if (whole) write_top(p, row, lane, 0, b);
+      else p.part_key[unit * p.k + lane] = 0;
+    }
   }
 }
 
+// the segments of a long row: at most 32 of them, their sums in one wave, their lists as the waves' above
 template <typename T>
-__global__ __launch_bounds__(ROW_T) void distill_bwd_kernel(const T* __restrict__ logits, int64_t ldl, const int64_t* __restrict__ tidx,
-                                                            const float* __restrict__ tlogp, const float* __restrict__ stats,
-                                                            const float* __restrict__ g_loss, T* __restrict__ dlogits, int64_t ldd, int C,
-                                                            int Cd, int K, float inv_t, int tail, int accumulate) {
-  __shared__ float sh[4];
-  __shared__ Listed L;
+__global__ __launch_bounds__(256) void token_logprobs_join_kernel(ScoreParams p) {
+  extern __shared__ __attribute__((aligned(16))) u64 score_lds[];   // [nseg][k]
   const int64_t row = blockIdx.x;
-  const Row<T> x{logits + row * ldl};
-  float mass;
-  load_listed(L, tidx + row * K, tlogp + row * K, K, C, inv_t, tail, mass, sh);
-  const float mx = stats[3 * row], logz = stats[3 * row + 1], logzr = stats[3 * row + 2];
-  const float left = tail && logzr > -INFINITY ? fmaxf(1.f - mass, 0.f) : 0.f;
-  const float g = g_loss[row] * inv_t;
-  for (int i = threadIdx.x; i < Cd; i += ROW_T) {
-    float d = 0.f;
-    if (i < C && mx != -INFINITY) {
-      const float u = (x[i] - mx) * inv_t;
-      const float q = __expf(u - logz);
-      float p = 0.f;
-      bool hit = false;
-      for (int j = 0; j < K; ++j)
-        if (L.idx[j] == i) { p += L.p[j]; hit = true; }
-      d = q * (mass + left) - p;
-      if (left > 0.f && !hit) d -= left * __expf(u - logzr);
-      d *= g;
+  const int lane = threadIdx.x & 63, nseg = p.sp.nseg, total = nseg * p.k;
+  for (int i = threadIdx.x; i < total; i += 256) score_lds[i] = p.part_key[row * total + i];
+  float4 s = make_float4(-FMAX, 0.f, 0.f, 0.f);
+  if (lane < nseg) s = p.part[row * nseg + lane];
+  RowSums a = {wave_max(s.x), 0.f, 0.f};
+  add_sums(a, s.x, s.y, s.z, a.m, p.inv_t * LOG2E);
+  a.z = wave_sum(a.z);
+  a.s = wave_sum(a.s);
+  if (threadIdx.x == 0) {
+    const int64_t tok = p.tokens[row];
+    const bool given = tok >= 0 && tok < p.C;
+    write_row(p, row, a, given, given ? (float)((const T*)p.logits)[row * p.ldl + tok] : 0.f);
+  }
+  if (!p.k) return;
+  __syncthreads();
+  int have = 0;
+  for (int i = lane; i < total; i += 64) have += score_lds[i] != 0;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) have += __shfl_xor(have, o, 64);
+  for (int i = threadIdx.x; i < total; i += 256) {
+    const u64 key = score_lds[i];
+    if (!key) continue;
+    const int r = merged_rank(score_lds, p.k, nseg, i / p.k, i % p.k, p.k, key);
+    if (r < p.k) write_top(p, row, r, key, a);
+  }
+  for (int r = threadIdx.x; r < p.k; r += 256)
+    if (r >= have) write_top(p, row, r, 0, a);
+}
+
+// (n / d, n % d) of a piece's number: in 32 bits where it fits (a 64-bit division costs as much as the piece's work)
+__device__ __forceinline__ void split_id(int64_t n, int d, int64_t& q, int& r) {
+  if ((uint64_t)n >> 32) { q = n / d; r = (int)(n % d); }
+  else { q = (uint32_t)n / (uint32_t)d; r = (int)((uint32_t)n % (uint32_t)d); }
+}
+
+// ---- gradient of the log-probabilities: one thread per 8 columns, everything of the row is known -------------------------
+template <typename T> __device__ __forceinline__ void store8(T* p, const float (&v)[8]);
+template <> __device__ __forceinline__ void store8<bf16>(bf16* p, const float (&v)[8]) {
+  bf16x8 r;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) r[j] = (bf16)v[j];
+  *reinterpret_cast<bf16x8*>(p) = r;
+}
+template <> __device__ __forceinline__ void store8<_Float16>(_Float16* p, const float (&v)[8]) {
+  f16x8 r;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) r[j] = (_Float16)v[j];
+  *reinterpret_cast<f16x8*>(p) = r;
+}
+template <> __device__ __forceinline__ void store8<float>(float* p, const float (&v)[8]) {
+  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+}
+
+struct ScoreGradParams {
+  const void* logits; int64_t ldl;
+  const int64_t* tokens;
+  const float *stats, *entropy, *g_logp, *g_entropy;
+  void* dlogits; int64_t ldd;
+  int C, Cd, per_row;   // per_row: 8-column pieces (aligned) or 512-column pieces (others) of a row
+  int64_t pieces;
+  float inv_t;
+};
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(ScoreGradParams p) {
+  const int64_t id = VEC ? (int64_t)blockIdx.x * 256 + threadIdx.x : (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (id >= p.pieces) return;
+  int64_t row;
+  int piece;
+  split_id(id, p.per_row, row, piece);
+  const int first = piece * (VEC ? 8 : 512) + (VEC ? 0 : (threadIdx.x & 63)), step = VEC ? 1 : 64;
+  const T* x = (const T*)p.logits + row * p.ldl;
+  T* d = (T*)p.dlogits + row * p.ldd;
+  float v[8];
+  if (VEC) {
+    if (first < p.C) load8<T>(x + first, p.C - first, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = first + 64 * j < p.C ? (float)x[first + 64 * j] : 0.f;
+  }
+  const float m = p.stats[2 * row], logz = p.stats[2 * row + 1], H = p.entropy[row];
+  const int64_t tok = p.tokens[row];
+  const bool given = tok >= 0 && tok < p.C;
+  const float gl = given ? p.g_logp[row] : 0.f, gh = p.g_entropy ? p.g_entropy[row] : 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int col = first + step * j;
+    float g = 0.f;
+    if (col < p.C && m != -INFINITY) {
+      const float y = (v[j] - m) * p.inv_t - logz;
+      const float q = __builtin_amdgcn_exp2f(y * LOG2E);
+      g = q == 0.f ? 0.f : -q * (gl + gh * (y + H));
+      if (given && col == (int)tok) g += gl;
+      g *= p.inv_t;
     }
-    T* o = dlogits + row * ldd + i;
-    if (accumulate) { if (i < C) *o = (T)((float)*o + d); }
-    else *o = (T)d;
+    v[j] = g;
+  }
+  if (VEC) {
+    if (first + 8 <= p.Cd) {
+      store8<T>(d + first, v);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (first + j < p.Cd) d[first + j] = (T)v[j];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (first + 64 * j < p.Cd) d[first + 64 * j] = (T)v[j];
+  }
+}
+
+// ---- distillation ---------------------------------------------------------------------------------------------------------
+// A row's list, two entries a lane: class (or -1), p and log p, and the list's mass.
+struct Listed { int id[2]; float p[2], logp[2], mass; };
+__device__ __forceinline__ Listed load_listed(const int64_t* idx, const float* tl, int K, int C, float inv_t, int tail, int lane) {
+  Listed L;
+  float t[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int j = lane + 64 * h;
+    L.id[h] = -1;
+    t[h] = -INFINITY;
+    if (j < K) {
+      const int64_t i = idx[j];
+      const float v = tl[j];
+      if (i >= 0 && i < C) { L.id[h] = (int)i; t[h] = v; }
+    }
+  }
+  if (tail) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      L.logp[h] = t[h];
+      L.p[h] = L.id[h] >= 0 ? __expf(t[h]) : 0.f;
+    }
+  } else {
+    const float m = fmaxf(wave_max(fmaxf(t[0], t[1])), -FMAX);
+    float e[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      L.logp[h] = (t[h] - m) * inv_t;
+      e[h] = L.id[h] >= 0 ? __expf(L.logp[h]) : 0.f;
+    }
+    const float z = wave_sum(e[0] + e[1]);
+    const float logz = __logf(z);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      L.p[h] = z == 0.f ? 0.f : e[h] / z;
+      L.logp[h] -= logz;
+    }
+  }
+  L.mass = wave_sum(L.p[0] + L.p[1]);
+  return L;
+}
+
+struct DistillParams {
+  const void* logits; int64_t ldl;
+  const int64_t* idx;
+  const float* tlogp;
+  float *row_loss, *stats;
+  float4* part;        // [R, nseg] (m, z of the listed classes, z of the others, -)
+  int R, C, K, tail;
+  float inv_t;
+  Split sp;
+};
+// by one wave: the row's loss from its sums (listed and other classes apart with tail, else all in zr) and the listed classes' logits
+__device__ __forceinline__ void finish_distill(const DistillParams& p, int64_t row, const Listed& L, const float (&xl)[2], float m, float zl, float zr,
+                                               int lane) {
+  const float z = zl + zr, logz = __logf(z);
+  float loss = 0.f;
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    if (L.p[h] != 0.f) loss += L.p[h] * (L.logp[h] - ((xl[h] - m) * p.inv_t - logz));
+  loss = wave_sum(loss);
+  if (lane == 0) {
+    const float left = 1.f - L.mass;
+    // log of the student's rest = -log(1 + listed / others): the difference of two log-sums would lose it where little is listed
+    if (p.tail && left > 0.f && zr > 0.f) loss += left * (log1pf(-L.mass) + log1pf(zl / zr));
+    const bool none = z == 0.f;
+    p.row_loss[row] = none ? 0.f : loss;
+    p.stats[3 * row] = none ? -INFINITY : m;
+    p.stats[3 * row + 1] = none ? -INFINITY : logz;
+    p.stats[3 * row + 2] = none || !p.tail ? 0.f : zl / zr;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void listed_logits(const T* row, const Listed& L, float (&xl)[2]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) xl[h] = L.id[h] >= 0 ? (float)row[L.id[h]] : 0.f;
+}
+
+// as token_logprobs_fwd_kernel; with tail each wave marks the listed classes of its columns in a bit map of its own
+template <typename T, bool VEC, bool MULTI>
+__global__ __launch_bounds__(MULTI ? 1024 : 256) void distill_fwd_kernel(DistillParams p) {
+  __shared__ uint32_t marks[MULTI ? MAX_WAVES : 4][WAVE_COLS / 32];
+  __shared__ RowSums sm[MAX_WAVES];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t unit = MULTI ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
+  const int64_t row = MULTI ? blockIdx.x / (unsigned)p.sp.nseg : unit;
+  if (row >= p.R) return;
+  const int seg = MULTI ? (int)(blockIdx.x % (unsigned)p.sp.nseg) : 0;
+  const T* lr = (const T*)p.logits + row * p.ldl;
+  const int send = MULTI ? min(p.C, (seg + 1) * p.sp.seg) : p.C;
+  const int c0 = MULTI ? seg * p.sp.seg + wave * p.sp.wave_cols : 0, cend = MULTI ? min(send, c0 + p.sp.wave_cols) : p.C;
+  const float c = p.inv_t * LOG2E;
+  float x[NV][8];
+  load_wave<T, VEC>(lr, c0, cend, lane, x);
+  const bool first = wave == 0 || !MULTI, whole = !MULTI || p.sp.nseg == 1;
+  Listed L;
+  float xl[2] = {0.f, 0.f};
+  if (p.tail || (first && whole)) L = load_listed(p.idx + row * p.K, p.tlogp + row * p.K, p.K, p.C, p.inv_t, p.tail, lane);
+  if (first && whole) listed_logits(lr, L, xl);
+  uint32_t* mark = marks[wave];
+  if (p.tail) {
+    mark[lane] = 0;
+    wave_fence();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int at = L.id[h] - c0;
+      if (L.id[h] >= c0 && L.id[h] < cend) atomicOr(&mark[at >> 5], 1u << (at & 31));
+    }
+    wave_fence();
+  }
+  float m = -FMAX;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = fmaxf(m, x[i][j]);
+  m = wave_max(m);
+  float zl = 0.f, zr = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (c0 + i * 512 >= cend) break;
+    const uint32_t bits = p.tail && VEC ? reinterpret_cast<const uint8_t*>(mark)[i * 64 + lane] : 0u;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float e = __builtin_amdgcn_exp2f((x[i][j] - m) * c);
+      bool hit = false;
+      if (p.tail) hit = VEC ? (bits >> j) & 1u : (mark[i * 16 + j * 2 + (lane >> 5)] >> (lane & 31)) & 1u;
+      zl += hit ? e : 0.f;
+      zr += hit ? 0.f : e;
+    }
+  }
+  zl = wave_sum(zl);
+  zr = wave_sum(zr);
+  if (!MULTI) {
+    finish_distill(p, row, L, xl, m, zl, zr, lane);
+    return;
+  }
+  if (lane == 0) sm[wave] = RowSums{m, zl, zr};
+  __syncthreads();
+  if (wave) return;
+  float M = sm[0].m, Zl = 0.f, Zr = 0.f;
+  for (int w = 1; w < p.sp.waves; ++w) M = fmaxf(M, sm[w].m);
+  for (int w = 0; w < p.sp.waves; ++w) {
+    const float f = __builtin_amdgcn_exp2f((sm[w].m - M) * c);
+    Zl += sm[w].z * f;
+    Zr += sm[w].s * f;
+  }
+  if (whole) finish_distill(p, row, L, xl, M, Zl, Zr, lane);
+  else if (lane == 0) p.part[unit] = make_float4(M, Zl, Zr, 0.f);
+}
+template <typename T>
+__global__ __launch_bounds__(256) void distill_join_kernel(DistillParams p) {   // a wave per row; at most 32 segments
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= p.R) return;
+  float4 s = make_float4(-FMAX, 0.f, 0.f, 0.f);
+  if (lane < p.sp.nseg) s = p.part[row * p.sp.nseg + lane];
+  const Listed L = load_listed(p.idx + row * p.K, p.tlogp + row * p.K, p.K, p.C, p.inv_t, p.tail, lane);
+  float xl[2];
+  listed_logits((const T*)p.logits + row * p.ldl, L, xl);
+  const float m = wave_max(s.x), f = __builtin_amdgcn_exp2f((s.x - m) * p.inv_t * LOG2E);
+  const float zl = wave_sum(s.y * f), zr = wave_sum(s.z * f);
+  finish_distill(p, row, L, xl, m, zl, zr, lane);
+}
+
+struct DistillGradParams {
+  const void* logits; int64_t ldl;
+  const int64_t* idx;
+  const float *tlogp, *stats, *g_loss;
+  void* dlogits; int64_t ldd;
+  int C, Cd, K, tail, accumulate, per_row, wave_cols;
+  int64_t units;
+  float inv_t;
+};
+// A wave on its own takes up to 2048 columns of a row.  A byte map of them in LDS names the list's entry (+ 1) of each class; of a class
+// named twice one entry's number stands there, and that entry's p becomes the sum, added in the list's order.  With
+// q = softmax(y) and w = (listed / other mass of the student), d / dy = q (mass - left w) on other classes (left the mass that the
+// list leaves out; 0 without tail) and q (mass + left) - p on the listed ones: one exponential per class.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void distill_bwd_kernel(DistillGradParams p) {
+  __shared__ uint32_t maps[4][WAVE_COLS / 4];
+  __shared__ float ps[4][TTTS_DISTILL_MAX_K + 1];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t unit = (int64_t)blockIdx.x * 4 + wave;
+  if (unit >= p.units) return;
+  int64_t row;
+  int piece;
+  split_id(unit, p.per_row, row, piece);
+  const int c0 = piece * p.wave_cols, dend = min(p.Cd, c0 + p.wave_cols), cend = min(p.C, dend);
+  const T* lr = (const T*)p.logits + row * p.ldl;
+  T* dr = (T*)p.dlogits + row * p.ldd;
+  float x[NV][8];
+  load_wave<T, VEC>(lr, c0, cend, lane, x);
+  uint32_t* map = maps[wave];
+  uint8_t* map8 = reinterpret_cast<uint8_t*>(map);
+  float* pl = ps[wave];
+#pragma unroll
+  for (int i = 0; i < WAVE_COLS / 4 / 64; ++i) map[i * 64 + lane] = 0;
+  const Listed L = load_listed(p.idx + row * p.K, p.tlogp + row * p.K, p.K, p.C, p.inv_t, p.tail, lane);
+  const float m = p.stats[3 * row], logz = p.stats[3 * row + 1], w = p.stats[3 * row + 2], g = p.g_loss[row] * p.inv_t;
+  wave_fence();
+  bool here[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    here[h] = L.id[h] >= c0 && L.id[h] < cend;
+    if (here[h]) map8[L.id[h] - c0] = (uint8_t)(lane + 64 * h + 1);
+    pl[lane + 64 * h] = L.p[h];
+  }
+  wave_fence();
+  bool twice = false;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) twice |= here[h] && map8[L.id[h] - c0] != (uint8_t)(lane + 64 * h + 1);
+  if (__any(twice)) {
+    float sum[2] = {0.f, 0.f};
+    for (int j = 0; j < p.K; ++j) {
+      const int idj = __shfl(j < 64 ? L.id[0] : L.id[1], j & 63, 64);
+      const float pj = __shfl(j < 64 ? L.p[0] : L.p[1], j & 63, 64);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) sum[h] += idj == L.id[h] ? pj : 0.f;
+    }
+    wave_fence();
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (here[h]) pl[lane + 64 * h] = sum[h];
+  }
+  wave_fence();
+  const bool held = p.tail && w < INFINITY;          // other classes than the listed ones hold something
+  const float left = held ? fmaxf(1.f - L.mass, 0.f) : 0.f;
+  const float on = L.mass + left, off = left > 0.f ? L.mass - left * w : L.mass;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (c0 + i * 512 >= dend) break;
+    uint2 marks = make_uint2(0u, 0u);
+    if (VEC) marks = *reinterpret_cast<const uint2*>(map8 + i * 512 + lane * 8);
+    float d[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float q = __builtin_amdgcn_exp2f(((x[i][j] - m) * p.inv_t - logz) * LOG2E);
+      const uint32_t e = VEC ? ((j < 4 ? marks.x : marks.y) >> (8 * (j & 3))) & 255u : map8[i * 512 + j * 64 + lane];
+      d[j] = e ? fmaf(q, on, -pl[e - 1]) : q * off;
+      d[j] = wave_col<VEC>(c0, i, j, lane) < p.C && m != -INFINITY ? d[j] * g : 0.f;
+    }
+    if (VEC && !p.accumulate && c0 + i * 512 + lane * 8 + 8 <= dend) {
+      store8<T>(dr + c0 + i * 512 + lane * 8, d);
+    } else if (VEC && p.accumulate && c0 + i * 512 + lane * 8 + 8 <= cend) {
+      float o[8];
+      T* at = dr + c0 + i * 512 + lane * 8;
+      load8<T>(at, 8, o);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[j] += d[j];
+      store8<T>(at, o);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int col = wave_col<VEC>(c0, i, j, lane);
+        if (p.accumulate) { if (col < cend) dr[col] = (T)((float)dr[col] + d[j]); }
+        else if (col < dend) dr[col] = (T)d[j];
+      }
+    }
   }
 }
 
@@ -266,7 +733,42 @@ static int check_logits(const char* what, const void* logits, int32_t dtype, int
   return TTTS_OK;
 }
 
-extern "C" int64_t ttts_token_logprobs_workspace_bytes(int32_t R, int32_t C, int32_t top_k) { return 0; }
+// rows whose addresses are all multiples of 16 bytes
+static bool rows16(const void* p, int64_t ld, int32_t dtype) { return aligned16(p) && (ld * (dtype == TTTS_DTYPE_F32 ? 4 : 2)) % 16 == 0; }
+static int need_workspace(const char* what, int64_t need, const void* ws, int64_t have) {
+  TTTS_REQUIRE(need == 0 || (ws && have >= need && aligned16(ws)), "%s: needs a 16-byte aligned workspace of %lld bytes", what, (long long)need);
+  return TTTS_OK;
+}
+static int need_grid(const char* what, int64_t grid) {
+  TTTS_REQUIRE(grid <= 0x7fffffff, "%s: more work than one launch holds", what);
+  return TTTS_OK;
+}
+
+extern "C" int64_t ttts_token_logprobs_workspace_bytes(int32_t R, int32_t C, int32_t top_k) {
+  if (R <= 0 || C <= 0 || top_k < 0) return 0;
+  const Split sp = split_row(C);
+  return sp.nseg > 1 ? cdiv((int64_t)R * sp.nseg * (16 + 8 * (int64_t)top_k), 16) * 16 : 0;
+}
+
+template <typename T, bool VEC>
+static int launch_score(const ScoreParams& p, hipStream_t st) {
+  const char* what = "token_logprobs_fwd";
+  if (p.sp.nseg == 1 && p.sp.waves == 1) {
+    token_logprobs_fwd_kernel<T, VEC, false><<<(unsigned)cdiv(p.R, 4), 256, p.k ? 4 * TOP_LDS * 8 : 0, st>>>(p);
+    return check_launch(what);
+  }
+  static OnceFlag once;
+  if (lds_opt_in(once, (const void*)token_logprobs_fwd_kernel<T, VEC, true>, MAX_WAVES * TOP_LDS * 8) != hipSuccess)
+    return fail(TTTS_EHIP, "%s: LDS opt-in failed", what);
+  const int64_t grid = (int64_t)p.R * p.sp.nseg;
+  int rc = need_grid(what, grid);
+  if (rc) return rc;
+  token_logprobs_fwd_kernel<T, VEC, true><<<(unsigned)grid, 64 * p.sp.waves, p.k ? p.sp.waves * TOP_LDS * 8 : 0, st>>>(p);
+  rc = check_launch(what);
+  if (rc || p.sp.nseg == 1) return rc;
+  token_logprobs_join_kernel<T><<<p.R, 256, p.sp.nseg * p.k * 8, st>>>(p);
+  return check_launch("token_logprobs_fwd join");
+}
 
 extern "C" int ttts_token_logprobs_fwd(const void* logits, int32_t dtype, int64_t ldl, const int64_t* tokens, float* logp, float* entropy,
                                        float* stats, float* top_logp, int64_t* top_idx, int32_t R, int32_t C, int32_t top_k,
@@ -276,10 +778,14 @@ extern "C" int ttts_token_logprobs_fwd(const void* logits, int32_t dtype, int64_
   TTTS_REQUIRE(top_k >= 0 && top_k <= TTTS_SCORE_MAX_TOP, "token_logprobs_fwd: need 0 <= top_k <= %d", TTTS_SCORE_MAX_TOP);
   if (R == 0) return TTTS_OK;
   TTTS_REQUIRE(tokens && logp && entropy && stats && (top_k == 0 || (top_logp && top_idx)), "token_logprobs_fwd: null pointer");
-  TTTS_BY_TYPE(dtype, "token_logprobs_fwd",
-               (token_logprobs_fwd_kernel<T><<<R, ROW_T, 0, as_stream(stream)>>>((const T*)logits, ldl, tokens, logp, entropy, stats, top_logp,
-                                                                                top_idx, C, top_k, 1.0f / temperature)));
-  return check_launch("token_logprobs_fwd");
+  rc = need_workspace("token_logprobs_fwd", ttts_token_logprobs_workspace_bytes(R, C, top_k), workspace, workspace_bytes);
+  if (rc) return rc;
+  ScoreParams p{logits, ldl, tokens, logp, entropy, stats, top_logp, top_idx, (float4*)workspace, nullptr, R, C, top_k, 1.0f / temperature, split_row(C)};
+  p.part_key = (u64*)(p.part + (int64_t)R * p.sp.nseg);
+  const bool vec = rows16(logits, ldl, dtype);
+  hipStream_t st = as_stream(stream);
+  TTTS_BY_TYPE(dtype, "token_logprobs_fwd", rc = (vec ? launch_score<T, true>(p, st) : launch_score<T, false>(p, st)));
+  return rc;
 }
 
 extern "C" int ttts_token_logprobs_bwd(const void* logits, int32_t dtype, int64_t ldl, const int64_t* tokens, const float* stats,
@@ -290,13 +796,41 @@ extern "C" int ttts_token_logprobs_bwd(const void* logits, int32_t dtype, int64_
   TTTS_REQUIRE(Cd >= C && ldd >= Cd, "token_logprobs_bwd: need C <= Cd <= ldd");
   if (R == 0) return TTTS_OK;
   TTTS_REQUIRE(tokens && stats && entropy && g_logp && dlogits, "token_logprobs_bwd: null pointer");
-  TTTS_BY_TYPE(dtype, "token_logprobs_bwd",
-               (token_logprobs_bwd_kernel<T><<<R, ROW_T, 0, as_stream(stream)>>>((const T*)logits, ldl, tokens, stats, entropy, g_logp, g_entropy,
-                                                                                (T*)dlogits, ldd, C, Cd, 1.0f / temperature)));
+  const bool vec = rows16(logits, ldl, dtype) && rows16(dlogits, ldd, dtype);
+  ScoreGradParams p{logits, ldl, tokens, stats, entropy, g_logp, g_entropy, dlogits, ldd, C, Cd, (int)cdiv(Cd, vec ? 8 : 512), 0, 1.0f / temperature};
+  p.pieces = (int64_t)R * p.per_row;
+  const int64_t grid = cdiv(p.pieces, vec ? 256 : 4);
+  rc = need_grid("token_logprobs_bwd", grid);
+  if (rc) return rc;
+  if (vec)
+    TTTS_BY_TYPE(dtype, "token_logprobs_bwd", (token_logprobs_bwd_kernel<T, true><<<(unsigned)grid, 256, 0, as_stream(stream)>>>(p)))
+  else
+    TTTS_BY_TYPE(dtype, "token_logprobs_bwd", (token_logprobs_bwd_kernel<T, false><<<(unsigned)grid, 256, 0, as_stream(stream)>>>(p)))
   return check_launch("token_logprobs_bwd");
 }
 
-extern "C" int64_t ttts_distill_workspace_bytes(int32_t R, int32_t C) { return 0; }
+extern "C" int64_t ttts_distill_workspace_bytes(int32_t R, int32_t C) {
+  if (R <= 0 || C <= 0) return 0;
+  const Split sp = split_row(C);
+  return sp.nseg > 1 ? (int64_t)R * sp.nseg * 16 : 0;
+}
+
+template <typename T, bool VEC>
+static int launch_distill(const DistillParams& p, hipStream_t st) {
+  const char* what = "distill_fwd";
+  if (p.sp.nseg == 1 && p.sp.waves == 1) {
+    distill_fwd_kernel<T, VEC, false><<<(unsigned)cdiv(p.R, 4), 256, 0, st>>>(p);
+    return check_launch(what);
+  }
+  const int64_t grid = (int64_t)p.R * p.sp.nseg;
+  int rc = need_grid(what, grid);
+  if (rc) return rc;
+  distill_fwd_kernel<T, VEC, true><<<(unsigned)grid, 64 * p.sp.waves, 0, st>>>(p);
+  rc = check_launch(what);
+  if (rc || p.sp.nseg == 1) return rc;
+  distill_join_kernel<T><<<(unsigned)cdiv(p.R, 4), 256, 0, st>>>(p);
+  return check_launch("distill_fwd join");
+}
 
 extern "C" int ttts_distill_fwd(const void* logits, int32_t dtype, int64_t ldl, const int64_t* teacher_idx, const float* teacher_logp,
                                 float* row_loss, float* stats, int32_t R, int32_t C, int32_t K, float temperature, int32_t tail,
@@ -306,10 +840,13 @@ extern "C" int ttts_distill_fwd(const void* logits, int32_t dtype, int64_t ldl, 
   TTTS_REQUIRE(K > 0 && K <= TTTS_DISTILL_MAX_K, "distill_fwd: need 0 < K <= %d", TTTS_DISTILL_MAX_K);
   if (R == 0) return TTTS_OK;
   TTTS_REQUIRE(teacher_idx && teacher_logp && row_loss && stats, "distill_fwd: null pointer");
-  TTTS_BY_TYPE(dtype, "distill_fwd",
-               (distill_fwd_kernel<T><<<R, ROW_T, 0, as_stream(stream)>>>((const T*)logits, ldl, teacher_idx, teacher_logp, row_loss, stats, C, K,
-                                                                         1.0f / temperature, tail)));
-  return check_launch("distill_fwd");
+  rc = need_workspace("distill_fwd", ttts_distill_workspace_bytes(R, C), workspace, workspace_bytes);
+  if (rc) return rc;
+  const DistillParams p{logits, ldl, teacher_idx, teacher_logp, row_loss, stats, (float4*)workspace, R, C, K, tail != 0, 1.0f / temperature, split_row(C)};
+  const bool vec = rows16(logits, ldl, dtype);
+  hipStream_t st = as_stream(stream);
+  TTTS_BY_TYPE(dtype, "distill_fwd", rc = (vec ? launch_distill<T, true>(p, st) : launch_distill<T, false>(p, st)));
+  return rc;
 }
 
 extern "C" int ttts_distill_bwd(const void* logits, int32_t dtype, int64_t ldl, const int64_t* teacher_idx, const float* teacher_logp,
@@ -321,8 +858,18 @@ extern "C" int ttts_distill_bwd(const void* logits, int32_t dtype, int64_t ldl, 
   TTTS_REQUIRE(Cd >= C && ldd >= Cd, "distill_bwd: need C <= Cd <= ldd");
   if (R == 0) return TTTS_OK;
   TTTS_REQUIRE(teacher_idx && teacher_logp && stats && g_loss && dlogits, "distill_bwd: null pointer");
-  TTTS_BY_TYPE(dtype, "distill_bwd",
-               (distill_bwd_kernel<T><<<R, ROW_T, 0, as_stream(stream)>>>((const T*)logits, ldl, teacher_idx, teacher_logp, stats, g_loss,
-                                                                         (T*)dlogits, ldd, C, Cd, K, 1.0f / temperature, tail, accumulate)));
+  const bool vec = rows16(logits, ldl, dtype) && rows16(dlogits, ldd, dtype);
+  DistillGradParams p{logits, ldl, teacher_idx, teacher_logp, stats, g_loss, dlogits, ldd, C, Cd, K, tail != 0, accumulate != 0, 0, 0, 0, 1.0f / temperature};
+  p.per_row = (int)cdiv(Cd, WAVE_COLS);
+  p.wave_cols = (int)cdiv(cdiv(Cd, p.per_row), 8) * 8;
+  p.per_row = (int)cdiv(Cd, p.wave_cols);
+  p.units = (int64_t)R * p.per_row;
+  const int64_t grid = cdiv(p.units, 4);
+  rc = need_grid("distill_bwd", grid);
+  if (rc) return rc;
+  if (vec)
+    TTTS_BY_TYPE(dtype, "distill_bwd", (distill_bwd_kernel<T, true><<<(unsigned)grid, 256, 0, as_stream(stream)>>>(p)))
+  else
+    TTTS_BY_TYPE(dtype, "distill_bwd", (distill_bwd_kernel<T, false><<<(unsigned)grid, 256, 0, as_stream(stream)>>>(p)))
   return check_launch("distill_bwd");
 }

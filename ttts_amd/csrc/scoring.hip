@@ -14,63 +14,61 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f, FMAX = 3
 
 // ---- one wave = up to 2048 columns of a row, held in registers as fp32 -------------------------------------------------
 // A row is read ONCE: maximum, sums, and the alternatives all come from the registers.  Rows up to 2048 columns take one wave, up to 32768
-// one workgroup of up to 16 waves that meet once in LDS, longer ones several workgroups (segments) and a second kernel that
-// joins their results.  Aligned rows: a lane holds 8 neighbouring columns per load; others: single columns, neighbouring lanes.
+// one workgroup of up to 16 waves that meet in LDS, longer ones several workgroups (segments) and a second kernel that joins
+// their results.  A lane holds 8 neighbouring columns per load (16 or 32 bytes, at whatever alignment the row has; only the row's last
+// columns are read one by one), 64 lanes 512 neighbouring ones: x[i][j] is column c0 + 512 i + 8 lane + j.
 constexpr int NV = 4, WAVE_COLS = NV * 512, MAX_WAVES = 16, SEG_COLS = WAVE_COLS * MAX_WAVES;
 
-struct Split {   // columns of a row -> segments (workgroups) -> waves
+struct Split {   // columns of a row -> segments (workgroups) -> waves, in whole 512s: the fewest steps over all waves
   int seg, nseg, waves, wave_cols;
 };
 static Split split_row(int C) {
   Split s;
   s.nseg = (int)cdiv(C, SEG_COLS);
-  s.seg = (int)cdiv(cdiv(C, s.nseg), 8) * 8;
+  s.seg = (int)cdiv(cdiv(C, 512), s.nseg) * 512;
   s.nseg = (int)cdiv(C, s.seg);
   s.waves = (int)cdiv(s.seg, WAVE_COLS);
-  s.wave_cols = (int)cdiv(cdiv(s.seg, s.waves), 8) * 8;
+  s.wave_cols = (int)cdiv(s.seg / 512, s.waves) * 512;
   return s;
 }
 
-template <typename T> __device__ __forceinline__ void load8(const T* p, int n, float (&v)[8]);   // n valid columns (1 .. 8) of an aligned 8
-template <> __device__ __forceinline__ void load8<bf16>(const bf16* p, int n, float (&v)[8]) {
-  const bf16x8 r = *reinterpret_cast<const bf16x8*>(p);
+template <typename T> struct Eight { typedef T type __attribute__((ext_vector_type(8), aligned(sizeof(T)))); };   // 8 columns, aligned to T only
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int n, float (&v)[8]) {   // the first n (>= 1) of 8 columns
+  if (n >= 8) {
+    const typename Eight<T>::type r = *reinterpret_cast<const typename Eight<T>::type*>(p);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = j < n ? (float)r[j] : -INFINITY;
-}
-template <> __device__ __forceinline__ void load8<_Float16>(const _Float16* p, int n, float (&v)[8]) {
-  const f16x8 r = *reinterpret_cast<const f16x8*>(p);
+    for (int j = 0; j < 8; ++j) v[j] = (float)r[j];
+  } else {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = j < n ? (float)r[j] : -INFINITY;
+    for (int j = 0; j < 8; ++j) v[j] = j < n ? (float)p[j] : -INFINITY;
+  }
 }
-template <> __device__ __forceinline__ void load8<float>(const float* p, int n, float (&v)[8]) {
-  const float4 a = *reinterpret_cast<const float4*>(p);
-  float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (n > 4) b = *reinterpret_cast<const float4*>(p + 4);   // (the pitch is a multiple of 4 only)
-  const float r[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+template <typename T>
+__device__ __forceinline__ void store8(T* p, int n, const float (&v)[8]) {
+  if (n >= 8) {
+    typename Eight<T>::type r;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = j < n ? r[j] : -INFINITY;
+    for (int j = 0; j < 8; ++j) r[j] = (T)v[j];
+    *reinterpret_cast<typename Eight<T>::type*>(p) = r;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < n) p[j] = (T)v[j];
+  }
 }
-
-// columns c0 .. cend - 1 of a row; columns outside are -inf.  Column of x[i][j]: wave_col(c0, i, j).
-template <bool VEC>
-__device__ __forceinline__ int wave_col(int c0, int i, int j, int lane) { return VEC ? c0 + i * 512 + lane * 8 + j : c0 + i * 512 + j * 64 + lane; }
-template <typename T, bool VEC>
+// columns c0 .. cend - 1 of a row; columns outside are -inf
+template <typename T>
 __device__ __forceinline__ void load_wave(const T* row, int c0, int cend, int lane, float (&x)[NV][8]) {
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
+    const int c = c0 + i * 512 + lane * 8;
+    if (c0 + i * 512 + 512 <= cend) {
+      load8<T>(row + c, 8, x[i]);
+    } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[i][j] = -INFINITY;
-    if (c0 + i * 512 < cend) {
-      if (VEC) {
-        const int c = c0 + i * 512 + lane * 8;
-        if (c < cend) load8<T>(row + c, cend - c, x[i]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int c = c0 + i * 512 + j * 64 + lane;
-          if (c < cend) x[i][j] = (float)row[c];
-        }
-      }
+      for (int j = 0; j < 8; ++j) x[i][j] = -INFINITY;
+      if (c < cend) load8<T>(row + c, cend - c, x[i]);
     }
   }
 }
@@ -88,7 +86,7 @@ __device__ __forceinline__ void wave_fence() {   // LDS written by this wave's l
   __builtin_amdgcn_wave_barrier();
 }
 
-// ---- the k best of a wave's columns ---------------------------------------------------------------------------------------
+// ---- the k best columns --------------------------------------------------------------------------------------------------
 // Order: larger value first, lower class first among equals.  A 64-bit key holds both: the value's bits in the order of the numbers
 // (zeros of both signs the same), and the class, inverted; key 0 is none.
 typedef unsigned long long u64;
@@ -100,104 +98,121 @@ __device__ __forceinline__ float unord(uint32_t u) { return __builtin_bit_cast(f
 __device__ __forceinline__ u64 top_key(float v, int c) { return ((u64)ord(v) << 32) | (uint32_t)~c; }
 __device__ __forceinline__ int key_class(u64 k) { return (int)~(uint32_t)k; }
 constexpr uint32_t ORD_NONE = 0x007fffffu;   // ord(-inf)
-
-constexpr int TOP_CAND = 64 * 8 + 64;        // candidates a wave keeps; TOP_LDS: and its sorted list, in u64
-constexpr int TOP_LDS = TOP_CAND + 2 + TTTS_SCORE_MAX_TOP;
 __device__ __forceinline__ int lanes_below(u64 mask) {
   return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
 }
-// A threshold first: the k-th largest of the 256 maxima of 8 columns each (vmax), found bit by bit with ballots, is at most the k-th
-// largest value, and what reaches it lies in few of those groups: about k + 10 % columns of ordinary rows.  These are ranked by
-// counting.  When values repeat (a constant row) any number of columns can reach it: then those above it are taken (under 64
-// groups of 8) and of those AT it the lowest classes, as many as are needed.
-template <bool VEC>
-__device__ __forceinline__ int wave_top(const float (&x)[NV][8], const float (&vmax)[NV], int c0, int cend, int k, int lane, u64* cand) {
-  u64* list = cand + TOP_CAND + 2;
-  uint32_t g[NV];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) g[i] = ord(vmax[i]);
+
+// A threshold first: the k-th largest of the maxima of groups of columns is at most the k-th largest column, and few columns reach it
+// (k + 10 .. 30 % of ordinary rows).  It is found bit by bit with ballots over n group maxima a lane, and any value that exactly k
+// groups reach will do (early).  What reaches it lies in at most k groups, unless values repeat at the threshold: then (exact) fewer
+// than k groups go above it, and of the columns AT it the lowest classes are taken, as many as are needed.
+template <int N>
+__device__ __forceinline__ float group_threshold(const uint32_t (&g)[N], int n, int k, bool early) {
   uint32_t t = 0;
   for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
     const uint32_t c = t | bit;
     int cnt = 0;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) cnt += __builtin_popcountll(__ballot(g[i] >= c));
+    for (int i = 0; i < N; ++i)
+      if (i < n) cnt += __builtin_popcountll(__ballot(g[i] >= c));
     if (cnt >= k) {
       t = c;
-      if (cnt == k) break;
+      if (early && cnt == k) break;
     }
   }
-  const float thr = t <= ORD_NONE ? -FMAX : unord(t);
-  int n = 0;
+  return t <= ORD_NONE ? -FMAX : unord(t);   // (a class at -inf is no alternative)
+}
+// bit 31 - (8 i + j): x[i][j] reaches the threshold / is above it
+template <bool ABOVE>
+__device__ __forceinline__ uint32_t reached(const float (&x)[NV][8], float thr, int c0, int cend) {
+  uint32_t bits = 0;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    if (c0 + i * 512 >= cend) break;
+    if (c0 + i * 512 < cend) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const bool in = x[i][j] >= thr;
-      const u64 mask = __ballot(in);
-      if (mask) {
-        const int at = n + lanes_below(mask);
-        if (in && at < TOP_CAND) cand[at] = top_key(x[i][j], wave_col<VEC>(c0, i, j, lane));
-        n += __builtin_popcountll(mask);
-      }
+      for (int j = 0; j < 8; ++j) bits = bits + bits + (ABOVE ? x[i][j] > thr : x[i][j] >= thr);
+    } else {
+      bits <<= 8;
     }
   }
-  if (n > TOP_CAND) {
-    n = 0;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const bool in = x[i][j] > thr;
-        const u64 mask = __ballot(in);
-        if (in) cand[n + lanes_below(mask)] = top_key(x[i][j], wave_col<VEC>(c0, i, j, lane));
-        n += __builtin_popcountll(mask);
-      }
-    const int end = max(n, k);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      if (VEC) {   // classes ascend with (lane, j)
-        int mine = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) mine += x[i][j] == thr;
-        int upto = mine;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-          const int v = __shfl_up(upto, o, 64);
-          if (lane >= o) upto += v;
-        }
-        int at = n + upto - mine;
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (x[i][j] == thr) {
-            if (at < end) cand[at] = top_key(x[i][j], wave_col<VEC>(c0, i, j, lane));
-            ++at;
-          }
-        n += __shfl(upto, 63, 64);
-      } else {     // classes ascend with (j, lane)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const bool in = x[i][j] == thr;
-          const u64 mask = __ballot(in);
-          const int at = n + lanes_below(mask);
-          if (in && at < end) cand[at] = top_key(x[i][j], wave_col<VEC>(c0, i, j, lane));
-          n += __builtin_popcountll(mask);
-        }
-      }
-      n = min(n, end);
+  return bits;
+}
+// the columns marked in `bits` become keys from place n on (those before `cap`); their values are read again (a register cannot be
+// indexed by a lane).  Returns the place behind the last.
+template <typename T, typename Place>
+__device__ __forceinline__ void collect(uint32_t bits, const T* row, int c0, int lane, u64* cand, int cap, Place place) {
+  for (u64 mask = __ballot(bits != 0); mask; mask = __ballot(bits != 0)) {
+    const int at = place(mask);
+    if (bits) {
+      const int e = __builtin_clz(bits), c = c0 + (e >> 3) * 512 + lane * 8 + (e & 7);
+      bits &= ~(0x80000000u >> e);
+      if (at < cap) cand[at] = top_key((float)row[c], c);
     }
   }
-  if (lane < 2) cand[n + lane] = 0;
-  if (lane < k) list[lane] = 0;
-  wave_fence();
-  for (int s = 0; s < n; s += 64) {
-    const u64 key = s + lane < n ? cand[s + lane] : 0;
+}
+// columns equal to thr, lowest classes first, become keys from place n on, up to `end`; first: ties of earlier waves.  Returns n + ties.
+__device__ __forceinline__ int collect_ties(const float (&x)[NV][8], float thr, int c0, int lane, u64* cand, int n, int end) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    int mine = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) mine += x[i][j] == thr;
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int v = __shfl_up(upto, o, 64);
+      if (lane >= o) upto += v;
+    }
+    int at = n + upto - mine;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (x[i][j] == thr) {
+        if (at < end) cand[at] = top_key(x[i][j], c0 + i * 512 + lane * 8 + j);
+        ++at;
+      }
+    n += __shfl(upto, 63, 64);
+  }
+  return n;
+}
+// f(rank, key) for the keys of rank < k among n distinct ones (cand[n] and cand[n + 1] writable): ranked by counting
+template <typename F>
+__device__ __forceinline__ void rank_keys(u64* cand, int n, int k, int thread, int threads, F f) {
+  for (int s = thread; s < n; s += threads) {
+    const u64 key = cand[s];
     int r = 0;
     for (int j = 0; j < n; j += 2) r += (cand[j] > key) + (cand[j + 1] > key);
-    if (s + lane < n && r < k) list[r] = key;
+    if (r < k) f(r, key);
   }
+}
+constexpr int WAVE_CAND = 64 * 8 + 64, WAVE_TOP_LDS = WAVE_CAND + 2;      // one wave: groups of 8 columns (exact)
+constexpr int GROUP_CAND = 64 * 32 + 64;                                  // a workgroup: a lane's 32 columns are a group
+// one wave: f(rank, key) of its k best; returns how many there are (<= k)
+template <typename T, typename F>
+__device__ __forceinline__ int wave_top(const float (&x)[NV][8], const float (&vmax)[NV], const T* row, int c0, int cend, int k, int lane, u64* cand,
+                                        F f) {
+  uint32_t g[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) g[i] = ord(vmax[i]);
+  float thr;
+  if (k <= 32) {          // groups of a lane's 32 columns: one ballot a bit
+    const uint32_t one[1] = {max(max(g[0], g[1]), max(g[2], g[3]))};
+    thr = group_threshold<1>(one, 1, k, true);
+  } else {                // of 8 columns: with 64 groups the least of them would have to do
+    thr = group_threshold<NV>(g, NV, k, true);
+  }
+  int n = 0;
+  auto next = [&](u64 mask) { const int at = n + lanes_below(mask); n += __builtin_popcountll(mask); return at; };
+  collect<T>(reached<false>(x, thr, c0, cend), row, c0, lane, cand, WAVE_CAND, next);
+  if (n > WAVE_CAND) {
+    thr = group_threshold<NV>(g, NV, k, false);
+    n = 0;
+    collect<T>(reached<true>(x, thr, c0, cend), row, c0, lane, cand, WAVE_CAND, next);
+    const int end = max(n, k);
+    n = min(end, collect_ties(x, thr, c0, lane, cand, n, end));
+  }
+  if (lane < 2) cand[n + lane] = 0;
   wave_fence();
+  rank_keys(cand, n, k, lane, 64, f);
   return min(n, k);
 }
 // place of list w's entry r among `lists` sorted lists of k (stride in u64): its own, and in each other one those above it
@@ -250,11 +265,13 @@ __device__ __forceinline__ void write_top(const ScoreParams& p, int64_t row, int
   p.top_logp[row * p.k + r] = have ? (unord((uint32_t)(key >> 32)) - a.m) * p.inv_t - __builtin_amdgcn_logf(a.z) * LN2 : nan ? a.z : -INFINITY;
 }
 
-// MULTI false: a wave per row, four rows a workgroup, no barrier.  MULTI: a workgroup per segment of a row.
-template <typename T, bool VEC, bool MULTI>
+// MULTI false: a wave per row, four rows a workgroup, no barrier.  MULTI: a workgroup per segment of a row; its alternatives come from one
+// threshold over all its lanes (with a list per wave, 64 alternatives of 100003 classes took 570 us instead of TOPTIME).
+template <typename T, bool MULTI>
 __global__ __launch_bounds__(MULTI ? 1024 : 256) void token_logprobs_fwd_kernel(ScoreParams p) {
   extern __shared__ __attribute__((aligned(16))) u64 score_lds[];
-  __shared__ RowSums sm[MAX_WAVES];
+  __shared__ RowSums sm[MULTI ? MAX_WAVES : 1];
+  __shared__ int sm_n[MAX_WAVES + 2];    // ties of each wave; [MAX_WAVES]: keys so far; [MAX_WAVES + 1]: the threshold's bits
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t unit = MULTI ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
   const int64_t row = MULTI ? blockIdx.x / (unsigned)p.sp.nseg : unit;
@@ -268,17 +285,17 @@ __global__ __launch_bounds__(MULTI ? 1024 : 256) void token_logprobs_fwd_kernel(
   const int c0 = MULTI ? seg * p.sp.seg + wave * p.sp.wave_cols : 0, cend = MULTI ? min(send, c0 + p.sp.wave_cols) : p.C;
   const float c = p.inv_t * LOG2E;
   float x[NV][8], vmax[NV];
-  load_wave<T, VEC>(lr, c0, cend, lane, x);
-  float m = -FMAX;
+  load_wave<T>(lr, c0, cend, lane, x);
+  float m = -FMAX, lmax = -INFINITY;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     vmax[i] = -INFINITY;
 #pragma unroll
     for (int j = 0; j < 8; ++j) vmax[i] = fmaxf(vmax[i], x[i][j]);
-    m = fmaxf(m, vmax[i]);
+    lmax = fmaxf(lmax, vmax[i]);
   }
   RowSums a;
-  a.m = wave_max(m);
+  a.m = wave_max(fmaxf(m, lmax));
   a.z = a.s = 0.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i)
@@ -292,17 +309,21 @@ __global__ __launch_bounds__(MULTI ? 1024 : 256) void token_logprobs_fwd_kernel(
       }
   a.z = wave_sum(a.z);
   a.s = wave_sum(a.s);
-  u64* cand = score_lds + (p.k ? wave * TOP_LDS : 0);
-  u64* list = cand + TOP_CAND + 2;
-  if (p.k) wave_top<VEC>(x, vmax, c0, cend, p.k, lane, cand);
   if (!MULTI) {
     if (lane == 0) write_row(p, row, a, given, xt);
-    if (lane < p.k) write_top(p, row, lane, list[lane], a);
+    if (p.k) {
+      const int have = wave_top<T>(x, vmax, lr, c0, cend, p.k, lane, score_lds + wave * WAVE_TOP_LDS, [&](int r, u64 key) { write_top(p, row, r, key, a); });
+      if (lane >= have && lane < p.k) write_top(p, row, lane, 0, a);
+    }
     return;
   }
-  if (lane == 0) sm[wave] = a;
-  __syncthreads();
   const int nw = p.sp.waves;
+  u64* cand = score_lds;                                                       // [GROUP_CAND + 2]
+  uint32_t* gmax = reinterpret_cast<uint32_t*>(score_lds + GROUP_CAND + 2);    // [nw][64]
+  if (lane == 0) sm[wave] = a;
+  if (p.k) gmax[threadIdx.x] = ord(lmax);
+  if (threadIdx.x == 0) sm_n[MAX_WAVES] = 0;
+  __syncthreads();
   RowSums b = {sm[0].m, 0.f, 0.f};
   for (int w = 1; w < nw; ++w) b.m = fmaxf(b.m, sm[w].m);
   for (int w = 0; w < nw; ++w) add_sums(b, sm[w].m, sm[w].z, sm[w].s, b.m, c);
@@ -311,22 +332,55 @@ __global__ __launch_bounds__(MULTI ? 1024 : 256) void token_logprobs_fwd_kernel(
     if (whole) write_row(p, row, b, given, xt);
     else p.part[unit] = make_float4(b.m, b.z, b.s, 0.f);
   }
-  if (p.k) {   // one entry of a wave's list per lane; places behind the last entry of all lists stay empty
-    u64* lists = score_lds + TOP_CAND + 2;
-    int have = 0;
-    for (int w = 0; w < nw; ++w) have += __builtin_popcountll(__ballot(lane < p.k && lists[w * TOP_LDS + lane] != 0));
-    const u64 key = lane < p.k ? list[lane] : 0;
-    if (key) {
-      const int r = merged_rank(lists, TOP_LDS, nw, wave, lane, p.k, key);
-      if (r < p.k) {
-        if (whole) write_top(p, row, r, key, b);
-        else p.part_key[unit * p.k + r] = key;
-      }
+  if (!p.k) return;
+  if (wave == 0) {
+    uint32_t g[MAX_WAVES];
+#pragma unroll
+    for (int w = 0; w < MAX_WAVES; ++w) g[w] = w < nw ? gmax[w * 64 + lane] : 0;
+    const float thr = group_threshold<MAX_WAVES>(g, nw, p.k, true);
+    if (lane == 0) sm_n[MAX_WAVES + 1] = __builtin_bit_cast(int, thr);
+  }
+  __syncthreads();
+  const float thr = __builtin_bit_cast(float, sm_n[MAX_WAVES + 1]);
+  auto next = [&](u64 mask) {
+    int base = 0;
+    if (lane == 0) base = atomicAdd(&sm_n[MAX_WAVES], __builtin_popcountll(mask));
+    return __builtin_amdgcn_readfirstlane(base) + lanes_below(mask);
+  };
+  if (__any(lmax >= thr)) collect<T>(reached<false>(x, thr, c0, cend), lr, c0, lane, cand, GROUP_CAND, next);
+  __syncthreads();
+  int n = sm_n[MAX_WAVES];
+  if (n > GROUP_CAND) {   // values repeat at the threshold (the k-th group's own then: exactly k groups hold no more than GROUP_CAND)
+    int ties = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ties += __builtin_popcountll(__ballot(x[i][j] == thr));
+    __syncthreads();
+    if (threadIdx.x == 0) sm_n[MAX_WAVES] = 0;
+    if (lane == 0) sm_n[wave] = ties;
+    __syncthreads();
+    collect<T>(reached<true>(x, thr, c0, cend), lr, c0, lane, cand, GROUP_CAND, next);
+    __syncthreads();
+    n = sm_n[MAX_WAVES];
+    const int end = max(n, p.k);
+    int all = n, mine = n;
+    for (int w = 0; w < nw; ++w) {
+      if (w < wave) mine += sm_n[w];
+      all += sm_n[w];
     }
-    if (wave == 0 && lane >= have && lane < p.k) {
-      if (whole) write_top(p, row, lane, 0, b);
-      else p.part_key[unit * p.k + lane] = 0;
-    }
+    if (mine < end) collect_ties(x, thr, c0, lane, cand, mine, end);
+    n = min(all, end);
+  }
+  if (threadIdx.x < 2) cand[n + threadIdx.x] = 0;
+  __syncthreads();
+  rank_keys(cand, n, p.k, threadIdx.x, 64 * nw, [&](int r, u64 key) {
+    if (whole) write_top(p, row, r, key, b);
+    else p.part_key[unit * p.k + r] = key;
+  });
+  for (int r = n + threadIdx.x; r < p.k; r += 64 * nw) {
+    if (whole) write_top(p, row, r, 0, b);
+    else p.part_key[unit * p.k + r] = 0;
   }
 }
 
@@ -371,80 +425,42 @@ __device__ __forceinline__ void split_id(int64_t n, int d, int64_t& q, int& r) {
 }
 
 // ---- gradient of the log-probabilities: one thread per 8 columns, everything of the row is known -------------------------
-template <typename T> __device__ __forceinline__ void store8(T* p, const float (&v)[8]);
-template <> __device__ __forceinline__ void store8<bf16>(bf16* p, const float (&v)[8]) {
-  bf16x8 r;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) r[j] = (bf16)v[j];
-  *reinterpret_cast<bf16x8*>(p) = r;
-}
-template <> __device__ __forceinline__ void store8<_Float16>(_Float16* p, const float (&v)[8]) {
-  f16x8 r;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) r[j] = (_Float16)v[j];
-  *reinterpret_cast<f16x8*>(p) = r;
-}
-template <> __device__ __forceinline__ void store8<float>(float* p, const float (&v)[8]) {
-  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-  *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
-}
-
 struct ScoreGradParams {
   const void* logits; int64_t ldl;
   const int64_t* tokens;
   const float *stats, *entropy, *g_logp, *g_entropy;
   void* dlogits; int64_t ldd;
-  int C, Cd, per_row;   // per_row: 8-column pieces (aligned) or 512-column pieces (others) of a row
+  int C, Cd, per_row;   // per_row: 8-column pieces of a row
   int64_t pieces;
   float inv_t;
 };
-template <typename T, bool VEC>
+template <typename T>
 __global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(ScoreGradParams p) {
-  const int64_t id = VEC ? (int64_t)blockIdx.x * 256 + threadIdx.x : (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (id >= p.pieces) return;
   int64_t row;
   int piece;
   split_id(id, p.per_row, row, piece);
-  const int first = piece * (VEC ? 8 : 512) + (VEC ? 0 : (threadIdx.x & 63)), step = VEC ? 1 : 64;
-  const T* x = (const T*)p.logits + row * p.ldl;
-  T* d = (T*)p.dlogits + row * p.ldd;
+  const int first = piece * 8;
   float v[8];
-  if (VEC) {
-    if (first < p.C) load8<T>(x + first, p.C - first, v);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = first + 64 * j < p.C ? (float)x[first + 64 * j] : 0.f;
-  }
+  if (first < p.C) load8<T>((const T*)p.logits + row * p.ldl + first, p.C - first, v);
   const float m = p.stats[2 * row], logz = p.stats[2 * row + 1], H = p.entropy[row];
   const int64_t tok = p.tokens[row];
   const bool given = tok >= 0 && tok < p.C;
   const float gl = given ? p.g_logp[row] : 0.f, gh = p.g_entropy ? p.g_entropy[row] : 0.f;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const int col = first + step * j;
     float g = 0.f;
-    if (col < p.C && m != -INFINITY) {
+    if (first + j < p.C && m != -INFINITY) {
       const float y = (v[j] - m) * p.inv_t - logz;
       const float q = __builtin_amdgcn_exp2f(y * LOG2E);
       g = q == 0.f ? 0.f : -q * (gl + gh * (y + H));
-      if (given && col == (int)tok) g += gl;
+      if (given && first + j == (int)tok) g += gl;
       g *= p.inv_t;
     }
     v[j] = g;
   }
-  if (VEC) {
-    if (first + 8 <= p.Cd) {
-      store8<T>(d + first, v);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (first + j < p.Cd) d[first + j] = (T)v[j];
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (first + 64 * j < p.Cd) d[first + 64 * j] = (T)v[j];
-  }
+  store8<T>((T*)p.dlogits + row * p.ldd + first, p.Cd - first, v);
 }
 
 // ---- distillation ---------------------------------------------------------------------------------------------------------
@@ -527,7 +543,7 @@ __device__ __forceinline__ void listed_logits(const T* row, const Listed& L, flo
 }
 
 // as token_logprobs_fwd_kernel; with tail each wave marks the listed classes of its columns in a bit map of its own
-template <typename T, bool VEC, bool MULTI>
+template <typename T, bool MULTI>
 __global__ __launch_bounds__(MULTI ? 1024 : 256) void distill_fwd_kernel(DistillParams p) {
   __shared__ uint32_t marks[MULTI ? MAX_WAVES : 4][WAVE_COLS / 32];
   __shared__ RowSums sm[MAX_WAVES];
@@ -541,7 +557,7 @@ __global__ __launch_bounds__(MULTI ? 1024 : 256) void distill_fwd_kernel(Distill
   const int c0 = MULTI ? seg * p.sp.seg + wave * p.sp.wave_cols : 0, cend = MULTI ? min(send, c0 + p.sp.wave_cols) : p.C;
   const float c = p.inv_t * LOG2E;
   float x[NV][8];
-  load_wave<T, VEC>(lr, c0, cend, lane, x);
+  load_wave<T>(lr, c0, cend, lane, x);
   const bool first = wave == 0 || !MULTI, whole = !MULTI || p.sp.nseg == 1;
   Listed L;
   float xl[2] = {0.f, 0.f};
@@ -565,20 +581,28 @@ __global__ __launch_bounds__(MULTI ? 1024 : 256) void distill_fwd_kernel(Distill
     for (int j = 0; j < 8; ++j) m = fmaxf(m, x[i][j]);
   m = wave_max(m);
   float zl = 0.f, zr = 0.f;
+  if (p.tail) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    if (c0 + i * 512 >= cend) break;
-    const uint32_t bits = p.tail && VEC ? reinterpret_cast<const uint8_t*>(mark)[i * 64 + lane] : 0u;
+    for (int i = 0; i < NV; ++i) {
+      if (c0 + i * 512 >= cend) break;
+      const uint32_t bits = reinterpret_cast<const uint8_t*>(mark)[i * 64 + lane];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float e = __builtin_amdgcn_exp2f((x[i][j] - m) * c);
-      bool hit = false;
-      if (p.tail) hit = VEC ? (bits >> j) & 1u : (mark[i * 16 + j * 2 + (lane >> 5)] >> (lane & 31)) & 1u;
-      zl += hit ? e : 0.f;
-      zr += hit ? 0.f : e;
+      for (int j = 0; j < 8; ++j) {
+        const float e = __builtin_amdgcn_exp2f((x[i][j] - m) * c);
+        const bool hit = (bits >> j) & 1u;
+        zl += hit ? e : 0.f;
+        zr += hit ? 0.f : e;
+      }
+    }
+    zl = wave_sum(zl);
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (c0 + i * 512 >= cend) break;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) zr += __builtin_amdgcn_exp2f((x[i][j] - m) * c);
     }
   }
-  zl = wave_sum(zl);
   zr = wave_sum(zr);
   if (!MULTI) {
     finish_distill(p, row, L, xl, m, zl, zr, lane);
@@ -621,14 +645,15 @@ struct DistillGradParams {
   int64_t units;
   float inv_t;
 };
-// A wave on its own takes up to 2048 columns of a row.  A byte map of them in LDS names the list's entry (+ 1) of each class; of a class
-// named twice one entry's number stands there, and that entry's p becomes the sum, added in the list's order.  With
-// q = softmax(y) and w = (listed / other mass of the student), d / dy = q (mass - left w) on other classes (left the mass that the
-// list leaves out; 0 without tail) and q (mass + left) - p on the listed ones: one exponential per class.
-template <typename T, bool VEC>
+// A wave on its own takes up to 2048 columns of a row.  With q = softmax(y) and w = (listed / other mass of the student),
+//   d / dy = q (mass - left w) on the classes that the list does not name (left: the mass it leaves out; 0 without tail)
+//          = q (mass + left) - p on those it names:
+// one exponential a class by the first form, then the few named ones again by the second, each by the lane that holds its entry (whose
+// logit, and what is accumulated to, is fetched beside the row; a wave's own stores to one address stay in order).  Entries that
+// name one class find out by leaving their number at its place in LDS: each then writes the sum of their p, in the list's order.
+template <typename T>
 __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillGradParams p) {
-  __shared__ uint32_t maps[4][WAVE_COLS / 4];
-  __shared__ float ps[4][TTTS_DISTILL_MAX_K + 1];
+  __shared__ uint8_t tags[4][WAVE_COLS];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t unit = (int64_t)blockIdx.x * 4 + wave;
   if (unit >= p.units) return;
@@ -639,26 +664,25 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillGradParams p) {
   const T* lr = (const T*)p.logits + row * p.ldl;
   T* dr = (T*)p.dlogits + row * p.ldd;
   float x[NV][8];
-  load_wave<T, VEC>(lr, c0, cend, lane, x);
-  uint32_t* map = maps[wave];
-  uint8_t* map8 = reinterpret_cast<uint8_t*>(map);
-  float* pl = ps[wave];
-#pragma unroll
-  for (int i = 0; i < WAVE_COLS / 4 / 64; ++i) map[i * 64 + lane] = 0;
-  const Listed L = load_listed(p.idx + row * p.K, p.tlogp + row * p.K, p.K, p.C, p.inv_t, p.tail, lane);
+  load_wave<T>(lr, c0, cend, lane, x);
+  Listed L = load_listed(p.idx + row * p.K, p.tlogp + row * p.K, p.K, p.C, p.inv_t, p.tail, lane);
   const float m = p.stats[3 * row], logz = p.stats[3 * row + 1], w = p.stats[3 * row + 2], g = p.g_loss[row] * p.inv_t;
-  wave_fence();
+  uint8_t* tag = tags[wave];
   bool here[2];
+  float xl[2] = {0.f, 0.f}, old[2] = {0.f, 0.f};
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     here[h] = L.id[h] >= c0 && L.id[h] < cend;
-    if (here[h]) map8[L.id[h] - c0] = (uint8_t)(lane + 64 * h + 1);
-    pl[lane + 64 * h] = L.p[h];
+    if (here[h]) {
+      tag[L.id[h] - c0] = (uint8_t)(lane + 64 * h);
+      xl[h] = (float)lr[L.id[h]];
+      if (p.accumulate) old[h] = (float)dr[L.id[h]];
+    }
   }
   wave_fence();
   bool twice = false;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) twice |= here[h] && map8[L.id[h] - c0] != (uint8_t)(lane + 64 * h + 1);
+  for (int h = 0; h < 2; ++h) twice |= here[h] && tag[L.id[h] - c0] != (uint8_t)(lane + 64 * h);
   if (__any(twice)) {
     float sum[2] = {0.f, 0.f};
     for (int j = 0; j < p.K; ++j) {
@@ -667,46 +691,43 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillGradParams p) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) sum[h] += idj == L.id[h] ? pj : 0.f;
     }
-    wave_fence();
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      if (here[h]) pl[lane + 64 * h] = sum[h];
+    L.p[0] = sum[0];
+    L.p[1] = sum[1];
   }
-  wave_fence();
   const bool held = p.tail && w < INFINITY;          // other classes than the listed ones hold something
   const float left = held ? fmaxf(1.f - L.mass, 0.f) : 0.f;
-  const float on = L.mass + left, off = left > 0.f ? L.mass - left * w : L.mass;
+  const bool none = m == -INFINITY;                  // every class at -inf: no gradient
+  const float on = L.mass + left, off = (left > 0.f ? L.mass - left * w : L.mass) * g;
+  const float c = p.inv_t * LOG2E, log2z = logz * LOG2E;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
+    const int first = c0 + i * 512 + lane * 8;
     if (c0 + i * 512 >= dend) break;
-    uint2 marks = make_uint2(0u, 0u);
-    if (VEC) marks = *reinterpret_cast<const uint2*>(map8 + i * 512 + lane * 8);
     float d[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float q = __builtin_amdgcn_exp2f(((x[i][j] - m) * p.inv_t - logz) * LOG2E);
-      const uint32_t e = VEC ? ((j < 4 ? marks.x : marks.y) >> (8 * (j & 3))) & 255u : map8[i * 512 + j * 64 + lane];
-      d[j] = e ? fmaf(q, on, -pl[e - 1]) : q * off;
-      d[j] = wave_col<VEC>(c0, i, j, lane) < p.C && m != -INFINITY ? d[j] * g : 0.f;
+    for (int j = 0; j < 8; ++j) d[j] = __builtin_amdgcn_exp2f((x[i][j] - m) * c - log2z) * off;
+    if (none || c0 + i * 512 + 512 > p.C) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) d[j] = first + j < p.C && !none ? d[j] : 0.f;
     }
-    if (VEC && !p.accumulate && c0 + i * 512 + lane * 8 + 8 <= dend) {
-      store8<T>(dr + c0 + i * 512 + lane * 8, d);
-    } else if (VEC && p.accumulate && c0 + i * 512 + lane * 8 + 8 <= cend) {
+    const int n = (p.accumulate ? cend : dend) - first;
+    if (n <= 0) continue;
+    if (p.accumulate) {
       float o[8];
-      T* at = dr + c0 + i * 512 + lane * 8;
-      load8<T>(at, 8, o);
+      load8<T>(dr + first, n, o);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) o[j] += d[j];
-      store8<T>(at, o);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int col = wave_col<VEC>(c0, i, j, lane);
-        if (p.accumulate) { if (col < cend) dr[col] = (T)((float)dr[col] + d[j]); }
-        else if (col < dend) dr[col] = (T)d[j];
-      }
+      for (int j = 0; j < 8; ++j) d[j] += o[j];
     }
+    store8<T>(dr + first, n, d);
   }
+  wave_fence();
+  if (none) return;
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    if (here[h]) {
+      const float q = __builtin_amdgcn_exp2f((xl[h] - m) * c - log2z);
+      dr[L.id[h]] = (T)(old[h] + fmaf(q, on, -L.p[h]) * g);
+    }
 }
 
 // run F<T> for the logits' type
@@ -733,8 +754,6 @@ static int check_logits(const char* what, const void* logits, int32_t dtype, int
   return TTTS_OK;
 }
 
-// rows whose addresses are all multiples of 16 bytes
-static bool rows16(const void* p, int64_t ld, int32_t dtype) { return aligned16(p) && (ld * (dtype == TTTS_DTYPE_F32 ? 4 : 2)) % 16 == 0; }
 static int need_workspace(const char* what, int64_t need, const void* ws, int64_t have) {
   TTTS_REQUIRE(need == 0 || (ws && have >= need && aligned16(ws)), "%s: needs a 16-byte aligned workspace of %lld bytes", what, (long long)need);
   return TTTS_OK;
@@ -750,20 +769,17 @@ extern "C" int64_t ttts_token_logprobs_workspace_bytes(int32_t R, int32_t C, int
   return sp.nseg > 1 ? cdiv((int64_t)R * sp.nseg * (16 + 8 * (int64_t)top_k), 16) * 16 : 0;
 }
 
-template <typename T, bool VEC>
+template <typename T>
 static int launch_score(const ScoreParams& p, hipStream_t st) {
   const char* what = "token_logprobs_fwd";
   if (p.sp.nseg == 1 && p.sp.waves == 1) {
-    token_logprobs_fwd_kernel<T, VEC, false><<<(unsigned)cdiv(p.R, 4), 256, p.k ? 4 * TOP_LDS * 8 : 0, st>>>(p);
+    token_logprobs_fwd_kernel<T, false><<<(unsigned)cdiv(p.R, 4), 256, p.k ? 4 * WAVE_TOP_LDS * 8 : 0, st>>>(p);
     return check_launch(what);
   }
-  static OnceFlag once;
-  if (lds_opt_in(once, (const void*)token_logprobs_fwd_kernel<T, VEC, true>, MAX_WAVES * TOP_LDS * 8) != hipSuccess)
-    return fail(TTTS_EHIP, "%s: LDS opt-in failed", what);
   const int64_t grid = (int64_t)p.R * p.sp.nseg;
   int rc = need_grid(what, grid);
   if (rc) return rc;
-  token_logprobs_fwd_kernel<T, VEC, true><<<(unsigned)grid, 64 * p.sp.waves, p.k ? p.sp.waves * TOP_LDS * 8 : 0, st>>>(p);
+  token_logprobs_fwd_kernel<T, true><<<(unsigned)grid, 64 * p.sp.waves, p.k ? (GROUP_CAND + 2) * 8 + p.sp.waves * 64 * 4 : 0, st>>>(p);
   rc = check_launch(what);
   if (rc || p.sp.nseg == 1) return rc;
   token_logprobs_join_kernel<T><<<p.R, 256, p.sp.nseg * p.k * 8, st>>>(p);
@@ -782,9 +798,7 @@ extern "C" int ttts_token_logprobs_fwd(const void* logits, int32_t dtype, int64_
   if (rc) return rc;
   ScoreParams p{logits, ldl, tokens, logp, entropy, stats, top_logp, top_idx, (float4*)workspace, nullptr, R, C, top_k, 1.0f / temperature, split_row(C)};
   p.part_key = (u64*)(p.part + (int64_t)R * p.sp.nseg);
-  const bool vec = rows16(logits, ldl, dtype);
-  hipStream_t st = as_stream(stream);
-  TTTS_BY_TYPE(dtype, "token_logprobs_fwd", rc = (vec ? launch_score<T, true>(p, st) : launch_score<T, false>(p, st)));
+  TTTS_BY_TYPE(dtype, "token_logprobs_fwd", rc = launch_score<T>(p, as_stream(stream)));
   return rc;
 }
 
@@ -796,16 +810,12 @@ extern "C" int ttts_token_logprobs_bwd(const void* logits, int32_t dtype, int64_
   TTTS_REQUIRE(Cd >= C && ldd >= Cd, "token_logprobs_bwd: need C <= Cd <= ldd");
   if (R == 0) return TTTS_OK;
   TTTS_REQUIRE(tokens && stats && entropy && g_logp && dlogits, "token_logprobs_bwd: null pointer");
-  const bool vec = rows16(logits, ldl, dtype) && rows16(dlogits, ldd, dtype);
-  ScoreGradParams p{logits, ldl, tokens, stats, entropy, g_logp, g_entropy, dlogits, ldd, C, Cd, (int)cdiv(Cd, vec ? 8 : 512), 0, 1.0f / temperature};
-  p.pieces = (int64_t)R * p.per_row;
-  const int64_t grid = cdiv(p.pieces, vec ? 256 : 4);
+  const int per_row = (int)cdiv(Cd, 8);
+  const ScoreGradParams p{logits, ldl, tokens, stats, entropy, g_logp, g_entropy, dlogits, ldd, C, Cd, per_row, (int64_t)R * per_row, 1.0f / temperature};
+  const int64_t grid = cdiv(p.pieces, 256);
   rc = need_grid("token_logprobs_bwd", grid);
   if (rc) return rc;
-  if (vec)
-    TTTS_BY_TYPE(dtype, "token_logprobs_bwd", (token_logprobs_bwd_kernel<T, true><<<(unsigned)grid, 256, 0, as_stream(stream)>>>(p)))
-  else
-    TTTS_BY_TYPE(dtype, "token_logprobs_bwd", (token_logprobs_bwd_kernel<T, false><<<(unsigned)grid, 256, 0, as_stream(stream)>>>(p)))
+  TTTS_BY_TYPE(dtype, "token_logprobs_bwd", (token_logprobs_bwd_kernel<T><<<(unsigned)grid, 256, 0, as_stream(stream)>>>(p)));
   return check_launch("token_logprobs_bwd");
 }
 
@@ -815,17 +825,17 @@ extern "C" int64_t ttts_distill_workspace_bytes(int32_t R, int32_t C) {
   return sp.nseg > 1 ? (int64_t)R * sp.nseg * 16 : 0;
 }
 
-template <typename T, bool VEC>
+template <typename T>
 static int launch_distill(const DistillParams& p, hipStream_t st) {
   const char* what = "distill_fwd";
   if (p.sp.nseg == 1 && p.sp.waves == 1) {
-    distill_fwd_kernel<T, VEC, false><<<(unsigned)cdiv(p.R, 4), 256, 0, st>>>(p);
+    distill_fwd_kernel<T, false><<<(unsigned)cdiv(p.R, 4), 256, 0, st>>>(p);
     return check_launch(what);
   }
   const int64_t grid = (int64_t)p.R * p.sp.nseg;
   int rc = need_grid(what, grid);
   if (rc) return rc;
-  distill_fwd_kernel<T, VEC, true><<<(unsigned)grid, 64 * p.sp.waves, 0, st>>>(p);
+  distill_fwd_kernel<T, true><<<(unsigned)grid, 64 * p.sp.waves, 0, st>>>(p);
   rc = check_launch(what);
   if (rc || p.sp.nseg == 1) return rc;
   distill_join_kernel<T><<<(unsigned)cdiv(p.R, 4), 256, 0, st>>>(p);
@@ -843,9 +853,7 @@ extern "C" int ttts_distill_fwd(const void* logits, int32_t dtype, int64_t ldl, 
   rc = need_workspace("distill_fwd", ttts_distill_workspace_bytes(R, C), workspace, workspace_bytes);
   if (rc) return rc;
   const DistillParams p{logits, ldl, teacher_idx, teacher_logp, row_loss, stats, (float4*)workspace, R, C, K, tail != 0, 1.0f / temperature, split_row(C)};
-  const bool vec = rows16(logits, ldl, dtype);
-  hipStream_t st = as_stream(stream);
-  TTTS_BY_TYPE(dtype, "distill_fwd", rc = (vec ? launch_distill<T, true>(p, st) : launch_distill<T, false>(p, st)));
+  TTTS_BY_TYPE(dtype, "distill_fwd", rc = launch_distill<T>(p, as_stream(stream)));
   return rc;
 }
 
@@ -858,18 +866,14 @@ extern "C" int ttts_distill_bwd(const void* logits, int32_t dtype, int64_t ldl, 
   TTTS_REQUIRE(Cd >= C && ldd >= Cd, "distill_bwd: need C <= Cd <= ldd");
   if (R == 0) return TTTS_OK;
   TTTS_REQUIRE(teacher_idx && teacher_logp && stats && g_loss && dlogits, "distill_bwd: null pointer");
-  const bool vec = rows16(logits, ldl, dtype) && rows16(dlogits, ldd, dtype);
   DistillGradParams p{logits, ldl, teacher_idx, teacher_logp, stats, g_loss, dlogits, ldd, C, Cd, K, tail != 0, accumulate != 0, 0, 0, 0, 1.0f / temperature};
   p.per_row = (int)cdiv(Cd, WAVE_COLS);
-  p.wave_cols = (int)cdiv(cdiv(Cd, p.per_row), 8) * 8;
+  p.wave_cols = (int)cdiv(cdiv(Cd, 512), p.per_row) * 512;
   p.per_row = (int)cdiv(Cd, p.wave_cols);
   p.units = (int64_t)R * p.per_row;
   const int64_t grid = cdiv(p.units, 4);
   rc = need_grid("distill_bwd", grid);
   if (rc) return rc;
-  if (vec)
-    TTTS_BY_TYPE(dtype, "distill_bwd", (distill_bwd_kernel<T, true><<<(unsigned)grid, 256, 0, as_stream(stream)>>>(p)))
-  else
-    TTTS_BY_TYPE(dtype, "distill_bwd", (distill_bwd_kernel<T, false><<<(unsigned)grid, 256, 0, as_stream(stream)>>>(p)))
+  TTTS_BY_TYPE(dtype, "distill_bwd", (distill_bwd_kernel<T><<<(unsigned)grid, 256, 0, as_stream(stream)>>>(p)));
   return check_launch("distill_bwd");
 }

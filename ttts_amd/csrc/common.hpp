@@ -121,6 +121,35 @@ __device__ __forceinline__ float wave_max(float v) {
   return v;
 }
 
+// The same without LDS traffic (register swaps and DPP instead of ds_bpermute), for any operation; every lane gets the result.
+//   over_rows: over the four lanes l & 15 of the wave's rows of 16;  over_wave: over all 64.
+template <typename F>
+__device__ __forceinline__ float over_rows(float x, F op) {
+  const unsigned u = __builtin_bit_cast(unsigned, x);
+  const auto h = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const unsigned h0 = h[0], h1 = h[1];   // (scalars of their own: a bit_cast of a vector's element reads element 0)
+  const unsigned v = __builtin_bit_cast(unsigned, op(__builtin_bit_cast(float, h0), __builtin_bit_cast(float, h1)));
+  const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  const unsigned r0 = r[0], r1 = r[1];
+  return op(__builtin_bit_cast(float, r0), __builtin_bit_cast(float, r1));
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp_mov(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, false));
+}
+template <typename F>
+__device__ __forceinline__ float over_wave(float x, F op) {
+  x = op(x, dpp_mov<0x128>(x));   // row_ror 8, 4, 2, 1: every lane of a row of 16 has the row's result
+  x = op(x, dpp_mov<0x124>(x));
+  x = op(x, dpp_mov<0x122>(x));
+  x = op(x, dpp_mov<0x121>(x));
+  return over_rows(x, op);
+}
+struct AddOp { __device__ __forceinline__ float operator()(float a, float b) const { return a + b; } };
+struct MaxOp { __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); } };
+constexpr AddOp add_op{};
+constexpr MaxOp max_op{};
+
 // LayerNorm row arithmetic shared by ln_fwd_kernel (elementwise.hip) and the fused residual-GEMM + LayerNorm kernel (gemm.hip): one
 // wave per row, a lane holds VPL float4 chunks.  Contraction is OFF in here so that both kernels form exactly the same roundings
 // whatever surrounds the call (the fused kernel's outputs are asserted bit-identical to the two-launch path).

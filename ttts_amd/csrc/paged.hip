@@ -43,18 +43,6 @@ template <> struct Frag<bf16> {
 template <> struct Frag<_Float16> {
   static __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
-// maximum / sum over the four lanes that hold one column (lane & 15): rows of 16 lanes, then halves, exchanged by register swaps
-template <typename F>
-__device__ __forceinline__ float over_rows(float x, F op) {
-  const unsigned u = __builtin_bit_cast(unsigned, x);
-  const auto h = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-  const unsigned h0 = h[0], h1 = h[1];   // (scalars of their own: a bit_cast of a vector's element reads element 0)
-  const unsigned v = __builtin_bit_cast(unsigned, op(__builtin_bit_cast(float, h0), __builtin_bit_cast(float, h1)));
-  const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-  const unsigned r0 = r[0], r1 = r[1];
-  return op(__builtin_bit_cast(float, r0), __builtin_bit_cast(float, r1));
-}
-
 // One workgroup = one chunk of keys of one (sequence, key / value head, 16 query rows); its waves take the chunk's 32-key tiles in turn,
 // each with a running maximum, sum and accumulator of its own, joined through LDS at the end.
 // A tile never touches LDS: both products are 16x16x32 MFMAs with the operand layout row = lane & 15, k = 8 (lane >> 4) ..+7,
@@ -154,7 +142,7 @@ __global__ __launch_bounds__(PAGED_WAVES * 64) void attn_paged_decode_kernel(Pag
         }
       }
       float mt = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
-      mt = over_rows(mt, [](float a, float b) { return fmaxf(a, b); });
+      mt = over_rows(mt, max_op);
       if (__any(mt > mx)) {
         const float mn = fmaxf(mx, mt), a = __builtin_amdgcn_exp2f(mx - mn);
         l *= a;
@@ -180,7 +168,7 @@ __global__ __launch_bounds__(PAGED_WAVES * 64) void attn_paged_decode_kernel(Pag
       cur = next;
     }
   }
-  l = over_rows(l, [](float a, float b) { return a + b; });
+  l = over_rows(l, add_op);
   // ---- join the waves
   float* sm_o = paged_lds;                       // [NW][rows][DH]
   float* sm_ml = paged_lds + NW * rows * DH;     // [NW][rows][2]

@@ -13,24 +13,14 @@ namespace ttts {
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f, FMAX = 3.402823466e38f;
 
 // ---- one wave = up to 2048 columns of a row, held in registers as fp32 -------------------------------------------------
-// A row is read ONCE: maximum, sums, and the alternatives all come from the registers.  Rows up to 2048 columns take one wave, up to 32768
-// one workgroup of up to 16 waves that meet in LDS, longer ones several workgroups (segments) and a second kernel that joins
-// their results.  A lane holds 8 neighbouring columns per load (16 or 32 bytes, at whatever alignment the row has; only the row's last
-// columns are read one by one), 64 lanes 512 neighbouring ones: x[i][j] is column c0 + 512 i + 8 lane + j.
-constexpr int NV = 4, WAVE_COLS = NV * 512, MAX_WAVES = 16, SEG_COLS = WAVE_COLS * MAX_WAVES;
-
-struct Split {   // columns of a row -> segments (workgroups) -> waves, in whole 512s: the fewest steps over all waves
-  int seg, nseg, waves, wave_cols;
-};
-static Split split_row(int C) {
-  Split s;
-  s.nseg = (int)cdiv(C, SEG_COLS);
-  s.seg = (int)cdiv(cdiv(C, 512), s.nseg) * 512;
-  s.nseg = (int)cdiv(C, s.seg);
-  s.waves = (int)cdiv(s.seg, WAVE_COLS);
-  s.wave_cols = (int)cdiv(s.seg / 512, s.waves) * 512;
-  return s;
-}
+// A row is read ONCE: maximum, sums, and the alternatives' threshold all come from the registers.  Rows up to 2048 columns take one wave;
+// longer ones a wave per 2048 columns, each on its own (a workgroup per row whose waves meet at barriers read 2.1 - 2.5 TB/s where
+// these read 4.4), and a second kernel that joins a row's parts.  A lane holds 8 neighbouring columns per load (16 or 32 bytes,
+// at whatever alignment the row has; only the row's last columns are read one by one), 64 lanes 512 neighbouring ones: x[i][j] is
+// column c0 + 512 i + 8 lane + j.
+constexpr int NV = 4, WAVE_COLS = NV * 512;
+__device__ __forceinline__ float sum_wave(float v) { return over_wave(v, add_op); }
+__device__ __forceinline__ float max_wave(float v) { return over_wave(v, max_op); }
 
 template <typename T> struct Eight { typedef T type __attribute__((ext_vector_type(8), aligned(sizeof(T)))); };   // 8 columns, aligned to T only
 template <typename T>
@@ -73,14 +63,25 @@ __device__ __forceinline__ void load_wave(const T* row, int c0, int cend, int la
   }
 }
 
-// e = 2^((x - m) c); t = (x - m) c kept finite (a class at -inf, or at the type's lowest value, has e = 0: e t must be 0, not NaN).
-// m is never -inf here (>= -FMAX), so -inf - m = -inf; NaN passes through e.  The difference comes first: lowest - lowest is 0.
-__device__ __forceinline__ float expo(float x, float m, float c, float& t) {
-  t = (x - m) * c;
-  const float e = __builtin_amdgcn_exp2f(t);
-  t = fmaxf(t, -200.f);
-  return e;
+// The exponent of a class from its row's (or wave's) maximum m >= -FMAX:  t = (x - m) c, in bits.  As fma(x, c, -m c) it is one
+// instruction and off by the one rounding of m c for the whole row, delta, which comes off the sums again; where m c is so large that
+// delta would matter (or not finite: a row of the type's lowest value) the difference is taken first.
+struct Exponent {
+  float m, c, mc, delta;
+  bool plain;   // uniform over the wave
+  __device__ __forceinline__ Exponent(float m_, float c_) : m(m_), c(c_) {
+    mc = m * c;
+    plain = fabsf(mc) <= 1048576.f;
+    delta = plain ? fmaf(m, c, -mc) : 0.f;
+  }
+  __device__ __forceinline__ float operator()(float x) const { return plain ? fmaf(x, c, -mc) : (x - m) * c; }
+};
+// (n / d, n % d) of a piece's number: in 32 bits where it fits (a 64-bit division costs as much as the piece's work)
+__device__ __forceinline__ void split_id(int64_t n, int d, int64_t& q, int& r) {
+  if ((uint64_t)n >> 32) { q = n / d; r = (int)(n % d); }
+  else { q = (uint32_t)n / (uint32_t)d; r = (int)((uint32_t)n % (uint32_t)d); }
 }
+
 __device__ __forceinline__ void wave_fence() {   // LDS written by this wave's lanes is read by its other lanes
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
@@ -215,26 +216,44 @@ __device__ __forceinline__ int wave_top(const float (&x)[NV][8], const float (&v
   rank_keys(cand, n, k, lane, 64, f);
   return min(n, k);
 }
-// place of list w's entry r among `lists` sorted lists of k (stride in u64): its own, and in each other one those above it
-__device__ __forceinline__ int merged_rank(const u64* base, int stride, int lists, int w, int r, int k, u64 key) {
-  int rank = r;
-  for (int o = 0; o < lists; ++o) {
-    if (o == w) continue;
-    const u64* l = base + o * stride;
-    int lo = 0, hi = k;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (l[mid] > key) lo = mid + 1; else hi = mid;
-    }
-    rank += lo;
-    if (rank >= k) break;
-  }
-  return rank;
-}
 
 struct RowSums { float m, z, s; };   // maximum, sum e, sum e t (t in bits, from the maximum)
-__device__ __forceinline__ void add_sums(RowSums& a, float m, float z, float s, float M, float c) {   // a's maximum is M already
-  const float d = fmaxf((m - M) * c, -200.f), f = __builtin_amdgcn_exp2f(d);
+// of one wave's columns
+template <int N>
+__device__ __forceinline__ RowSums wave_sums(const float (&x)[N][8], float lmax, int steps, float c) {
+  RowSums a;
+  a.m = max_wave(fmaxf(lmax, -FMAX));
+  a.z = a.s = 0.f;
+  const Exponent ex(a.m, c);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (i >= steps) break;
+    float least = x[i][0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) least = fminf(least, x[i][j]);
+    if (ex.plain && !__any(least < -1e30f)) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float t = fmaf(x[i][j], c, -ex.mc), e = __builtin_amdgcn_exp2f(t);
+        a.z += e;
+        a.s = fmaf(e, t, a.s);
+      }
+    } else {   // a class at -inf, or at the type's lowest value, has e = 0: e t must be 0, not NaN (a NaN passes through e)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float t = ex(x[i][j]), e = __builtin_amdgcn_exp2f(t);
+        a.z += e;
+        a.s = fmaf(e, fmaxf(t, -200.f), a.s);
+      }
+    }
+  }
+  const float f = __builtin_amdgcn_exp2f(-ex.delta);
+  a.z = sum_wave(a.z) * f;
+  a.s = sum_wave(a.s) * f - ex.delta * a.z;
+  return a;
+}
+__device__ __forceinline__ void add_sums(RowSums& a, float m, float z, float s, float c) {   // a.m is the row's maximum already
+  const float d = fmaxf((m - a.m) * c, -200.f), f = __builtin_amdgcn_exp2f(d);
   a.z += z * f;
   a.s += f * (s + z * d);
 }
@@ -244,11 +263,10 @@ struct ScoreParams {
   const int64_t* tokens;
   float *logp, *entropy, *stats, *top_logp;
   int64_t* top_idx;
-  float4* part;      // [R, nseg] (m, z, s, -) of the segments of a long row, and their sorted keys [R, nseg, k]
-  u64* part_key;
-  int R, C, k;
+  float4* part;          // long rows: [R, units] (m, z, s, -) of each wave's 2048 columns,
+  uint32_t* part_max;    // and with alternatives [R, units, 64]: ord() of the maximum of each lane's 32 columns
+  int R, C, k, units;
   float inv_t;
-  Split sp;
 };
 
 __device__ __forceinline__ void write_row(const ScoreParams& p, int64_t row, const RowSums& a, bool given, float xt) {
@@ -265,163 +283,217 @@ __device__ __forceinline__ void write_top(const ScoreParams& p, int64_t row, int
   p.top_logp[row * p.k + r] = have ? (unord((uint32_t)(key >> 32)) - a.m) * p.inv_t - __builtin_amdgcn_logf(a.z) * LN2 : nan ? a.z : -INFINITY;
 }
 
-// MULTI false: a wave per row, four rows a workgroup, no barrier.  MULTI: a workgroup per segment of a row; its alternatives come from one
-// threshold over all its lanes (with a list per wave, 64 alternatives of 100003 classes took 570 us instead of TOPTIME).
-template <typename T, bool MULTI>
-__global__ __launch_bounds__(MULTI ? 1024 : 256) void token_logprobs_fwd_kernel(ScoreParams p) {
+// one wave per row (LONG false), or per 2048 columns of a row
+template <typename T, bool LONG>
+__global__ __launch_bounds__(256) void token_logprobs_fwd_kernel(ScoreParams p) {
   extern __shared__ __attribute__((aligned(16))) u64 score_lds[];
-  __shared__ RowSums sm[MULTI ? MAX_WAVES : 1];
-  __shared__ int sm_n[MAX_WAVES + 2];    // ties of each wave; [MAX_WAVES]: keys so far; [MAX_WAVES + 1]: the threshold's bits
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t unit = MULTI ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
-  const int64_t row = MULTI ? blockIdx.x / (unsigned)p.sp.nseg : unit;
+  const int64_t id = (int64_t)blockIdx.x * 4 + wave;
+  int64_t row = id;
+  int unit = 0;
+  if (LONG) split_id(id, p.units, row, unit);
   if (row >= p.R) return;
-  const int seg = MULTI ? (int)(blockIdx.x % (unsigned)p.sp.nseg) : 0;
   const T* lr = (const T*)p.logits + row * p.ldl;
-  const int64_t tok = p.tokens[row];
-  const bool given = tok >= 0 && tok < p.C;
-  const float xt = given ? (float)lr[tok] : 0.f;      // (its latency runs beside the row's)
-  const int send = MULTI ? min(p.C, (seg + 1) * p.sp.seg) : p.C;
-  const int c0 = MULTI ? seg * p.sp.seg + wave * p.sp.wave_cols : 0, cend = MULTI ? min(send, c0 + p.sp.wave_cols) : p.C;
-  const float c = p.inv_t * LOG2E;
-  float x[NV][8], vmax[NV];
+  const int c0 = unit * WAVE_COLS, cend = min(p.C, c0 + WAVE_COLS);
+  int64_t tok = -1;
+  float xt = 0.f;
+  if (!LONG) {
+    tok = p.tokens[row];
+    if (tok >= 0 && tok < p.C) xt = (float)lr[tok];      // (its latency runs beside the row's)
+  }
+  float x[NV][8], vmax[NV], lmax = -INFINITY;
   load_wave<T>(lr, c0, cend, lane, x);
-  float m = -FMAX, lmax = -INFINITY;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    vmax[i] = -INFINITY;
+    vmax[i] = x[i][0];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) vmax[i] = fmaxf(vmax[i], x[i][j]);
+    for (int j = 1; j < 8; ++j) vmax[i] = fmaxf(vmax[i], x[i][j]);
     lmax = fmaxf(lmax, vmax[i]);
   }
-  RowSums a;
-  a.m = wave_max(fmaxf(m, lmax));
-  a.z = a.s = 0.f;
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-    if (c0 + i * 512 < cend)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        float t;
-        const float e = expo(x[i][j], a.m, c, t);
-        a.z += e;
-        a.s = fmaf(e, t, a.s);
-      }
-  a.z = wave_sum(a.z);
-  a.s = wave_sum(a.s);
-  if (!MULTI) {
-    if (lane == 0) write_row(p, row, a, given, xt);
-    if (p.k) {
-      const int have = wave_top<T>(x, vmax, lr, c0, cend, p.k, lane, score_lds + wave * WAVE_TOP_LDS, [&](int r, u64 key) { write_top(p, row, r, key, a); });
-      if (lane >= have && lane < p.k) write_top(p, row, lane, 0, a);
-    }
+  const RowSums a = wave_sums(x, lmax, (cend - c0 + 511) >> 9, p.inv_t * LOG2E);
+  if (LONG) {
+    if (lane == 0) p.part[id] = make_float4(a.m, a.z, a.s, 0.f);
+    if (p.k) p.part_max[id * 64 + lane] = ord(fmaxf(lmax, -INFINITY));
     return;
   }
-  const int nw = p.sp.waves;
-  u64* cand = score_lds;                                                       // [GROUP_CAND + 2]
-  uint32_t* gmax = reinterpret_cast<uint32_t*>(score_lds + GROUP_CAND + 2);    // [nw][64]
-  if (lane == 0) sm[wave] = a;
-  if (p.k) gmax[threadIdx.x] = ord(lmax);
-  if (threadIdx.x == 0) sm_n[MAX_WAVES] = 0;
-  __syncthreads();
-  RowSums b = {sm[0].m, 0.f, 0.f};
-  for (int w = 1; w < nw; ++w) b.m = fmaxf(b.m, sm[w].m);
-  for (int w = 0; w < nw; ++w) add_sums(b, sm[w].m, sm[w].z, sm[w].s, b.m, c);
-  const bool whole = p.sp.nseg == 1;
-  if (threadIdx.x == 0) {
-    if (whole) write_row(p, row, b, given, xt);
-    else p.part[unit] = make_float4(b.m, b.z, b.s, 0.f);
-  }
-  if (!p.k) return;
-  if (wave == 0) {
-    uint32_t g[MAX_WAVES];
+  if (lane == 0) write_row(p, row, a, tok >= 0 && tok < p.C, xt);
+  if (p.k) {
 #pragma unroll
-    for (int w = 0; w < MAX_WAVES; ++w) g[w] = w < nw ? gmax[w * 64 + lane] : 0;
-    const float thr = group_threshold<MAX_WAVES>(g, nw, p.k, true);
-    if (lane == 0) sm_n[MAX_WAVES + 1] = __builtin_bit_cast(int, thr);
-  }
-  __syncthreads();
-  const float thr = __builtin_bit_cast(float, sm_n[MAX_WAVES + 1]);
-  auto next = [&](u64 mask) {
-    int base = 0;
-    if (lane == 0) base = atomicAdd(&sm_n[MAX_WAVES], __builtin_popcountll(mask));
-    return __builtin_amdgcn_readfirstlane(base) + lanes_below(mask);
-  };
-  if (__any(lmax >= thr)) collect<T>(reached<false>(x, thr, c0, cend), lr, c0, lane, cand, GROUP_CAND, next);
-  __syncthreads();
-  int n = sm_n[MAX_WAVES];
-  if (n > GROUP_CAND) {   // values repeat at the threshold (the k-th group's own then: exactly k groups hold no more than GROUP_CAND)
-    int ties = 0;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) ties += __builtin_popcountll(__ballot(x[i][j] == thr));
-    __syncthreads();
-    if (threadIdx.x == 0) sm_n[MAX_WAVES] = 0;
-    if (lane == 0) sm_n[wave] = ties;
-    __syncthreads();
-    collect<T>(reached<true>(x, thr, c0, cend), lr, c0, lane, cand, GROUP_CAND, next);
-    __syncthreads();
-    n = sm_n[MAX_WAVES];
-    const int end = max(n, p.k);
-    int all = n, mine = n;
-    for (int w = 0; w < nw; ++w) {
-      if (w < wave) mine += sm_n[w];
-      all += sm_n[w];
-    }
-    if (mine < end) collect_ties(x, thr, c0, lane, cand, mine, end);
-    n = min(all, end);
-  }
-  if (threadIdx.x < 2) cand[n + threadIdx.x] = 0;
-  __syncthreads();
-  rank_keys(cand, n, p.k, threadIdx.x, 64 * nw, [&](int r, u64 key) {
-    if (whole) write_top(p, row, r, key, b);
-    else p.part_key[unit * p.k + r] = key;
-  });
-  for (int r = n + threadIdx.x; r < p.k; r += 64 * nw) {
-    if (whole) write_top(p, row, r, 0, b);
-    else p.part_key[unit * p.k + r] = 0;
+    for (int i = 0; i < NV; ++i) vmax[i] = fmaxf(vmax[i], -INFINITY);   // (a group of NaN only)
+    const int have = wave_top<T>(x, vmax, lr, c0, cend, p.k, lane, score_lds + wave * WAVE_TOP_LDS, [&](int r, u64 key) { write_top(p, row, r, key, a); });
+    if (lane >= have && lane < p.k) write_top(p, row, lane, 0, a);
   }
 }
 
-// the segments of a long row: at most 32 of them, their sums in one wave, their lists as the waves' above
+// a long row's sums, by one wave, from its units' parts; every lane gets them
+__device__ __forceinline__ RowSums join_sums(const ScoreParams& p, int64_t row, int lane) {
+  const float4* part = p.part + row * p.units;
+  float m = -FMAX;
+  for (int u = lane; u < p.units; u += 64) m = fmaxf(m, part[u].x);
+  RowSums a = {max_wave(m), 0.f, 0.f};
+  for (int u = lane; u < p.units; u += 64) {
+    const float4 s = part[u];
+    add_sums(a, s.x, s.y, s.z, p.inv_t * LOG2E);
+  }
+  a.z = sum_wave(a.z);
+  a.s = sum_wave(a.s);
+  return a;
+}
 template <typename T>
-__global__ __launch_bounds__(256) void token_logprobs_join_kernel(ScoreParams p) {
-  extern __shared__ __attribute__((aligned(16))) u64 score_lds[];   // [nseg][k]
-  const int64_t row = blockIdx.x;
-  const int lane = threadIdx.x & 63, nseg = p.sp.nseg, total = nseg * p.k;
-  for (int i = threadIdx.x; i < total; i += 256) score_lds[i] = p.part_key[row * total + i];
-  float4 s = make_float4(-FMAX, 0.f, 0.f, 0.f);
-  if (lane < nseg) s = p.part[row * nseg + lane];
-  RowSums a = {wave_max(s.x), 0.f, 0.f};
-  add_sums(a, s.x, s.y, s.z, a.m, p.inv_t * LOG2E);
-  a.z = wave_sum(a.z);
-  a.s = wave_sum(a.s);
-  if (threadIdx.x == 0) {
-    const int64_t tok = p.tokens[row];
-    const bool given = tok >= 0 && tok < p.C;
-    write_row(p, row, a, given, given ? (float)((const T*)p.logits)[row * p.ldl + tok] : 0.f);
-  }
-  if (!p.k) return;
-  __syncthreads();
-  int have = 0;
-  for (int i = lane; i < total; i += 64) have += score_lds[i] != 0;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) have += __shfl_xor(have, o, 64);
-  for (int i = threadIdx.x; i < total; i += 256) {
-    const u64 key = score_lds[i];
-    if (!key) continue;
-    const int r = merged_rank(score_lds, p.k, nseg, i / p.k, i % p.k, p.k, key);
-    if (r < p.k) write_top(p, row, r, key, a);
-  }
-  for (int r = threadIdx.x; r < p.k; r += 256)
-    if (r >= have) write_top(p, row, r, 0, a);
+__device__ __forceinline__ void write_long_row(const ScoreParams& p, int64_t row, const RowSums& a) {
+  const int64_t tok = p.tokens[row];
+  const bool given = tok >= 0 && tok < p.C;
+  write_row(p, row, a, given, given ? (float)((const T*)p.logits)[row * p.ldl + tok] : 0.f);
+}
+template <typename T>
+__global__ __launch_bounds__(256) void token_logprobs_join_kernel(ScoreParams p) {   // no alternatives: a wave per row
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= p.R) return;
+  const RowSums a = join_sums(p, row, threadIdx.x & 63);
+  if ((threadIdx.x & 63) == 0) write_long_row<T>(p, row, a);
 }
 
-// (n / d, n % d) of a piece's number: in 32 bits where it fits (a 64-bit division costs as much as the piece's work)
-__device__ __forceinline__ void split_id(int64_t n, int d, int64_t& q, int& r) {
-  if ((uint64_t)n >> 32) { q = n / d; r = (int)(n % d); }
-  else { q = (uint32_t)n / (uint32_t)d; r = (int)((uint32_t)n % (uint32_t)d); }
+// Alternatives of a long row: W waves, up to W * N * 64 groups of 32 columns.  Each wave's own k-th largest group maximum is at most the
+// row's, so the largest of these bounds is one too and keeps at most k groups a wave; among those one wave finds the exact
+// threshold, the k or so groups that reach it are read again, and their columns that do are ranked.  Where values repeat at a
+// threshold, so that more groups reach it than there is room for: the exact threshold over all groups, the fewer than k groups above
+// it, and then the row's columns AT it in the order of the classes until there are k.
+template <typename T, int W, int N>
+__global__ __launch_bounds__(W * 64) void token_logprobs_top_kernel(ScoreParams p) {
+  constexpr int LIST = 64 * W;
+  __shared__ u64 cand[GROUP_CAND + 2];
+  __shared__ uint32_t list_max[LIST];
+  __shared__ int list_id[LIST];
+  __shared__ float sm_thr[W + 1];
+  __shared__ int sm_n, sm_list, sm_cnt[W];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t row = blockIdx.x;
+  const T* lr = (const T*)p.logits + row * p.ldl;
+  const int k = p.k, groups = p.units * 64;
+  const uint32_t* gm = p.part_max + row * groups;
+  if (tid == 0) sm_n = sm_list = 0;
+  uint32_t g[N];
+  int steps = 0;                              // groups id = (i W + wave) 64 + lane: neighbouring units in different waves
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int u = i * W + wave;
+    g[i] = 0;
+    if (u < p.units) { g[i] = gm[u * 64 + lane]; steps = i + 1; }
+  }
+  const RowSums a = join_sums(p, row, lane);
+  if (tid == 0) write_long_row<T>(p, row, a);
+  const float mine = steps ? group_threshold<N>(g, steps, k, true) : -FMAX;
+  if (lane == 0) sm_thr[wave] = mine;
+  __syncthreads();
+  float thr = sm_thr[0];
+  for (int w = 1; w < W; ++w) thr = fmaxf(thr, sm_thr[w]);
+  // push(bits-of-value test): the columns of group id that pass become keys
+  auto push_eight = [&](int id, int i, float t, bool above) {
+    const int c = (id >> 6) * WAVE_COLS + i * 512 + (id & 63) * 8;
+    if (c >= p.C) return;
+    float v[8];
+    load8<T>(lr + c, p.C - c, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (above ? v[j] > t : v[j] >= t) {
+        const int at = atomicAdd(&sm_n, 1);
+        if (at < GROUP_CAND) cand[at] = top_key(v[j], c + j);
+      }
+  };
+  {
+    const uint32_t tb = ord(thr);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < steps && g[i] >= tb) {
+        const int at = atomicAdd(&sm_list, 1);
+        if (at < LIST) { list_max[at] = g[i]; list_id[at] = (i * W + wave) * 64 + lane; }
+      }
+  }
+  __syncthreads();
+  const int listed = sm_list;
+  bool full = listed > LIST;                  // (uniform over the workgroup)
+  if (!full) {
+    if (wave == 0) {
+      uint32_t q[W];
+#pragma unroll
+      for (int i = 0; i < W; ++i) q[i] = i * 64 + lane < listed ? list_max[i * 64 + lane] : 0;
+      const float t = fmaxf(thr, group_threshold<W>(q, (listed + 63) >> 6, k, true));   // (fewer than k groups: the bound itself)
+      if (lane == 0) sm_thr[W] = t;
+    }
+    __syncthreads();
+    const float t = sm_thr[W];
+    const uint32_t tb = ord(t);
+    for (int task = tid; task < listed * NV; task += W * 64)
+      if (list_max[task / NV] >= tb) push_eight(list_id[task / NV], task % NV, t, false);
+    __syncthreads();
+    full = sm_n > GROUP_CAND;
+  }
+  if (full) {
+    uint32_t t = 0;                           // the exact threshold over all groups of the row
+    for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
+      int cnt = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (i < steps) cnt += __builtin_popcountll(__ballot(g[i] >= (t | bit)));
+      __syncthreads();
+      if (lane == 0) sm_cnt[wave] = cnt;
+      __syncthreads();
+      cnt = 0;
+      for (int w = 0; w < W; ++w) cnt += sm_cnt[w];
+      if (cnt >= k) t |= bit;
+    }
+    thr = t <= ORD_NONE ? -FMAX : unord(t);
+    __syncthreads();
+    if (tid == 0) sm_n = 0;
+    __syncthreads();
+    const uint32_t tb = ord(thr);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < steps && g[i] > tb)
+        for (int e = 0; e < NV; ++e) push_eight((i * W + wave) * 64 + lane, e, thr, true);
+    __syncthreads();
+    int n = sm_n;
+    const int end = max(n, k);
+    for (int c0 = 0; c0 < p.C && n < end; c0 += W * 512) {
+      const int c = c0 + tid * 8;
+      float v[8];
+      int mine_n = 0;
+      if (c < p.C) {
+        load8<T>(lr + c, p.C - c, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) mine_n += v[j] == thr;
+      }
+      int upto = mine_n;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int s = __shfl_up(upto, o, 64);
+        if (lane >= o) upto += s;
+      }
+      __syncthreads();
+      if (lane == 63) sm_cnt[wave] = upto;
+      __syncthreads();
+      int at = n + upto - mine_n;
+      for (int w = 0; w < W; ++w) {
+        if (w < wave) at += sm_cnt[w];
+        n += sm_cnt[w];
+      }
+      if (mine_n)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (v[j] == thr) {
+            if (at < end) cand[at] = top_key(v[j], c + j);
+            ++at;
+          }
+    }
+    __syncthreads();
+    if (tid == 0) sm_n = min(n, end);
+    __syncthreads();
+  }
+  const int n = sm_n;
+  if (tid < 2) cand[n + tid] = 0;
+  __syncthreads();
+  rank_keys(cand, n, k, tid, W * 64, [&](int r, u64 key) { write_top(p, row, r, key, a); });
+  for (int r = n + tid; r < k; r += W * 64) write_top(p, row, r, 0, a);
 }
 
 // ---- gradient of the log-probabilities: one thread per 8 columns, everything of the row is known -------------------------
@@ -487,14 +559,14 @@ __device__ __forceinline__ Listed load_listed(const int64_t* idx, const float* t
       L.p[h] = L.id[h] >= 0 ? __expf(t[h]) : 0.f;
     }
   } else {
-    const float m = fmaxf(wave_max(fmaxf(t[0], t[1])), -FMAX);
+    const float m = fmaxf(max_wave(fmaxf(t[0], t[1])), -FMAX);
     float e[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       L.logp[h] = (t[h] - m) * inv_t;
       e[h] = L.id[h] >= 0 ? __expf(L.logp[h]) : 0.f;
     }
-    const float z = wave_sum(e[0] + e[1]);
+    const float z = sum_wave(e[0] + e[1]);
     const float logz = __logf(z);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -502,7 +574,7 @@ __device__ __forceinline__ Listed load_listed(const int64_t* idx, const float* t
       L.logp[h] -= logz;
     }
   }
-  L.mass = wave_sum(L.p[0] + L.p[1]);
+  L.mass = sum_wave(L.p[0] + L.p[1]);
   return L;
 }
 
@@ -511,10 +583,9 @@ struct DistillParams {
   const int64_t* idx;
   const float* tlogp;
   float *row_loss, *stats;
-  float4* part;        // [R, nseg] (m, z of the listed classes, z of the others, -)
-  int R, C, K, tail;
+  float4* part;        // long rows: [R, units] (m, z of the listed classes, z of the others, -) of each wave's 2048 columns
+  int R, C, K, tail, units;
   float inv_t;
-  Split sp;
 };
 // by one wave: the row's loss from its sums (listed and other classes apart with tail, else all in zr) and the listed classes' logits
 __device__ __forceinline__ void finish_distill(const DistillParams& p, int64_t row, const Listed& L, const float (&xl)[2], float m, float zl, float zr,
@@ -524,7 +595,7 @@ __device__ __forceinline__ void finish_distill(const DistillParams& p, int64_t r
 #pragma unroll
   for (int h = 0; h < 2; ++h)
     if (L.p[h] != 0.f) loss += L.p[h] * (L.logp[h] - ((xl[h] - m) * p.inv_t - logz));
-  loss = wave_sum(loss);
+  loss = sum_wave(loss);
   if (lane == 0) {
     const float left = 1.f - L.mass;
     // log of the student's rest = -log(1 + listed / others): the difference of two log-sums would lose it where little is listed
@@ -543,34 +614,33 @@ __device__ __forceinline__ void listed_logits(const T* row, const Listed& L, flo
 }
 
 // as token_logprobs_fwd_kernel; with tail each wave marks the listed classes of its columns in a bit map of its own
-template <typename T, bool MULTI>
-__global__ __launch_bounds__(MULTI ? 1024 : 256) void distill_fwd_kernel(DistillParams p) {
-  __shared__ uint32_t marks[MULTI ? MAX_WAVES : 4][WAVE_COLS / 32];
-  __shared__ RowSums sm[MAX_WAVES];
+template <typename T, bool LONG>
+__global__ __launch_bounds__(256) void distill_fwd_kernel(DistillParams p) {
+  __shared__ uint32_t marks[4][WAVE_COLS / 32];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t unit = MULTI ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
-  const int64_t row = MULTI ? blockIdx.x / (unsigned)p.sp.nseg : unit;
+  const int64_t id = (int64_t)blockIdx.x * 4 + wave;
+  int64_t row = id;
+  int unit = 0;
+  if (LONG) split_id(id, p.units, row, unit);
   if (row >= p.R) return;
-  const int seg = MULTI ? (int)(blockIdx.x % (unsigned)p.sp.nseg) : 0;
   const T* lr = (const T*)p.logits + row * p.ldl;
-  const int send = MULTI ? min(p.C, (seg + 1) * p.sp.seg) : p.C;
-  const int c0 = MULTI ? seg * p.sp.seg + wave * p.sp.wave_cols : 0, cend = MULTI ? min(send, c0 + p.sp.wave_cols) : p.C;
-  const float c = p.inv_t * LOG2E;
+  const int c0 = unit * WAVE_COLS, cend = min(p.C, c0 + WAVE_COLS);
   float x[NV][8];
   load_wave<T>(lr, c0, cend, lane, x);
-  const bool first = wave == 0 || !MULTI, whole = !MULTI || p.sp.nseg == 1;
   Listed L;
   float xl[2] = {0.f, 0.f};
-  if (p.tail || (first && whole)) L = load_listed(p.idx + row * p.K, p.tlogp + row * p.K, p.K, p.C, p.inv_t, p.tail, lane);
-  if (first && whole) listed_logits(lr, L, xl);
+  if (!LONG) {
+    L = load_listed(p.idx + row * p.K, p.tlogp + row * p.K, p.K, p.C, p.inv_t, p.tail, lane);
+    listed_logits(lr, L, xl);
+  }
   uint32_t* mark = marks[wave];
   if (p.tail) {
     mark[lane] = 0;
     wave_fence();
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int at = L.id[h] - c0;
-      if (L.id[h] >= c0 && L.id[h] < cend) atomicOr(&mark[at >> 5], 1u << (at & 31));
+      const int64_t c = LONG ? (lane + 64 * h < p.K ? p.idx[row * p.K + lane + 64 * h] : -1) : L.id[h];
+      if (c >= c0 && c < cend) atomicOr(&mark[(c - c0) >> 5], 1u << ((c - c0) & 31));
     }
     wave_fence();
   }
@@ -579,61 +649,57 @@ __global__ __launch_bounds__(MULTI ? 1024 : 256) void distill_fwd_kernel(Distill
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int j = 0; j < 8; ++j) m = fmaxf(m, x[i][j]);
-  m = wave_max(m);
+  m = max_wave(m);
+  const Exponent ex(m, p.inv_t * LOG2E);
   float zl = 0.f, zr = 0.f;
+  const int steps = (cend - c0 + 511) >> 9;
   if (p.tail) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      if (c0 + i * 512 >= cend) break;
+      if (i >= steps) break;
       const uint32_t bits = reinterpret_cast<const uint8_t*>(mark)[i * 64 + lane];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float e = __builtin_amdgcn_exp2f((x[i][j] - m) * c);
+        const float e = __builtin_amdgcn_exp2f(ex(x[i][j]));
         const bool hit = (bits >> j) & 1u;
         zl += hit ? e : 0.f;
         zr += hit ? 0.f : e;
       }
     }
-    zl = wave_sum(zl);
+    zl = sum_wave(zl);
   } else {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      if (c0 + i * 512 >= cend) break;
+      if (i >= steps) break;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) zr += __builtin_amdgcn_exp2f((x[i][j] - m) * c);
+      for (int j = 0; j < 8; ++j) zr += __builtin_amdgcn_exp2f(ex(x[i][j]));
     }
   }
-  zr = wave_sum(zr);
-  if (!MULTI) {
-    finish_distill(p, row, L, xl, m, zl, zr, lane);
-    return;
-  }
-  if (lane == 0) sm[wave] = RowSums{m, zl, zr};
-  __syncthreads();
-  if (wave) return;
-  float M = sm[0].m, Zl = 0.f, Zr = 0.f;
-  for (int w = 1; w < p.sp.waves; ++w) M = fmaxf(M, sm[w].m);
-  for (int w = 0; w < p.sp.waves; ++w) {
-    const float f = __builtin_amdgcn_exp2f((sm[w].m - M) * c);
-    Zl += sm[w].z * f;
-    Zr += sm[w].s * f;
-  }
-  if (whole) finish_distill(p, row, L, xl, M, Zl, Zr, lane);
-  else if (lane == 0) p.part[unit] = make_float4(M, Zl, Zr, 0.f);
+  const float f = __builtin_amdgcn_exp2f(-ex.delta);
+  zl *= f;
+  zr = sum_wave(zr) * f;
+  if (!LONG) finish_distill(p, row, L, xl, m, zl, zr, lane);
+  else if (lane == 0) p.part[id] = make_float4(m, zl, zr, 0.f);
 }
 template <typename T>
-__global__ __launch_bounds__(256) void distill_join_kernel(DistillParams p) {   // a wave per row; at most 32 segments
+__global__ __launch_bounds__(256) void distill_join_kernel(DistillParams p) {   // a wave per row
   const int lane = threadIdx.x & 63;
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= p.R) return;
-  float4 s = make_float4(-FMAX, 0.f, 0.f, 0.f);
-  if (lane < p.sp.nseg) s = p.part[row * p.sp.nseg + lane];
   const Listed L = load_listed(p.idx + row * p.K, p.tlogp + row * p.K, p.K, p.C, p.inv_t, p.tail, lane);
   float xl[2];
   listed_logits((const T*)p.logits + row * p.ldl, L, xl);
-  const float m = wave_max(s.x), f = __builtin_amdgcn_exp2f((s.x - m) * p.inv_t * LOG2E);
-  const float zl = wave_sum(s.y * f), zr = wave_sum(s.z * f);
-  finish_distill(p, row, L, xl, m, zl, zr, lane);
+  const float4* part = p.part + row * p.units;
+  float m = -FMAX, zl = 0.f, zr = 0.f;
+  for (int u = lane; u < p.units; u += 64) m = fmaxf(m, part[u].x);
+  m = max_wave(m);
+  for (int u = lane; u < p.units; u += 64) {
+    const float4 s = part[u];
+    const float f = __builtin_amdgcn_exp2f((s.x - m) * p.inv_t * LOG2E);
+    zl = fmaf(s.y, f, zl);
+    zr = fmaf(s.z, f, zr);
+  }
+  finish_distill(p, row, L, xl, m, sum_wave(zl), sum_wave(zr), lane);
 }
 
 struct DistillGradParams {
@@ -763,26 +829,30 @@ static int need_grid(const char* what, int64_t grid) {
   return TTTS_OK;
 }
 
+// waves of a long row; 1: the row is one wave's
+static int row_units(int C) { return (int)cdiv(C, WAVE_COLS); }
+
 extern "C" int64_t ttts_token_logprobs_workspace_bytes(int32_t R, int32_t C, int32_t top_k) {
-  if (R <= 0 || C <= 0 || top_k < 0) return 0;
-  const Split sp = split_row(C);
-  return sp.nseg > 1 ? cdiv((int64_t)R * sp.nseg * (16 + 8 * (int64_t)top_k), 16) * 16 : 0;
+  if (R <= 0 || C <= WAVE_COLS || top_k < 0) return 0;
+  return (int64_t)R * row_units(C) * (16 + (top_k > 0 ? 256 : 0));
 }
 
 template <typename T>
 static int launch_score(const ScoreParams& p, hipStream_t st) {
   const char* what = "token_logprobs_fwd";
-  if (p.sp.nseg == 1 && p.sp.waves == 1) {
-    token_logprobs_fwd_kernel<T, false><<<(unsigned)cdiv(p.R, 4), 256, p.k ? 4 * WAVE_TOP_LDS * 8 : 0, st>>>(p);
-    return check_launch(what);
-  }
-  const int64_t grid = (int64_t)p.R * p.sp.nseg;
+  const int64_t grid = cdiv((int64_t)p.R * p.units, 4);
   int rc = need_grid(what, grid);
   if (rc) return rc;
-  token_logprobs_fwd_kernel<T, true><<<(unsigned)grid, 64 * p.sp.waves, p.k ? (GROUP_CAND + 2) * 8 + p.sp.waves * 64 * 4 : 0, st>>>(p);
+  if (p.units == 1) {
+    token_logprobs_fwd_kernel<T, false><<<(unsigned)grid, 256, p.k ? 4 * WAVE_TOP_LDS * 8 : 0, st>>>(p);
+    return check_launch(what);
+  }
+  token_logprobs_fwd_kernel<T, true><<<(unsigned)grid, 256, 0, st>>>(p);
   rc = check_launch(what);
-  if (rc || p.sp.nseg == 1) return rc;
-  token_logprobs_join_kernel<T><<<p.R, 256, p.sp.nseg * p.k * 8, st>>>(p);
+  if (rc) return rc;
+  if (p.k == 0) token_logprobs_join_kernel<T><<<(unsigned)cdiv(p.R, 4), 256, 0, st>>>(p);
+  else if (p.units <= 64) token_logprobs_top_kernel<T, 4, 16><<<p.R, 256, 0, st>>>(p);    // up to 131072 classes
+  else token_logprobs_top_kernel<T, 16, 32><<<p.R, 1024, 0, st>>>(p);                     // up to TTTS_SCORE_MAX_CLASSES
   return check_launch("token_logprobs_fwd join");
 }
 
@@ -796,8 +866,8 @@ extern "C" int ttts_token_logprobs_fwd(const void* logits, int32_t dtype, int64_
   TTTS_REQUIRE(tokens && logp && entropy && stats && (top_k == 0 || (top_logp && top_idx)), "token_logprobs_fwd: null pointer");
   rc = need_workspace("token_logprobs_fwd", ttts_token_logprobs_workspace_bytes(R, C, top_k), workspace, workspace_bytes);
   if (rc) return rc;
-  ScoreParams p{logits, ldl, tokens, logp, entropy, stats, top_logp, top_idx, (float4*)workspace, nullptr, R, C, top_k, 1.0f / temperature, split_row(C)};
-  p.part_key = (u64*)(p.part + (int64_t)R * p.sp.nseg);
+  ScoreParams p{logits, ldl, tokens, logp, entropy, stats, top_logp, top_idx, (float4*)workspace, nullptr, R, C, top_k, row_units(C), 1.0f / temperature};
+  p.part_max = (uint32_t*)(p.part + (int64_t)R * p.units);
   TTTS_BY_TYPE(dtype, "token_logprobs_fwd", rc = launch_score<T>(p, as_stream(stream)));
   return rc;
 }
@@ -819,25 +889,21 @@ extern "C" int ttts_token_logprobs_bwd(const void* logits, int32_t dtype, int64_
   return check_launch("token_logprobs_bwd");
 }
 
-extern "C" int64_t ttts_distill_workspace_bytes(int32_t R, int32_t C) {
-  if (R <= 0 || C <= 0) return 0;
-  const Split sp = split_row(C);
-  return sp.nseg > 1 ? (int64_t)R * sp.nseg * 16 : 0;
-}
+extern "C" int64_t ttts_distill_workspace_bytes(int32_t R, int32_t C) { return R > 0 && C > WAVE_COLS ? (int64_t)R * row_units(C) * 16 : 0; }
 
 template <typename T>
 static int launch_distill(const DistillParams& p, hipStream_t st) {
   const char* what = "distill_fwd";
-  if (p.sp.nseg == 1 && p.sp.waves == 1) {
-    distill_fwd_kernel<T, false><<<(unsigned)cdiv(p.R, 4), 256, 0, st>>>(p);
-    return check_launch(what);
-  }
-  const int64_t grid = (int64_t)p.R * p.sp.nseg;
+  const int64_t grid = cdiv((int64_t)p.R * p.units, 4);
   int rc = need_grid(what, grid);
   if (rc) return rc;
-  distill_fwd_kernel<T, true><<<(unsigned)grid, 64 * p.sp.waves, 0, st>>>(p);
+  if (p.units == 1) {
+    distill_fwd_kernel<T, false><<<(unsigned)grid, 256, 0, st>>>(p);
+    return check_launch(what);
+  }
+  distill_fwd_kernel<T, true><<<(unsigned)grid, 256, 0, st>>>(p);
   rc = check_launch(what);
-  if (rc || p.sp.nseg == 1) return rc;
+  if (rc) return rc;
   distill_join_kernel<T><<<(unsigned)cdiv(p.R, 4), 256, 0, st>>>(p);
   return check_launch("distill_fwd join");
 }
@@ -852,7 +918,7 @@ extern "C" int ttts_distill_fwd(const void* logits, int32_t dtype, int64_t ldl, 
   TTTS_REQUIRE(teacher_idx && teacher_logp && row_loss && stats, "distill_fwd: null pointer");
   rc = need_workspace("distill_fwd", ttts_distill_workspace_bytes(R, C), workspace, workspace_bytes);
   if (rc) return rc;
-  const DistillParams p{logits, ldl, teacher_idx, teacher_logp, row_loss, stats, (float4*)workspace, R, C, K, tail != 0, 1.0f / temperature, split_row(C)};
+  const DistillParams p{logits, ldl, teacher_idx, teacher_logp, row_loss, stats, (float4*)workspace, R, C, K, tail != 0, row_units(C), 1.0f / temperature};
   TTTS_BY_TYPE(dtype, "distill_fwd", rc = launch_distill<T>(p, as_stream(stream)));
   return rc;
 }

@@ -63,6 +63,9 @@ __device__ __forceinline__ void load_wave(const T* row, int c0, int cend, int la
   }
 }
 
+// max(a, b) without the two instructions that would first make signalling NaNs quiet; a NaN is passed over, as by fmaxf
+__device__ __forceinline__ float max_med(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); }
+
 // The exponent of a class from its row's (or wave's) maximum m >= -FMAX:  t = (x - m) c, in bits.  As fma(x, c, -m c) it is one
 // instruction and off by the one rounding of m c for the whole row, delta, which comes off the sums again; where m c is so large that
 // delta would matter (or not finite: a row of the type's lowest value) the difference is taken first.
@@ -74,7 +77,6 @@ struct Exponent {
     plain = fabsf(mc) <= 1048576.f;
     delta = plain ? fmaf(m, c, -mc) : 0.f;
   }
-  __device__ __forceinline__ float operator()(float x) const { return plain ? fmaf(x, c, -mc) : (x - m) * c; }
 };
 // (n / d, n % d) of a piece's number: in 32 bits where it fits (a 64-bit division costs as much as the piece's work)
 __device__ __forceinline__ void split_id(int64_t n, int d, int64_t& q, int& r) {
@@ -103,14 +105,24 @@ __device__ __forceinline__ int lanes_below(u64 mask) {
   return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
 }
 
+// bits of ord() that values of the type leave alike (below a 16-bit type's mantissa): nothing to search there
+template <typename T> struct LowBits { static constexpr int n = 0; };
+template <> struct LowBits<bf16> { static constexpr int n = 16; };
+template <> struct LowBits<_Float16> { static constexpr int n = 13; };
+
 // A threshold first: the k-th largest of the maxima of groups of columns is at most the k-th largest column, and few columns reach it
 // (k + 10 .. 30 % of ordinary rows).  It is found bit by bit with ballots over n group maxima a lane, and any value that exactly k
 // groups reach will do (early).  What reaches it lies in at most k groups, unless values repeat at the threshold: then (exact) fewer
 // than k groups go above it, and of the columns AT it the lowest classes are taken, as many as are needed.
-template <int N>
+template <typename T>
+__device__ __forceinline__ float threshold_of(uint32_t t) {   // (a class at -inf is no alternative)
+  if (LowBits<T>::n && !(t >> 31)) t |= (1u << LowBits<T>::n) - 1;   // below zero ord() has ones there
+  return t <= ORD_NONE ? -FMAX : unord(t);
+}
+template <typename T, int N>
 __device__ __forceinline__ float group_threshold(const uint32_t (&g)[N], int n, int k, bool early) {
   uint32_t t = 0;
-  for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
+  for (uint32_t bit = 0x80000000u; bit >> LowBits<T>::n; bit >>= 1) {
     const uint32_t c = t | bit;
     int cnt = 0;
 #pragma unroll
@@ -121,7 +133,7 @@ __device__ __forceinline__ float group_threshold(const uint32_t (&g)[N], int n, 
       if (early && cnt == k) break;
     }
   }
-  return t <= ORD_NONE ? -FMAX : unord(t);   // (a class at -inf is no alternative)
+  return threshold_of<T>(t);
 }
 // bit 31 - (8 i + j): x[i][j] reaches the threshold / is above it
 template <bool ABOVE>
@@ -197,15 +209,15 @@ __device__ __forceinline__ int wave_top(const float (&x)[NV][8], const float (&v
   float thr;
   if (k <= 32) {          // groups of a lane's 32 columns: one ballot a bit
     const uint32_t one[1] = {max(max(g[0], g[1]), max(g[2], g[3]))};
-    thr = group_threshold<1>(one, 1, k, true);
+    thr = group_threshold<T, 1>(one, 1, k, true);
   } else {                // of 8 columns: with 64 groups the least of them would have to do
-    thr = group_threshold<NV>(g, NV, k, true);
+    thr = group_threshold<T, NV>(g, NV, k, true);
   }
   int n = 0;
   auto next = [&](u64 mask) { const int at = n + lanes_below(mask); n += __builtin_popcountll(mask); return at; };
   collect<T>(reached<false>(x, thr, c0, cend), row, c0, lane, cand, WAVE_CAND, next);
   if (n > WAVE_CAND) {
-    thr = group_threshold<NV>(g, NV, k, false);
+    thr = group_threshold<T, NV>(g, NV, k, false);
     n = 0;
     collect<T>(reached<true>(x, thr, c0, cend), row, c0, lane, cand, WAVE_CAND, next);
     const int end = max(n, k);
@@ -218,38 +230,40 @@ __device__ __forceinline__ int wave_top(const float (&x)[NV][8], const float (&v
 }
 
 struct RowSums { float m, z, s; };   // maximum, sum e, sum e t (t in bits, from the maximum)
-// of one wave's columns
-template <int N>
-__device__ __forceinline__ RowSums wave_sums(const float (&x)[N][8], float lmax, int steps, float c) {
+// of one wave's columns.  A class at -inf, or at the type's lowest value, has e = 0: e t must be 0, not NaN, so t is kept finite
+// there (a NaN passes through e).
+__device__ __forceinline__ RowSums wave_sums(const float (&x)[NV][8], float lmax, int steps, float c) {
   RowSums a;
   a.m = max_wave(fmaxf(lmax, -FMAX));
   a.z = a.s = 0.f;
   const Exponent ex(a.m, c);
+  if (ex.plain) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    if (i >= steps) break;
-    float least = x[i][0];
-#pragma unroll
-    for (int j = 1; j < 8; ++j) least = fminf(least, x[i][j]);
-    if (ex.plain && !__any(least < -1e30f)) {
+    for (int i = 0; i < NV; ++i) {
+      if (i >= steps) break;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float t = fmaf(x[i][j], c, -ex.mc), e = __builtin_amdgcn_exp2f(t);
         a.z += e;
-        a.s = fmaf(e, t, a.s);
-      }
-    } else {   // a class at -inf, or at the type's lowest value, has e = 0: e t must be 0, not NaN (a NaN passes through e)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float t = ex(x[i][j]), e = __builtin_amdgcn_exp2f(t);
-        a.z += e;
         a.s = fmaf(e, fmaxf(t, -200.f), a.s);
       }
     }
+    const float f = __builtin_amdgcn_exp2f(-ex.delta);
+    a.z = sum_wave(a.z) * f;
+    a.s = sum_wave(a.s) * f - ex.delta * a.z;
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < NV; ++i)
+      if (i < steps)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float t = ((i == 0 ? x[0][j] : i == 1 ? x[1][j] : i == 2 ? x[2][j] : x[3][j]) - a.m) * c, e = __builtin_amdgcn_exp2f(t);
+          a.z += e;
+          a.s = fmaf(e, fmaxf(t, -200.f), a.s);
+        }
+    a.z = sum_wave(a.z);
+    a.s = sum_wave(a.s);
   }
-  const float f = __builtin_amdgcn_exp2f(-ex.delta);
-  a.z = sum_wave(a.z) * f;
-  a.s = sum_wave(a.s) * f - ex.delta * a.z;
   return a;
 }
 __device__ __forceinline__ void add_sums(RowSums& a, float m, float z, float s, float c) {   // a.m is the row's maximum already
@@ -305,21 +319,19 @@ __global__ __launch_bounds__(256) void token_logprobs_fwd_kernel(ScoreParams p) 
   load_wave<T>(lr, c0, cend, lane, x);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    vmax[i] = x[i][0];
+    vmax[i] = -INFINITY;
 #pragma unroll
-    for (int j = 1; j < 8; ++j) vmax[i] = fmaxf(vmax[i], x[i][j]);
-    lmax = fmaxf(lmax, vmax[i]);
+    for (int j = 0; j < 8; ++j) vmax[i] = max_med(vmax[i], x[i][j]);
+    lmax = max_med(lmax, vmax[i]);
   }
   const RowSums a = wave_sums(x, lmax, (cend - c0 + 511) >> 9, p.inv_t * LOG2E);
   if (LONG) {
     if (lane == 0) p.part[id] = make_float4(a.m, a.z, a.s, 0.f);
-    if (p.k) p.part_max[id * 64 + lane] = ord(fmaxf(lmax, -INFINITY));
+    if (p.k) p.part_max[id * 64 + lane] = ord(lmax);
     return;
   }
   if (lane == 0) write_row(p, row, a, tok >= 0 && tok < p.C, xt);
   if (p.k) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) vmax[i] = fmaxf(vmax[i], -INFINITY);   // (a group of NaN only)
     const int have = wave_top<T>(x, vmax, lr, c0, cend, p.k, lane, score_lds + wave * WAVE_TOP_LDS, [&](int r, u64 key) { write_top(p, row, r, key, a); });
     if (lane >= have && lane < p.k) write_top(p, row, lane, 0, a);
   }
@@ -353,18 +365,19 @@ __global__ __launch_bounds__(256) void token_logprobs_join_kernel(ScoreParams p)
   if ((threadIdx.x & 63) == 0) write_long_row<T>(p, row, a);
 }
 
-// Alternatives of a long row: W waves, up to W * N * 64 groups of 32 columns.  Each wave's own k-th largest group maximum is at most the
-// row's, so the largest of these bounds is one too and keeps at most k groups a wave; among those one wave finds the exact
-// threshold, the k or so groups that reach it are read again, and their columns that do are ranked.  Where values repeat at a
-// threshold, so that more groups reach it than there is room for: the exact threshold over all groups, the fewer than k groups above
-// it, and then the row's columns AT it in the order of the classes until there are k.
+// Alternatives of a long row: W waves, up to W * N * 64 groups of 32 columns.  Each wave bounds the threshold from its own groups (the k-th
+// largest of the maxima of up to 4 sets of them a lane); the largest of these bounds keeps little more than k groups a wave, among
+// those one wave finds the exact threshold, the k or so groups that reach it are read again, and their columns that do are ranked.
+// Where values repeat at a threshold, so that more reach it than there is room for: the exact threshold over all groups, the
+// fewer than k groups above it, and then the row's columns AT it in the order of the classes until there are k.
 template <typename T, int W, int N>
 __global__ __launch_bounds__(W * 64) void token_logprobs_top_kernel(ScoreParams p) {
-  constexpr int LIST = 64 * W;
+  constexpr int LIST = 128 * W, SETS = N < 4 ? N : 4;
   __shared__ u64 cand[GROUP_CAND + 2];
   __shared__ uint32_t list_max[LIST];
   __shared__ int list_id[LIST];
   __shared__ float sm_thr[W + 1];
+  __shared__ RowSums sm_row;
   __shared__ int sm_n, sm_list, sm_cnt[W];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t row = blockIdx.x;
@@ -372,23 +385,46 @@ __global__ __launch_bounds__(W * 64) void token_logprobs_top_kernel(ScoreParams 
   const int k = p.k, groups = p.units * 64;
   const uint32_t* gm = p.part_max + row * groups;
   if (tid == 0) sm_n = sm_list = 0;
-  uint32_t g[N];
-  int steps = 0;                              // groups id = (i W + wave) 64 + lane: neighbouring units in different waves
+  {
+    uint32_t g[N], q[SETS];                   // wave w has the units w, w + W, ..; group id = unit * 64 + lane
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int u = i * W + wave;
-    g[i] = 0;
-    if (u < p.units) { g[i] = gm[u * 64 + lane]; steps = i + 1; }
+    for (int i = 0; i < N; ++i) g[i] = i * W + wave < p.units ? gm[(i * W + wave) * 64 + lane] : 0;
+    if (wave == W - 1) {                      // (beside the others' search)
+      const RowSums a = join_sums(p, row, lane);
+      if (lane == 0) {
+        sm_row = a;
+        write_long_row<T>(p, row, a);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < SETS; ++i) {
+      q[i] = g[i];
+#pragma unroll
+      for (int j = i + SETS; j < N; j += SETS) q[i] = max(q[i], g[j]);
+    }
+    const float mine = group_threshold<T, SETS>(q, SETS, k, true);
+    if (lane == 0) sm_thr[wave] = mine;
+    __syncthreads();
+    float bound = sm_thr[0];
+    for (int w = 1; w < W; ++w) bound = fmaxf(bound, sm_thr[w]);
+    const uint32_t tb = ord(bound);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (g[i] >= tb) {
+        const int at = atomicAdd(&sm_list, 1);
+        if (at < LIST) { list_max[at] = g[i]; list_id[at] = (i * W + wave) * 64 + lane; }
+      }
+    __syncthreads();
+    if (wave == 0 && sm_list <= LIST) {
+      uint32_t l[LIST / 64];
+#pragma unroll
+      for (int i = 0; i < LIST / 64; ++i) l[i] = i * 64 + lane < sm_list ? list_max[i * 64 + lane] : 0;
+      const float t = fmaxf(bound, group_threshold<T, LIST / 64>(l, (sm_list + 63) >> 6, k, true));   // (fewer than k groups: the bound)
+      if (lane == 0) sm_thr[W] = t;
+    }
+    __syncthreads();
   }
-  const RowSums a = join_sums(p, row, lane);
-  if (tid == 0) write_long_row<T>(p, row, a);
-  const float mine = steps ? group_threshold<N>(g, steps, k, true) : -FMAX;
-  if (lane == 0) sm_thr[wave] = mine;
-  __syncthreads();
-  float thr = sm_thr[0];
-  for (int w = 1; w < W; ++w) thr = fmaxf(thr, sm_thr[w]);
-  // push(bits-of-value test): the columns of group id that pass become keys
-  auto push_eight = [&](int id, int i, float t, bool above) {
+  auto push_eight = [&](int id, int i, float t, bool above) {   // columns that reach t (or lie above it) become keys
     const int c = (id >> 6) * WAVE_COLS + i * 512 + (id & 63) * 8;
     if (c >= p.C) return;
     float v[8];
@@ -400,27 +436,9 @@ __global__ __launch_bounds__(W * 64) void token_logprobs_top_kernel(ScoreParams 
         if (at < GROUP_CAND) cand[at] = top_key(v[j], c + j);
       }
   };
-  {
-    const uint32_t tb = ord(thr);
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (i < steps && g[i] >= tb) {
-        const int at = atomicAdd(&sm_list, 1);
-        if (at < LIST) { list_max[at] = g[i]; list_id[at] = (i * W + wave) * 64 + lane; }
-      }
-  }
-  __syncthreads();
   const int listed = sm_list;
   bool full = listed > LIST;                  // (uniform over the workgroup)
   if (!full) {
-    if (wave == 0) {
-      uint32_t q[W];
-#pragma unroll
-      for (int i = 0; i < W; ++i) q[i] = i * 64 + lane < listed ? list_max[i * 64 + lane] : 0;
-      const float t = fmaxf(thr, group_threshold<W>(q, (listed + 63) >> 6, k, true));   // (fewer than k groups: the bound itself)
-      if (lane == 0) sm_thr[W] = t;
-    }
-    __syncthreads();
     const float t = sm_thr[W];
     const uint32_t tb = ord(t);
     for (int task = tid; task < listed * NV; task += W * 64)
@@ -430,11 +448,9 @@ __global__ __launch_bounds__(W * 64) void token_logprobs_top_kernel(ScoreParams 
   }
   if (full) {
     uint32_t t = 0;                           // the exact threshold over all groups of the row
-    for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
+    for (uint32_t bit = 0x80000000u; bit >> LowBits<T>::n; bit >>= 1) {
       int cnt = 0;
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (i < steps) cnt += __builtin_popcountll(__ballot(g[i] >= (t | bit)));
+      for (int u = wave; u < p.units; u += W) cnt += __builtin_popcountll(__ballot(gm[u * 64 + lane] >= (t | bit)));
       __syncthreads();
       if (lane == 0) sm_cnt[wave] = cnt;
       __syncthreads();
@@ -442,28 +458,28 @@ __global__ __launch_bounds__(W * 64) void token_logprobs_top_kernel(ScoreParams 
       for (int w = 0; w < W; ++w) cnt += sm_cnt[w];
       if (cnt >= k) t |= bit;
     }
-    thr = t <= ORD_NONE ? -FMAX : unord(t);
+    const float thr = threshold_of<T>(t);
+    const uint32_t tb = ord(thr);
     __syncthreads();
     if (tid == 0) sm_n = 0;
     __syncthreads();
-    const uint32_t tb = ord(thr);
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (i < steps && g[i] > tb)
-        for (int e = 0; e < NV; ++e) push_eight((i * W + wave) * 64 + lane, e, thr, true);
+    for (int u = wave; u < p.units; u += W)
+      if (gm[u * 64 + lane] > tb)
+#pragma unroll 1
+        for (int e = 0; e < NV; ++e) push_eight(u * 64 + lane, e, thr, true);
     __syncthreads();
     int n = sm_n;
     const int end = max(n, k);
     for (int c0 = 0; c0 < p.C && n < end; c0 += W * 512) {
       const int c = c0 + tid * 8;
       float v[8];
-      int mine_n = 0;
+      int mine = 0;
       if (c < p.C) {
         load8<T>(lr + c, p.C - c, v);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) mine_n += v[j] == thr;
+        for (int j = 0; j < 8; ++j) mine += v[j] == thr;
       }
-      int upto = mine_n;
+      int upto = mine;
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
         const int s = __shfl_up(upto, o, 64);
@@ -472,12 +488,12 @@ __global__ __launch_bounds__(W * 64) void token_logprobs_top_kernel(ScoreParams 
       __syncthreads();
       if (lane == 63) sm_cnt[wave] = upto;
       __syncthreads();
-      int at = n + upto - mine_n;
+      int at = n + upto - mine;
       for (int w = 0; w < W; ++w) {
         if (w < wave) at += sm_cnt[w];
         n += sm_cnt[w];
       }
-      if (mine_n)
+      if (mine)
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           if (v[j] == thr) {
@@ -490,6 +506,7 @@ __global__ __launch_bounds__(W * 64) void token_logprobs_top_kernel(ScoreParams 
     __syncthreads();
   }
   const int n = sm_n;
+  const RowSums a = sm_row;
   if (tid < 2) cand[n + tid] = 0;
   __syncthreads();
   rank_keys(cand, n, k, tid, W * 64, [&](int r, u64 key) { write_top(p, row, r, key, a); });
@@ -648,33 +665,37 @@ __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillParams p) {
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m = fmaxf(m, x[i][j]);
+    for (int j = 0; j < 8; ++j) m = max_med(m, x[i][j]);
   m = max_wave(m);
   const Exponent ex(m, p.inv_t * LOG2E);
   float zl = 0.f, zr = 0.f;
   const int steps = (cend - c0 + 511) >> 9;
-  if (p.tail) {
+  auto add_up = [&](auto exponent) {
+    if (p.tail) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      if (i >= steps) break;
-      const uint32_t bits = reinterpret_cast<const uint8_t*>(mark)[i * 64 + lane];
+      for (int i = 0; i < NV; ++i) {
+        if (i >= steps) break;
+        const uint32_t bits = reinterpret_cast<const uint8_t*>(mark)[i * 64 + lane];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float e = __builtin_amdgcn_exp2f(ex(x[i][j]));
-        const bool hit = (bits >> j) & 1u;
-        zl += hit ? e : 0.f;
-        zr += hit ? 0.f : e;
+        for (int j = 0; j < 8; ++j) {
+          const float e = __builtin_amdgcn_exp2f(exponent(x[i][j]));
+          const bool hit = (bits >> j) & 1u;
+          zl += hit ? e : 0.f;
+          zr += hit ? 0.f : e;
+        }
+      }
+      zl = sum_wave(zl);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        if (i >= steps) break;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) zr += __builtin_amdgcn_exp2f(exponent(x[i][j]));
       }
     }
-    zl = sum_wave(zl);
-  } else {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      if (i >= steps) break;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) zr += __builtin_amdgcn_exp2f(ex(x[i][j]));
-    }
-  }
+  };
+  if (ex.plain) add_up([&](float v) { return fmaf(v, ex.c, -ex.mc); });
+  else add_up([&](float v) { return (v - ex.m) * ex.c; });
   const float f = __builtin_amdgcn_exp2f(-ex.delta);
   zl *= f;
   zr = sum_wave(zr) * f;
@@ -851,8 +872,9 @@ static int launch_score(const ScoreParams& p, hipStream_t st) {
   rc = check_launch(what);
   if (rc) return rc;
   if (p.k == 0) token_logprobs_join_kernel<T><<<(unsigned)cdiv(p.R, 4), 256, 0, st>>>(p);
-  else if (p.units <= 64) token_logprobs_top_kernel<T, 4, 16><<<p.R, 256, 0, st>>>(p);    // up to 131072 classes
-  else token_logprobs_top_kernel<T, 16, 32><<<p.R, 1024, 0, st>>>(p);                     // up to TTTS_SCORE_MAX_CLASSES
+  else if (p.units <= 8) token_logprobs_top_kernel<T, 4, 2><<<p.R, 256, 0, st>>>(p);       // up to 16384 classes
+  else if (p.units <= 64) token_logprobs_top_kernel<T, 4, 16><<<p.R, 256, 0, st>>>(p);     // up to 131072
+  else token_logprobs_top_kernel<T, 16, 32><<<p.R, 1024, 0, st>>>(p);                      // up to TTTS_SCORE_MAX_CLASSES
   return check_launch("token_logprobs_fwd join");
 }
 

@@ -47,20 +47,37 @@ __device__ __forceinline__ void store8(T* p, int n, const float (&v)[8]) {
       if (j < n) p[j] = (T)v[j];
   }
 }
-// columns c0 .. cend - 1 of a row; columns outside are -inf
+// Columns c0 .. cend - 1 of a row, as they lie in memory (all loads on their way before the first is waited for); as fp32, columns outside
+// are -inf.
+template <typename T> struct Raw { typename Eight<T>::type v[NV]; };
 template <typename T>
-__device__ __forceinline__ void load_wave(const T* row, int c0, int cend, int lane, float (&x)[NV][8]) {
+__device__ __forceinline__ void load_raw(Raw<T>& r, const T* row, int c0, int cend, int lane) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = c0 + i * 512 + lane * 8;
+    if (c0 + i * 512 + 512 <= cend || c + 8 <= cend) r.v[i] = *reinterpret_cast<const typename Eight<T>::type*>(row + c);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void expand(const Raw<T>& r, const T* row, int c0, int cend, int lane, float (&x)[NV][8]) {
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = c0 + i * 512 + lane * 8;
     if (c0 + i * 512 + 512 <= cend) {
-      load8<T>(row + c, 8, x[i]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[i][j] = (float)r.v[i][j];
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[i][j] = -INFINITY;
-      if (c < cend) load8<T>(row + c, cend - c, x[i]);
+      for (int j = 0; j < 8; ++j) x[i][j] = c + 8 <= cend ? (float)r.v[i][j] : -INFINITY;
+      if (c < cend && c + 8 > cend) load8<T>(row + c, cend - c, x[i]);
     }
   }
+}
+template <typename T>
+__device__ __forceinline__ void load_wave(const T* row, int c0, int cend, int lane, float (&x)[NV][8]) {
+  Raw<T> r;
+  load_raw(r, row, c0, cend, lane);
+  expand(r, row, c0, cend, lane, x);
 }
 
 // max(a, b) without the two instructions that would first make signalling NaNs quiet; a NaN is passed over, as by fmaxf
@@ -297,7 +314,8 @@ __device__ __forceinline__ void write_top(const ScoreParams& p, int64_t row, int
   p.top_logp[row * p.k + r] = have ? (unord((uint32_t)(key >> 32)) - a.m) * p.inv_t - __builtin_amdgcn_logf(a.z) * LN2 : nan ? a.z : -INFINITY;
 }
 
-// one wave per row (LONG false), or per 2048 columns of a row
+// One wave per row (LONG false), or per 2048 columns of a row.  (Waves that went through several of them, the next one's loads under this
+// one's arithmetic, were slower at every grid: 118 - 125 us instead of 109 for logits of 2048 x 100003 with 64 alternatives.)
 template <typename T, bool LONG>
 __global__ __launch_bounds__(256) void token_logprobs_fwd_kernel(ScoreParams p) {
   extern __shared__ __attribute__((aligned(16))) u64 score_lds[];
@@ -309,14 +327,18 @@ __global__ __launch_bounds__(256) void token_logprobs_fwd_kernel(ScoreParams p) 
   if (row >= p.R) return;
   const T* lr = (const T*)p.logits + row * p.ldl;
   const int c0 = unit * WAVE_COLS, cend = min(p.C, c0 + WAVE_COLS);
+  float x[NV][8], vmax[NV], lmax = -INFINITY;
   int64_t tok = -1;
   float xt = 0.f;
-  if (!LONG) {
-    tok = p.tokens[row];
-    if (tok >= 0 && tok < p.C) xt = (float)lr[tok];      // (its latency runs beside the row's)
+  {
+    Raw<T> raw;
+    load_raw(raw, lr, c0, cend, lane);
+    if (!LONG) {
+      tok = p.tokens[row];
+      if (tok >= 0 && tok < p.C) xt = (float)lr[tok];      // (its latency runs beside the row's)
+    }
+    expand(raw, lr, c0, cend, lane, x);
   }
-  float x[NV][8], vmax[NV], lmax = -INFINITY;
-  load_wave<T>(lr, c0, cend, lane, x);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     vmax[i] = -INFINITY;
@@ -642,8 +664,8 @@ __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillParams p) {
   if (row >= p.R) return;
   const T* lr = (const T*)p.logits + row * p.ldl;
   const int c0 = unit * WAVE_COLS, cend = min(p.C, c0 + WAVE_COLS);
-  float x[NV][8];
-  load_wave<T>(lr, c0, cend, lane, x);
+  Raw<T> raw;
+  load_raw(raw, lr, c0, cend, lane);
   Listed L;
   float xl[2] = {0.f, 0.f};
   if (!LONG) {
@@ -661,7 +683,8 @@ __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillParams p) {
     }
     wave_fence();
   }
-  float m = -FMAX;
+  float x[NV][8], m = -FMAX;
+  expand(raw, lr, c0, cend, lane, x);
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -671,11 +694,11 @@ __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillParams p) {
   float zl = 0.f, zr = 0.f;
   const int steps = (cend - c0 + 511) >> 9;
   auto add_up = [&](auto exponent) {
-    if (p.tail) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        if (i >= steps) break;
-        const uint32_t bits = reinterpret_cast<const uint8_t*>(mark)[i * 64 + lane];
+    for (int i = 0; i < NV; ++i) {
+      if (i >= steps) break;
+      const uint32_t bits = p.tail ? reinterpret_cast<const uint8_t*>(mark)[i * 64 + lane] : 0u;
+      if (p.tail && __any(bits != 0)) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const float e = __builtin_amdgcn_exp2f(exponent(x[i][j]));
@@ -683,12 +706,7 @@ __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillParams p) {
           zl += hit ? e : 0.f;
           zr += hit ? 0.f : e;
         }
-      }
-      zl = sum_wave(zl);
-    } else {
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        if (i >= steps) break;
+      } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) zr += __builtin_amdgcn_exp2f(exponent(x[i][j]));
       }
@@ -697,8 +715,8 @@ __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillParams p) {
   if (ex.plain) add_up([&](float v) { return fmaf(v, ex.c, -ex.mc); });
   else add_up([&](float v) { return (v - ex.m) * ex.c; });
   const float f = __builtin_amdgcn_exp2f(-ex.delta);
-  zl *= f;
   zr = sum_wave(zr) * f;
+  if (p.tail) zl = sum_wave(zl) * f;
   if (!LONG) finish_distill(p, row, L, xl, m, zl, zr, lane);
   else if (lane == 0) p.part[id] = make_float4(m, zl, zr, 0.f);
 }

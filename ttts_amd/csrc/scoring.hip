@@ -167,21 +167,41 @@ __device__ __forceinline__ uint32_t reached(const float (&x)[NV][8], float thr, 
   }
   return bits;
 }
-// the columns marked in `bits` become keys from place n on (those before `cap`); their values are read again (a register cannot be
-// indexed by a lane).  Returns the place behind the last.
+// A wave's own keys of a 16-bit type fit 32 bits: the ord() that the type has, and the column within the wave's 2048, inverted.
+template <typename T> struct WaveKey {
+  typedef u64 type;
+  static __device__ __forceinline__ type make(float v, int at, int c0) { return top_key(v, c0 + at); }
+  static __device__ __forceinline__ u64 full(type k, int) { return k; }
+};
+template <typename T> struct WaveKey16 {
+  typedef uint32_t type;
+  static __device__ __forceinline__ type make(float v, int at, int) { return (ord(v) >> LowBits<T>::n << 11) | (uint32_t)(WAVE_COLS - 1 - at); }
+  static __device__ __forceinline__ u64 full(type k, int c0) {
+    uint32_t o = k >> 11 << LowBits<T>::n;
+    if (!(o >> 31)) o |= (1u << LowBits<T>::n) - 1;   // below zero ord() has ones there
+    return ((u64)o << 32) | (uint32_t)~(c0 + WAVE_COLS - 1 - (int)(k & (WAVE_COLS - 1)));
+  }
+};
+template <> struct WaveKey<bf16> : WaveKey16<bf16> {};
+template <> struct WaveKey<_Float16> : WaveKey16<_Float16> {};
+static_assert(WAVE_COLS == 2048, "11 bits of a wave's key are a column");
+
+// the columns marked in `bits` become keys at the places that place() deals out (those before `cap`); their values are read again (a
+// register cannot be indexed by a lane)
 template <typename T, typename Place>
-__device__ __forceinline__ void collect(uint32_t bits, const T* row, int c0, int lane, u64* cand, int cap, Place place) {
+__device__ __forceinline__ void collect(uint32_t bits, const T* row, int c0, int lane, typename WaveKey<T>::type* cand, int cap, Place place) {
   for (u64 mask = __ballot(bits != 0); mask; mask = __ballot(bits != 0)) {
     const int at = place(mask);
     if (bits) {
-      const int e = __builtin_clz(bits), c = c0 + (e >> 3) * 512 + lane * 8 + (e & 7);
+      const int e = __builtin_clz(bits), c = (e >> 3) * 512 + lane * 8 + (e & 7);
       bits &= ~(0x80000000u >> e);
-      if (at < cap) cand[at] = top_key((float)row[c], c);
+      if (at < cap) cand[at] = WaveKey<T>::make((float)row[c0 + c], c, c0);
     }
   }
 }
-// columns equal to thr, lowest classes first, become keys from place n on, up to `end`; first: ties of earlier waves.  Returns n + ties.
-__device__ __forceinline__ int collect_ties(const float (&x)[NV][8], float thr, int c0, int lane, u64* cand, int n, int end) {
+// columns equal to thr, lowest classes first, become keys from place n on, up to `end`; returns n + ties
+template <typename T>
+__device__ __forceinline__ int collect_ties(const float (&x)[NV][8], float thr, int c0, int lane, typename WaveKey<T>::type* cand, int n, int end) {
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     int mine = 0;
@@ -197,29 +217,29 @@ __device__ __forceinline__ int collect_ties(const float (&x)[NV][8], float thr, 
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       if (x[i][j] == thr) {
-        if (at < end) cand[at] = top_key(x[i][j], c0 + i * 512 + lane * 8 + j);
+        if (at < end) cand[at] = WaveKey<T>::make(x[i][j], i * 512 + lane * 8 + j, c0);
         ++at;
       }
     n += __shfl(upto, 63, 64);
   }
   return n;
 }
-// f(rank, key) for the keys of rank < k among n distinct ones (cand[n] and cand[n + 1] writable): ranked by counting
-template <typename F>
-__device__ __forceinline__ void rank_keys(u64* cand, int n, int k, int thread, int threads, F f) {
+// f(rank, key) for the keys of rank < k among n distinct ones (four places behind them writable): ranked by counting
+template <typename K, typename F>
+__device__ __forceinline__ void rank_keys(const K* cand, int n, int k, int thread, int threads, F f) {
   for (int s = thread; s < n; s += threads) {
-    const u64 key = cand[s];
+    const K key = cand[s];
     int r = 0;
-    for (int j = 0; j < n; j += 2) r += (cand[j] > key) + (cand[j + 1] > key);
+    for (int j = 0; j < n; j += 4) r += (cand[j] > key) + (cand[j + 1] > key) + (cand[j + 2] > key) + (cand[j + 3] > key);
     if (r < k) f(r, key);
   }
 }
-constexpr int WAVE_CAND = 64 * 8 + 64, WAVE_TOP_LDS = WAVE_CAND + 2;      // one wave: groups of 8 columns (exact)
+constexpr int WAVE_CAND = 64 * 8 + 64, WAVE_TOP_LDS = WAVE_CAND + 4;      // one wave: groups of 8 columns (exact)
 constexpr int GROUP_CAND = 64 * 32 + 64;                                  // a workgroup: a lane's 32 columns are a group
 // one wave: f(rank, key) of its k best; returns how many there are (<= k)
 template <typename T, typename F>
-__device__ __forceinline__ int wave_top(const float (&x)[NV][8], const float (&vmax)[NV], const T* row, int c0, int cend, int k, int lane, u64* cand,
-                                        F f) {
+__device__ __forceinline__ int wave_top(const float (&x)[NV][8], const float (&vmax)[NV], const T* row, int c0, int cend, int k, int lane,
+                                        typename WaveKey<T>::type* cand, F f) {
   uint32_t g[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) g[i] = ord(vmax[i]);
@@ -238,11 +258,11 @@ __device__ __forceinline__ int wave_top(const float (&x)[NV][8], const float (&v
     n = 0;
     collect<T>(reached<true>(x, thr, c0, cend), row, c0, lane, cand, WAVE_CAND, next);
     const int end = max(n, k);
-    n = min(end, collect_ties(x, thr, c0, lane, cand, n, end));
+    n = min(end, collect_ties<T>(x, thr, c0, lane, cand, n, end));
   }
-  if (lane < 2) cand[n + lane] = 0;
+  if (lane < 4) cand[n + lane] = 0;
   wave_fence();
-  rank_keys(cand, n, k, lane, 64, f);
+  rank_keys(cand, n, k, lane, 64, [&](int r, typename WaveKey<T>::type key) { f(r, WaveKey<T>::full(key, c0)); });
   return min(n, k);
 }
 
@@ -318,7 +338,7 @@ __device__ __forceinline__ void write_top(const ScoreParams& p, int64_t row, int
 // one's arithmetic, were slower at every grid: 118 - 125 us instead of 109 for logits of 2048 x 100003 with 64 alternatives.)
 template <typename T, bool LONG>
 __global__ __launch_bounds__(256) void token_logprobs_fwd_kernel(ScoreParams p) {
-  extern __shared__ __attribute__((aligned(16))) u64 score_lds[];
+  extern __shared__ __attribute__((aligned(16))) unsigned char score_lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t id = (int64_t)blockIdx.x * 4 + wave;
   int64_t row = id;
@@ -354,7 +374,7 @@ __global__ __launch_bounds__(256) void token_logprobs_fwd_kernel(ScoreParams p) 
   }
   if (lane == 0) write_row(p, row, a, tok >= 0 && tok < p.C, xt);
   if (p.k) {
-    const int have = wave_top<T>(x, vmax, lr, c0, cend, p.k, lane, score_lds + wave * WAVE_TOP_LDS, [&](int r, u64 key) { write_top(p, row, r, key, a); });
+    const int have = wave_top<T>(x, vmax, lr, c0, cend, p.k, lane, reinterpret_cast<typename WaveKey<T>::type*>(score_lds) + wave * WAVE_TOP_LDS, [&](int r, u64 key) { write_top(p, row, r, key, a); });
     if (lane >= have && lane < p.k) write_top(p, row, lane, 0, a);
   }
 }
@@ -395,7 +415,7 @@ __global__ __launch_bounds__(256) void token_logprobs_join_kernel(ScoreParams p)
 template <typename T, int W, int N>
 __global__ __launch_bounds__(W * 64) void token_logprobs_top_kernel(ScoreParams p) {
   constexpr int LIST = 128 * W, SETS = N < 4 ? N : 4;
-  __shared__ u64 cand[GROUP_CAND + 2];
+  __shared__ __attribute__((aligned(16))) u64 cand[GROUP_CAND + 4];
   __shared__ uint32_t list_max[LIST];
   __shared__ int list_id[LIST];
   __shared__ float sm_thr[W + 1];
@@ -529,7 +549,7 @@ __global__ __launch_bounds__(W * 64) void token_logprobs_top_kernel(ScoreParams 
   }
   const int n = sm_n;
   const RowSums a = sm_row;
-  if (tid < 2) cand[n + tid] = 0;
+  if (tid < 4) cand[n + tid] = 0;
   __syncthreads();
   rank_keys(cand, n, k, tid, W * 64, [&](int r, u64 key) { write_top(p, row, r, key, a); });
   for (int r = n + tid; r < k; r += W * 64) write_top(p, row, r, 0, a);
@@ -575,7 +595,7 @@ __global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(ScoreGradParams
 }
 
 // ---- distillation ---------------------------------------------------------------------------------------------------------
-// A row's list, two entries a lane: class (or -1), p and log p, and the list's mass.
+// A row's list, two entries a lane (one, and no work for the other, up to 64 entries): class (or -1), p and log p, and the list's mass.
 struct Listed { int id[2]; float p[2], logp[2], mass; };
 __device__ __forceinline__ Listed load_listed(const int64_t* idx, const float* tl, int K, int C, float inv_t, int tail, int lane) {
   Listed L;
@@ -584,7 +604,8 @@ __device__ __forceinline__ Listed load_listed(const int64_t* idx, const float* t
   for (int h = 0; h < 2; ++h) {
     const int j = lane + 64 * h;
     L.id[h] = -1;
-    t[h] = -INFINITY;
+    L.p[h] = 0.f;
+    L.logp[h] = t[h] = -INFINITY;
     if (j < K) {
       const int64_t i = idx[j];
       const float v = tl[j];
@@ -593,27 +614,29 @@ __device__ __forceinline__ Listed load_listed(const int64_t* idx, const float* t
   }
   if (tail) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      L.logp[h] = t[h];
-      L.p[h] = L.id[h] >= 0 ? __expf(t[h]) : 0.f;
-    }
-  } else {
-    const float m = fmaxf(max_wave(fmaxf(t[0], t[1])), -FMAX);
-    float e[2];
+    for (int h = 0; h < 2; ++h)
+      if (h * 64 < K) {
+        L.logp[h] = t[h];
+        L.p[h] = L.id[h] >= 0 ? __expf(t[h]) : 0.f;
+      }
+    L.mass = sum_wave(L.p[0] + L.p[1]);
+    return L;
+  }
+  const float m = fmaxf(max_wave(K > 64 ? fmaxf(t[0], t[1]) : t[0]), -FMAX);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+  for (int h = 0; h < 2; ++h)
+    if (h * 64 < K) {
       L.logp[h] = (t[h] - m) * inv_t;
-      e[h] = L.id[h] >= 0 ? __expf(L.logp[h]) : 0.f;
+      L.p[h] = L.id[h] >= 0 ? __expf(L.logp[h]) : 0.f;
     }
-    const float z = sum_wave(e[0] + e[1]);
-    const float logz = __logf(z);
+  const float z = sum_wave(L.p[0] + L.p[1]), over = 1.f / z, logz = __logf(z);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      L.p[h] = z == 0.f ? 0.f : e[h] / z;
+  for (int h = 0; h < 2; ++h)
+    if (h * 64 < K) {
+      L.p[h] = z == 0.f ? 0.f : L.p[h] * over;
       L.logp[h] -= logz;
     }
-  }
-  L.mass = sum_wave(L.p[0] + L.p[1]);
+  L.mass = z == 0.f ? 0.f : z * over;   // 1; 0 of a row without entries; NaN of one with
   return L;
 }
 
@@ -883,7 +906,7 @@ static int launch_score(const ScoreParams& p, hipStream_t st) {
   int rc = need_grid(what, grid);
   if (rc) return rc;
   if (p.units == 1) {
-    token_logprobs_fwd_kernel<T, false><<<(unsigned)grid, 256, p.k ? 4 * WAVE_TOP_LDS * 8 : 0, st>>>(p);
+    token_logprobs_fwd_kernel<T, false><<<(unsigned)grid, 256, p.k ? 4 * WAVE_TOP_LDS * sizeof(typename WaveKey<T>::type) : 0, st>>>(p);
     return check_launch(what);
   }
   token_logprobs_fwd_kernel<T, true><<<(unsigned)grid, 256, 0, st>>>(p);

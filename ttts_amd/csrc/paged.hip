@@ -53,10 +53,9 @@ template <> struct Frag<_Float16> {
 // The next tile's keys are loaded as soon as this one's have been multiplied, its values after the second product (held twice over,
 // 209 instead of 145 registers at 128 columns, they were no faster), the table entries another tile ahead.  The queries of a shared
 // head fill rows of the products that are there anyway, so a cached key is read once for up to 16 of them.
-constexpr int PAGED_WAVES = 8;
-template <typename T, int DH>
-__global__ __launch_bounds__(PAGED_WAVES * 64) void attn_paged_decode_kernel(PagedParams p) {
-  constexpr int NW = PAGED_WAVES, W = DH / 16, KC = DH / 32;
+template <typename T, int DH, int NW>
+__global__ __launch_bounds__(NW * 64) void attn_paged_decode_kernel(PagedParams p) {
+  constexpr int W = DH / 16, KC = DH / 32;
   typedef T T8 __attribute__((ext_vector_type(8)));
   typedef T TW __attribute__((ext_vector_type(W)));
   extern __shared__ __attribute__((aligned(16))) float paged_lds[];
@@ -204,47 +203,52 @@ __global__ __launch_bounds__(PAGED_WAVES * 64) void attn_paged_decode_kernel(Pag
   }
 }
 
-// the chunks of a split sequence: one workgroup per (sequence, query head).  First every chunk's weight 2^(m - M), a chunk per thread, then
-// DH / 4 lanes per chunk add up the weighted parts: two rounds of independent loads, whatever the number of chunks (<= PAGED_MAX_CHUNKS).
+// The chunks of a split sequence: one workgroup per (sequence, query head).  Every chunk's weight 2^(m - M), a chunk per thread, and DH / 4
+// lanes per chunk that add up the weighted parts; the first 8 parts of a thread are on their way before the weights (and the
+// length) are known, so it takes one round of loads up to 8 * 1024 / DH chunks.
 constexpr int PAGED_MAX_CHUNKS = 2048;
 template <typename T, int DH>
 __global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedParams p) {
-  constexpr int LPC = DH / 4, G = 256 / LPC;
+  constexpr int LPC = DH / 4, G = 256 / LPC, AHEAD = 8;
   __shared__ float sm_w[PAGED_MAX_CHUNKS];
   __shared__ float4 sm_o[G][LPC];
   __shared__ float sm_r[2][4];
   const int64_t mh = blockIdx.x, m = mh / p.H;
   const int tid = threadIdx.x, sub = tid % LPC, grp = tid / LPC;
-  const int len = min(p.lens[m], p.width << p.page_shift);
-  const int n = len > 0 ? (len + p.chunk - 1) / p.chunk : 0;
   const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + mh * p.chunks;
   const float4* po = reinterpret_cast<const float4*>(p.part_o) + mh * p.chunks * LPC + sub;
-  float M = -3.0e38f;
-  for (int c = tid; c < n; c += 256) M = fmaxf(M, ml[c].x);
+  const int len = min(p.lens[m], p.width << p.page_shift);
+  float4 ahead[AHEAD];                       // (parts behind the sequence's end were not written: whatever the memory holds, not used)
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+  for (int i = 0; i < AHEAD; ++i) ahead[i] = po[(int64_t)min(grp + i * G, p.chunks - 1) * LPC];
+  const float2 s0 = ml[min(tid, p.chunks - 1)];
+  const int n = len > 0 ? (len + p.chunk - 1) / p.chunk : 0;
+  float M = tid < n ? s0.x : -3.0e38f;
+  for (int c = tid + 256; c < n; c += 256) M = fmaxf(M, ml[c].x);
+  M = over_wave(M, max_op);
   if ((tid & 63) == 0) sm_r[0][tid >> 6] = M;
   __syncthreads();
   M = fmaxf(fmaxf(sm_r[0][0], sm_r[0][1]), fmaxf(sm_r[0][2], sm_r[0][3]));
   float L = 0.f;
   for (int c = tid; c < n; c += 256) {
-    const float2 s = ml[c];
+    const float2 s = c < 256 ? s0 : ml[c];
     const float w = __builtin_amdgcn_exp2f(s.x - M);
     sm_w[c] = w;
     L += s.y * w;
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) L += __shfl_xor(L, o, 64);
+  L = over_wave(L, add_op);
   if ((tid & 63) == 0) sm_r[1][tid >> 6] = L;
   __syncthreads();
   L = (sm_r[1][0] + sm_r[1][1]) + (sm_r[1][2] + sm_r[1][3]);
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-  for (int c = grp; c < n; c += G) {
-    const float4 v = po[(int64_t)c * LPC];
-    const float w = sm_w[c];
+  auto add = [&](const float4& v, float w) {
     o.x = fmaf(v.x, w, o.x); o.y = fmaf(v.y, w, o.y); o.z = fmaf(v.z, w, o.z); o.w = fmaf(v.w, w, o.w);
-  }
+  };
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i)
+    if (grp + i * G < n) add(ahead[i], sm_w[grp + i * G]);
+#pragma unroll 8
+  for (int c = grp + AHEAD * G; c < n; c += G) add(po[(int64_t)c * LPC], sm_w[c]);
   sm_o[grp][sub] = o;
   __syncthreads();
   if (tid < DH) {
@@ -256,25 +260,34 @@ __global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedParams p) {
   }
 }
 
-// How sequences of up to `longest` keys (what the table holds; their lengths stay on the device) are split into chunks, one workgroup each:
-//  * not at all up to 768 keys (three tiles a wave): 613 keys of one sequence, 8 heads of 64: 6.0 us; split 6.4 - 7.0, two launches.
+// How sequences of up to `longest` keys (what the table holds; their lengths stay on the device) are split into chunks, one workgroup each;
+// units = workgroups of an unsplit call:
+//  * not at all up to 768 keys (three tiles for each of 8 waves): 613 keys of one sequence, 8 heads of 64: 6.0 us; split 6.4 - 7.0.
+//    Nor up to 4096 keys where the units alone give every CU two workgroups (of 4 waves then): 64 sequences up to 2404, 8 heads:
+//    40.7 us, 42.5 split; 96 up to 4096, 8 heads of 128: 148 us, 150 - 170 split in two to four.
 //  * into 256 keys, one tile a wave, while that gives the card's 256 CUs one workgroup each at most: 2404 keys of one sequence
 //    6.9 us, against 10.8 in chunks of 1024; more workgroups than CUs cost more than they give (20000 keys: 12.2 us, 14.2 with 512).
 //  * beyond that into 1024 keys or more, about 1024 workgroups (4 sequences of 130000 keys: 178 us, 188 with 2048), or about 2048
-//    where a sequence gets few chunks, which a ragged batch fills unevenly (96 sequences up to 4096: 150 us, 173 with 1024).
-static void paged_split(int64_t units, int64_t longest, int& chunk, int& chunks) {
+//    where a sequence gets few chunks, and chunks of at most 4096 keys while there are under 16384 of them: the lengths may be
+//    anything up to the longest, and a workgroup's chunk is what the others wait for.
+struct PagedSplit { int chunk, chunks, waves; };
+static PagedSplit paged_split(int64_t units, int64_t longest) {
   auto least = [](int64_t a, int64_t b) { return a < b ? a : b; };
+  auto most = [](int64_t a, int64_t b) { return a > b ? a : b; };
+  PagedSplit s;
   int64_t n = 1;
-  if (longest > 768) {
+  const bool many = units >= 512;
+  if (longest > (many ? 4096 : 768)) {
     int64_t wide = cdiv(1024, units);
     if (wide < 8) wide = cdiv(2048, units);
-    n = least(cdiv(longest, 1024), wide);
-    const int64_t fine = least(cdiv(longest, 256), 256 / units);
-    n = n > fine ? n : fine;
+    n = most(least(cdiv(longest, 1024), wide), least(cdiv(longest, 256), 256 / units));
+    n = most(n, least(cdiv(longest, 4096), 16384 / units));
   }
-  const int64_t c = cdiv(cdiv(longest, n), 32 * PAGED_WAVES) * 32 * PAGED_WAVES;
-  chunk = (int)c;
-  chunks = (int)cdiv(longest, c);
+  s.waves = many && n == 1 ? 4 : 8;
+  const int64_t c = cdiv(cdiv(longest, n), 32 * s.waves) * 32 * s.waves;
+  s.chunk = (int)c;
+  s.chunks = (int)cdiv(longest, c);
+  return s;
 }
 
 }  // namespace ttts
@@ -314,19 +327,21 @@ static int64_t paged_bytes(int64_t M, int64_t H, int dh, int chunks) { return ch
 
 extern "C" int64_t ttts_attn_paged_decode_workspace_bytes(int32_t M, int32_t H, int32_t Hkv, int32_t head_dim, int32_t page, int32_t width) {
   if (M <= 0 || Hkv <= 0 || H < Hkv || head_dim <= 0 || page <= 0 || width <= 0) return 0;
-  int chunk, chunks;
-  paged_split(M * (int64_t)Hkv * paged_tiles(H, Hkv), (int64_t)width * page, chunk, chunks);
-  return paged_bytes(M, H, head_dim, chunks);
+  return paged_bytes(M, H, head_dim, paged_split(M * (int64_t)Hkv * paged_tiles(H, Hkv), (int64_t)width * page).chunks);
 }
 
-template <typename T, int DH>
-static int launch_paged(const PagedParams& p, int64_t grid, int64_t rows, hipStream_t st) {
+template <typename T, int DH, int NW>
+static int launch_paged_waves(const PagedParams& p, int64_t grid, hipStream_t st) {
   static OnceFlag once;
-  const int lds = PAGED_WAVES * (p.group < 16 ? p.group : 16) * (DH + 2) * 4;
-  if (lds_opt_in(once, (const void*)attn_paged_decode_kernel<T, DH>, PAGED_WAVES * 16 * (DH + 2) * 4) != hipSuccess)
+  const int lds = NW * (p.group < 16 ? p.group : 16) * (DH + 2) * 4;
+  if (lds_opt_in(once, (const void*)attn_paged_decode_kernel<T, DH, NW>, NW * 16 * (DH + 2) * 4) != hipSuccess)
     return fail(TTTS_EHIP, "attn_paged_decode: LDS opt-in failed");
-  attn_paged_decode_kernel<T, DH><<<(unsigned)grid, PAGED_WAVES * 64, lds, st>>>(p);
-  const int rc = check_launch("attn_paged_decode");
+  attn_paged_decode_kernel<T, DH, NW><<<(unsigned)grid, NW * 64, lds, st>>>(p);
+  return check_launch("attn_paged_decode");
+}
+template <typename T, int DH>
+static int launch_paged(const PagedParams& p, int waves, int64_t grid, int64_t rows, hipStream_t st) {
+  const int rc = waves == 4 ? launch_paged_waves<T, DH, 4>(p, grid, st) : launch_paged_waves<T, DH, 8>(p, grid, st);
   if (rc || p.chunks == 1) return rc;
   attn_paged_join_kernel<T, DH><<<(unsigned)rows, 256, 0, st>>>(p);
   return check_launch("attn_paged_decode join");
@@ -353,7 +368,8 @@ extern "C" int ttts_attn_paged_decode(const void* q, int64_t q_stride_m, int64_t
   p.H = H; p.Hkv = Hkv; p.group = H / Hkv; p.tiles = (int)paged_tiles(H, Hkv); p.page_shift = __builtin_ctz(page); p.P = P; p.width = width;
   p.scale_log2 = scale * 1.4426950408889634f;
   const int64_t units = M * (int64_t)Hkv * p.tiles;
-  paged_split(units, (int64_t)width * page, p.chunk, p.chunks);
+  const PagedSplit sp = paged_split(units, (int64_t)width * page);
+  p.chunk = sp.chunk; p.chunks = sp.chunks;
   const int64_t grid = units * p.chunks, rows = (int64_t)M * H, need = paged_bytes(M, H, head_dim, p.chunks);
   TTTS_REQUIRE(grid <= 0x7fffffff && rows <= 0x7fffffff, "attn_paged_decode: more work than one launch holds (M %d, H %d)", M, H);
   TTTS_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned16(workspace)),
@@ -362,8 +378,8 @@ extern "C" int ttts_attn_paged_decode(const void* q, int64_t q_stride_m, int64_t
   p.part_ml = p.part_o + rows * p.chunks * head_dim;
   hipStream_t st = as_stream(stream);
   if (dtype == TTTS_DTYPE_BF16)
-    return head_dim == 32 ? launch_paged<bf16, 32>(p, grid, rows, st) : head_dim == 64 ? launch_paged<bf16, 64>(p, grid, rows, st)
-                                                                                       : launch_paged<bf16, 128>(p, grid, rows, st);
-  return head_dim == 32 ? launch_paged<_Float16, 32>(p, grid, rows, st) : head_dim == 64 ? launch_paged<_Float16, 64>(p, grid, rows, st)
-                                                                                         : launch_paged<_Float16, 128>(p, grid, rows, st);
+    return head_dim == 32 ? launch_paged<bf16, 32>(p, sp.waves, grid, rows, st) : head_dim == 64 ? launch_paged<bf16, 64>(p, sp.waves, grid, rows, st)
+                                                                                       : launch_paged<bf16, 128>(p, sp.waves, grid, rows, st);
+  return head_dim == 32 ? launch_paged<_Float16, 32>(p, sp.waves, grid, rows, st) : head_dim == 64 ? launch_paged<_Float16, 64>(p, sp.waves, grid, rows, st)
+                                                                                         : launch_paged<_Float16, 128>(p, sp.waves, grid, rows, st);
 }

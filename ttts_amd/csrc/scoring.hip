@@ -314,9 +314,9 @@ struct ScoreParams {
   const int64_t* tokens;
   float *logp, *entropy, *stats, *top_logp;
   int64_t* top_idx;
-  float4* part;          // long rows: [R, units] (m, z, s, -) of each wave's 2048 columns,
+  float4* part;          // long rows: [R, units] (m, z, s, -) of each wave's columns,
   uint32_t* part_max;    // and with alternatives [R, units, 64]: ord() of the maximum of each lane's 32 columns
-  int R, C, k, units;
+  int R, C, k, units, unit_cols;
   float inv_t;
 };
 
@@ -334,7 +334,7 @@ __device__ __forceinline__ void write_top(const ScoreParams& p, int64_t row, int
   p.top_logp[row * p.k + r] = have ? (unord((uint32_t)(key >> 32)) - a.m) * p.inv_t - __builtin_amdgcn_logf(a.z) * LN2 : nan ? a.z : -INFINITY;
 }
 
-// One wave per row (LONG false), or per 2048 columns of a row.  (Waves that went through several of them, the next one's loads under this
+// One wave per row (LONG false), or per unit of up to 2048 columns of a row.  (Waves that went through several of them, the next one's loads under this
 // one's arithmetic, were slower at every grid: 118 - 125 us instead of 109 for logits of 2048 x 100003 with 64 alternatives.)
 template <typename T, bool LONG>
 __global__ __launch_bounds__(256) void token_logprobs_fwd_kernel(ScoreParams p) {
@@ -346,7 +346,7 @@ __global__ __launch_bounds__(256) void token_logprobs_fwd_kernel(ScoreParams p) 
   if (LONG) split_id(id, p.units, row, unit);
   if (row >= p.R) return;
   const T* lr = (const T*)p.logits + row * p.ldl;
-  const int c0 = unit * WAVE_COLS, cend = min(p.C, c0 + WAVE_COLS);
+  const int c0 = unit * p.unit_cols, cend = min(p.C, c0 + p.unit_cols);
   float x[NV][8], vmax[NV], lmax = -INFINITY;
   int64_t tok = -1;
   float xt = 0.f;
@@ -467,8 +467,8 @@ __global__ __launch_bounds__(W * 64) void token_logprobs_top_kernel(ScoreParams 
     __syncthreads();
   }
   auto push_eight = [&](int id, int i, float t, bool above) {   // columns that reach t (or lie above it) become keys
-    const int c = (id >> 6) * WAVE_COLS + i * 512 + (id & 63) * 8;
-    if (c >= p.C) return;
+    const int c = (id >> 6) * p.unit_cols + i * 512 + (id & 63) * 8;
+    if (i * 512 >= p.unit_cols || c >= p.C) return;
     float v[8];
     load8<T>(lr + c, p.C - c, v);
 #pragma unroll
@@ -553,6 +553,118 @@ __global__ __launch_bounds__(W * 64) void token_logprobs_top_kernel(ScoreParams 
   __syncthreads();
   rank_keys(cand, n, k, tid, W * 64, [&](int r, u64 key) { write_top(p, row, r, key, a); });
   for (int r = n + tid; r < k; r += W * 64) write_top(p, row, r, 0, a);
+}
+
+// The same for rows of up to 8 units by one wave each, four rows a workgroup and no barrier: all 512 groups are in its registers, so the
+// threshold is exact at once (rows of 8194 classes, 25000 of them, 20 alternatives: 135 us, 197 with a workgroup each).  Where the
+// candidates do not fit (values that repeat, or a row whose largest ones crowd into few groups): the k-th largest column itself,
+// searched by counting over the row, the fewer than k columns above it, and the lowest classes at it.
+template <typename T>
+__global__ __launch_bounds__(256) void token_logprobs_top_wave_kernel(ScoreParams p) {
+  constexpr int UNITS = 8, CAND = 320, LIST = 128;
+  __shared__ __attribute__((aligned(16))) u64 sm_cand[4][CAND + 4];
+  __shared__ int sm_list[4][LIST];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t row = (int64_t)blockIdx.x * 4 + wave;
+  if (row >= p.R) return;
+  const T* lr = (const T*)p.logits + row * p.ldl;
+  const uint32_t* gm = p.part_max + row * p.units * 64;
+  u64* cand = sm_cand[wave];
+  int* list = sm_list[wave];
+  const int k = p.k;
+  uint32_t g[UNITS];
+#pragma unroll
+  for (int i = 0; i < UNITS; ++i) g[i] = i < p.units ? gm[i * 64 + lane] : 0;
+  const RowSums a = join_sums(p, row, lane);
+  if (lane == 0) write_long_row<T>(p, row, a);
+  float thr = group_threshold<T, UNITS>(g, p.units, k, true);
+  int n = 0, listed = 0;
+  {
+    const uint32_t tb = ord(thr);
+#pragma unroll
+    for (int i = 0; i < UNITS; ++i) {
+      const u64 mask = __ballot(g[i] >= tb);
+      if (mask) {
+        const int at = listed + lanes_below(mask);
+        if (g[i] >= tb && at < LIST) list[at] = i * 64 + lane;
+        listed += __builtin_popcountll(mask);
+      }
+    }
+  }
+  wave_fence();
+  // v: the lane's 8 columns from c on; test(v) of them become keys
+  auto push = [&](const float (&v)[8], int c, auto test) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const bool in = test(v[j]);
+      const u64 mask = __ballot(in);
+      if (mask) {
+        const int at = n + lanes_below(mask);
+        if (in && at < CAND) cand[at] = top_key(v[j], c + j);
+        n += __builtin_popcountll(mask);
+      }
+    }
+  };
+  auto eight = [&](int c, bool mine, float (&v)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = -INFINITY;
+    if (mine && c < p.C) load8<T>(lr + c, p.C - c, v);
+  };
+  bool full = listed > LIST;
+  if (!full) {
+    for (int s = 0; s < listed * NV; s += 64) {
+      const int task = s + lane, id = task < listed * NV ? list[task / NV] : 0;
+      const int c = (id >> 6) * p.unit_cols + (task % NV) * 512 + (id & 63) * 8;
+      float v[8];
+      eight(c, task < listed * NV && (task % NV) * 512 < p.unit_cols, v);
+      push(v, c, [&](float x) { return x >= thr; });
+    }
+    full = n > CAND;
+  }
+  if (full) {
+    float v[8];
+    uint32_t t = 0;
+    for (uint32_t bit = 0x80000000u; bit >> LowBits<T>::n; bit >>= 1) {
+      float cnt = 0.f;                        // (whole numbers up to 16384)
+      for (int c0 = 0; c0 < p.C; c0 += 512) {
+        eight(c0 + lane * 8, true, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) cnt += ord(v[j]) >= (t | bit) && v[j] == v[j] ? 1.f : 0.f;
+      }
+      if (sum_wave(cnt) >= (float)k) t |= bit;
+    }
+    thr = threshold_of<T>(t);
+    n = 0;
+    for (int c0 = 0; c0 < p.C; c0 += 512) {
+      eight(c0 + lane * 8, true, v);
+      push(v, c0 + lane * 8, [&](float x) { return x > thr; });
+    }
+    for (int c0 = 0; c0 < p.C && n < k; c0 += 512) {
+      eight(c0 + lane * 8, true, v);
+      int mine = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) mine += v[j] == thr;
+      int upto = mine;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(upto, o, 64);
+        if (lane >= o) upto += u;
+      }
+      int at = n + upto - mine;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (v[j] == thr) {
+          if (at < k) cand[at] = top_key(v[j], c0 + lane * 8 + j);
+          ++at;
+        }
+      n = min(k, n + __shfl(upto, 63, 64));
+    }
+    n = min(n, k);
+  }
+  if (lane < 4) cand[n + lane] = 0;
+  wave_fence();
+  rank_keys(cand, n, k, lane, 64, [&](int r, u64 key) { write_top(p, row, r, key, a); });
+  if (lane >= n && lane < k) write_top(p, row, lane, 0, a);
 }
 
 // ---- gradient of the log-probabilities: one thread per 8 columns, everything of the row is known -------------------------
@@ -645,8 +757,8 @@ struct DistillParams {
   const int64_t* idx;
   const float* tlogp;
   float *row_loss, *stats;
-  float4* part;        // long rows: [R, units] (m, z of the listed classes, z of the others, -) of each wave's 2048 columns
-  int R, C, K, tail, units;
+  float4* part;        // long rows: [R, units] (m, z of the listed classes, z of the others, -) of each wave's columns
+  int R, C, K, tail, units, unit_cols;
   float inv_t;
 };
 // by one wave: the row's loss from its sums (listed and other classes apart with tail, else all in zr) and the listed classes' logits
@@ -686,7 +798,7 @@ __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillParams p) {
   if (LONG) split_id(id, p.units, row, unit);
   if (row >= p.R) return;
   const T* lr = (const T*)p.logits + row * p.ldl;
-  const int c0 = unit * WAVE_COLS, cend = min(p.C, c0 + WAVE_COLS);
+  const int c0 = unit * p.unit_cols, cend = min(p.C, c0 + p.unit_cols);
   Raw<T> raw;
   load_raw(raw, lr, c0, cend, lane);
   Listed L;
@@ -891,8 +1003,9 @@ static int need_grid(const char* what, int64_t grid) {
   return TTTS_OK;
 }
 
-// waves of a long row; 1: the row is one wave's
-static int row_units(int C) { return (int)cdiv(C, WAVE_COLS); }
+// waves of a long row (1: the row is one wave's) and the columns of each, whole 512s: as few steps as 2048 each, but no small rest
+static int unit_columns(int C) { return (int)(cdiv(cdiv(C, 512), cdiv(C, WAVE_COLS)) * 512); }
+static int row_units(int C) { return (int)cdiv(C, unit_columns(C)); }
 
 extern "C" int64_t ttts_token_logprobs_workspace_bytes(int32_t R, int32_t C, int32_t top_k) {
   if (R <= 0 || C <= WAVE_COLS || top_k < 0) return 0;
@@ -913,7 +1026,7 @@ static int launch_score(const ScoreParams& p, hipStream_t st) {
   rc = check_launch(what);
   if (rc) return rc;
   if (p.k == 0) token_logprobs_join_kernel<T><<<(unsigned)cdiv(p.R, 4), 256, 0, st>>>(p);
-  else if (p.units <= 8) token_logprobs_top_kernel<T, 4, 2><<<p.R, 256, 0, st>>>(p);       // up to 16384 classes
+  else if (p.units <= 8) token_logprobs_top_wave_kernel<T><<<(unsigned)cdiv(p.R, 4), 256, 0, st>>>(p);   // up to 16384 classes
   else if (p.units <= 64) token_logprobs_top_kernel<T, 4, 16><<<p.R, 256, 0, st>>>(p);     // up to 131072
   else token_logprobs_top_kernel<T, 16, 32><<<p.R, 1024, 0, st>>>(p);                      // up to TTTS_SCORE_MAX_CLASSES
   return check_launch("token_logprobs_fwd join");
@@ -929,7 +1042,7 @@ extern "C" int ttts_token_logprobs_fwd(const void* logits, int32_t dtype, int64_
   TTTS_REQUIRE(tokens && logp && entropy && stats && (top_k == 0 || (top_logp && top_idx)), "token_logprobs_fwd: null pointer");
   rc = need_workspace("token_logprobs_fwd", ttts_token_logprobs_workspace_bytes(R, C, top_k), workspace, workspace_bytes);
   if (rc) return rc;
-  ScoreParams p{logits, ldl, tokens, logp, entropy, stats, top_logp, top_idx, (float4*)workspace, nullptr, R, C, top_k, row_units(C), 1.0f / temperature};
+  ScoreParams p{logits, ldl, tokens, logp, entropy, stats, top_logp, top_idx, (float4*)workspace, nullptr, R, C, top_k, row_units(C), unit_columns(C), 1.0f / temperature};
   p.part_max = (uint32_t*)(p.part + (int64_t)R * p.units);
   TTTS_BY_TYPE(dtype, "token_logprobs_fwd", rc = launch_score<T>(p, as_stream(stream)));
   return rc;
@@ -981,7 +1094,7 @@ extern "C" int ttts_distill_fwd(const void* logits, int32_t dtype, int64_t ldl, 
   TTTS_REQUIRE(teacher_idx && teacher_logp && row_loss && stats, "distill_fwd: null pointer");
   rc = need_workspace("distill_fwd", ttts_distill_workspace_bytes(R, C), workspace, workspace_bytes);
   if (rc) return rc;
-  const DistillParams p{logits, ldl, teacher_idx, teacher_logp, row_loss, stats, (float4*)workspace, R, C, K, tail != 0, row_units(C), 1.0f / temperature};
+  const DistillParams p{logits, ldl, teacher_idx, teacher_logp, row_loss, stats, (float4*)workspace, R, C, K, tail != 0, row_units(C), unit_columns(C), 1.0f / temperature};
   TTTS_BY_TYPE(dtype, "distill_fwd", rc = launch_distill<T>(p, as_stream(stream)));
   return rc;
 }

@@ -113,6 +113,27 @@ def test_attn_paged_decode_long_and_ragged(dtype, dh, Hkv, group, page, lens):
     _check(out, lse, _ref(q, kp, vp, table, lens, dh ** -0.5), lens, dtype)
 
 
+@pytest.mark.parametrize("dtype,dh,M,Hkv,group,page,longest", [
+    (torch.bfloat16, 64, 70, 8, 1, 16, 300), (torch.float16, 128, 33, 16, 2, 32, 200), (torch.bfloat16, 32, 520, 1, 5, 16, 90),
+    (torch.bfloat16, 64, 70, 8, 1, 16, 5001)])
+def test_many_sequences(dtype, dh, M, Hkv, group, page, longest):
+    """As many sequences and heads as fill the card: no split up to 4096 keys, chunks beyond."""
+    from ttts_amd import ops
+    g = _gen(M)
+    lens = torch.randint(0, min(longest, 130), (M,), generator=g).tolist()
+    lens[3], lens[M - 1] = longest, 1
+    table, P, free = _tables(lens, page, 1)
+    kp, vp = _cache(P, Hkv, page, dh, dtype, 2)
+    _poison(kp, vp, table, lens, page, free)
+    q = (torch.randn(M, Hkv * group, dh, generator=_gen(4)) * 2).to(dtype).cuda()
+    out, lse = ops.attn_paged_decode(q, kp, vp, table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), dh ** -0.5)
+    some = sorted({0, 3, 4, 5, M // 2, M - 2, M - 1})
+    pick = torch.tensor(some)
+    ref = _ref(q[pick.cuda()], kp, vp, table[pick], [lens[i] for i in some], dh ** -0.5)
+    _check(out[pick.cuda()], lse[pick.cuda()], ref, lens, dtype)
+    assert torch.isfinite(out).all() and torch.equal(torch.isinf(lse).all(dim=1).cpu(), torch.tensor(lens) == 0)
+
+
 def test_lengths_and_tables_out_of_range():
     """A negative length, one beyond the table, table entries outside the cache in the middle and over a whole sequence."""
     from ttts_amd import ops

@@ -169,6 +169,32 @@ def test_token_logprobs_special_rows(dtype, C):
     _inside(d.cpu()[keep], ref, size * (4 * _r(C) + 8 * U * 100) + 4 * U + _half_step(ref, dtype), "dlogits")
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("C", [65, 100, 2048, 2049, 2561, 5000, 8194, 16384, 16385, 40000, 131072, 131081, 600001])
+@pytest.mark.parametrize("top_k", [1, 33, 64])
+def test_alternatives_where_values_repeat_or_crowd(dtype, C, top_k):
+    """Rows whose largest values sit in few of a wave's lanes, sorted rows, rows of one, two and few values, few classes left: the
+    alternatives are the stable order's, whatever the search for them runs into."""
+    from ttts_amd import ops
+    g = _gen(C + top_k)
+    base = torch.randn(C, generator=g)
+    at = torch.arange(C)
+    rows = [base + 30.0 * ((at // 8) % 64 == 5),                        # one lane's columns
+            base + 30.0 * ((at // 8) % 64 == 5) * (at % 8 == 3) + 20.0 * (at % 8 == 0),
+            base.sort().values, base.sort(descending=True).values,
+            torch.full((C,), -2.5), torch.where(torch.rand(C, generator=g) < 0.5, 1.0, 0.0), torch.where(at == C - 1, 1.0, 0.0),
+            torch.randint(-3, 1, (C,), generator=g).float(),            # values below zero, repeated
+            torch.where(at % 97 == 64, base, torch.tensor(-math.inf)),
+            4096.0 + (at % 7).float() * 2.0 ** -11 if dtype == torch.float32 else base.round(),
+            torch.where(at < C // 2, torch.tensor(LOWEST[dtype]), torch.tensor(-math.inf)),
+            -base.abs() - 3.0]
+    x = torch.stack(rows).to(dtype).cuda()
+    r = ops.token_logprobs_fwd(x, torch.zeros(len(rows), dtype=torch.int64, device="cuda"), top_k=top_k)
+    _, _, tl, ti, _, _ = _ref_logprobs(x, torch.zeros(len(rows), dtype=torch.int64), C, top_k, 1.0)
+    assert torch.equal(r.top_idx.cpu(), ti)
+    _inside(r.top_logp, tl, _r(C) + 4 * U * tl.abs().nan_to_num(posinf=0.0), "top_logp")
+
+
 def test_logits_far_from_zero():
     """The statistics hand the maximum and log Z on apart: rows around 4096 lose nothing of their gradient."""
     from ttts_amd import ops

@@ -179,6 +179,8 @@ class GptEngine:
         self._graph_key = None
         # buffers / descriptor tables / captured graphs of the last few batch shapes (see _ensure_buffers)
         self._shape_cache = collections.OrderedDict()
+        self._teacher = None         # a teacher's alternatives for the tokens last set (train_step's `teacher`)
+        self.distill_loss = None     # their loss after the backward: device scalar
         self._capture_error = None   # one line on why a hipGraph capture was refused (bench.py reports it), else None
 
     # ---- parameter plumbing -------------------------------------------------------------------------------
@@ -405,6 +407,7 @@ class GptEngine:
         if Tt > self.c["max_text_tokens"] + 2 or Tm > self.c["max_mel_tokens"] + 2:
             raise ValueError("sequence exceeds the learned position tables (text %d, mel %d)" % (Tt, Tm))
         self._ensure_buffers(B, Tt, Tm)
+        self._teacher = None             # it belonged to the last tokens
         b = self.b
         b["text_inp"].copy_(text_inp, non_blocking=True)
         b["text_tar"].copy_(text_tar.reshape(-1), non_blocking=True)
@@ -427,6 +430,7 @@ class GptEngine:
         if Tt + 2 > c["max_text_tokens"] + 2 or Tm + 2 > c["max_mel_tokens"] + 2:
             raise ValueError("sequence exceeds the learned position tables (text %d, mel %d)" % (Tt + 2, Tm + 2))
         self._ensure_buffers(B, Tt + 2, Tm + 2)
+        self._teacher = None             # it belonged to the last tokens
         b = self.b
         ops.gpt_prepare_tokens(text_inputs, mel_codes, [int(w) // comp + 1 for w in wl], Tt, Tm, c["start_text_token"],
                                c["stop_text_token"], c["start_mel_token"], c["stop_mel_token"], b["text_inp"], b["text_tar"],
@@ -572,6 +576,11 @@ class GptEngine:
         G = lambda k: self.view(self.grads, k)   # noqa: E731
         ops.ce_bwd(b["logits_t"], b["text_tar"], b["rows_t"][1], b["dlog_t"], self.nt, w_text, g_text_dev)
         ops.ce_bwd(b["logits_m"], b["mel_tar"], b["rows_m"][1], b["dlog_m"], self.nm, w_mel, g_mel_dev)
+        if self._teacher is not None:
+            idx, logp, g_rows, kw = self._teacher
+            rows, stats = ops.distill_fwd(b["logits_m"], idx, logp, C=self.nm, **kw)
+            ops.distill_bwd(b["logits_m"], idx, logp, stats, g_rows, C=self.nm, dlogits=b["dlog_m"], accumulate=True, **kw)
+            self.distill_loss = rows.mean()
         enc_t, enc_m = b["enc"][:B * Tt], b["enc"][B * Tt:]
         fork()
         with torch.cuda.stream(side):
@@ -705,7 +714,26 @@ class GptEngine:
         state-dict order: embeddings, h.0 .. h.L-1, ln_f, position tables, final_norm, heads."""
         return exchange_ranges(self.offsets, self.n_arena, self.c["layers"], split)
 
-    def train_step(self, tokens, w_text=0.01, w_mel=1.0, capture=False, exchange=None, exchange_range=None, **opt):
+    def set_teacher(self, teacher_idx, teacher_logp=None, weight=1.0, temperature=1.0, tail=True):
+        """The backward of the tokens last set also descends weight * mean over the mel positions of KL(teacher || student), from a
+        teacher's alternatives: teacher_idx int64 / teacher_logp f32 [B, Tm, K], as UnifiedVoice.score returns them (at the same
+        temperature; tail False: any logits of the listed classes).  The loss is left in `distill_loss` (device scalar).
+        set_teacher(None), other tokens, and the next train_step without a teacher end it."""
+        if teacher_idx is None:
+            self._teacher = None
+            return
+        if self._bufs_key is None:
+            raise TttsError("set_teacher: set the tokens first")
+        B, _, Tm = self._bufs_key
+        if teacher_idx.dim() != 3 or teacher_idx.shape[:2] != (B, Tm) or teacher_logp.shape != teacher_idx.shape:
+            raise TttsError("set_teacher: need [%d, %d, K] indices and log-probabilities, got %s and %s"
+                            % (B, Tm, tuple(teacher_idx.shape), tuple(teacher_logp.shape)))
+        rows = B * Tm
+        g_rows = torch.full((rows,), float(weight) / rows, dtype=torch.float32, device=self.device)
+        self._teacher = (teacher_idx.reshape(rows, -1).contiguous(), teacher_logp.reshape(rows, -1).contiguous(), g_rows,
+                         dict(temperature=float(temperature), tail=bool(tail)))
+
+    def train_step(self, tokens, w_text=0.01, w_mel=1.0, capture=False, exchange=None, exchange_range=None, teacher=None, **opt):
         """tokens = (text_inp, text_tar, mel_inp, mel_tar) int64 tensors (see model.prepare_tokens).
         exchange: optional callable run between backward and the optimizer (the data-parallel gradient all-reduce).
         exchange_range: optional callable (lo, hi) -> handle with .wait(): asynchronous all-reduce of grads[lo:hi].  With it
@@ -714,9 +742,13 @@ class GptEngine:
         capture=True replays the step from hipGraphs: one graph without an exchange, two (forward+backward | optimizer)
         around `exchange`, three (forward + backward part 0 | backward part 1 | optimizer) around `exchange_range`.
         tokens=None: the token buffers were already filled (set_tokens_raw).
+        teacher: arguments of set_teacher as a dict, for this step's tokens; such a step runs launch by launch (capture is refused).
         Returns nothing: losses stay on the device (no host sync in the hot loop)."""
+        if teacher is not None and capture:
+            raise TttsError("train_step: a step with a teacher is not captured (its alternatives change with the batch)")
         if tokens is not None:
             self.set_tokens(*tokens)
+        self.set_teacher(**teacher) if teacher is not None else self.set_teacher(None)
         mode = "range" if exchange_range is not None else ("whole" if exchange is not None else "none")
         graphs = None
         if capture:

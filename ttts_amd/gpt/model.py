@@ -14,6 +14,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .. import ops
 from .decode import GptDecoder
 from .engine import GptEngine, resolve_config
 
@@ -182,6 +183,25 @@ class UnifiedVoice(nn.Module):
         lo = eng.b["losses"]
         return lo[0].clone(), lo[1].clone(), eng.mel_logits()
 
+
+    @torch.no_grad()
+    def score(self, text_inputs, text_lengths, mel_codes, wav_lengths, types=None, clip_inputs=True, top_k=0, temperature=1.0):
+        """What the model gives each mel target of a batch (the arguments of `forward`), without dropout: `ops.TokenLogprobs` of
+        logp / entropy f32 [B, Tm], top_logp f32 / top_idx int64 [B, Tm, top_k] (None for top_k 0), stats f32 [B, Tm, 2].  Targets are
+        forward's: the codes, STOP at the padding and twice at the end.  The alternatives of one model are another's teacher
+        (GptEngine.train_step)."""
+        if types is not None:
+            text_inputs = text_inputs * (1 + types).unsqueeze(-1)
+        eng = self.engine
+        eng.set_tokens(*prepare_tokens(self.cfg, text_inputs, text_lengths, mel_codes, wav_lengths, clip_inputs))
+        was_training, eng.training = eng.training, False
+        try:
+            eng.forward()
+        finally:
+            eng.training = was_training
+        B, _, Tm = eng._bufs_key
+        r = ops.token_logprobs_fwd(eng.b["logits_m"], eng.b["mel_tar"], C=eng.nm, top_k=top_k, temperature=temperature)
+        return r._replace(**{k: v.view((B, Tm) + v.shape[1:]) for k, v in r._asdict().items() if v is not None})
 
     # ---- inference (ttts/gpt/model.py:357-396, 533-562) ---------------------------------------------------------------
     def post_init_gpt2_config(self, use_deepspeed=False, kv_cache=False, half=False):

@@ -17,7 +17,7 @@ from .lib import (EPI_DGELU_BF16, EPI_GELU_BF16, EPI_RESID_ADD_F32, EPI_STORE_BF
 __all__ = ["gemm_nt", "gemm_tn_accum", "colsum_accum", "attn_fwd", "attn_bwd", "layernorm_fwd", "layernorm_bwd",
            "embed_fwd", "embed_bwd", "ce_fwd", "ce_bwd", "gradnorm", "adamw", "adamw_schedule", "vq_nearest",
            "vq_commit", "vq_ema_update", "stft_mag", "mel_log", "CastPlan", "TransposePlan", "ColsumPlan", "LnFinalizePlan", "TnPlan", "probe_layout", "device_info",
-           "token_logprobs_fwd", "token_logprobs_bwd", "distill_fwd", "distill_bwd", "kv_page_write", "attn_paged_decode"]
+           "TokenLogprobs", "token_logprobs_fwd", "token_logprobs_bwd", "distill_fwd", "distill_bwd", "kv_page_write", "attn_paged_decode"]
 
 
 def _raw_stream(index=None):

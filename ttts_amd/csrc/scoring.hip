@@ -17,8 +17,20 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f, FMAX = 3
 // longer ones a wave per 2048 columns, each on its own (a workgroup per row whose waves meet at barriers read 2.1 - 2.5 TB/s where
 // these read 4.4), and a second kernel that joins a row's parts.  A lane holds 8 neighbouring columns per load (16 or 32 bytes,
 // at whatever alignment the row has; only the row's last columns are read one by one), 64 lanes 512 neighbouring ones: x[i][j] is
-// column c0 + 512 i + 8 lane + j.
-constexpr int NV = 4, WAVE_COLS = NV * 512;
+// column c0 + 512 i + 8 lane + j.  A rest of up to 64 columns behind the last whole 512 -- a codebook and its few special classes --
+// is one more column a lane (`narrow`) instead of a step of eight.
+constexpr int NV = 4, WAVE_COLS = NV * 512, NARROW = 64;
+struct Cols {   // a wave's columns: c0 .. wide - 1 in `steps` of 512, wide .. end - 1 one a lane
+  int c0, wide, end, steps;
+  __device__ __forceinline__ Cols(int first, int last) : c0(first), wide(last), end(last), steps((last - first + 511) >> 9) {
+    const int rest = (last - first) & 511;
+    if (rest && rest <= NARROW) { --steps; wide -= rest; }
+  }
+  __device__ __forceinline__ bool narrow() const { return wide < end; }
+  template <typename T> __device__ __forceinline__ float load_narrow(const T* row, int lane) const {
+    return wide + lane < end ? (float)row[wide + lane] : -INFINITY;
+  }
+};
 __device__ __forceinline__ float sum_wave(float v) { return over_wave(v, add_op); }
 __device__ __forceinline__ float max_wave(float v) { return over_wave(v, max_op); }
 
@@ -154,11 +166,11 @@ __device__ __forceinline__ float group_threshold(const uint32_t (&g)[N], int n, 
 }
 // bit 31 - (8 i + j): x[i][j] reaches the threshold / is above it
 template <bool ABOVE>
-__device__ __forceinline__ uint32_t reached(const float (&x)[NV][8], float thr, int c0, int cend) {
+__device__ __forceinline__ uint32_t reached(const float (&x)[NV][8], float thr, int steps) {
   uint32_t bits = 0;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    if (c0 + i * 512 < cend) {
+    if (i < steps) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) bits = bits + bits + (ABOVE ? x[i][j] > thr : x[i][j] >= thr);
     } else {
@@ -167,7 +179,7 @@ __device__ __forceinline__ uint32_t reached(const float (&x)[NV][8], float thr, 
   }
   return bits;
 }
-// A wave's own keys of a 16-bit type fit 32 bits: the ord() that the type has, and the column within the wave's 2048, inverted.
+// A wave's own keys of a 16-bit type fit 32 bits: the ord() that the type has, and the column among the wave's, inverted.
 template <typename T> struct WaveKey {
   typedef u64 type;
   static __device__ __forceinline__ type make(float v, int at, int c0) { return top_key(v, c0 + at); }
@@ -175,21 +187,27 @@ template <typename T> struct WaveKey {
 };
 template <typename T> struct WaveKey16 {
   typedef uint32_t type;
-  static __device__ __forceinline__ type make(float v, int at, int) { return (ord(v) >> LowBits<T>::n << 11) | (uint32_t)(WAVE_COLS - 1 - at); }
+  static __device__ __forceinline__ type make(float v, int at, int) { return (ord(v) >> LowBits<T>::n << 12) | (uint32_t)(4095 - at); }
   static __device__ __forceinline__ u64 full(type k, int c0) {
-    uint32_t o = k >> 11 << LowBits<T>::n;
+    uint32_t o = k >> 12 << LowBits<T>::n;
     if (!(o >> 31)) o |= (1u << LowBits<T>::n) - 1;   // below zero ord() has ones there
-    return ((u64)o << 32) | (uint32_t)~(c0 + WAVE_COLS - 1 - (int)(k & (WAVE_COLS - 1)));
+    return ((u64)o << 32) | (uint32_t)~(c0 + 4095 - (int)(k & 4095));
   }
 };
 template <> struct WaveKey<bf16> : WaveKey16<bf16> {};
 template <> struct WaveKey<_Float16> : WaveKey16<_Float16> {};
-static_assert(WAVE_COLS == 2048, "11 bits of a wave's key are a column");
+static_assert(WAVE_COLS + NARROW <= 4096, "12 bits of a wave's key are a column");
 
 // the columns marked in `bits` become keys at the places that place() deals out (those before `cap`); their values are read again (a
 // register cannot be indexed by a lane)
 template <typename T, typename Place>
-__device__ __forceinline__ void collect(uint32_t bits, const T* row, int c0, int lane, typename WaveKey<T>::type* cand, int cap, Place place) {
+__device__ __forceinline__ void collect(uint32_t bits, bool narrow, float xn, const T* row, const Cols& cols, int lane,
+                                        typename WaveKey<T>::type* cand, int cap, Place place) {
+  const int c0 = cols.c0;
+  if (const u64 mask = __ballot(narrow)) {
+    const int at = place(mask);
+    if (narrow && at < cap) cand[at] = WaveKey<T>::make(xn, cols.wide - c0 + lane, c0);
+  }
   for (u64 mask = __ballot(bits != 0); mask; mask = __ballot(bits != 0)) {
     const int at = place(mask);
     if (bits) {
@@ -201,7 +219,9 @@ __device__ __forceinline__ void collect(uint32_t bits, const T* row, int c0, int
 }
 // columns equal to thr, lowest classes first, become keys from place n on, up to `end`; returns n + ties
 template <typename T>
-__device__ __forceinline__ int collect_ties(const float (&x)[NV][8], float thr, int c0, int lane, typename WaveKey<T>::type* cand, int n, int end) {
+__device__ __forceinline__ int collect_ties(const float (&x)[NV][8], float xn, float thr, const Cols& cols, int lane,
+                                            typename WaveKey<T>::type* cand, int n, int end) {
+  const int c0 = cols.c0;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     int mine = 0;
@@ -222,7 +242,10 @@ __device__ __forceinline__ int collect_ties(const float (&x)[NV][8], float thr, 
       }
     n += __shfl(upto, 63, 64);
   }
-  return n;
+  const u64 mask = __ballot(xn == thr);
+  const int at = n + lanes_below(mask);
+  if (xn == thr && at < end) cand[at] = WaveKey<T>::make(xn, cols.wide - c0 + lane, c0);
+  return n + __builtin_popcountll(mask);
 }
 // f(rank, key) for the keys of rank < k among n distinct ones (four places behind them writable): ranked by counting
 template <typename K, typename F>
@@ -234,11 +257,11 @@ __device__ __forceinline__ void rank_keys(const K* cand, int n, int k, int threa
     if (r < k) f(r, key);
   }
 }
-constexpr int WAVE_CAND = 64 * 8 + 64, WAVE_TOP_LDS = WAVE_CAND + 4;      // one wave: groups of 8 columns (exact)
-constexpr int GROUP_CAND = 64 * 32 + 64;                                  // a workgroup: a lane's 32 columns are a group
+constexpr int WAVE_CAND = 64 * 9, WAVE_TOP_LDS = WAVE_CAND + 4;           // one wave: groups of 8 or 9 columns (exact)
+constexpr int GROUP_CAND = 64 * 33;                                       // a workgroup: a lane's 32 or 33 columns are a group
 // one wave: f(rank, key) of its k best; returns how many there are (<= k)
 template <typename T, typename F>
-__device__ __forceinline__ int wave_top(const float (&x)[NV][8], const float (&vmax)[NV], const T* row, int c0, int cend, int k, int lane,
+__device__ __forceinline__ int wave_top(const float (&x)[NV][8], float xn, const float (&vmax)[NV], const T* row, const Cols& cols, int k, int lane,
                                         typename WaveKey<T>::type* cand, F f) {
   uint32_t g[NV];
 #pragma unroll
@@ -252,24 +275,25 @@ __device__ __forceinline__ int wave_top(const float (&x)[NV][8], const float (&v
   }
   int n = 0;
   auto next = [&](u64 mask) { const int at = n + lanes_below(mask); n += __builtin_popcountll(mask); return at; };
-  collect<T>(reached<false>(x, thr, c0, cend), row, c0, lane, cand, WAVE_CAND, next);
+  collect<T>(reached<false>(x, thr, cols.steps), xn >= thr, xn, row, cols, lane, cand, WAVE_CAND, next);
   if (n > WAVE_CAND) {
     thr = group_threshold<T, NV>(g, NV, k, false);
     n = 0;
-    collect<T>(reached<true>(x, thr, c0, cend), row, c0, lane, cand, WAVE_CAND, next);
+    collect<T>(reached<true>(x, thr, cols.steps), xn > thr, xn, row, cols, lane, cand, WAVE_CAND, next);
     const int end = max(n, k);
-    n = min(end, collect_ties<T>(x, thr, c0, lane, cand, n, end));
+    n = min(end, collect_ties<T>(x, xn, thr, cols, lane, cand, n, end));
   }
   if (lane < 4) cand[n + lane] = 0;
   wave_fence();
-  rank_keys(cand, n, k, lane, 64, [&](int r, typename WaveKey<T>::type key) { f(r, WaveKey<T>::full(key, c0)); });
+  rank_keys(cand, n, k, lane, 64, [&](int r, typename WaveKey<T>::type key) { f(r, WaveKey<T>::full(key, cols.c0)); });
   return min(n, k);
 }
 
 struct RowSums { float m, z, s; };   // maximum, sum e, sum e t (t in bits, from the maximum)
 // of one wave's columns.  A class at -inf, or at the type's lowest value, has e = 0: e t must be 0, not NaN, so t is kept finite
 // there (a NaN passes through e).
-__device__ __forceinline__ RowSums wave_sums(const float (&x)[NV][8], float lmax, int steps, float c) {
+__device__ __forceinline__ RowSums wave_sums(const float (&x)[NV][8], float xn, const Cols& cols, float lmax, float c) {
+  const int steps = cols.steps;
   RowSums a;
   a.m = max_wave(fmaxf(lmax, -FMAX));
   a.z = a.s = 0.f;
@@ -285,6 +309,11 @@ __device__ __forceinline__ RowSums wave_sums(const float (&x)[NV][8], float lmax
         a.s = fmaf(e, fmaxf(t, -200.f), a.s);
       }
     }
+    if (cols.narrow()) {
+      const float t = fmaf(xn, c, -ex.mc), e = __builtin_amdgcn_exp2f(t);
+      a.z += e;
+      a.s = fmaf(e, fmaxf(t, -200.f), a.s);
+    }
     const float f = __builtin_amdgcn_exp2f(-ex.delta);
     a.z = sum_wave(a.z) * f;
     a.s = sum_wave(a.s) * f - ex.delta * a.z;
@@ -298,6 +327,9 @@ __device__ __forceinline__ RowSums wave_sums(const float (&x)[NV][8], float lmax
           a.z += e;
           a.s = fmaf(e, fmaxf(t, -200.f), a.s);
         }
+    const float t = (xn - a.m) * c, e = __builtin_amdgcn_exp2f(t);
+    a.z += e;
+    a.s = fmaf(e, fmaxf(t, -200.f), a.s);
     a.z = sum_wave(a.z);
     a.s = sum_wave(a.s);
   }
@@ -316,7 +348,7 @@ struct ScoreParams {
   int64_t* top_idx;
   float4* part;          // long rows: [R, units] (m, z, s, -) of each wave's columns,
   uint32_t* part_max;    // and with alternatives [R, units, 64]: ord() of the maximum of each lane's 32 columns
-  int R, C, k, units, unit_cols;
+  int R, C, k, units, unit_cols, narrow_at;   // the row's columns from narrow_at on are its last unit's narrow ones
   float inv_t;
 };
 
@@ -346,19 +378,21 @@ __global__ __launch_bounds__(256) void token_logprobs_fwd_kernel(ScoreParams p) 
   if (LONG) split_id(id, p.units, row, unit);
   if (row >= p.R) return;
   const T* lr = (const T*)p.logits + row * p.ldl;
-  const int c0 = unit * p.unit_cols, cend = min(p.C, c0 + p.unit_cols);
-  float x[NV][8], vmax[NV], lmax = -INFINITY;
+  const Cols cols(unit * p.unit_cols, unit == p.units - 1 ? p.C : (unit + 1) * p.unit_cols);
+  float x[NV][8], vmax[NV];
   int64_t tok = -1;
   float xt = 0.f;
   {
     Raw<T> raw;
-    load_raw(raw, lr, c0, cend, lane);
+    load_raw(raw, lr, cols.c0, cols.wide, lane);
     if (!LONG) {
       tok = p.tokens[row];
       if (tok >= 0 && tok < p.C) xt = (float)lr[tok];      // (its latency runs beside the row's)
     }
-    expand(raw, lr, c0, cend, lane, x);
+    expand(raw, lr, cols.c0, cols.wide, lane, x);
   }
+  const float xn = cols.load_narrow(lr, lane);
+  float lmax = xn;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     vmax[i] = -INFINITY;
@@ -366,7 +400,9 @@ __global__ __launch_bounds__(256) void token_logprobs_fwd_kernel(ScoreParams p) 
     for (int j = 0; j < 8; ++j) vmax[i] = max_med(vmax[i], x[i][j]);
     lmax = max_med(lmax, vmax[i]);
   }
-  const RowSums a = wave_sums(x, lmax, (cend - c0 + 511) >> 9, p.inv_t * LOG2E);
+  vmax[0] = max_med(vmax[0], xn);
+  lmax = max_med(lmax, -INFINITY);                         // (xn may be NaN)
+  const RowSums a = wave_sums(x, xn, cols, lmax, p.inv_t * LOG2E);
   if (LONG) {
     if (lane == 0) p.part[id] = make_float4(a.m, a.z, a.s, 0.f);
     if (p.k) p.part_max[id * 64 + lane] = ord(lmax);
@@ -374,7 +410,7 @@ __global__ __launch_bounds__(256) void token_logprobs_fwd_kernel(ScoreParams p) 
   }
   if (lane == 0) write_row(p, row, a, tok >= 0 && tok < p.C, xt);
   if (p.k) {
-    const int have = wave_top<T>(x, vmax, lr, c0, cend, p.k, lane, reinterpret_cast<typename WaveKey<T>::type*>(score_lds) + wave * WAVE_TOP_LDS, [&](int r, u64 key) { write_top(p, row, r, key, a); });
+    const int have = wave_top<T>(x, xn, vmax, lr, cols, p.k, lane, reinterpret_cast<typename WaveKey<T>::type*>(score_lds) + wave * WAVE_TOP_LDS, [&](int r, u64 key) { write_top(p, row, r, key, a); });
     if (lane >= have && lane < p.k) write_top(p, row, lane, 0, a);
   }
 }
@@ -414,7 +450,7 @@ __global__ __launch_bounds__(256) void token_logprobs_join_kernel(ScoreParams p)
 // fewer than k groups above it, and then the row's columns AT it in the order of the classes until there are k.
 template <typename T, int W, int N>
 __global__ __launch_bounds__(W * 64) void token_logprobs_top_kernel(ScoreParams p) {
-  constexpr int LIST = 128 * W, SETS = N < 4 ? N : 4;
+  constexpr int LIST = 96 * W, SETS = N < 4 ? N : 4;
   __shared__ __attribute__((aligned(16))) u64 cand[GROUP_CAND + 4];
   __shared__ uint32_t list_max[LIST];
   __shared__ int list_id[LIST];
@@ -467,10 +503,16 @@ __global__ __launch_bounds__(W * 64) void token_logprobs_top_kernel(ScoreParams 
     __syncthreads();
   }
   auto push_eight = [&](int id, int i, float t, bool above) {   // columns that reach t (or lie above it) become keys
-    const int c = (id >> 6) * p.unit_cols + i * 512 + (id & 63) * 8;
-    if (i * 512 >= p.unit_cols || c >= p.C) return;
+    int c = (id >> 6) * p.unit_cols + i * 512 + (id & 63) * 8, end = p.narrow_at;
+    if (i == NV) {                              // the unit's narrow columns
+      c = p.narrow_at + (id & 63);
+      end = (id >> 6) == p.units - 1 ? min(p.C, c + 1) : 0;
+    } else if (i * 512 >= p.unit_cols) {
+      return;
+    }
+    if (c >= end) return;
     float v[8];
-    load8<T>(lr + c, p.C - c, v);
+    load8<T>(lr + c, end - c, v);
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       if (above ? v[j] > t : v[j] >= t) {
@@ -483,8 +525,8 @@ __global__ __launch_bounds__(W * 64) void token_logprobs_top_kernel(ScoreParams 
   if (!full) {
     const float t = sm_thr[W];
     const uint32_t tb = ord(t);
-    for (int task = tid; task < listed * NV; task += W * 64)
-      if (list_max[task / NV] >= tb) push_eight(list_id[task / NV], task % NV, t, false);
+    for (int task = tid; task < listed * (NV + 1); task += W * 64)
+      if (list_max[task / (NV + 1)] >= tb) push_eight(list_id[task / (NV + 1)], task % (NV + 1), t, false);
     __syncthreads();
     full = sm_n > GROUP_CAND;
   }
@@ -508,7 +550,7 @@ __global__ __launch_bounds__(W * 64) void token_logprobs_top_kernel(ScoreParams 
     for (int u = wave; u < p.units; u += W)
       if (gm[u * 64 + lane] > tb)
 #pragma unroll 1
-        for (int e = 0; e < NV; ++e) push_eight(u * 64 + lane, e, thr, true);
+        for (int e = 0; e <= NV; ++e) push_eight(u * 64 + lane, e, thr, true);
     __syncthreads();
     int n = sm_n;
     const int end = max(n, k);
@@ -605,18 +647,22 @@ __global__ __launch_bounds__(256) void token_logprobs_top_wave_kernel(ScoreParam
       }
     }
   };
-  auto eight = [&](int c, bool mine, float (&v)[8]) {
+  auto eight = [&](int c, int end, float (&v)[8]) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = -INFINITY;
-    if (mine && c < p.C) load8<T>(lr + c, p.C - c, v);
+    if (c < end) load8<T>(lr + c, end - c, v);
   };
   bool full = listed > LIST;
   if (!full) {
-    for (int s = 0; s < listed * NV; s += 64) {
-      const int task = s + lane, id = task < listed * NV ? list[task / NV] : 0;
-      const int c = (id >> 6) * p.unit_cols + (task % NV) * 512 + (id & 63) * 8;
+    for (int s = 0; s < listed * (NV + 1); s += 64) {
+      const int task = s + lane, i = task % (NV + 1), id = task < listed * (NV + 1) ? list[task / (NV + 1)] : 0;
+      int c = (id >> 6) * p.unit_cols + i * 512 + (id & 63) * 8, end = i * 512 < p.unit_cols ? p.narrow_at : 0;
+      if (i == NV) {                              // the unit's narrow columns
+        c = p.narrow_at + (id & 63);
+        end = (id >> 6) == p.units - 1 ? min(p.C, c + 1) : 0;
+      }
       float v[8];
-      eight(c, task < listed * NV && (task % NV) * 512 < p.unit_cols, v);
+      eight(c, task < listed * (NV + 1) ? end : 0, v);
       push(v, c, [&](float x) { return x >= thr; });
     }
     full = n > CAND;
@@ -627,7 +673,7 @@ __global__ __launch_bounds__(256) void token_logprobs_top_wave_kernel(ScoreParam
     for (uint32_t bit = 0x80000000u; bit >> LowBits<T>::n; bit >>= 1) {
       float cnt = 0.f;                        // (whole numbers up to 16384)
       for (int c0 = 0; c0 < p.C; c0 += 512) {
-        eight(c0 + lane * 8, true, v);
+        eight(c0 + lane * 8, p.C, v);
 #pragma unroll
         for (int j = 0; j < 8; ++j) cnt += ord(v[j]) >= (t | bit) && v[j] == v[j] ? 1.f : 0.f;
       }
@@ -636,11 +682,11 @@ __global__ __launch_bounds__(256) void token_logprobs_top_wave_kernel(ScoreParam
     thr = threshold_of<T>(t);
     n = 0;
     for (int c0 = 0; c0 < p.C; c0 += 512) {
-      eight(c0 + lane * 8, true, v);
+      eight(c0 + lane * 8, p.C, v);
       push(v, c0 + lane * 8, [&](float x) { return x > thr; });
     }
     for (int c0 = 0; c0 < p.C && n < k; c0 += 512) {
-      eight(c0 + lane * 8, true, v);
+      eight(c0 + lane * 8, p.C, v);
       int mine = 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j) mine += v[j] == thr;
@@ -790,7 +836,7 @@ __device__ __forceinline__ void listed_logits(const T* row, const Listed& L, flo
 // as token_logprobs_fwd_kernel; with tail each wave marks the listed classes of its columns in a bit map of its own
 template <typename T, bool LONG>
 __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillParams p) {
-  __shared__ uint32_t marks[4][WAVE_COLS / 32];
+  __shared__ uint32_t marks[4][(WAVE_COLS + NARROW) / 32];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t id = (int64_t)blockIdx.x * 4 + wave;
   int64_t row = id;
@@ -798,9 +844,10 @@ __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillParams p) {
   if (LONG) split_id(id, p.units, row, unit);
   if (row >= p.R) return;
   const T* lr = (const T*)p.logits + row * p.ldl;
-  const int c0 = unit * p.unit_cols, cend = min(p.C, c0 + p.unit_cols);
+  const Cols cols(unit * p.unit_cols, unit == p.units - 1 ? p.C : (unit + 1) * p.unit_cols);
   Raw<T> raw;
-  load_raw(raw, lr, c0, cend, lane);
+  load_raw(raw, lr, cols.c0, cols.wide, lane);
+  const float xn = cols.load_narrow(lr, lane);
   Listed L;
   float xl[2] = {0.f, 0.f};
   if (!LONG) {
@@ -810,16 +857,17 @@ __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillParams p) {
   uint32_t* mark = marks[wave];
   if (p.tail) {
     mark[lane] = 0;
+    if (lane < NARROW / 32) mark[64 + lane] = 0;
     wave_fence();
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int64_t c = LONG ? (lane + 64 * h < p.K ? p.idx[row * p.K + lane + 64 * h] : -1) : L.id[h];
-      if (c >= c0 && c < cend) atomicOr(&mark[(c - c0) >> 5], 1u << ((c - c0) & 31));
+      if (c >= cols.c0 && c < cols.end) atomicOr(&mark[(c - cols.c0) >> 5], 1u << ((c - cols.c0) & 31));
     }
     wave_fence();
   }
-  float x[NV][8], m = -FMAX;
-  expand(raw, lr, c0, cend, lane, x);
+  float x[NV][8], m = fmaxf(xn, -FMAX);
+  expand(raw, lr, cols.c0, cols.wide, lane, x);
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -827,11 +875,10 @@ __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillParams p) {
   m = max_wave(m);
   const Exponent ex(m, p.inv_t * LOG2E);
   float zl = 0.f, zr = 0.f;
-  const int steps = (cend - c0 + 511) >> 9;
   auto add_up = [&](auto exponent) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      if (i >= steps) break;
+      if (i >= cols.steps) break;
       const uint32_t bits = p.tail ? reinterpret_cast<const uint8_t*>(mark)[i * 64 + lane] : 0u;
       if (p.tail && __any(bits != 0)) {
 #pragma unroll
@@ -845,6 +892,13 @@ __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillParams p) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) zr += __builtin_amdgcn_exp2f(exponent(x[i][j]));
       }
+    }
+    if (cols.narrow()) {
+      const float e = __builtin_amdgcn_exp2f(exponent(xn));
+      const int at = cols.steps * 512 + lane;
+      const bool hit = p.tail && (mark[at >> 5] >> (at & 31)) & 1u;
+      zl += hit ? e : 0.f;
+      zr += hit ? 0.f : e;
     }
   };
   if (ex.plain) add_up([&](float v) { return fmaf(v, ex.c, -ex.mc); });
@@ -860,15 +914,16 @@ __global__ __launch_bounds__(256) void distill_join_kernel(DistillParams p) {   
   const int lane = threadIdx.x & 63;
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= p.R) return;
+  const float4* part = p.part + row * p.units;
+  const float4 first = lane < p.units ? part[lane] : make_float4(-FMAX, 0.f, 0.f, 0.f);   // (on its way beside the list)
   const Listed L = load_listed(p.idx + row * p.K, p.tlogp + row * p.K, p.K, p.C, p.inv_t, p.tail, lane);
   float xl[2];
   listed_logits((const T*)p.logits + row * p.ldl, L, xl);
-  const float4* part = p.part + row * p.units;
-  float m = -FMAX, zl = 0.f, zr = 0.f;
-  for (int u = lane; u < p.units; u += 64) m = fmaxf(m, part[u].x);
+  float m = first.x, zl = 0.f, zr = 0.f;
+  for (int u = lane + 64; u < p.units; u += 64) m = fmaxf(m, part[u].x);
   m = max_wave(m);
   for (int u = lane; u < p.units; u += 64) {
-    const float4 s = part[u];
+    const float4 s = u < 64 ? first : part[u];
     const float f = __builtin_amdgcn_exp2f((s.x - m) * p.inv_t * LOG2E);
     zl = fmaf(s.y, f, zl);
     zr = fmaf(s.z, f, zr);
@@ -893,18 +948,21 @@ struct DistillGradParams {
 // name one class find out by leaving their number at its place in LDS: each then writes the sum of their p, in the list's order.
 template <typename T>
 __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillGradParams p) {
-  __shared__ uint8_t tags[4][WAVE_COLS];
+  __shared__ uint8_t tags[4][WAVE_COLS + NARROW];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t unit = (int64_t)blockIdx.x * 4 + wave;
   if (unit >= p.units) return;
   int64_t row;
   int piece;
   split_id(unit, p.per_row, row, piece);
-  const int c0 = piece * p.wave_cols, dend = min(p.Cd, c0 + p.wave_cols), cend = min(p.C, dend);
+  const int c0 = piece * p.wave_cols;
+  const Cols cols(c0, piece == p.per_row - 1 ? p.Cd : c0 + p.wave_cols);   // of what is written; the classes end at cend
+  const int dend = cols.wide, cend = min(p.C, cols.end);
   const T* lr = (const T*)p.logits + row * p.ldl;
   T* dr = (T*)p.dlogits + row * p.ldd;
   float x[NV][8];
-  load_wave<T>(lr, c0, cend, lane, x);
+  load_wave<T>(lr, c0, min(p.C, cols.wide), lane, x);
+  const float xn = cols.wide + lane < cend ? (float)lr[cols.wide + lane] : -INFINITY;
   Listed L = load_listed(p.idx + row * p.K, p.tlogp + row * p.K, p.K, p.C, p.inv_t, p.tail, lane);
   const float m = p.stats[3 * row], logz = p.stats[3 * row + 1], w = p.stats[3 * row + 2], g = p.g_loss[row] * p.inv_t;
   uint8_t* tag = tags[wave];
@@ -950,7 +1008,7 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillGradParams p) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) d[j] = first + j < p.C && !none ? d[j] : 0.f;
     }
-    const int n = (p.accumulate ? cend : dend) - first;
+    const int n = (p.accumulate ? min(cend, dend) : dend) - first;
     if (n <= 0) continue;
     if (p.accumulate) {
       float o[8];
@@ -959,6 +1017,14 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillGradParams p) {
       for (int j = 0; j < 8; ++j) d[j] += o[j];
     }
     store8<T>(dr + first, n, d);
+  }
+  {
+    const int col = cols.wide + lane;
+    float d = col < p.C && !none ? __builtin_amdgcn_exp2f((xn - m) * c - log2z) * off : 0.f;
+    if (col < (p.accumulate ? cend : cols.end)) {
+      if (p.accumulate) d += (float)dr[col];
+      dr[col] = (T)d;
+    }
   }
   wave_fence();
   if (none) return;
@@ -1003,13 +1069,22 @@ static int need_grid(const char* what, int64_t grid) {
   return TTTS_OK;
 }
 
-// waves of a long row (1: the row is one wave's) and the columns of each, whole 512s: as few steps as 2048 each, but no small rest
-static int unit_columns(int C) { return (int)(cdiv(cdiv(C, 512), cdiv(C, WAVE_COLS)) * 512); }
-static int row_units(int C) { return (int)cdiv(C, unit_columns(C)); }
+// n columns -> waves (1: one wave's) and the columns of each but the last, which takes the rest: whole 512s, as few steps as there can
+// be, and no small rest but a narrow one
+struct Units { int units, cols, narrow_at; };
+static Units split_columns(int n) {
+  const int rest = n % 512, narrow = rest <= NARROW ? rest : 0, steps = (int)cdiv(n - narrow, 512);
+  Units u;
+  u.units = steps > NV ? (int)cdiv(steps, NV) : 1;
+  u.cols = steps > 0 ? (int)cdiv(steps, u.units) * 512 : 512;
+  u.units = steps > 0 ? (int)cdiv(steps * 512, u.cols) : 1;
+  u.narrow_at = n - narrow;
+  return u;
+}
 
 extern "C" int64_t ttts_token_logprobs_workspace_bytes(int32_t R, int32_t C, int32_t top_k) {
-  if (R <= 0 || C <= WAVE_COLS || top_k < 0) return 0;
-  return (int64_t)R * row_units(C) * (16 + (top_k > 0 ? 256 : 0));
+  const int units = C > 0 ? split_columns(C).units : 1;
+  return R > 0 && units > 1 ? (int64_t)R * units * (16 + (top_k > 0 ? 256 : 0)) : 0;
 }
 
 template <typename T>
@@ -1026,8 +1101,8 @@ static int launch_score(const ScoreParams& p, hipStream_t st) {
   rc = check_launch(what);
   if (rc) return rc;
   if (p.k == 0) token_logprobs_join_kernel<T><<<(unsigned)cdiv(p.R, 4), 256, 0, st>>>(p);
-  else if (p.units <= 8) token_logprobs_top_wave_kernel<T><<<(unsigned)cdiv(p.R, 4), 256, 0, st>>>(p);   // up to 16384 classes
-  else if (p.units <= 64) token_logprobs_top_kernel<T, 4, 16><<<p.R, 256, 0, st>>>(p);     // up to 131072
+  else if (p.units <= 8) token_logprobs_top_wave_kernel<T><<<(unsigned)cdiv(p.R, 4), 256, 0, st>>>(p);   // up to 16448 classes
+  else if (p.units <= 64) token_logprobs_top_kernel<T, 4, 16><<<p.R, 256, 0, st>>>(p);     // up to 131136
   else token_logprobs_top_kernel<T, 16, 32><<<p.R, 1024, 0, st>>>(p);                      // up to TTTS_SCORE_MAX_CLASSES
   return check_launch("token_logprobs_fwd join");
 }
@@ -1042,7 +1117,8 @@ extern "C" int ttts_token_logprobs_fwd(const void* logits, int32_t dtype, int64_
   TTTS_REQUIRE(tokens && logp && entropy && stats && (top_k == 0 || (top_logp && top_idx)), "token_logprobs_fwd: null pointer");
   rc = need_workspace("token_logprobs_fwd", ttts_token_logprobs_workspace_bytes(R, C, top_k), workspace, workspace_bytes);
   if (rc) return rc;
-  ScoreParams p{logits, ldl, tokens, logp, entropy, stats, top_logp, top_idx, (float4*)workspace, nullptr, R, C, top_k, row_units(C), unit_columns(C), 1.0f / temperature};
+  const Units u = split_columns(C);
+  ScoreParams p{logits, ldl, tokens, logp, entropy, stats, top_logp, top_idx, (float4*)workspace, nullptr, R, C, top_k, u.units, u.cols, u.narrow_at, 1.0f / temperature};
   p.part_max = (uint32_t*)(p.part + (int64_t)R * p.units);
   TTTS_BY_TYPE(dtype, "token_logprobs_fwd", rc = launch_score<T>(p, as_stream(stream)));
   return rc;
@@ -1065,7 +1141,10 @@ extern "C" int ttts_token_logprobs_bwd(const void* logits, int32_t dtype, int64_
   return check_launch("token_logprobs_bwd");
 }
 
-extern "C" int64_t ttts_distill_workspace_bytes(int32_t R, int32_t C) { return R > 0 && C > WAVE_COLS ? (int64_t)R * row_units(C) * 16 : 0; }
+extern "C" int64_t ttts_distill_workspace_bytes(int32_t R, int32_t C) {
+  const int units = C > 0 ? split_columns(C).units : 1;
+  return R > 0 && units > 1 ? (int64_t)R * units * 16 : 0;
+}
 
 template <typename T>
 static int launch_distill(const DistillParams& p, hipStream_t st) {
@@ -1094,7 +1173,8 @@ extern "C" int ttts_distill_fwd(const void* logits, int32_t dtype, int64_t ldl, 
   TTTS_REQUIRE(teacher_idx && teacher_logp && row_loss && stats, "distill_fwd: null pointer");
   rc = need_workspace("distill_fwd", ttts_distill_workspace_bytes(R, C), workspace, workspace_bytes);
   if (rc) return rc;
-  const DistillParams p{logits, ldl, teacher_idx, teacher_logp, row_loss, stats, (float4*)workspace, R, C, K, tail != 0, row_units(C), unit_columns(C), 1.0f / temperature};
+  const Units u = split_columns(C);
+  const DistillParams p{logits, ldl, teacher_idx, teacher_logp, row_loss, stats, (float4*)workspace, R, C, K, tail != 0, u.units, u.cols, 1.0f / temperature};
   TTTS_BY_TYPE(dtype, "distill_fwd", rc = launch_distill<T>(p, as_stream(stream)));
   return rc;
 }
@@ -1109,9 +1189,9 @@ extern "C" int ttts_distill_bwd(const void* logits, int32_t dtype, int64_t ldl, 
   if (R == 0) return TTTS_OK;
   TTTS_REQUIRE(teacher_idx && teacher_logp && stats && g_loss && dlogits, "distill_bwd: null pointer");
   DistillGradParams p{logits, ldl, teacher_idx, teacher_logp, stats, g_loss, dlogits, ldd, C, Cd, K, tail != 0, accumulate != 0, 0, 0, 0, 1.0f / temperature};
-  p.per_row = (int)cdiv(Cd, WAVE_COLS);
-  p.wave_cols = (int)cdiv(cdiv(Cd, 512), p.per_row) * 512;
-  p.per_row = (int)cdiv(Cd, p.wave_cols);
+  const Units u = split_columns(Cd);
+  p.per_row = u.units;
+  p.wave_cols = u.cols;
   p.units = (int64_t)R * p.per_row;
   const int64_t grid = cdiv(p.units, 4);
   rc = need_grid("distill_bwd", grid);

@@ -3,7 +3,6 @@ the current HIP stream and (elsewhere) torch.distributed.  Every function requir
 raises `TttsError` on any failure -- there is no eager / CPU fallback.
 """
 import collections
-import contextlib
 import ctypes
 
 import numpy as np
@@ -891,18 +890,16 @@ def decode_advance(ctr, finished):
 _DTYPE_CODES = {torch.float32: _l.DTYPE_F32, torch.bfloat16: _l.DTYPE_BF16, torch.float16: _l.DTYPE_F16}
 
 
-_NO_GUARD = contextlib.nullcontext()
-
-
 def _on(what, *tensors):
-    """All of the tensors (None: left out) live on one GPU: a context that makes it the current device, so that the launch goes to torch's
-    current stream of THAT device.  Raises for a CPU tensor or two devices."""
+    """All of the tensors (None: left out) live on one GPU: its index if that is not the current device (the call is then made again with it
+    as the current one, so that the launch goes to torch's current stream of THAT device), else None.  Raises for a CPU tensor
+    or two devices."""
     index = tensors[0].get_device()
     for t in tensors:
         if t is not None and (index < 0 or t.get_device() != index):
             raise TttsError("%s: every tensor must live on the GPU, all on the same one (no CPU fallback in ttts_amd); got %s"
                             % (what, ", ".join(sorted({str(x.device) for x in tensors if x is not None}))))
-    return _NO_GUARD if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
+    return None if index == torch._C._cuda_getDevice() else index
 
 
 def _a(t):
@@ -959,32 +956,42 @@ def token_logprobs_fwd(logits, tokens, C=None, top_k=0, temperature=1.0):
     token, logp 0).  Returns TokenLogprobs(logp f32 [R], entropy f32 [R], top_logp f32 [R, top_k] | None, top_idx int64 [R, top_k] |
     None, stats f32 [R, 2] for the backward).  Alternatives: best first, equal logits by ascending class; -inf / -1 where a row has
     fewer classes above -inf.  Rows of -inf only and rows with NaN: include/ttts_hip.h."""
-    what = "token_logprobs_fwd"
+    what, lib = "token_logprobs_fwd", _l.get()
     code, ld, R, C = _logits(logits, C, what)
     _vec(tokens, torch.int64, (R,), what, "tokens")
     k = int(top_k)
-    with _on(what, logits, tokens):
-        f = lambda *shape, dt=torch.float32: torch.empty(shape, dtype=dt, device=logits.device)  # noqa: E731
-        r = TokenLogprobs(f(R), f(R), f(R, k) if k > 0 else None, f(R, k, dt=torch.int64) if k > 0 else None, f(R, 2))
-        n = _l.get().ttts_token_logprobs_workspace_bytes(R, C, k)
-        ws = _workspace(n, logits.device)
-        check(_l.get().ttts_token_logprobs_fwd(_a(logits), code, ld, _a(tokens), _a(r.logp), _a(r.entropy), _a(r.stats), _a(r.top_logp),
-                                               _a(r.top_idx), R, C, k, float(temperature), _a(ws), n, _raw_stream()), what)
+    other = _on(what, logits, tokens)
+    if other is not None:
+        with torch.cuda.device(other):
+            return token_logprobs_fwd(logits, tokens, C, top_k, temperature)
+    f = lambda *shape, dt=torch.float32: torch.empty(shape, dtype=dt, device=logits.device)  # noqa: E731
+    r = TokenLogprobs(f(R), f(R), f(R, k) if k > 0 else None, f(R, k, dt=torch.int64) if k > 0 else None, f(R, 2))
+    n = lib.ttts_token_logprobs_workspace_bytes(R, C, k)
+    ws = _workspace(n, logits.device)
+    rc = lib.ttts_token_logprobs_fwd(_a(logits), code, ld, _a(tokens), _a(r.logp), _a(r.entropy), _a(r.stats), _a(r.top_logp),
+                                     _a(r.top_idx), R, C, k, float(temperature), _a(ws), n, _raw_stream())
+    if rc:
+        check(rc, what)
     return r
 
 
 def token_logprobs_bwd(logits, tokens, stats, entropy, g_logp, g_entropy=None, C=None, temperature=1.0, dlogits=None):
     """Gradient of token_logprobs_fwd's logp and entropy to the logits: dlogits (new, or the given tensor; `logits` itself is allowed)
     of the logits' type and shape, columns from C on zero.  g_logp / g_entropy f32 [R]."""
-    what = "token_logprobs_bwd"
+    what, lib = "token_logprobs_bwd", _l.get()
     code, ld, R, C = _logits(logits, C, what)
     _vec(tokens, torch.int64, (R,), what, "tokens"); _vec(stats, torch.float32, (R, 2), what, "stats")
     for t, name in ((entropy, "entropy"), (g_logp, "g_logp"), (g_entropy, "g_entropy")):
         _vec(t, torch.float32, (R,), what, name)
-    with _on(what, logits, tokens, stats, entropy, g_logp, g_entropy, dlogits):
-        dlogits, ldd = _grad_rows(dlogits, logits, what)
-        check(_l.get().ttts_token_logprobs_bwd(_a(logits), code, ld, _a(tokens), _a(stats), _a(entropy), _a(g_logp), _a(g_entropy),
-                                               _a(dlogits), ldd, R, C, logits.shape[1], float(temperature), _raw_stream()), what)
+    other = _on(what, logits, tokens, stats, entropy, g_logp, g_entropy, dlogits)
+    if other is not None:
+        with torch.cuda.device(other):
+            return token_logprobs_bwd(logits, tokens, stats, entropy, g_logp, g_entropy, C, temperature, dlogits)
+    dlogits, ldd = _grad_rows(dlogits, logits, what)
+    rc = lib.ttts_token_logprobs_bwd(_a(logits), code, ld, _a(tokens), _a(stats), _a(entropy), _a(g_logp), _a(g_entropy),
+                                     _a(dlogits), ldd, R, C, logits.shape[1], float(temperature), _raw_stream())
+    if rc:
+        check(rc, what)
     return dlogits
 
 
@@ -993,16 +1000,21 @@ def distill_fwd(logits, teacher_idx, teacher_logp, C=None, temperature=1.0, tail
     (an index outside [0, C): an empty entry).  tail False: teacher_logp / temperature is normalised over the row's entries; tail
     True: they are log-probabilities at that temperature, and the mass that they leave out is compared with the student's on all
     other classes.  Returns (row_loss f32 [R], stats f32 [R, 3] for the backward)."""
-    what = "distill_fwd"
+    what, lib = "distill_fwd", _l.get()
     code, ld, R, C = _logits(logits, C, what)
     K = _teacher(teacher_idx, teacher_logp, R, what)
-    with _on(what, logits, teacher_idx, teacher_logp):
-        loss = torch.empty(R, dtype=torch.float32, device=logits.device)
-        stats = torch.empty(R, 3, dtype=torch.float32, device=logits.device)
-        n = _l.get().ttts_distill_workspace_bytes(R, C)
-        ws = _workspace(n, logits.device)
-        check(_l.get().ttts_distill_fwd(_a(logits), code, ld, _a(teacher_idx), _a(teacher_logp), _a(loss), _a(stats), R, C, K,
-                                        float(temperature), int(bool(tail)), _a(ws), n, _raw_stream()), what)
+    other = _on(what, logits, teacher_idx, teacher_logp)
+    if other is not None:
+        with torch.cuda.device(other):
+            return distill_fwd(logits, teacher_idx, teacher_logp, C, temperature, tail)
+    loss = torch.empty(R, dtype=torch.float32, device=logits.device)
+    stats = torch.empty(R, 3, dtype=torch.float32, device=logits.device)
+    n = lib.ttts_distill_workspace_bytes(R, C)
+    ws = _workspace(n, logits.device)
+    rc = lib.ttts_distill_fwd(_a(logits), code, ld, _a(teacher_idx), _a(teacher_logp), _a(loss), _a(stats), R, C, K,
+                              float(temperature), int(bool(tail)), _a(ws), n, _raw_stream())
+    if rc:
+        check(rc, what)
     return loss, stats
 
 
@@ -1017,16 +1029,21 @@ def distill_bwd(logits, teacher_idx, teacher_logp, stats, g_loss, C=None, temper
     """Gradient of distill_fwd's row losses to the logits, weighted by g_loss f32 [R]: dlogits (new, or the given tensor; `logits`
     itself is allowed) of the logits' type and shape, columns from C on zero.  accumulate: added to the given dlogits instead
     (columns from C on stay)."""
-    what = "distill_bwd"
+    what, lib = "distill_bwd", _l.get()
     code, ld, R, C = _logits(logits, C, what)
     K = _teacher(teacher_idx, teacher_logp, R, what)
     _vec(stats, torch.float32, (R, 3), what, "stats"); _vec(g_loss, torch.float32, (R,), what, "g_loss")
-    if accumulate and (dlogits is None or dlogits.data_ptr() == logits.data_ptr()):
+    if accumulate and (dlogits is None or (dlogits.data_ptr() == logits.data_ptr() and R > 0)):
         raise TttsError("%s: accumulate needs a dlogits of its own" % what)
-    with _on(what, logits, teacher_idx, teacher_logp, stats, g_loss, dlogits):
-        dlogits, ldd = _grad_rows(dlogits, logits, what)
-        check(_l.get().ttts_distill_bwd(_a(logits), code, ld, _a(teacher_idx), _a(teacher_logp), _a(stats), _a(g_loss), _a(dlogits), ldd, R, C,
-                                        logits.shape[1], K, float(temperature), int(bool(tail)), int(bool(accumulate)), _raw_stream()), what)
+    other = _on(what, logits, teacher_idx, teacher_logp, stats, g_loss, dlogits)
+    if other is not None:
+        with torch.cuda.device(other):
+            return distill_bwd(logits, teacher_idx, teacher_logp, stats, g_loss, C, temperature, tail, dlogits, accumulate)
+    dlogits, ldd = _grad_rows(dlogits, logits, what)
+    rc = lib.ttts_distill_bwd(_a(logits), code, ld, _a(teacher_idx), _a(teacher_logp), _a(stats), _a(g_loss), _a(dlogits), ldd, R, C,
+                                    logits.shape[1], K, float(temperature), int(bool(tail)), int(bool(accumulate)), _raw_stream())
+    if rc:
+        check(rc, what)
     return dlogits
 
 
@@ -1053,16 +1070,21 @@ def kv_page_write(k, v, k_pages, v_pages, slots):
     parts of a packed projection) goes to position slots[n] % page of page slots[n] // page of k_pages / v_pages [pages, heads, page
     size, head_dim], bf16 or fp16.  slots int64 [N]; one outside the cache (-1: a padding row) writes nothing.  The slots of a call
     differ from each other."""
-    what = "kv_page_write"
+    what, lib = "kv_page_write", _l.get()
     code = _pages(k_pages, v_pages, what)
     P, H, page, dh = k_pages.shape
     N = slots.shape[0] if slots.dim() == 1 else -1
     _vec(slots, torch.int64, (N,), what, "slots")
     ksn, ksh = _heads(k, k_pages.dtype, (N, H, dh), what, "k")
     vsn, vsh = _heads(v, k_pages.dtype, (N, H, dh), what, "v")
-    with _on(what, k, v, k_pages, v_pages, slots):
-        check(_l.get().ttts_kv_page_write(_a(k), _a(v), ksn, ksh, vsn, vsh, _a(k_pages), _a(v_pages),
-                                          _a(slots), code, N, H, dh, page, P, _raw_stream()), what)
+    other = _on(what, k, v, k_pages, v_pages, slots)
+    if other is not None:
+        with torch.cuda.device(other):
+            return kv_page_write(k, v, k_pages, v_pages, slots)
+    rc = lib.ttts_kv_page_write(_a(k), _a(v), ksn, ksh, vsn, vsh, _a(k_pages), _a(v_pages),
+                                      _a(slots), code, N, H, dh, page, P, _raw_stream())
+    if rc:
+        check(rc, what)
 
 
 def attn_paged_decode(q, k_pages, v_pages, block_table, seq_lens, scale, out=None):
@@ -1070,7 +1092,7 @@ def attn_paged_decode(q, k_pages, v_pages, block_table, seq_lens, scale, out=Non
     of the cache's heads (shared by neighbours); block_table int32 [M, width]: a sequence's pages in order; seq_lens int32 [M]: its
     keys, the new token's among them.  Returns (out [M, H, head_dim] of q's type, lse f32 [M, H]).  A sequence without keys gets 0 and
     -inf; keys of a table entry outside the cache are left out.  A slice block_table[:, :n] bounds the lengths to n pages."""
-    what = "attn_paged_decode"
+    what, lib = "attn_paged_decode", _l.get()
     code = _pages(k_pages, v_pages, what)
     P, Hkv, page, dh = k_pages.shape
     if q.dim() != 3 or block_table.dim() != 2 or block_table.dtype != torch.int32:
@@ -1081,16 +1103,21 @@ def attn_paged_decode(q, k_pages, v_pages, block_table, seq_lens, scale, out=Non
     ts, tm, width = _rows(block_table, what, "block_table")
     if tm != M:
         raise TttsError("%s: block_table has %d rows for %d sequences" % (what, tm, M))
-    with _on(what, q, k_pages, v_pages, block_table, seq_lens, out):
-        if out is None:
-            out = torch.empty(M, H, dh, dtype=q.dtype, device=q.device)
-        osm, osh = _heads(out, q.dtype, (M, H, dh), what, "out")
-        lse = torch.empty(M, H, dtype=torch.float32, device=q.device)
-        n = _l.get().ttts_attn_paged_decode_workspace_bytes(M, H, Hkv, dh, page, width)
-        ws = _workspace(n, q.device)
-        check(_l.get().ttts_attn_paged_decode(_a(q), qsm, qsh, _a(k_pages), _a(v_pages), _a(block_table), ts, _a(seq_lens),
-                                              _a(out), osm, osh, _a(lse), code, M, H, Hkv, dh, page, P, width,
-                                              float(scale), _a(ws), n, _raw_stream()), what)
+    other = _on(what, q, k_pages, v_pages, block_table, seq_lens, out)
+    if other is not None:
+        with torch.cuda.device(other):
+            return attn_paged_decode(q, k_pages, v_pages, block_table, seq_lens, scale, out)
+    if out is None:
+        out = torch.empty(M, H, dh, dtype=q.dtype, device=q.device)
+    osm, osh = _heads(out, q.dtype, (M, H, dh), what, "out")
+    lse = torch.empty(M, H, dtype=torch.float32, device=q.device)
+    n = lib.ttts_attn_paged_decode_workspace_bytes(M, H, Hkv, dh, page, width)
+    ws = _workspace(n, q.device)
+    rc = lib.ttts_attn_paged_decode(_a(q), qsm, qsh, _a(k_pages), _a(v_pages), _a(block_table), ts, _a(seq_lens),
+                                    _a(out), osm, osh, _a(lse), code, M, H, Hkv, dh, page, P, width,
+                                    float(scale), _a(ws), n, _raw_stream())
+    if rc:
+        check(rc, what)
     return out, lse
 
 

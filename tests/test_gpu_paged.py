@@ -115,6 +115,7 @@ def test_attn_paged_decode_long_and_ragged(dtype, dh, Hkv, group, page, lens):
 
 @pytest.mark.parametrize("dtype,dh,M,Hkv,group,page,longest", [
     (torch.bfloat16, 64, 70, 8, 1, 16, 300), (torch.float16, 128, 33, 16, 2, 32, 200), (torch.bfloat16, 32, 520, 1, 5, 16, 90),
+    (torch.bfloat16, 64, 512, 1, 1, 16, 100), (torch.float16, 32, 257, 2, 3, 16, 60),
     (torch.bfloat16, 64, 70, 8, 1, 16, 5001)])
 def test_many_sequences(dtype, dh, M, Hkv, group, page, longest):
     """As many sequences and heads as fill the card: no split up to 4096 keys, chunks beyond."""
@@ -190,7 +191,7 @@ def test_views_and_sliced_tables():
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("N,H,dh,page", [(1, 8, 64, 16), (7, 1, 32, 32), (300, 3, 128, 16), (5000, 2, 64, 1024)])
+@pytest.mark.parametrize("N,H,dh,page", [(1, 8, 64, 16), (7, 1, 32, 32), (300, 3, 128, 16), (5000, 2, 64, 1024), (65, 17, 128, 16), (40, 64, 64, 32)])
 def test_kv_page_write(dtype, N, H, dh, page):
     from ttts_amd import ops
     P = -(-N // page) + 2

@@ -9,20 +9,26 @@
 
 namespace ttts {
 
-// one 16-byte piece per thread: piece (n, which, h, c) of row n
+// One 16-byte piece of a row's keys and of its values per thread; pieces of a row run over (head, column).  Bound by HBM: 30011 rows of 8
+// heads of 128, 232 MB read and written, take 46.5 us = 5.0 TB/s, what a large copy reaches.
 __global__ __launch_bounds__(256) void kv_page_write_kernel(const uint4* __restrict__ k, const uint4* __restrict__ v, int64_t ks_n, int64_t ks_h,
                                                             int64_t vs_n, int64_t vs_h, uint4* __restrict__ kp, uint4* __restrict__ vp,
-                                                            const int64_t* __restrict__ slots, int64_t total, int H, int chunks, int page,
-                                                            int64_t n_slots) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int c = (int)(i % chunks);
-    const int h = (int)(i / chunks % H);
-    const int64_t n = i / chunks / H;
-    const int64_t slot = slots[n];
-    if (slot < 0 || slot >= n_slots) continue;
-    const int64_t dst = (((slot / page) * H + h) * page + slot % page) * chunks + c;
-    kp[dst] = k[n * ks_n + h * ks_h + c];
-    vp[dst] = v[n * vs_n + h * vs_h + c];
+                                                            const int64_t* __restrict__ slots, int N, unsigned pieces, unsigned chunks,
+                                                            int page_shift, int64_t n_slots) {
+  const unsigned rows = 256 / pieces;                 // of a workgroup (at least one; longer rows: several rounds)
+  const unsigned r = rows ? threadIdx.x / pieces : 0;
+  const int64_t n = (int64_t)blockIdx.x * (rows ? rows : 1) + r;
+  if (n >= N || (rows && r >= rows)) return;
+  const int64_t slot = slots[n];
+  if (slot < 0 || slot >= n_slots) return;
+  const int64_t page = slot >> page_shift, at = slot & ((1 << page_shift) - 1);
+  const unsigned heads = pieces / chunks;
+  for (unsigned i = rows ? threadIdx.x % pieces : threadIdx.x; i < pieces; i += rows ? pieces : 256) {
+    const unsigned h = i / chunks, c = i % chunks;
+    const int64_t dst = (((page * heads + h) << page_shift) + at) * chunks + c;
+    const uint4 x = k[n * ks_n + h * ks_h + c], y = v[n * vs_n + h * vs_h + c];
+    kp[dst] = x;
+    vp[dst] = y;
   }
 }
 
@@ -32,9 +38,35 @@ struct PagedParams {
   float *lse, *part_o, *part_ml;          // partial results of split sequences: [M, H, chunks, DH] and [M, H, chunks][2]
   const int32_t *table, *lens;
   int64_t qs_m, qs_h, os_m, os_h, ts_m;   // strides in elements
-  int H, Hkv, group, tiles, page_shift, P, width, chunk, chunks;   // tiles: 16-row tiles of a head group; width: pages of a table row
+  int M, H, Hkv, group, tiles, page_shift, P, width, chunk, chunks, ordered;   // tiles: 16-row tiles of a head group; width: pages of a table row
   float scale_log2;
 };
+
+// The i-th sequence of a batch by length, longest first, in 16 steps of length, for up to PAGED_ORDERED sequences: a batch that fills the card
+// several times over then ends with its short sequences (96 ragged ones up to 4096 keys: 160 -> 151 us; 64 up to 2404: 33.9 -> 29.6).
+// Every workgroup works it out for itself, from one load a lane and 64 sequences.
+constexpr int PAGED_ORDERED = 512;
+__device__ __forceinline__ int ordered_sequence(const int32_t* lens, int M, int i, int longest, int lane) {
+  constexpr int N = PAGED_ORDERED / 64;
+  const float per = 16.f / (float)longest;
+  int level[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) level[j] = j * 64 + lane < M ? max(0, min(15, (int)((float)lens[j * 64 + lane] * per))) : -1;
+  for (int l = 15; l >= 0; --l) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (j * 64 >= M) break;
+      const unsigned long long mask = __ballot(level[j] == l);
+      const int n = __builtin_popcountll(mask);
+      if (i < n) {
+        const int below = __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+        return j * 64 + __builtin_ctzll(__ballot(level[j] == l && below == i));
+      }
+      i -= n;
+    }
+  }
+  return 0;   // (not reached: every sequence has a level)
+}
 
 template <typename T> struct Frag;
 template <> struct Frag<bf16> {
@@ -64,7 +96,7 @@ __global__ __launch_bounds__(NW * 64) void attn_paged_decode_kernel(PagedParams 
   const int hk = id % p.Hkv; id /= p.Hkv;
   const int tile = id % p.tiles; id /= p.tiles;
   const int chunk = id % p.chunks;
-  const int64_t m = id / p.chunks;
+  const int64_t m = p.ordered ? ordered_sequence(p.lens, p.M, id / p.chunks, p.width << p.page_shift, lane) : id / p.chunks;
   const int len = min(p.lens[m], p.width << p.page_shift);
   const int c0 = chunk * p.chunk, c1 = min(len, c0 + p.chunk);
   if (c0 >= len && !(chunk == 0 && p.chunks == 1)) return;   // (the join looks at no chunk behind the sequence's end)
@@ -264,7 +296,7 @@ __global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedParams p) {
 // units = workgroups of an unsplit call:
 //  * not at all up to 768 keys (three tiles for each of 8 waves): 613 keys of one sequence, 8 heads of 64: 6.0 us; split 6.4 - 7.0.
 //    Nor up to 4096 keys where the units alone give every CU two workgroups (of 4 waves then): 64 sequences up to 2404, 8 heads:
-//    40.7 us, 42.5 split; 96 up to 4096, 8 heads of 128: 148 us, 150 - 170 split in two to four.
+//    40.7 us, 42.5 split; 96 up to 4096, 8 heads of 128: 148 us, 150 - 170 split in two to four (38.8 and 139 longest first).
 //  * into 256 keys, one tile a wave, while that gives the card's 256 CUs one workgroup each at most: 2404 keys of one sequence
 //    6.9 us, against 10.8 in chunks of 1024; more workgroups than CUs cost more than they give (20000 keys: 12.2 us, 14.2 with 512).
 //  * beyond that into 1024 keys or more, about 1024 workgroups (4 sequences of 130000 keys: 178 us, 188 with 2048), or about 2048
@@ -312,12 +344,11 @@ extern "C" int ttts_kv_page_write(const void* k, const void* v, int64_t k_stride
   TTTS_REQUIRE(k && v && k_pages && v_pages && slots, "kv_page_write: null pointer");
   TTTS_REQUIRE(aligned16(k) && aligned16(v) && aligned16(k_pages) && aligned16(v_pages), "kv_page_write: 16-byte aligned bases are needed");
   TTTS_REQUIRE(((k_stride_n | k_stride_h | v_stride_n | v_stride_h) & 7) == 0, "kv_page_write: strides must be multiples of 8 elements");
-  const int chunks = head_dim / 8;
-  const int64_t total = (int64_t)N * H * chunks;
-  const int grid = (int)(cdiv(total, 256) < 1048576 ? cdiv(total, 256) : 1048576);
-  kv_page_write_kernel<<<grid, 256, 0, as_stream(stream)>>>((const uint4*)k, (const uint4*)v, k_stride_n / 8, k_stride_h / 8, v_stride_n / 8,
-                                                             v_stride_h / 8, (uint4*)k_pages, (uint4*)v_pages, slots, total, H, chunks, page,
-                                                             (int64_t)P * page);
+  const unsigned chunks = head_dim / 8, pieces = H * chunks, rows = pieces < 256 ? 256 / pieces : 1;
+  TTTS_REQUIRE(H <= 65536, "kv_page_write: %d heads", H);
+  kv_page_write_kernel<<<(unsigned)cdiv(N, rows), 256, 0, as_stream(stream)>>>((const uint4*)k, (const uint4*)v, k_stride_n / 8, k_stride_h / 8,
+                                                                               v_stride_n / 8, v_stride_h / 8, (uint4*)k_pages, (uint4*)v_pages,
+                                                                               slots, N, pieces, chunks, __builtin_ctz(page), (int64_t)P * page);
   return check_launch("kv_page_write");
 }
 
@@ -365,11 +396,12 @@ extern "C" int ttts_attn_paged_decode(const void* q, int64_t q_stride_m, int64_t
   PagedParams p{};
   p.q = q; p.kp = k_pages; p.vp = v_pages; p.out = out; p.lse = lse; p.table = block_table; p.lens = seq_lens;
   p.qs_m = q_stride_m; p.qs_h = q_stride_h; p.os_m = o_stride_m; p.os_h = o_stride_h; p.ts_m = table_stride;
-  p.H = H; p.Hkv = Hkv; p.group = H / Hkv; p.tiles = (int)paged_tiles(H, Hkv); p.page_shift = __builtin_ctz(page); p.P = P; p.width = width;
+  p.M = M; p.H = H; p.Hkv = Hkv; p.group = H / Hkv; p.tiles = (int)paged_tiles(H, Hkv); p.page_shift = __builtin_ctz(page); p.P = P; p.width = width;
   p.scale_log2 = scale * 1.4426950408889634f;
   const int64_t units = M * (int64_t)Hkv * p.tiles;
   const PagedSplit sp = paged_split(units, (int64_t)width * page);
   p.chunk = sp.chunk; p.chunks = sp.chunks;
+  p.ordered = units >= 512 && M <= PAGED_ORDERED;
   const int64_t grid = units * p.chunks, rows = (int64_t)M * H, need = paged_bytes(M, H, head_dim, p.chunks);
   TTTS_REQUIRE(grid <= 0x7fffffff && rows <= 0x7fffffff, "attn_paged_decode: more work than one launch holds (M %d, H %d)", M, H);
   TTTS_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned16(workspace)),

@@ -422,6 +422,7 @@ int ttts_diffusion_loss_bwd_f32(const float* model_out, const float* x_start, co
                                 int32_t C, int32_t T, void* stream);
 
 /* ---- scoring of given tokens and distillation on a teacher's alternatives ------------------------------------------
+ * (Added to ABI version 11; nothing that was there changes.)
  * Beside ttts_ce_fwd_bf16 (the mean loss alone) and ttts_sample_logits_f32 (the drawn token alone): what a token was worth, what
  * else was likely, and a student's loss on that.  logits [R, ldl] of `dtype`, C classes per row (columns C .. ldl - 1 are never
  * looked at), any row pitch >= C, aligned to the type only;
@@ -435,7 +436,8 @@ enum { TTTS_DTYPE_F32 = 0, TTTS_DTYPE_BF16 = 1, TTTS_DTYPE_F16 = 2 };
  *   stats f32 [R, 2] = (max of the row's logits, log sum e^(y - max / temperature)) for the backward -- their sum, the first over
  *   the temperature, is the log-sum-exp; top_logp f32 / top_idx int64 [R, top_k]: the top_k <= TTTS_SCORE_MAX_TOP best classes, best
  *   first, equal logits by ascending class (top_k 0: not written, may be NULL); where a row has fewer, -inf and -1.
- *   All classes at -inf: logp -inf (0 without a token), entropy 0, no alternatives.  NaN rows: every float NaN, every index -1.
+ *   All classes at -inf: logp -inf (0 without a token), entropy 0, no alternatives.  NaN rows: logp (0 without a token), entropy
+ *   and top_logp NaN, every index -1.
  * workspace: ttts_token_logprobs_workspace_bytes (16-byte aligned; may be 0 -> NULL), the call's own until it has run. */
 int64_t ttts_token_logprobs_workspace_bytes(int32_t R, int32_t C, int32_t top_k);
 int ttts_token_logprobs_fwd(const void* logits, int32_t dtype, int64_t ldl, const int64_t* tokens, float* logp, float* entropy,
@@ -443,8 +445,8 @@ int ttts_token_logprobs_fwd(const void* logits, int32_t dtype, int64_t ldl, cons
                             float temperature, void* workspace, int64_t workspace_bytes, void* stream);
 /* bwd: dlogits [R, ldd] of the logits' type = [g_logp (1[class = token] - p) - g_entropy p (log p + entropy)] / temperature, from the
  *   forward's stats and entropy; g_logp / g_entropy f32 [R] (g_entropy may be NULL); rows without a token ignore g_logp.  Columns
- *   C .. Cd - 1 are written as zeros (C <= Cd <= ldd).  dlogits may be the logits' own buffer (same pitch).  A row whose classes are
- *   all -inf gets zeros. */
+ *   C .. Cd - 1 are written as zeros (C <= Cd <= ldd).  dlogits is the logits' own buffer (same pitch) or shares no memory with them.
+ *   A row whose classes are all -inf gets zeros. */
 int ttts_token_logprobs_bwd(const void* logits, int32_t dtype, int64_t ldl, const int64_t* tokens, const float* stats,
                             const float* entropy, const float* g_logp, const float* g_entropy, void* dlogits, int64_t ldd,
                             int32_t R, int32_t C, int32_t Cd, float temperature, void* stream);
@@ -469,7 +471,7 @@ int ttts_distill_bwd(const void* logits, int32_t dtype, int64_t ldl, const int64
 /* ---- paged key / value cache and the attention of one new token that reads it ---------------------------------------
  * Beside ttts_kv_cache_fill_bf16 / ttts_attn_decode_bf16 (one block per sequence, all of one length): sequences of any length share
  * pages.  k_pages / v_pages [P, Hkv, page, head_dim] of bf16 or fp16, contiguous, page a power of two 16 .. 1024, head_dim in
- * {32, 64, 128}.  What comes from device memory is checked there and never reaches outside the cache.
+ * {32, 64, 128}, at most 65536 heads.  What comes from device memory is checked there and never reaches outside the cache.
  *  ttts_kv_page_write: row n of k / v [N, Hkv, head_dim] (strides in elements, multiples of 8; 16-byte aligned) -> position
  *    slots[n] % page of page slots[n] / page.  A slot outside [0, P page) writes nothing (padding rows: -1).  The slots of one call
  *    differ; where two rows name the same one, its 16-byte pieces are one row's or the other's.

@@ -185,6 +185,10 @@ def test_views_and_sliced_tables():
     out, lse = ops.attn_paged_decode(q, kp, vp, table.cuda(), L, 0.1, out=wide[:, 1::2])
     _check(out, lse, _ref(q, kp, vp, table, lens, 0.1), lens, dtype)
     assert (wide[:, ::2] == 7.0).all()
+    one = torch.randn(1, (H + 2 * Hkv) * dh + 4, generator=_gen(2)).to(dtype).cuda()[:, :(H + 2 * Hkv) * dh]   # one row: its pitch says nothing
+    ops.kv_page_write(one[:, H * dh:(H + Hkv) * dh].view(1, Hkv, dh), one[:, (H + Hkv) * dh:].view(1, Hkv, dh), kp, vp,
+                      torch.tensor([int(table[2, 3]) * page + 15]).cuda())
+    assert torch.equal(kp[int(table[2, 3]), :, 15], one[0, H * dh:(H + Hkv) * dh].view(Hkv, dh))
     cut = table.cuda()[:, :3]
     out, lse = ops.attn_paged_decode(q, kp, vp, cut, L, 0.1)
     _check(out, lse, _ref(q, kp, vp, table[:, :3], lens, 0.1), lens, dtype)

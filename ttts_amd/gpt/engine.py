@@ -725,9 +725,9 @@ class GptEngine:
         if self._bufs_key is None:
             raise TttsError("set_teacher: set the tokens first")
         B, _, Tm = self._bufs_key
-        if teacher_idx.dim() != 3 or teacher_idx.shape[:2] != (B, Tm) or teacher_logp.shape != teacher_idx.shape:
+        if teacher_logp is None or teacher_idx.dim() != 3 or teacher_idx.shape[:2] != (B, Tm) or teacher_logp.shape != teacher_idx.shape:
             raise TttsError("set_teacher: need [%d, %d, K] indices and log-probabilities, got %s and %s"
-                            % (B, Tm, tuple(teacher_idx.shape), tuple(teacher_logp.shape)))
+                            % (B, Tm, tuple(teacher_idx.shape), None if teacher_logp is None else tuple(teacher_logp.shape)))
         rows = B * Tm
         g_rows = torch.full((rows,), float(weight) / rows, dtype=torch.float32, device=self.device)
         self._teacher = (teacher_idx.reshape(rows, -1).contiguous(), teacher_logp.reshape(rows, -1).contiguous(), g_rows,

@@ -976,8 +976,8 @@ def token_logprobs_fwd(logits, tokens, C=None, top_k=0, temperature=1.0):
 
 
 def token_logprobs_bwd(logits, tokens, stats, entropy, g_logp, g_entropy=None, C=None, temperature=1.0, dlogits=None):
-    """Gradient of token_logprobs_fwd's logp and entropy to the logits: dlogits (new, or the given tensor; `logits` itself is allowed)
-    of the logits' type and shape, columns from C on zero.  g_logp / g_entropy f32 [R]."""
+    """Gradient of token_logprobs_fwd's logp and entropy to the logits: dlogits (new, or the given tensor: `logits` itself, or one that
+    shares no memory with it) of the logits' type and shape, columns from C on zero.  g_logp / g_entropy f32 [R]."""
     what, lib = "token_logprobs_bwd", _l.get()
     code, ld, R, C = _logits(logits, C, what)
     _vec(tokens, torch.int64, (R,), what, "tokens"); _vec(stats, torch.float32, (R, 2), what, "stats")
@@ -1026,9 +1026,9 @@ def _teacher(idx, logp, R, what):
 
 
 def distill_bwd(logits, teacher_idx, teacher_logp, stats, g_loss, C=None, temperature=1.0, tail=False, dlogits=None, accumulate=False):
-    """Gradient of distill_fwd's row losses to the logits, weighted by g_loss f32 [R]: dlogits (new, or the given tensor; `logits`
-    itself is allowed) of the logits' type and shape, columns from C on zero.  accumulate: added to the given dlogits instead
-    (columns from C on stay)."""
+    """Gradient of distill_fwd's row losses to the logits, weighted by g_loss f32 [R]: dlogits (new, or the given tensor: `logits`
+    itself, or one that shares no memory with it) of the logits' type and shape, columns from C on zero.  accumulate: added to the
+    given dlogits (not the logits) instead; columns from C on stay."""
     what, lib = "distill_bwd", _l.get()
     code, ld, R, C = _logits(logits, C, what)
     K = _teacher(teacher_idx, teacher_logp, R, what)
@@ -1057,12 +1057,12 @@ def _pages(k_pages, v_pages, what):
 
 
 def _heads(t, dtype, shape, what, name):
-    """Strides of rows and heads of a [rows, heads, head_dim] view with contiguous heads."""
+    """Strides of rows and heads of a [rows, heads, head_dim] view with contiguous heads (0 for the one row or head that has none)."""
     strides = t.stride()
     if t.shape != shape or t.dtype != dtype or strides[2] != 1:
         raise TttsError("%s: %s must be a %s tensor of shape %s with contiguous heads, got %s %s strides %s"
                         % (what, name, dtype, tuple(shape), t.dtype, tuple(t.shape), strides))
-    return strides[0], strides[1]
+    return strides[0] if shape[0] > 1 else 0, strides[1] if shape[1] > 1 else 0
 
 
 def kv_page_write(k, v, k_pages, v_pages, slots):

@@ -27,8 +27,10 @@ struct Cols {   // a wave's columns: c0 .. wide - 1 in `steps` of 512, wide .. e
     if (rest && rest <= NARROW) { --steps; wide -= rest; }
   }
   __device__ __forceinline__ bool narrow() const { return wide < end; }
-  template <typename T> __device__ __forceinline__ float load_narrow(const T* row, int lane) const {
-    return wide + lane < end ? (float)row[wide + lane] : -INFINITY;
+  // its load, of some column of the row where the lane has none (no branch, so that nothing waits for it there), and its value
+  template <typename T> __device__ __forceinline__ T load_narrow(const T* row, int last, int lane) const { return row[min(wide + lane, last)]; }
+  template <typename T> __device__ __forceinline__ float narrow_value(T v, int cend, int lane) const {
+    return wide + lane < min(end, cend) ? (float)v : -INFINITY;
   }
 };
 __device__ __forceinline__ float sum_wave(float v) { return over_wave(v, add_op); }
@@ -84,12 +86,6 @@ __device__ __forceinline__ void expand(const Raw<T>& r, const T* row, int c0, in
       if (c < cend && c + 8 > cend) load8<T>(row + c, cend - c, x[i]);
     }
   }
-}
-template <typename T>
-__device__ __forceinline__ void load_wave(const T* row, int c0, int cend, int lane, float (&x)[NV][8]) {
-  Raw<T> r;
-  load_raw(r, row, c0, cend, lane);
-  expand(r, row, c0, cend, lane, x);
 }
 
 // max(a, b) without the two instructions that would first make signalling NaNs quiet; a NaN is passed over, as by fmaxf
@@ -381,17 +377,18 @@ __global__ __launch_bounds__(256) void token_logprobs_fwd_kernel(ScoreParams p) 
   const Cols cols(unit * p.unit_cols, unit == p.units - 1 ? p.C : (unit + 1) * p.unit_cols);
   float x[NV][8], vmax[NV];
   int64_t tok = -1;
-  float xt = 0.f;
+  float xt = 0.f, xn;
   {
     Raw<T> raw;
+    if (!LONG) tok = p.tokens[row];
     load_raw(raw, lr, cols.c0, cols.wide, lane);
-    if (!LONG) {
-      tok = p.tokens[row];
-      if (tok >= 0 && tok < p.C) xt = (float)lr[tok];      // (its latency runs beside the row's)
-    }
+    const T narrow = cols.load_narrow(lr, p.C - 1, lane);
+    const bool given = tok >= 0 && tok < p.C;
+    const T at_tok = LONG ? T(0.f) : lr[given ? tok : 0];   // (its latency runs beside the row's)
     expand(raw, lr, cols.c0, cols.wide, lane, x);
+    xn = cols.narrow_value(narrow, p.C, lane);
+    xt = given ? (float)at_tok : 0.f;
   }
-  const float xn = cols.load_narrow(lr, lane);
   float lmax = xn;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -754,21 +751,34 @@ __global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(ScoreGradParams
 
 // ---- distillation ---------------------------------------------------------------------------------------------------------
 // A row's list, two entries a lane (one, and no work for the other, up to 64 entries): class (or -1), p and log p, and the list's mass.
+// Its loads go first and without branches: everything behind them in the wave then has one wait for them, not one each.
+struct ListLoads { int64_t id[2]; float t[2]; };
+__device__ __forceinline__ ListLoads load_list(const int64_t* idx, const float* tl, int K, int lane) {
+  ListLoads r;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    r.id[h] = -1;
+    r.t[h] = 0.f;
+    if (h * 64 < K) {
+      const int j = min(lane + 64 * h, K - 1);
+      r.id[h] = idx[j];
+      r.t[h] = tl[j];
+    }
+  }
+  return r;
+}
 struct Listed { int id[2]; float p[2], logp[2], mass; };
-__device__ __forceinline__ Listed load_listed(const int64_t* idx, const float* tl, int K, int C, float inv_t, int tail, int lane) {
-  Listed L;
+__device__ __forceinline__ void list_classes(Listed& L, const ListLoads& r, int K, int C, int lane) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) L.id[h] = lane + 64 * h < K && r.id[h] >= 0 && r.id[h] < C ? (int)r.id[h] : -1;
+}
+__device__ __forceinline__ void list_weights(Listed& L, const ListLoads& r, int K, float inv_t, int tail) {
   float t[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const int j = lane + 64 * h;
-    L.id[h] = -1;
+    t[h] = L.id[h] >= 0 ? r.t[h] : -INFINITY;
     L.p[h] = 0.f;
-    L.logp[h] = t[h] = -INFINITY;
-    if (j < K) {
-      const int64_t i = idx[j];
-      const float v = tl[j];
-      if (i >= 0 && i < C) { L.id[h] = (int)i; t[h] = v; }
-    }
+    L.logp[h] = -INFINITY;
   }
   if (tail) {
 #pragma unroll
@@ -778,7 +788,7 @@ __device__ __forceinline__ Listed load_listed(const int64_t* idx, const float* t
         L.p[h] = L.id[h] >= 0 ? __expf(t[h]) : 0.f;
       }
     L.mass = sum_wave(L.p[0] + L.p[1]);
-    return L;
+    return;
   }
   const float m = fmaxf(max_wave(K > 64 ? fmaxf(t[0], t[1]) : t[0]), -FMAX);
 #pragma unroll
@@ -795,7 +805,6 @@ __device__ __forceinline__ Listed load_listed(const int64_t* idx, const float* t
       L.logp[h] -= logz;
     }
   L.mass = z == 0.f ? 0.f : z * over;   // 1; 0 of a row without entries; NaN of one with
-  return L;
 }
 
 struct DistillParams {
@@ -808,13 +817,13 @@ struct DistillParams {
   float inv_t;
 };
 // by one wave: the row's loss from its sums (listed and other classes apart with tail, else all in zr) and the listed classes' logits
-__device__ __forceinline__ void finish_distill(const DistillParams& p, int64_t row, const Listed& L, const float (&xl)[2], float m, float zl, float zr,
+__device__ __forceinline__ void finish_distill(const DistillParams& p, int64_t row, const Listed& L, float x0, float x1, float m, float zl, float zr,
                                                int lane) {
   const float z = zl + zr, logz = __logf(z);
   float loss = 0.f;
 #pragma unroll
   for (int h = 0; h < 2; ++h)
-    if (L.p[h] != 0.f) loss += L.p[h] * (L.logp[h] - ((xl[h] - m) * p.inv_t - logz));
+    if (h * 64 < p.K && L.p[h] != 0.f) loss += L.p[h] * (L.logp[h] - (((h ? x1 : x0) - m) * p.inv_t - logz));
   loss = sum_wave(loss);
   if (lane == 0) {
     const float left = 1.f - L.mass;
@@ -828,9 +837,9 @@ __device__ __forceinline__ void finish_distill(const DistillParams& p, int64_t r
   }
 }
 template <typename T>
-__device__ __forceinline__ void listed_logits(const T* row, const Listed& L, float (&xl)[2]) {
+__device__ __forceinline__ void listed_logits(const T* row, const Listed& L, int K, T (&xl)[2]) {   // (some column's for an empty entry)
 #pragma unroll
-  for (int h = 0; h < 2; ++h) xl[h] = L.id[h] >= 0 ? (float)row[L.id[h]] : 0.f;
+  for (int h = 0; h < 2; ++h) xl[h] = h * 64 < K ? row[max(L.id[h], 0)] : T(0.f);
 }
 
 // as token_logprobs_fwd_kernel; with tail each wave marks the listed classes of its columns in a bit map of its own
@@ -845,15 +854,15 @@ __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillParams p) {
   if (row >= p.R) return;
   const T* lr = (const T*)p.logits + row * p.ldl;
   const Cols cols(unit * p.unit_cols, unit == p.units - 1 ? p.C : (unit + 1) * p.unit_cols);
+  ListLoads list;
+  if (!LONG || p.tail) list = load_list(p.idx + row * p.K, p.tlogp + row * p.K, p.K, lane);
   Raw<T> raw;
   load_raw(raw, lr, cols.c0, cols.wide, lane);
-  const float xn = cols.load_narrow(lr, lane);
+  const T narrow = cols.load_narrow(lr, p.C - 1, lane);
   Listed L;
-  float xl[2] = {0.f, 0.f};
-  if (!LONG) {
-    L = load_listed(p.idx + row * p.K, p.tlogp + row * p.K, p.K, p.C, p.inv_t, p.tail, lane);
-    listed_logits(lr, L, xl);
-  }
+  T xl[2] = {T(0.f), T(0.f)};
+  if (!LONG || p.tail) list_classes(L, list, p.K, p.C, lane);
+  if (!LONG) listed_logits(lr, L, p.K, xl);
   uint32_t* mark = marks[wave];
   if (p.tail) {
     mark[lane] = 0;
@@ -861,11 +870,13 @@ __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillParams p) {
     wave_fence();
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int64_t c = LONG ? (lane + 64 * h < p.K ? p.idx[row * p.K + lane + 64 * h] : -1) : L.id[h];
+      const int c = L.id[h];
       if (c >= cols.c0 && c < cols.end) atomicOr(&mark[(c - cols.c0) >> 5], 1u << ((c - cols.c0) & 31));
     }
     wave_fence();
   }
+  if (!LONG) list_weights(L, list, p.K, p.inv_t, p.tail);
+  const float xn = cols.narrow_value(narrow, p.C, lane);
   float x[NV][8], m = fmaxf(xn, -FMAX);
   expand(raw, lr, cols.c0, cols.wide, lane, x);
 #pragma unroll
@@ -906,7 +917,7 @@ __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillParams p) {
   const float f = __builtin_amdgcn_exp2f(-ex.delta);
   zr = sum_wave(zr) * f;
   if (p.tail) zl = sum_wave(zl) * f;
-  if (!LONG) finish_distill(p, row, L, xl, m, zl, zr, lane);
+  if (!LONG) finish_distill(p, row, L, (float)xl[0], (float)xl[1], m, zl, zr, lane);
   else if (lane == 0) p.part[id] = make_float4(m, zl, zr, 0.f);
 }
 template <typename T>
@@ -915,10 +926,14 @@ __global__ __launch_bounds__(256) void distill_join_kernel(DistillParams p) {   
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= p.R) return;
   const float4* part = p.part + row * p.units;
-  const float4 first = lane < p.units ? part[lane] : make_float4(-FMAX, 0.f, 0.f, 0.f);   // (on its way beside the list)
-  const Listed L = load_listed(p.idx + row * p.K, p.tlogp + row * p.K, p.K, p.C, p.inv_t, p.tail, lane);
-  float xl[2];
-  listed_logits((const T*)p.logits + row * p.ldl, L, xl);
+  const ListLoads list = load_list(p.idx + row * p.K, p.tlogp + row * p.K, p.K, lane);
+  float4 first = part[min(lane, p.units - 1)];
+  if (lane >= p.units) first = make_float4(-FMAX, 0.f, 0.f, 0.f);
+  Listed L;
+  list_classes(L, list, p.K, p.C, lane);
+  T xl[2];
+  listed_logits((const T*)p.logits + row * p.ldl, L, p.K, xl);
+  list_weights(L, list, p.K, p.inv_t, p.tail);
   float m = first.x, zl = 0.f, zr = 0.f;
   for (int u = lane + 64; u < p.units; u += 64) m = fmaxf(m, part[u].x);
   m = max_wave(m);
@@ -928,7 +943,7 @@ __global__ __launch_bounds__(256) void distill_join_kernel(DistillParams p) {   
     zl = fmaf(s.y, f, zl);
     zr = fmaf(s.z, f, zr);
   }
-  finish_distill(p, row, L, xl, m, sum_wave(zl), sum_wave(zr), lane);
+  finish_distill(p, row, L, (float)xl[0], (float)xl[1], m, sum_wave(zl), sum_wave(zr), lane);
 }
 
 struct DistillGradParams {
@@ -960,23 +975,32 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillGradParams p) {
   const int dend = cols.wide, cend = min(p.C, cols.end);
   const T* lr = (const T*)p.logits + row * p.ldl;
   T* dr = (T*)p.dlogits + row * p.ldd;
-  float x[NV][8];
-  load_wave<T>(lr, c0, min(p.C, cols.wide), lane, x);
-  const float xn = cols.wide + lane < cend ? (float)lr[cols.wide + lane] : -INFINITY;
-  Listed L = load_listed(p.idx + row * p.K, p.tlogp + row * p.K, p.K, p.C, p.inv_t, p.tail, lane);
-  const float m = p.stats[3 * row], logz = p.stats[3 * row + 1], w = p.stats[3 * row + 2], g = p.g_loss[row] * p.inv_t;
-  uint8_t* tag = tags[wave];
+  const ListLoads list = load_list(p.idx + row * p.K, p.tlogp + row * p.K, p.K, lane);
+  Raw<T> raw;
+  load_raw(raw, lr, c0, min(p.C, cols.wide), lane);
+  const T narrow = cols.load_narrow(lr, p.C - 1, lane);
+  Listed L;
+  list_classes(L, list, p.K, p.C, lane);
   bool here[2];
-  float xl[2] = {0.f, 0.f}, old[2] = {0.f, 0.f};
+  T xl[2], old[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     here[h] = L.id[h] >= c0 && L.id[h] < cend;
-    if (here[h]) {
-      tag[L.id[h] - c0] = (uint8_t)(lane + 64 * h);
-      xl[h] = (float)lr[L.id[h]];
-      if (p.accumulate) old[h] = (float)dr[L.id[h]];
+    xl[h] = old[h] = T(0.f);
+    if (h * 64 < p.K) {
+      xl[h] = lr[here[h] ? L.id[h] : 0];
+      if (p.accumulate) old[h] = dr[here[h] ? L.id[h] : 0];
     }
   }
+  const float m = p.stats[3 * row], logz = p.stats[3 * row + 1], w = p.stats[3 * row + 2], g = p.g_loss[row] * p.inv_t;
+  uint8_t* tag = tags[wave];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    if (here[h]) tag[L.id[h] - c0] = (uint8_t)(lane + 64 * h);
+  list_weights(L, list, p.K, p.inv_t, p.tail);
+  float x[NV][8];
+  expand(raw, lr, c0, min(p.C, cols.wide), lane, x);
+  const float xn = cols.narrow_value(narrow, p.C, lane);
   wave_fence();
   bool twice = false;
 #pragma unroll
@@ -1031,8 +1055,8 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillGradParams p) {
 #pragma unroll
   for (int h = 0; h < 2; ++h)
     if (here[h]) {
-      const float q = __builtin_amdgcn_exp2f((xl[h] - m) * c - log2z);
-      dr[L.id[h]] = (T)(old[h] + fmaf(q, on, -L.p[h]) * g);
+      const float q = __builtin_amdgcn_exp2f(((float)xl[h] - m) * c - log2z);
+      dr[L.id[h]] = (T)((float)old[h] + fmaf(q, on, -L.p[h]) * g);
     }
 }
 

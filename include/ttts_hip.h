@@ -427,7 +427,8 @@ int ttts_diffusion_loss_bwd_f32(const float* model_out, const float* x_start, co
  * else was likely, and a student's loss on that.  logits [R, ldl] of `dtype`, C classes per row (columns C .. ldl - 1 are never
  * looked at), any row pitch >= C, aligned to the type only;
  * y = logits / temperature; sums and statistics are fp32.  A class at -inf has no probability and is no alternative.
- * Rows: one whose classes are all -inf has no distribution (below); one that holds a NaN or +inf gets NaN. */
+ * Rows: one whose classes are all -inf has no distribution (below); one that holds a NaN or +inf gets NaN.
+ * Calls that would need 2^32 threads of one launch (some 67 million rows of up to 2048 classes) are refused, here and below. */
 enum { TTTS_DTYPE_F32 = 0, TTTS_DTYPE_BF16 = 1, TTTS_DTYPE_F16 = 2 };
 #define TTTS_SCORE_MAX_CLASSES 1048576
 #define TTTS_SCORE_MAX_TOP 64
@@ -474,13 +475,13 @@ int ttts_distill_bwd(const void* logits, int32_t dtype, int64_t ldl, const int64
  * {32, 64, 128}, at most 65536 heads.  What comes from device memory is checked there and never reaches outside the cache.
  *  ttts_kv_page_write: row n of k / v [N, Hkv, head_dim] (strides in elements, multiples of 8; 16-byte aligned) -> position
  *    slots[n] % page of page slots[n] / page.  A slot outside [0, P page) writes nothing (padding rows: -1).  The slots of one call
- *    differ; where two rows name the same one, its 16-byte pieces are one row's or the other's.
+ *    differ; where two rows name the same one, its 16-byte pieces are one row's or the other's.  k / v share no memory with the pages.
  *  ttts_attn_paged_decode: q [M, H, head_dim] (strides as above), heads h H/Hkv .. share key / value head h; block_table
  *    int32 [M, width] (row pitch table_stride): pages of sequence m in order; seq_lens int32 [M]: its keys, the new token's among
  *    them (write it first).  out [M, H, head_dim] = softmax(scale q K^T) V over keys 0 .. seq_lens[m] - 1, lse f32 [M, H] =
  *    log sum exp(scaled scores).  A length beyond width * page ends there; keys of a table entry outside [0, P) are left out;
- *    without keys (length <= 0) out is 0 and lse -inf.  fp32 softmax and sums; the weights are rounded to the cache's type for the
- *    product with V.  workspace: ttts_attn_paged_decode_workspace_bytes (16-byte aligned), the call's own until it has run. */
+ *    without keys (length <= 0) out is 0 and lse -inf.  fp32 softmax and sums; the weights are rounded to the cache's type (fp16: as
+ *    2^15 times themselves) for the product with V.  workspace: ttts_attn_paged_decode_workspace_bytes (16-byte aligned), the call's own until it has run. */
 int ttts_kv_page_write(const void* k, const void* v, int64_t k_stride_n, int64_t k_stride_h, int64_t v_stride_n,
                        int64_t v_stride_h, void* k_pages, void* v_pages, const int64_t* slots, int32_t dtype, int32_t N,
                        int32_t Hkv, int32_t head_dim, int32_t page, int32_t P, void* stream);

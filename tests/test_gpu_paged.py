@@ -301,3 +301,64 @@ def test_refusals_on_the_gpu():
         with pytest.raises(TttsError):
             f()
             pytest.fail("refusal %d did not come" % n)
+
+
+def _one_far(n, far, dtype, dh=32, page=64, big=1024.0):
+    """One sequence of n keys: the first scores 0 (bits) with value 0, the others `far` bits below with value `big`."""
+    table, P, _ = _tables([n], page, 4)
+    kp, vp = torch.zeros(P, 1, page, dh, dtype=dtype), torch.zeros(P, 1, page, dh, dtype=dtype)
+    for pg in table[0].tolist():
+        kp[pg, :, :, 0], vp[pg] = 1.0, big
+    kp[int(table[0, 0]), :, 0], vp[int(table[0, 0]), :, 0] = 0.0, 0.0
+    q = torch.zeros(1, 1, dh, dtype=dtype)
+    q[0, 0, 0] = -far
+    return q.cuda(), kp.cuda(), vp.cuda(), table
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,far", [(4096, 25.5), (500, 20.0), (30000, 28.0)])
+def test_attn_paged_decode_small_weights_add_up(dtype, n, far):
+    """Weights of 2^-20 .. 2^-28 of the largest, thousands of them: less than fp16's own steps, and all there is of the result."""
+    from ttts_amd import ops
+    q, kp, vp, table = _one_far(n, far, dtype)
+    out, lse = ops.attn_paged_decode(q, kp, vp, table.cuda(), torch.tensor([n], dtype=torch.int32).cuda(), math.log(2.0))
+    ref, _, rl, S = _ref(q, kp, vp, table, [n], math.log(2.0))
+    e = torch.finfo(dtype).eps / 2                       # the weights once, the result once
+    r = (n / 64 + 32) * U
+    assert ((out.double().cpu() - ref).abs() <= ref.abs() * (2.1 * e + 4 * (S[..., None] + r))).all(), (out[0, 0, 0].item(), ref[0, 0, 0].item())
+    assert ((lse.double().cpu() - rl).abs() <= 2 * S + r).all()
+
+
+@pytest.mark.parametrize("n", [1, 40, 1500])
+def test_attn_paged_decode_scores_at_the_end_of_the_range(n):
+    """Scores (in bits) between -3.0e38 and the lowest fp32 number are scores: equal ones share the values."""
+    from ttts_amd import ops
+    table, P, _ = _tables([n], 64, 5)
+    kp, vp = _cache(P, 1, 64, 32, torch.bfloat16, 6)
+    kp.zero_()
+    kp[..., 0] = -(2.0 ** 64)
+    q = torch.zeros(1, 1, 32, dtype=torch.bfloat16).cuda()
+    q[0, 0, 0] = 1.7265625 * 2.0 ** 63                   # product -2.93e38; times 0.75 log2 e: -3.18e38
+    out, lse = ops.attn_paged_decode(q, kp, vp, table.cuda(), torch.tensor([n], dtype=torch.int32).cuda(), 0.75)
+    ref, mag, rl, _ = _ref(q, kp, vp, table, [n], 0.75)
+    e = torch.finfo(torch.bfloat16).eps / 2
+    assert ((out.double().cpu() - ref).abs() <= e * (mag + ref.abs()) * 1.1 + (n / 64 + 32) * U * mag).all()
+    assert ((lse.double().cpu() - rl).abs() <= 8 * U * rl.abs()).all()
+
+
+def test_attn_paged_decode_out_must_not_overlap():
+    from ttts_amd import ops
+    from ttts_amd.lib import TttsError
+    table, P, _ = _tables([5, 6], 16, 7)
+    kp, vp = _cache(P, 2, 16, 32, torch.bfloat16, 8)
+    q = torch.randn(2, 4, 32, generator=_gen(9)).to(torch.bfloat16).cuda()
+    args = (q, kp, vp, table.cuda(), torch.tensor([5, 6], dtype=torch.int32).cuda(), 0.2)
+    want, _ = ops.attn_paged_decode(*args)
+    one = torch.zeros(1, 1, 32, dtype=torch.bfloat16).cuda()
+    for out in (one.expand(2, 4, 32), torch.zeros(2, 1, 32, dtype=torch.bfloat16).cuda().expand(2, 4, 32),
+                torch.zeros(512, dtype=torch.bfloat16).cuda().as_strided((2, 4, 32), (32, 32, 1))):
+        with pytest.raises(TttsError, match="overlap"):
+            ops.attn_paged_decode(*args, out=out)
+    across = torch.zeros(4, 2, 40, dtype=torch.bfloat16).cuda()[..., :32].transpose(0, 1)   # heads first in memory, with a pitch
+    got, _ = ops.attn_paged_decode(*args, out=across)
+    assert got is across and torch.equal(across, want)

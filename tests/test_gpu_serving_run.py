@@ -163,3 +163,25 @@ def test_gpt_score_and_teacher():
         eng.train_step(dev_tokens, capture=True, teacher=dict(teacher_idx=r.top_idx, teacher_logp=r.top_logp))
     with pytest.raises(TttsError):
         eng.set_teacher(r.top_idx[:, :-1], r.top_logp[:, :-1])
+
+
+def test_teacher_arguments_are_checked_before_the_step():
+    from ttts_amd.gpt.model import prepare_tokens
+    from ttts_amd.lib import TttsError
+    cfg, (teacher, student), batch = _models()
+    r = teacher.score(*batch, top_k=5)
+    eng = student.engine
+    tokens = [t.cuda() for t in prepare_tokens(teacher.cfg, *batch)]
+    before = eng.params.clone()
+    wide = r.top_idx.repeat(1, 1, 26)
+    for bad in (dict(teacher_idx=r.top_idx.int(), teacher_logp=r.top_logp), dict(teacher_idx=r.top_idx, teacher_logp=r.top_logp.double()),
+                dict(teacher_idx=r.top_idx.cpu(), teacher_logp=r.top_logp.cpu()), dict(teacher_idx=r.top_idx[..., :0], teacher_logp=r.top_logp[..., :0]),
+                dict(teacher_idx=wide, teacher_logp=r.top_logp.repeat(1, 1, 26)), dict(teacher_idx=r.top_idx),
+                dict(teacher_idx=r.top_idx, teacher_logp=r.top_logp, temperature=0.0)):
+        with pytest.raises(TttsError):
+            eng.train_step(tokens, teacher=bad)
+        assert eng._teacher is None and torch.equal(eng.params, before) and not eng.grads.any()
+    eng.train_step(tokens, teacher=dict(teacher_idx=r.top_idx, teacher_logp=r.top_logp))
+    assert math.isfinite(eng.distill_loss.item())
+    eng.train_step(tokens)
+    assert eng.distill_loss is None                      # no loss of an earlier step's teacher

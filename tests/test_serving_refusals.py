@@ -122,3 +122,14 @@ def test_wrappers_refuse_cpu_tensors():
     for f in calls:
         with pytest.raises(TttsError, match="must live on the GPU"):
             f()
+
+
+def test_more_than_one_launch_holds(lib):
+    """2^32 threads of one launch, or more: refused by name, nothing is launched."""
+    big = 1 << 30
+    _refused(lib, "ttts_token_logprobs_fwd", FWD, "one launch", R=big)
+    _refused(lib, "ttts_token_logprobs_bwd", BWD, "one launch", R=(1 << 31) - 1, C=16)
+    _refused(lib, "ttts_distill_fwd", DFWD, "one launch", R=big)
+    _refused(lib, "ttts_distill_bwd", DBWD, "one launch", R=big)
+    _refused(lib, "ttts_kv_page_write", WRITE, "one launch", N=big, H=64, ksn=4096, vsn=4096)
+    _refused(lib, "ttts_attn_paged_decode", ATT, "one launch", M=big, width=4)

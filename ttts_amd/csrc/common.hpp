@@ -51,6 +51,8 @@ inline int check_launch(const char* what) {
   if (e != hipSuccess) return fail(TTTS_EHIP, "%s: %s", what, hipGetErrorString(e));
   return TTTS_OK;
 }
+// a launch has fewer than 2^32 threads
+inline bool one_launch(int64_t workgroups, int threads) { return workgroups <= 0xffffffffLL / threads; }
 #define TTTS_REQUIRE(cond, ...) \
   do {                          \
     if (!(cond)) return ::ttts::fail(TTTS_EINVAL, __VA_ARGS__); \

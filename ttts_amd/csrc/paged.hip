@@ -3,6 +3,7 @@
 //   attn_paged_decode : softmax(scale q K^T) V of one new token per sequence over the keys its table lists
 // Everything that comes from device memory (slots, table entries, lengths) is checked there: a slot outside the cache writes
 // nothing, keys of a page outside the cache are left out, a length beyond the table ends with it.
+#include <float.h>
 #include <math.h>
 
 #include "common.hpp"
@@ -70,9 +71,12 @@ __device__ __forceinline__ int ordered_sequence(const int32_t* lens, int M, int 
 
 template <typename T> struct Frag;
 template <> struct Frag<bf16> {
+  static constexpr float weight = 1.f;
   static __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 template <> struct Frag<_Float16> {
+  static constexpr float weight = 32768.f;   // a weight of one enters the product as this: fp16 then holds them down to 2^-39 of the
+                                             // largest, 2^-29 in full (thousands of keys 2^-25 below it are part of the result)
   static __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 // One workgroup = one chunk of keys of one (sequence, key / value head, 16 query rows); its waves take the chunk's 32-key tiles in turn,
@@ -108,7 +112,7 @@ __global__ __launch_bounds__(NW * 64) void attn_paged_decode_kernel(PagedParams 
     qf[c] = T8{};
     if (col < rows) qf[c] = *reinterpret_cast<const T8*>((const T*)p.q + m * p.qs_m + (int64_t)(h0 + col) * p.qs_h + 32 * c + 8 * g);
   }
-  float mx = -3.0e38f, l = 0.f;
+  float mx = -FLT_MAX, l = 0.f;
   f32x4 acc[W];
 #pragma unroll
   for (int r = 0; r < W; ++r) acc[r] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -186,7 +190,7 @@ __global__ __launch_bounds__(NW * 64) void attn_paged_decode_kernel(PagedParams 
       for (int j = 0; j < 8; ++j) {
         const float e = __builtin_amdgcn_exp2f(s[j] - mx);
         l += e;
-        pf[j] = (T)e;
+        pf[j] = (T)(e * Frag<T>::weight);
       }
 #pragma unroll
       for (int r = 0; r < W; ++r) {
@@ -208,7 +212,7 @@ __global__ __launch_bounds__(NW * 64) void attn_paged_decode_kernel(PagedParams 
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int r = 0; r < W; ++r) o[i * W + r] = acc[r][i];
+      for (int r = 0; r < W; ++r) o[i * W + r] = acc[r][i] * (1.f / Frag<T>::weight);
     if (g == 0) { sm_ml[(wave * rows + col) * 2] = mx; sm_ml[(wave * rows + col) * 2 + 1] = l; }
   }
   __syncthreads();
@@ -255,7 +259,7 @@ __global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedParams p) {
   for (int i = 0; i < AHEAD; ++i) ahead[i] = po[(int64_t)min(grp + i * G, p.chunks - 1) * LPC];
   const float2 s0 = ml[min(tid, p.chunks - 1)];
   const int n = len > 0 ? (len + p.chunk - 1) / p.chunk : 0;
-  float M = tid < n ? s0.x : -3.0e38f;
+  float M = tid < n ? s0.x : -FLT_MAX;
   for (int c = tid + 256; c < n; c += 256) M = fmaxf(M, ml[c].x);
   M = over_wave(M, max_op);
   if ((tid & 63) == 0) sm_r[0][tid >> 6] = M;
@@ -346,6 +350,7 @@ extern "C" int ttts_kv_page_write(const void* k, const void* v, int64_t k_stride
   TTTS_REQUIRE(((k_stride_n | k_stride_h | v_stride_n | v_stride_h) & 7) == 0, "kv_page_write: strides must be multiples of 8 elements");
   const unsigned chunks = head_dim / 8, pieces = H * chunks, rows = pieces < 256 ? 256 / pieces : 1;
   TTTS_REQUIRE(H <= 65536, "kv_page_write: %d heads", H);
+  TTTS_REQUIRE(one_launch(cdiv(N, rows), 256), "kv_page_write: more work than one launch holds (%d rows)", N);
   kv_page_write_kernel<<<(unsigned)cdiv(N, rows), 256, 0, as_stream(stream)>>>((const uint4*)k, (const uint4*)v, k_stride_n / 8, k_stride_h / 8,
                                                                                v_stride_n / 8, v_stride_h / 8, (uint4*)k_pages, (uint4*)v_pages,
                                                                                slots, N, pieces, chunks, __builtin_ctz(page), (int64_t)P * page);
@@ -403,7 +408,7 @@ extern "C" int ttts_attn_paged_decode(const void* q, int64_t q_stride_m, int64_t
   p.chunk = sp.chunk; p.chunks = sp.chunks;
   p.ordered = units >= 512 && M <= PAGED_ORDERED;
   const int64_t grid = units * p.chunks, rows = (int64_t)M * H, need = paged_bytes(M, H, head_dim, p.chunks);
-  TTTS_REQUIRE(grid <= 0x7fffffff && rows <= 0x7fffffff, "attn_paged_decode: more work than one launch holds (M %d, H %d)", M, H);
+  TTTS_REQUIRE(one_launch(grid, sp.waves * 64) && one_launch(rows, 256), "attn_paged_decode: more work than one launch holds (M %d, H %d)", M, H);
   TTTS_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned16(workspace)),
                "attn_paged_decode: needs a 16-byte aligned workspace of %lld bytes", (long long)need);
   p.part_o = (float*)workspace;

@@ -1088,8 +1088,8 @@ static int need_workspace(const char* what, int64_t need, const void* ws, int64_
   TTTS_REQUIRE(need == 0 || (ws && have >= need && aligned16(ws)), "%s: needs a 16-byte aligned workspace of %lld bytes", what, (long long)need);
   return TTTS_OK;
 }
-static int need_grid(const char* what, int64_t grid) {
-  TTTS_REQUIRE(grid <= 0x7fffffff, "%s: more work than one launch holds", what);
+static int need_grid(const char* what, int64_t grid, int threads = 256) {
+  TTTS_REQUIRE(one_launch(grid, threads), "%s: more work than one launch holds", what);
   return TTTS_OK;
 }
 
@@ -1116,6 +1116,7 @@ static int launch_score(const ScoreParams& p, hipStream_t st) {
   const char* what = "token_logprobs_fwd";
   const int64_t grid = cdiv((int64_t)p.R * p.units, 4);
   int rc = need_grid(what, grid);
+  if (!rc && p.k && p.units > 8) rc = need_grid(what, p.R, p.units <= 64 ? 256 : 1024);
   if (rc) return rc;
   if (p.units == 1) {
     token_logprobs_fwd_kernel<T, false><<<(unsigned)grid, 256, p.k ? 4 * WAVE_TOP_LDS * sizeof(typename WaveKey<T>::type) : 0, st>>>(p);

@@ -23,7 +23,7 @@ import os
 import torch
 
 from .. import ops
-from ..lib import EPI_DGELU_BF16, EPI_GELU_BF16, EPI_RESID_ADD_F32, EPI_STORE_BF16, TttsError
+from ..lib import DISTILL_MAX_K, EPI_DGELU_BF16, EPI_GELU_BF16, EPI_RESID_ADD_F32, EPI_STORE_BF16, TttsError
 
 DEFAULTS = dict(layers=8, model_dim=512, heads=8, max_text_tokens=120, max_mel_tokens=250,
                 max_conditioning_inputs=1, mel_length_compression=1024, number_text_tokens=256,
@@ -407,7 +407,7 @@ class GptEngine:
         if Tt > self.c["max_text_tokens"] + 2 or Tm > self.c["max_mel_tokens"] + 2:
             raise ValueError("sequence exceeds the learned position tables (text %d, mel %d)" % (Tt, Tm))
         self._ensure_buffers(B, Tt, Tm)
-        self._teacher = None             # it belonged to the last tokens
+        self._teacher = self.distill_loss = None   # they belonged to the last tokens
         b = self.b
         b["text_inp"].copy_(text_inp, non_blocking=True)
         b["text_tar"].copy_(text_tar.reshape(-1), non_blocking=True)
@@ -430,7 +430,7 @@ class GptEngine:
         if Tt + 2 > c["max_text_tokens"] + 2 or Tm + 2 > c["max_mel_tokens"] + 2:
             raise ValueError("sequence exceeds the learned position tables (text %d, mel %d)" % (Tt + 2, Tm + 2))
         self._ensure_buffers(B, Tt + 2, Tm + 2)
-        self._teacher = None             # it belonged to the last tokens
+        self._teacher = self.distill_loss = None   # they belonged to the last tokens
         b = self.b
         ops.gpt_prepare_tokens(text_inputs, mel_codes, [int(w) // comp + 1 for w in wl], Tt, Tm, c["start_text_token"],
                                c["stop_text_token"], c["start_mel_token"], c["stop_mel_token"], b["text_inp"], b["text_tar"],
@@ -719,8 +719,8 @@ class GptEngine:
         teacher's alternatives: teacher_idx int64 / teacher_logp f32 [B, Tm, K], as UnifiedVoice.score returns them (at the same
         temperature; tail False: any logits of the listed classes).  The loss is left in `distill_loss` (device scalar).
         set_teacher(None), other tokens, and the next train_step without a teacher end it."""
+        self._teacher = self.distill_loss = None
         if teacher_idx is None:
-            self._teacher = None
             return
         if self._bufs_key is None:
             raise TttsError("set_teacher: set the tokens first")
@@ -728,6 +728,13 @@ class GptEngine:
         if teacher_logp is None or teacher_idx.dim() != 3 or teacher_idx.shape[:2] != (B, Tm) or teacher_logp.shape != teacher_idx.shape:
             raise TttsError("set_teacher: need [%d, %d, K] indices and log-probabilities, got %s and %s"
                             % (B, Tm, tuple(teacher_idx.shape), None if teacher_logp is None else tuple(teacher_logp.shape)))
+        for t, dtype in ((teacher_idx, torch.int64), (teacher_logp, torch.float32)):
+            if t.dtype != dtype or t.device != self.params.device:
+                raise TttsError("set_teacher: need int64 indices and float32 log-probabilities on %s, got %s on %s"
+                                % (self.params.device, t.dtype, t.device))
+        if not 0 < teacher_idx.shape[2] <= DISTILL_MAX_K or not 0.0 < float(temperature) < float("inf"):
+            raise TttsError("set_teacher: need 1 .. %d entries and a positive temperature (got %d, %s)"
+                            % (DISTILL_MAX_K, teacher_idx.shape[2], temperature))
         rows = B * Tm
         g_rows = torch.full((rows,), float(weight) / rows, dtype=torch.float32, device=self.device)
         self._teacher = (teacher_idx.reshape(rows, -1).contiguous(), teacher_logp.reshape(rows, -1).contiguous(), g_rows,

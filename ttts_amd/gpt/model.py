@@ -189,7 +189,7 @@ class UnifiedVoice(nn.Module):
         """What the model gives each mel target of a batch (the arguments of `forward`), without dropout: `ops.TokenLogprobs` of
         logp / entropy f32 [B, Tm], top_logp f32 / top_idx int64 [B, Tm, top_k] (None for top_k 0), stats f32 [B, Tm, 2].  Targets are
         forward's: the codes, STOP at the padding and twice at the end.  The alternatives of one model are another's teacher
-        (GptEngine.train_step)."""
+        (GptEngine.train_step).  The activations of the last forward are overwritten: call its backward first."""
         if types is not None:
             text_inputs = text_inputs * (1 + types).unsqueeze(-1)
         eng = self.engine

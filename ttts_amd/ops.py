@@ -1069,7 +1069,7 @@ def kv_page_write(k, v, k_pages, v_pages, slots):
     """Keys and values of new tokens enter a paged cache: row n of k / v [N, heads, head_dim] (views with strides of multiples of 8, as the
     parts of a packed projection) goes to position slots[n] % page of page slots[n] // page of k_pages / v_pages [pages, heads, page
     size, head_dim], bf16 or fp16.  slots int64 [N]; one outside the cache (-1: a padding row) writes nothing.  The slots of a call
-    differ from each other."""
+    differ from each other, and k / v share no memory with the pages."""
     what, lib = "kv_page_write", _l.get()
     code = _pages(k_pages, v_pages, what)
     P, H, page, dh = k_pages.shape
@@ -1110,6 +1110,8 @@ def attn_paged_decode(q, k_pages, v_pages, block_table, seq_lens, scale, out=Non
     if out is None:
         out = torch.empty(M, H, dh, dtype=q.dtype, device=q.device)
     osm, osh = _heads(out, q.dtype, (M, H, dh), what, "out")
+    if (H > 1 and osh < dh) or (M > 1 and osm < dh) or (H > 1 and M > 1 and max(osm, osh) < min(osm, osh) * ((M if osm < osh else H) - 1) + dh):
+        raise TttsError("%s: rows of out overlap (strides %s)" % (what, out.stride()))
     lse = torch.empty(M, H, dtype=torch.float32, device=q.device)
     n = lib.ttts_attn_paged_decode_workspace_bytes(M, H, Hkv, dh, page, width)
     ws = _workspace(n, q.device)

@@ -933,7 +933,7 @@ def _logits(logits, C, what):
 
 def _grad_rows(dlogits, logits, what):
     if dlogits is None:
-        dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        dlogits = logits.new_empty(*logits.shape)
     if dlogits.dtype != logits.dtype or dlogits.shape != logits.shape:
         raise TttsError("%s: dlogits must have the type and the shape of logits" % what)
     ldd, _, _ = _rows(dlogits, what, "dlogits")
@@ -964,8 +964,9 @@ def token_logprobs_fwd(logits, tokens, C=None, top_k=0, temperature=1.0):
     if other is not None:
         with torch.cuda.device(other):
             return token_logprobs_fwd(logits, tokens, C, top_k, temperature)
-    f = lambda *shape, dt=torch.float32: torch.empty(shape, dtype=dt, device=logits.device)  # noqa: E731
-    r = TokenLogprobs(f(R), f(R), f(R, k) if k > 0 else None, f(R, k, dt=torch.int64) if k > 0 else None, f(R, 2))
+    stats = logits.new_empty(R, 2, dtype=torch.float32)          # (the others from it: the cheapest way to a tensor, and there are five)
+    r = TokenLogprobs(stats.new_empty(R), stats.new_empty(R), stats.new_empty(R, k) if k > 0 else None,
+                      tokens.new_empty(R, k) if k > 0 else None, stats)
     n = lib.ttts_token_logprobs_workspace_bytes(R, C, k)
     ws = _workspace(n, logits.device)
     rc = lib.ttts_token_logprobs_fwd(_a(logits), code, ld, _a(tokens), _a(r.logp), _a(r.entropy), _a(r.stats), _a(r.top_logp),
@@ -1007,8 +1008,7 @@ def distill_fwd(logits, teacher_idx, teacher_logp, C=None, temperature=1.0, tail
     if other is not None:
         with torch.cuda.device(other):
             return distill_fwd(logits, teacher_idx, teacher_logp, C, temperature, tail)
-    loss = torch.empty(R, dtype=torch.float32, device=logits.device)
-    stats = torch.empty(R, 3, dtype=torch.float32, device=logits.device)
+    loss, stats = teacher_logp.new_empty(R), teacher_logp.new_empty(R, 3)
     n = lib.ttts_distill_workspace_bytes(R, C)
     ws = _workspace(n, logits.device)
     rc = lib.ttts_distill_fwd(_a(logits), code, ld, _a(teacher_idx), _a(teacher_logp), _a(loss), _a(stats), R, C, K,
@@ -1108,11 +1108,11 @@ def attn_paged_decode(q, k_pages, v_pages, block_table, seq_lens, scale, out=Non
         with torch.cuda.device(other):
             return attn_paged_decode(q, k_pages, v_pages, block_table, seq_lens, scale, out)
     if out is None:
-        out = torch.empty(M, H, dh, dtype=q.dtype, device=q.device)
+        out = q.new_empty(M, H, dh)
     osm, osh = _heads(out, q.dtype, (M, H, dh), what, "out")
     if (H > 1 and osh < dh) or (M > 1 and osm < dh) or (H > 1 and M > 1 and max(osm, osh) < min(osm, osh) * ((M if osm < osh else H) - 1) + dh):
         raise TttsError("%s: rows of out overlap (strides %s)" % (what, out.stride()))
-    lse = torch.empty(M, H, dtype=torch.float32, device=q.device)
+    lse = q.new_empty(M, H, dtype=torch.float32)
     n = lib.ttts_attn_paged_decode_workspace_bytes(M, H, Hkv, dh, page, width)
     ws = _workspace(n, q.device)
     rc = lib.ttts_attn_paged_decode(_a(q), qsm, qsh, _a(k_pages), _a(v_pages), _a(block_table), ts, _a(seq_lens),

@@ -195,6 +195,23 @@ def test_alternatives_where_values_repeat_or_crowd(dtype, C, top_k):
     _inside(r.top_logp, tl, _r(C) + 4 * U * tl.abs().nan_to_num(posinf=0.0), "top_logp")
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("C,every,top_k", [(40000, 4, 64), (40000, 4, 9), (100003, 4, 33), (300000, 16, 64), (20000, 10, 20)])
+def test_alternatives_crowd_into_few_parts_of_a_row(dtype, C, every, top_k):
+    """The largest classes all in every `every`-th stretch of 2048, or all in one: few waves hold them, the others' bounds say little."""
+    from ttts_amd import ops
+    R = 5
+    x = torch.randn(R, C, generator=torch.Generator().manual_seed(C + every))
+    part = torch.arange(C) // 2048
+    x[:3, part % every == 1] += 30.0
+    x[3, part == every - 1] += 30.0
+    x[4] = -x[4].abs() - 1.0                              # below zero throughout
+    x = x.to(dtype).cuda()
+    r = ops.token_logprobs_fwd(x, torch.zeros(R, dtype=torch.int64).cuda(), top_k=top_k)
+    want = torch.sort(x.float().cpu(), dim=1, descending=True, stable=True).indices[:, :top_k]
+    assert torch.equal(r.top_idx.cpu(), want)
+
+
 def test_logits_far_from_zero():
     """The statistics hand the maximum and log Z on apart: rows around 4096 lose nothing of their gradient."""
     from ttts_amd import ops

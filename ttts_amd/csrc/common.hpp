@@ -137,7 +137,7 @@ __device__ __forceinline__ float over_rows(float x, F op) {
 }
 template <int CTRL>
 __device__ __forceinline__ float dpp_mov(float x) {
-  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, false));
+  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));   // (every lane has a source)
 }
 template <typename F>
 __device__ __forceinline__ float over_wave(float x, F op) {
@@ -148,7 +148,8 @@ __device__ __forceinline__ float over_wave(float x, F op) {
   return over_rows(x, op);
 }
 struct AddOp { __device__ __forceinline__ float operator()(float a, float b) const { return a + b; } };
-struct MaxOp { __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); } };
+// as fmaxf (a NaN is passed over), without the instructions that would first make signalling NaNs quiet
+struct MaxOp { __device__ __forceinline__ float operator()(float a, float b) const { return __builtin_amdgcn_fmed3f(a, b, INFINITY); } };
 constexpr AddOp add_op{};
 constexpr MaxOp max_op{};
 

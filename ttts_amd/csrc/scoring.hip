@@ -18,8 +18,9 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f, FMAX = 3
 // these read 4.4), and a second kernel that joins a row's parts.  A lane holds 8 neighbouring columns per load (16 or 32 bytes,
 // at whatever alignment the row has; only the row's last columns are read one by one), 64 lanes 512 neighbouring ones: x[i][j] is
 // column c0 + 512 i + 8 lane + j.  A rest of up to 64 columns behind the last whole 512 -- a codebook and its few special classes --
-// is one more column a lane (`narrow`) instead of a step of eight.
-constexpr int NV = 4, WAVE_COLS = NV * 512, NARROW = 64;
+// is one more column a lane (`narrow`) instead of a step of eight.  NV: the steps of 512 that a kernel is compiled for; rows up to 1088
+// columns have one of two (the instructions of two empty steps were a fifth of all).
+constexpr int STEPS = 4, WAVE_COLS = STEPS * 512, NARROW = 64;
 struct Cols {   // a wave's columns: c0 .. wide - 1 in `steps` of 512, wide .. end - 1 one a lane
   int c0, wide, end, steps;
   __device__ __forceinline__ Cols(int first, int last) : c0(first), wide(last), end(last), steps((last - first + 511) >> 9) {
@@ -63,17 +64,17 @@ __device__ __forceinline__ void store8(T* p, int n, const float (&v)[8]) {
 }
 // Columns c0 .. cend - 1 of a row, as they lie in memory (all loads on their way before the first is waited for); as fp32, columns outside
 // are -inf.
-template <typename T> struct Raw { typename Eight<T>::type v[NV]; };
-template <typename T>
-__device__ __forceinline__ void load_raw(Raw<T>& r, const T* row, int c0, int cend, int lane) {
+template <typename T, int NV> struct Raw { typename Eight<T>::type v[NV]; };
+template <typename T, int NV>
+__device__ __forceinline__ void load_raw(Raw<T, NV>& r, const T* row, int c0, int cend, int lane) {
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = c0 + i * 512 + lane * 8;
     if (c0 + i * 512 + 512 <= cend || c + 8 <= cend) r.v[i] = *reinterpret_cast<const typename Eight<T>::type*>(row + c);
   }
 }
-template <typename T>
-__device__ __forceinline__ void expand(const Raw<T>& r, const T* row, int c0, int cend, int lane, float (&x)[NV][8]) {
+template <typename T, int NV>
+__device__ __forceinline__ void expand(const Raw<T, NV>& r, const T* row, int c0, int cend, int lane, float (&x)[NV][8]) {
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = c0 + i * 512 + lane * 8;
@@ -99,7 +100,7 @@ struct Exponent {
   bool plain;   // uniform over the wave
   __device__ __forceinline__ Exponent(float m_, float c_) : m(m_), c(c_) {
     mc = m * c;
-    plain = fabsf(mc) <= 1048576.f;
+    plain = __builtin_amdgcn_readfirstlane(fabsf(mc) <= 1048576.f);
     delta = plain ? fmaf(m, c, -mc) : 0.f;
   }
 };
@@ -145,14 +146,14 @@ __device__ __forceinline__ float threshold_of(uint32_t t) {   // (a class at -in
   return t <= ORD_NONE ? -FMAX : unord(t);
 }
 template <typename T, int N>
-__device__ __forceinline__ float group_threshold(const uint32_t (&g)[N], int n, int k, bool early) {
-  uint32_t t = 0;
-  for (uint32_t bit = 0x80000000u; bit >> LowBits<T>::n; bit >>= 1) {
+__device__ __forceinline__ float group_threshold(const uint32_t (&g)[N], int k, bool early, uint32_t lo = 0, uint32_t hi = 0xffffffffu) {
+  if (lo == hi) return threshold_of<T>(lo);
+  uint32_t bit = 0x80000000u >> __builtin_clz(lo ^ hi), t = lo & ~(bit + bit - 1);   // lo <= it <= hi: it begins as both do
+  for (; bit >> LowBits<T>::n; bit >>= 1) {
     const uint32_t c = t | bit;
     int cnt = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (i < n) cnt += __builtin_popcountll(__ballot(g[i] >= c));
+    for (int i = 0; i < N; ++i) cnt += __builtin_popcountll(__ballot(g[i] >= c));
     if (cnt >= k) {
       t = c;
       if (early && cnt == k) break;
@@ -160,8 +161,13 @@ __device__ __forceinline__ float group_threshold(const uint32_t (&g)[N], int n, 
   }
   return threshold_of<T>(t);
 }
+// bounds of the k-th largest (k <= 64) of a wave's groups, from the largest of each lane's
+__device__ __forceinline__ void lane_bounds(float most, uint32_t& lo, uint32_t& hi) {
+  lo = __builtin_amdgcn_readfirstlane(ord(-max_wave(-most)));
+  hi = __builtin_amdgcn_readfirstlane(ord(max_wave(most)));
+}
 // bit 31 - (8 i + j): x[i][j] reaches the threshold / is above it
-template <bool ABOVE>
+template <bool ABOVE, int NV>
 __device__ __forceinline__ uint32_t reached(const float (&x)[NV][8], float thr, int steps) {
   uint32_t bits = 0;
 #pragma unroll
@@ -173,7 +179,7 @@ __device__ __forceinline__ uint32_t reached(const float (&x)[NV][8], float thr, 
       bits <<= 8;
     }
   }
-  return bits;
+  return bits << (32 - 8 * NV);
 }
 // A wave's own keys of a 16-bit type fit 32 bits: the ord() that the type has, and the column among the wave's, inverted.
 template <typename T> struct WaveKey {
@@ -214,7 +220,7 @@ __device__ __forceinline__ void collect(uint32_t bits, bool narrow, float xn, co
   }
 }
 // columns equal to thr, lowest classes first, become keys from place n on, up to `end`; returns n + ties
-template <typename T>
+template <typename T, int NV>
 __device__ __forceinline__ int collect_ties(const float (&x)[NV][8], float xn, float thr, const Cols& cols, int lane,
                                             typename WaveKey<T>::type* cand, int n, int end) {
   const int c0 = cols.c0;
@@ -256,7 +262,7 @@ __device__ __forceinline__ void rank_keys(const K* cand, int n, int k, int threa
 constexpr int WAVE_CAND = 64 * 9, WAVE_TOP_LDS = WAVE_CAND + 4;           // one wave: groups of 8 or 9 columns (exact)
 constexpr int GROUP_CAND = 64 * 33;                                       // a workgroup: a lane's 32 or 33 columns are a group
 // one wave: f(rank, key) of its k best; returns how many there are (<= k)
-template <typename T, typename F>
+template <typename T, int NV, typename F>
 __device__ __forceinline__ int wave_top(const float (&x)[NV][8], float xn, const float (&vmax)[NV], const T* row, const Cols& cols, int k, int lane,
                                         typename WaveKey<T>::type* cand, F f) {
   uint32_t g[NV];
@@ -264,20 +270,22 @@ __device__ __forceinline__ int wave_top(const float (&x)[NV][8], float xn, const
   for (int i = 0; i < NV; ++i) g[i] = ord(vmax[i]);
   float thr;
   if (k <= 32) {          // groups of a lane's 32 columns: one ballot a bit
-    const uint32_t one[1] = {max(max(g[0], g[1]), max(g[2], g[3]))};
-    thr = group_threshold<T, 1>(one, 1, k, true);
+    uint32_t one[1] = {g[0]};
+#pragma unroll
+    for (int i = 1; i < NV; ++i) one[0] = max(one[0], g[i]);
+    thr = group_threshold<T, 1>(one, k, true);
   } else {                // of 8 columns: with 64 groups the least of them would have to do
-    thr = group_threshold<T, NV>(g, NV, k, true);
+    thr = group_threshold<T, NV>(g, k, true);
   }
   int n = 0;
   auto next = [&](u64 mask) { const int at = n + lanes_below(mask); n += __builtin_popcountll(mask); return at; };
-  collect<T>(reached<false>(x, thr, cols.steps), xn >= thr, xn, row, cols, lane, cand, WAVE_CAND, next);
+  collect<T>(reached<false, NV>(x, thr, cols.steps), xn >= thr, xn, row, cols, lane, cand, WAVE_CAND, next);
   if (n > WAVE_CAND) {
-    thr = group_threshold<T, NV>(g, NV, k, false);
+    thr = group_threshold<T, NV>(g, k, false);
     n = 0;
-    collect<T>(reached<true>(x, thr, cols.steps), xn > thr, xn, row, cols, lane, cand, WAVE_CAND, next);
+    collect<T>(reached<true, NV>(x, thr, cols.steps), xn > thr, xn, row, cols, lane, cand, WAVE_CAND, next);
     const int end = max(n, k);
-    n = min(end, collect_ties<T>(x, xn, thr, cols, lane, cand, n, end));
+    n = min(end, collect_ties<T, NV>(x, xn, thr, cols, lane, cand, n, end));
   }
   if (lane < 4) cand[n + lane] = 0;
   wave_fence();
@@ -288,47 +296,32 @@ __device__ __forceinline__ int wave_top(const float (&x)[NV][8], float xn, const
 struct RowSums { float m, z, s; };   // maximum, sum e, sum e t (t in bits, from the maximum)
 // of one wave's columns.  A class at -inf, or at the type's lowest value, has e = 0: e t must be 0, not NaN, so t is kept finite
 // there (a NaN passes through e).
+template <int NV>
 __device__ __forceinline__ RowSums wave_sums(const float (&x)[NV][8], float xn, const Cols& cols, float lmax, float c) {
   const int steps = cols.steps;
   RowSums a;
   a.m = max_wave(fmaxf(lmax, -FMAX));
   a.z = a.s = 0.f;
   const Exponent ex(a.m, c);
-  if (ex.plain) {
+  auto add = [&](float t) {
+    const float e = __builtin_amdgcn_exp2f(t);
+    a.z += e;
+    a.s = fmaf(e, fmaxf(t, -200.f), a.s);
+  };
+  auto add_up = [&](auto exponent) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       if (i >= steps) break;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float t = fmaf(x[i][j], c, -ex.mc), e = __builtin_amdgcn_exp2f(t);
-        a.z += e;
-        a.s = fmaf(e, fmaxf(t, -200.f), a.s);
-      }
+      for (int j = 0; j < 8; ++j) add(exponent(x[i][j]));
     }
-    if (cols.narrow()) {
-      const float t = fmaf(xn, c, -ex.mc), e = __builtin_amdgcn_exp2f(t);
-      a.z += e;
-      a.s = fmaf(e, fmaxf(t, -200.f), a.s);
-    }
-    const float f = __builtin_amdgcn_exp2f(-ex.delta);
-    a.z = sum_wave(a.z) * f;
-    a.s = sum_wave(a.s) * f - ex.delta * a.z;
-  } else {
-#pragma unroll 1
-    for (int i = 0; i < NV; ++i)
-      if (i < steps)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float t = ((i == 0 ? x[0][j] : i == 1 ? x[1][j] : i == 2 ? x[2][j] : x[3][j]) - a.m) * c, e = __builtin_amdgcn_exp2f(t);
-          a.z += e;
-          a.s = fmaf(e, fmaxf(t, -200.f), a.s);
-        }
-    const float t = (xn - a.m) * c, e = __builtin_amdgcn_exp2f(t);
-    a.z += e;
-    a.s = fmaf(e, fmaxf(t, -200.f), a.s);
-    a.z = sum_wave(a.z);
-    a.s = sum_wave(a.s);
-  }
+    if (cols.narrow()) add(exponent(xn));
+  };
+  if (ex.plain) add_up([&](float v) { return fmaf(v, c, -ex.mc); });
+  else add_up([&](float v) { return (v - a.m) * c; });
+  const float f = __builtin_amdgcn_exp2f(-ex.delta);
+  a.z = sum_wave(a.z) * f;
+  a.s = sum_wave(a.s) * f - ex.delta * a.z;
   return a;
 }
 __device__ __forceinline__ void add_sums(RowSums& a, float m, float z, float s, float c) {   // a.m is the row's maximum already
@@ -337,13 +330,24 @@ __device__ __forceinline__ void add_sums(RowSums& a, float m, float z, float s, 
   a.s += f * (s + z * d);
 }
 
+// Groups of a long row's unit, 64 of 32 neighbouring columns each: from the maxima of a lane's 8 columns a step (and its narrow column) lane
+// l gets that of step l & 3 of the four lanes around it, columns 512 (l & 3) + 32 (l / 4) ..+31 of the unit (and narrow column l).
+// (A lane's own 4 x 8 columns as a group lay in four places when they were read again.)
+__device__ __forceinline__ float group_max(const float (&v)[STEPS], float xn, int lane) {
+  static_assert(STEPS == 4, "four lanes, four steps");
+  const bool odd = lane & 1, high = lane & 2;
+  const float a = max_med(odd ? v[1] : v[0], dpp_mov<0xb1>(odd ? v[0] : v[1]));   // quad_perm 1, 0, 3, 2
+  const float b = max_med(odd ? v[3] : v[2], dpp_mov<0xb1>(odd ? v[2] : v[3]));
+  const float m = max_med(high ? b : a, dpp_mov<0x4e>(high ? a : b));             // quad_perm 2, 3, 0, 1
+  return max_med(max_med(m, xn), -INFINITY);
+}
 struct ScoreParams {
   const void* logits; int64_t ldl;
   const int64_t* tokens;
   float *logp, *entropy, *stats, *top_logp;
   int64_t* top_idx;
   float4* part;          // long rows: [R, units] (m, z, s, -) of each wave's columns,
-  uint32_t* part_max;    // and with alternatives [R, units, 64]: ord() of the maximum of each lane's 32 columns
+  void* part_max;        // and with alternatives [R, units, 64] of the logits' type: the maximum of each group of columns (group_max)
   int R, C, k, units, unit_cols, narrow_at;   // the row's columns from narrow_at on are its last unit's narrow ones
   float inv_t;
 };
@@ -364,7 +368,7 @@ __device__ __forceinline__ void write_top(const ScoreParams& p, int64_t row, int
 
 // One wave per row (LONG false), or per unit of up to 2048 columns of a row.  (Waves that went through several of them, the next one's loads under this
 // one's arithmetic, were slower at every grid: 118 - 125 us instead of 109 for logits of 2048 x 100003 with 64 alternatives.)
-template <typename T, bool LONG>
+template <typename T, bool LONG, int NV>
 __global__ __launch_bounds__(256) void token_logprobs_fwd_kernel(ScoreParams p) {
   extern __shared__ __attribute__((aligned(16))) unsigned char score_lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -379,7 +383,7 @@ __global__ __launch_bounds__(256) void token_logprobs_fwd_kernel(ScoreParams p) 
   int64_t tok = -1;
   float xt = 0.f, xn;
   {
-    Raw<T> raw;
+    Raw<T, NV> raw;
     if (!LONG) tok = p.tokens[row];
     load_raw(raw, lr, cols.c0, cols.wide, lane);
     const T narrow = cols.load_narrow(lr, p.C - 1, lane);
@@ -397,119 +401,125 @@ __global__ __launch_bounds__(256) void token_logprobs_fwd_kernel(ScoreParams p) 
     for (int j = 0; j < 8; ++j) vmax[i] = max_med(vmax[i], x[i][j]);
     lmax = max_med(lmax, vmax[i]);
   }
-  vmax[0] = max_med(vmax[0], xn);
+  if (!LONG) vmax[0] = max_med(vmax[0], xn);
   lmax = max_med(lmax, -INFINITY);                         // (xn may be NaN)
   const RowSums a = wave_sums(x, xn, cols, lmax, p.inv_t * LOG2E);
-  if (LONG) {
+  if constexpr (LONG) {
     if (lane == 0) p.part[id] = make_float4(a.m, a.z, a.s, 0.f);
-    if (p.k) p.part_max[id * 64 + lane] = ord(lmax);
+    if (p.k) ((T*)p.part_max)[id * 64 + lane] = (T)group_max(vmax, xn, lane);
     return;
   }
   if (lane == 0) write_row(p, row, a, tok >= 0 && tok < p.C, xt);
   if (p.k) {
-    const int have = wave_top<T>(x, xn, vmax, lr, cols, p.k, lane, reinterpret_cast<typename WaveKey<T>::type*>(score_lds) + wave * WAVE_TOP_LDS, [&](int r, u64 key) { write_top(p, row, r, key, a); });
+    const int have = wave_top<T, NV>(x, xn, vmax, lr, cols, p.k, lane, reinterpret_cast<typename WaveKey<T>::type*>(score_lds) + wave * WAVE_TOP_LDS, [&](int r, u64 key) { write_top(p, row, r, key, a); });
     if (lane >= have && lane < p.k) write_top(p, row, lane, 0, a);
   }
 }
 
-// a long row's sums, by one wave, from its units' parts; every lane gets them
-__device__ __forceinline__ RowSums join_sums(const ScoreParams& p, int64_t row, int lane) {
+// A long row's sums, by one wave, from its units' parts; every lane gets them.  What it takes from memory is asked for first, and by every
+// lane, so that its way is short when it is needed.
+struct LongRow { float4 first; int tok; float xt; };   // tok: -1 if none is given
+template <typename T>
+__device__ __forceinline__ LongRow load_long_row(const ScoreParams& p, int64_t row, int lane) {
+  LongRow r;
+  const int64_t tok = p.tokens[row];
+  r.first = p.part[row * p.units + min(lane, p.units - 1)];
+  r.tok = tok >= 0 && tok < p.C ? (int)tok : -1;
+  r.xt = (float)((const T*)p.logits)[row * p.ldl + max(r.tok, 0)];
+  return r;
+}
+__device__ __forceinline__ RowSums join_sums(const ScoreParams& p, int64_t row, const LongRow& r, int lane) {
   const float4* part = p.part + row * p.units;
-  float m = -FMAX;
-  for (int u = lane; u < p.units; u += 64) m = fmaxf(m, part[u].x);
+  const float c = p.inv_t * LOG2E;
+  float m = r.first.x;
+  for (int u = lane + 64; u < p.units; u += 64) m = fmaxf(m, part[u].x);
   RowSums a = {max_wave(m), 0.f, 0.f};
-  for (int u = lane; u < p.units; u += 64) {
+  if (lane < p.units) add_sums(a, r.first.x, r.first.y, r.first.z, c);
+  for (int u = lane + 64; u < p.units; u += 64) {
     const float4 s = part[u];
-    add_sums(a, s.x, s.y, s.z, p.inv_t * LOG2E);
+    add_sums(a, s.x, s.y, s.z, c);
   }
   a.z = sum_wave(a.z);
   a.s = sum_wave(a.s);
   return a;
 }
 template <typename T>
-__device__ __forceinline__ void write_long_row(const ScoreParams& p, int64_t row, const RowSums& a) {
-  const int64_t tok = p.tokens[row];
-  const bool given = tok >= 0 && tok < p.C;
-  write_row(p, row, a, given, given ? (float)((const T*)p.logits)[row * p.ldl + tok] : 0.f);
-}
-template <typename T>
 __global__ __launch_bounds__(256) void token_logprobs_join_kernel(ScoreParams p) {   // no alternatives: a wave per row
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= p.R) return;
-  const RowSums a = join_sums(p, row, threadIdx.x & 63);
-  if ((threadIdx.x & 63) == 0) write_long_row<T>(p, row, a);
+  const int lane = threadIdx.x & 63;
+  const LongRow r = load_long_row<T>(p, row, lane);
+  const RowSums a = join_sums(p, row, r, lane);
+  if (lane == 0) write_row(p, row, a, r.tok >= 0, r.xt);
 }
 
-// Alternatives of a long row: W waves, up to W * N * 64 groups of 32 columns.  Each wave bounds the threshold from its own groups (the k-th
-// largest of the maxima of up to 4 sets of them a lane); the largest of these bounds keeps little more than k groups a wave, among
-// those one wave finds the exact threshold, the k or so groups that reach it are read again, and their columns that do are ranked.
-// Where values repeat at a threshold, so that more reach it than there is room for: the exact threshold over all groups, the
+// Alternatives of a long row: W waves, up to W * N * 64 groups of 32 columns.  A bound that k groups reach: the least of the waves' own
+// (k / W)-th largest of the maxima of 2 or 4 sets of their groups a lane; a third more than k groups reach it where the row's largest
+// are spread over the waves' units (a wave has every W-th).  Where they are not, and more reach it than are listed: the largest of the waves' own
+// k-th largest.  The columns of the listed groups are read again, and those that reach the bound ranked.
+// Where values repeat at the bound, so that more reach it than there is room for: the exact threshold over all groups, the
 // fewer than k groups above it, and then the row's columns AT it in the order of the classes until there are k.
 template <typename T, int W, int N>
-__global__ __launch_bounds__(W * 64) void token_logprobs_top_kernel(ScoreParams p) {
-  constexpr int LIST = 96 * W, SETS = N < 4 ? N : 4;
+__global__ __launch_bounds__(W * 64, 8) void token_logprobs_top_kernel(ScoreParams p) {
+  constexpr int LIST = 96 * W, SETS = N > 16 ? 2 : 4;   // (with 32 groups a lane four sets would not fit 64 registers)
   __shared__ __attribute__((aligned(16))) u64 cand[GROUP_CAND + 4];
-  __shared__ uint32_t list_max[LIST];
   __shared__ int list_id[LIST];
-  __shared__ float sm_thr[W + 1];
+  __shared__ float sm_thr[W];
   __shared__ RowSums sm_row;
-  __shared__ int sm_n, sm_list, sm_cnt[W];
+  __shared__ int sm_n, sm_list[2], sm_cnt[W];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t row = blockIdx.x;
   const T* lr = (const T*)p.logits + row * p.ldl;
   const int k = p.k, groups = p.units * 64;
-  const uint32_t* gm = p.part_max + row * groups;
-  if (tid == 0) sm_n = sm_list = 0;
+  const T* gm = (const T*)p.part_max + row * groups;
+  if (tid == 0) sm_n = sm_list[0] = sm_list[1] = 0;
+  float bound;
+  int listed;
+  LongRow r;
+  if (wave == W - 1) r = load_long_row<T>(p, row, lane);
   {
-    uint32_t g[N], q[SETS];                   // wave w has the units w, w + W, ..; group id = unit * 64 + lane
+    float v[N];                               // wave w has the units w, w + W, ..; group id = unit * 64 + lane
 #pragma unroll
-    for (int i = 0; i < N; ++i) g[i] = i * W + wave < p.units ? gm[(i * W + wave) * 64 + lane] : 0;
-    if (wave == W - 1) {                      // (beside the others' search)
-      const RowSums a = join_sums(p, row, lane);
-      if (lane == 0) {
-        sm_row = a;
-        write_long_row<T>(p, row, a);
-      }
-    }
+    for (int i = 0; i < N; ++i) v[i] = (float)(gm + min(i * W + wave, p.units - 1) * 64)[lane];
+    uint32_t q[SETS], lo, hi;
+    float most = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = i * W + wave < p.units ? v[i] : -INFINITY;
 #pragma unroll
     for (int i = 0; i < SETS; ++i) {
-      q[i] = g[i];
+      float set = v[i];
 #pragma unroll
-      for (int j = i + SETS; j < N; j += SETS) q[i] = max(q[i], g[j]);
+      for (int j = i + SETS; j < N; j += SETS) set = max_med(set, v[j]);
+      most = max_med(most, set);
+      q[i] = ord(set);
     }
-    const float mine = group_threshold<T, SETS>(q, SETS, k, true);
-    if (lane == 0) sm_thr[wave] = mine;
-    __syncthreads();
-    float bound = sm_thr[0];
-    for (int w = 1; w < W; ++w) bound = fmaxf(bound, sm_thr[w]);
-    const uint32_t tb = ord(bound);
+    lane_bounds(most, lo, hi);
+    for (int round = 0; round < 2; ++round) {
+      const float mine = group_threshold<T, SETS>(q, round ? k : (k + W - 1) / W, true, lo, hi);
+      if (lane == 0) sm_thr[wave] = mine;
+      __syncthreads();
+      bound = sm_thr[0];
+      for (int w = 1; w < W; ++w) bound = round ? fmaxf(bound, sm_thr[w]) : fminf(bound, sm_thr[w]);
+      int at = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (g[i] >= tb) {
-        const int at = atomicAdd(&sm_list, 1);
-        if (at < LIST) { list_max[at] = g[i]; list_id[at] = (i * W + wave) * 64 + lane; }
+      for (int i = 0; i < N; ++i) at += v[i] >= bound;
+      if (at) at = atomicAdd(&sm_list[round], at);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (v[i] >= bound) {
+          if (at < LIST) list_id[at] = (i * W + wave) * 64 + lane;
+          ++at;
+        }
+      if (wave == W - 1 && round == 0) {
+        const RowSums a = join_sums(p, row, r, lane);
+        if (lane == 0) sm_row = a;
       }
-    __syncthreads();
-    if (wave == 0 && sm_list <= LIST) {
-      uint32_t l[LIST / 64];
-#pragma unroll
-      for (int i = 0; i < LIST / 64; ++i) l[i] = i * 64 + lane < sm_list ? list_max[i * 64 + lane] : 0;
-      const float t = fmaxf(bound, group_threshold<T, LIST / 64>(l, (sm_list + 63) >> 6, k, true));   // (fewer than k groups: the bound)
-      if (lane == 0) sm_thr[W] = t;
+      __syncthreads();
+      listed = sm_list[round];
+      if (listed <= LIST) break;              // (uniform over the workgroup)
     }
-    __syncthreads();
   }
-  auto push_eight = [&](int id, int i, float t, bool above) {   // columns that reach t (or lie above it) become keys
-    int c = (id >> 6) * p.unit_cols + i * 512 + (id & 63) * 8, end = p.narrow_at;
-    if (i == NV) {                              // the unit's narrow columns
-      c = p.narrow_at + (id & 63);
-      end = (id >> 6) == p.units - 1 ? min(p.C, c + 1) : 0;
-    } else if (i * 512 >= p.unit_cols) {
-      return;
-    }
-    if (c >= end) return;
-    float v[8];
-    load8<T>(lr + c, end - c, v);
+  auto push = [&](const float (&v)[8], int c, float t, bool above) {   // columns that reach t (or lie above it) become keys
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       if (above ? v[j] > t : v[j] >= t) {
@@ -517,13 +527,49 @@ __global__ __launch_bounds__(W * 64) void token_logprobs_top_kernel(ScoreParams 
         if (at < GROUP_CAND) cand[at] = top_key(v[j], c + j);
       }
   };
-  const int listed = sm_list;
-  bool full = listed > LIST;                  // (uniform over the workgroup)
+  // where piece i of a group lies: `end - c` columns, none if that is not positive; its narrow column goes with piece 0
+  auto piece = [&](int id, int i, int& c, int& end, int& cn) {
+    c = (id >> 6) * p.unit_cols + (id & 3) * 512 + (id & 60) * 8 + i * 8;
+    end = (id & 3) * 512 < p.unit_cols ? p.narrow_at : 0;
+    cn = i == 0 && (id >> 6) == p.units - 1 ? p.narrow_at + (id & 63) : p.C;
+  };
+  auto push_narrow = [&](T x, int cn, float t, bool above) {
+    const float v = (float)x;
+    if (cn < p.C && (above ? v > t : v >= t)) {
+      const int at = atomicAdd(&sm_n, 1);
+      if (at < GROUP_CAND) cand[at] = top_key(v, cn);
+    }
+  };
+  bool full = listed > LIST;
   if (!full) {
-    const float t = sm_thr[W];
-    const uint32_t tb = ord(t);
-    for (int task = tid; task < listed * (NV + 1); task += W * 64)
-      if (list_max[task / (NV + 1)] >= tb) push_eight(list_id[task / (NV + 1)], task % (NV + 1), t, false);
+    const int tasks = listed * STEPS;
+    for (int s = tid; s < tasks; s += 2 * W * 64) {   // two pieces a thread, their loads together
+      typename Eight<T>::type r[2];
+      T rn[2];
+      int c[2], end[2], cn[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int task = s + h * W * 64;
+        piece(list_id[min(task, tasks - 1) / STEPS], task % STEPS, c[h], end[h], cn[h]);
+        if (task >= tasks) { end[h] = 0; cn[h] = p.C; }
+        if (c[h] + 8 <= end[h]) r[h] = *reinterpret_cast<const typename Eight<T>::type*>(lr + c[h]);
+        rn[h] = lr[min(cn[h], p.C - 1)];
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (c[h] < end[h]) {
+          float v[8];
+          if (c[h] + 8 <= end[h]) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = (float)r[h][j];
+          } else {
+            load8<T>(lr + c[h], end[h] - c[h], v);
+          }
+          push(v, c[h], bound, false);
+        }
+        push_narrow(rn[h], cn[h], bound, false);
+      }
+    }
     __syncthreads();
     full = sm_n > GROUP_CAND;
   }
@@ -531,7 +577,7 @@ __global__ __launch_bounds__(W * 64) void token_logprobs_top_kernel(ScoreParams 
     uint32_t t = 0;                           // the exact threshold over all groups of the row
     for (uint32_t bit = 0x80000000u; bit >> LowBits<T>::n; bit >>= 1) {
       int cnt = 0;
-      for (int u = wave; u < p.units; u += W) cnt += __builtin_popcountll(__ballot(gm[u * 64 + lane] >= (t | bit)));
+      for (int u = wave; u < p.units; u += W) cnt += __builtin_popcountll(__ballot(ord((float)gm[u * 64 + lane]) >= (t | bit)));
       __syncthreads();
       if (lane == 0) sm_cnt[wave] = cnt;
       __syncthreads();
@@ -545,9 +591,18 @@ __global__ __launch_bounds__(W * 64) void token_logprobs_top_kernel(ScoreParams 
     if (tid == 0) sm_n = 0;
     __syncthreads();
     for (int u = wave; u < p.units; u += W)
-      if (gm[u * 64 + lane] > tb)
+      if (ord((float)gm[u * 64 + lane]) > tb)
 #pragma unroll 1
-        for (int e = 0; e <= NV; ++e) push_eight(u * 64 + lane, e, thr, true);
+        for (int e = 0; e < STEPS; ++e) {
+          int c, end, cn;
+          piece(u * 64 + lane, e, c, end, cn);
+          if (c < end) {
+            float v[8];
+            load8<T>(lr + c, end - c, v);
+            push(v, c, thr, true);
+          }
+          if (cn < p.C) push_narrow(lr[cn], cn, thr, true);
+        }
     __syncthreads();
     int n = sm_n;
     const int end = max(n, k);
@@ -591,7 +646,8 @@ __global__ __launch_bounds__(W * 64) void token_logprobs_top_kernel(ScoreParams 
   if (tid < 4) cand[n + tid] = 0;
   __syncthreads();
   rank_keys(cand, n, k, tid, W * 64, [&](int r, u64 key) { write_top(p, row, r, key, a); });
-  for (int r = n + tid; r < k; r += W * 64) write_top(p, row, r, 0, a);
+  for (int e = n + tid; e < k; e += W * 64) write_top(p, row, e, 0, a);
+  if (wave == W - 1 && lane == 0) write_row(p, row, a, r.tok >= 0, r.xt);
 }
 
 // The same for rows of up to 8 units by one wave each, four rows a workgroup and no barrier: all 512 groups are in its registers, so the
@@ -607,16 +663,26 @@ __global__ __launch_bounds__(256) void token_logprobs_top_wave_kernel(ScoreParam
   const int64_t row = (int64_t)blockIdx.x * 4 + wave;
   if (row >= p.R) return;
   const T* lr = (const T*)p.logits + row * p.ldl;
-  const uint32_t* gm = p.part_max + row * p.units * 64;
+  const T* gm = (const T*)p.part_max + row * p.units * 64;
   u64* cand = sm_cand[wave];
   int* list = sm_list[wave];
   const int k = p.k;
-  uint32_t g[UNITS];
+  T raw[UNITS];
 #pragma unroll
-  for (int i = 0; i < UNITS; ++i) g[i] = i < p.units ? gm[i * 64 + lane] : 0;
-  const RowSums a = join_sums(p, row, lane);
-  if (lane == 0) write_long_row<T>(p, row, a);
-  float thr = group_threshold<T, UNITS>(g, p.units, k, true);
+  for (int i = 0; i < UNITS; ++i) raw[i] = gm[min(i, p.units - 1) * 64 + lane];
+  const LongRow r = load_long_row<T>(p, row, lane);
+  uint32_t g[UNITS], lo, hi;
+  float most = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < UNITS; ++i) {
+    const float v = i < p.units ? (float)raw[i] : -INFINITY;
+    g[i] = ord(v);
+    most = max_med(most, v);
+  }
+  const RowSums a = join_sums(p, row, r, lane);
+  if (lane == 0) write_row(p, row, a, r.tok >= 0, r.xt);
+  lane_bounds(most, lo, hi);
+  float thr = group_threshold<T, UNITS>(g, k, true, lo, hi);
   int n = 0, listed = 0;
   {
     const uint32_t tb = ord(thr);
@@ -651,15 +717,15 @@ __global__ __launch_bounds__(256) void token_logprobs_top_wave_kernel(ScoreParam
   };
   bool full = listed > LIST;
   if (!full) {
-    for (int s = 0; s < listed * (NV + 1); s += 64) {
-      const int task = s + lane, i = task % (NV + 1), id = task < listed * (NV + 1) ? list[task / (NV + 1)] : 0;
-      int c = (id >> 6) * p.unit_cols + i * 512 + (id & 63) * 8, end = i * 512 < p.unit_cols ? p.narrow_at : 0;
-      if (i == NV) {                              // the unit's narrow columns
+    for (int s = 0; s < listed * (STEPS + 1); s += 64) {
+      const int task = s + lane, i = task % (STEPS + 1), id = task < listed * (STEPS + 1) ? list[task / (STEPS + 1)] : 0;
+      int c = (id >> 6) * p.unit_cols + (id & 3) * 512 + (id & 60) * 8 + i * 8, end = (id & 3) * 512 < p.unit_cols ? p.narrow_at : 0;
+      if (i == STEPS) {                              // the unit's narrow columns
         c = p.narrow_at + (id & 63);
         end = (id >> 6) == p.units - 1 ? min(p.C, c + 1) : 0;
       }
       float v[8];
-      eight(c, task < listed * (NV + 1) ? end : 0, v);
+      eight(c, task < listed * (STEPS + 1) ? end : 0, v);
       push(v, c, [&](float x) { return x >= thr; });
     }
     full = n > CAND;
@@ -843,7 +909,7 @@ __device__ __forceinline__ void listed_logits(const T* row, const Listed& L, int
 }
 
 // as token_logprobs_fwd_kernel; with tail each wave marks the listed classes of its columns in a bit map of its own
-template <typename T, bool LONG>
+template <typename T, bool LONG, int NV>
 __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillParams p) {
   __shared__ uint32_t marks[4][(WAVE_COLS + NARROW) / 32];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -856,7 +922,7 @@ __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillParams p) {
   const Cols cols(unit * p.unit_cols, unit == p.units - 1 ? p.C : (unit + 1) * p.unit_cols);
   ListLoads list;
   if (!LONG || p.tail) list = load_list(p.idx + row * p.K, p.tlogp + row * p.K, p.K, lane);
-  Raw<T> raw;
+  Raw<T, NV> raw;
   load_raw(raw, lr, cols.c0, cols.wide, lane);
   const T narrow = cols.load_narrow(lr, p.C - 1, lane);
   Listed L;
@@ -961,7 +1027,7 @@ struct DistillGradParams {
 // one exponential a class by the first form, then the few named ones again by the second, each by the lane that holds its entry (whose
 // logit, and what is accumulated to, is fetched beside the row; a wave's own stores to one address stay in order).  Entries that
 // name one class find out by leaving their number at its place in LDS: each then writes the sum of their p, in the list's order.
-template <typename T>
+template <typename T, int NV>
 __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillGradParams p) {
   __shared__ uint8_t tags[4][WAVE_COLS + NARROW];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -976,7 +1042,7 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillGradParams p) {
   const T* lr = (const T*)p.logits + row * p.ldl;
   T* dr = (T*)p.dlogits + row * p.ldd;
   const ListLoads list = load_list(p.idx + row * p.K, p.tlogp + row * p.K, p.K, lane);
-  Raw<T> raw;
+  Raw<T, NV> raw;
   load_raw(raw, lr, c0, min(p.C, cols.wide), lane);
   const T narrow = cols.load_narrow(lr, p.C - 1, lane);
   Listed L;
@@ -1099,7 +1165,7 @@ struct Units { int units, cols, narrow_at; };
 static Units split_columns(int n) {
   const int rest = n % 512, narrow = rest <= NARROW ? rest : 0, steps = (int)cdiv(n - narrow, 512);
   Units u;
-  u.units = steps > NV ? (int)cdiv(steps, NV) : 1;
+  u.units = steps > STEPS ? (int)cdiv(steps, STEPS) : 1;
   u.cols = steps > 0 ? (int)cdiv(steps, u.units) * 512 : 512;
   u.units = steps > 0 ? (int)cdiv(steps * 512, u.cols) : 1;
   u.narrow_at = n - narrow;
@@ -1119,10 +1185,12 @@ static int launch_score(const ScoreParams& p, hipStream_t st) {
   if (!rc && p.k && p.units > 8) rc = need_grid(what, p.R, p.units <= 64 ? 256 : 1024);
   if (rc) return rc;
   if (p.units == 1) {
-    token_logprobs_fwd_kernel<T, false><<<(unsigned)grid, 256, p.k ? 4 * WAVE_TOP_LDS * sizeof(typename WaveKey<T>::type) : 0, st>>>(p);
+    const size_t lds = p.k ? 4 * WAVE_TOP_LDS * sizeof(typename WaveKey<T>::type) : 0;
+    if (p.narrow_at <= 1024) token_logprobs_fwd_kernel<T, false, 2><<<(unsigned)grid, 256, lds, st>>>(p);
+    else token_logprobs_fwd_kernel<T, false, STEPS><<<(unsigned)grid, 256, lds, st>>>(p);
     return check_launch(what);
   }
-  token_logprobs_fwd_kernel<T, true><<<(unsigned)grid, 256, 0, st>>>(p);
+  token_logprobs_fwd_kernel<T, true, STEPS><<<(unsigned)grid, 256, 0, st>>>(p);
   rc = check_launch(what);
   if (rc) return rc;
   if (p.k == 0) token_logprobs_join_kernel<T><<<(unsigned)cdiv(p.R, 4), 256, 0, st>>>(p);
@@ -1144,7 +1212,7 @@ extern "C" int ttts_token_logprobs_fwd(const void* logits, int32_t dtype, int64_
   if (rc) return rc;
   const Units u = split_columns(C);
   ScoreParams p{logits, ldl, tokens, logp, entropy, stats, top_logp, top_idx, (float4*)workspace, nullptr, R, C, top_k, u.units, u.cols, u.narrow_at, 1.0f / temperature};
-  p.part_max = (uint32_t*)(p.part + (int64_t)R * p.units);
+  p.part_max = p.part + (int64_t)R * p.units;
   TTTS_BY_TYPE(dtype, "token_logprobs_fwd", rc = launch_score<T>(p, as_stream(stream)));
   return rc;
 }
@@ -1178,10 +1246,11 @@ static int launch_distill(const DistillParams& p, hipStream_t st) {
   int rc = need_grid(what, grid);
   if (rc) return rc;
   if (p.units == 1) {
-    distill_fwd_kernel<T, false><<<(unsigned)grid, 256, 0, st>>>(p);
+    if (split_columns(p.C).narrow_at <= 1024) distill_fwd_kernel<T, false, 2><<<(unsigned)grid, 256, 0, st>>>(p);
+    else distill_fwd_kernel<T, false, STEPS><<<(unsigned)grid, 256, 0, st>>>(p);
     return check_launch(what);
   }
-  distill_fwd_kernel<T, true><<<(unsigned)grid, 256, 0, st>>>(p);
+  distill_fwd_kernel<T, true, STEPS><<<(unsigned)grid, 256, 0, st>>>(p);
   rc = check_launch(what);
   if (rc) return rc;
   distill_join_kernel<T><<<(unsigned)cdiv(p.R, 4), 256, 0, st>>>(p);
@@ -1221,6 +1290,7 @@ extern "C" int ttts_distill_bwd(const void* logits, int32_t dtype, int64_t ldl, 
   const int64_t grid = cdiv(p.units, 4);
   rc = need_grid("distill_bwd", grid);
   if (rc) return rc;
-  TTTS_BY_TYPE(dtype, "distill_bwd", (distill_bwd_kernel<T><<<(unsigned)grid, 256, 0, as_stream(stream)>>>(p)));
+  if (u.units == 1 && u.narrow_at <= 1024) TTTS_BY_TYPE(dtype, "distill_bwd", (distill_bwd_kernel<T, 2><<<(unsigned)grid, 256, 0, as_stream(stream)>>>(p)))
+  else TTTS_BY_TYPE(dtype, "distill_bwd", (distill_bwd_kernel<T, STEPS><<<(unsigned)grid, 256, 0, as_stream(stream)>>>(p)))
   return check_launch("distill_bwd");
 }

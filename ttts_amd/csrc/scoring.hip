@@ -200,24 +200,26 @@ template <> struct WaveKey<bf16> : WaveKey16<bf16> {};
 template <> struct WaveKey<_Float16> : WaveKey16<_Float16> {};
 static_assert(WAVE_COLS + NARROW <= 4096, "12 bits of a wave's key are a column");
 
-// the columns marked in `bits` become keys at the places that place() deals out (those before `cap`); their values are read again (a
-// register cannot be indexed by a lane)
-template <typename T, typename Place>
-__device__ __forceinline__ void collect(uint32_t bits, bool narrow, float xn, const T* row, const Cols& cols, int lane,
-                                        typename WaveKey<T>::type* cand, int cap, Place place) {
-  const int c0 = cols.c0;
+// The marked columns (bits, narrow) are listed, n of them with what was there, those before `cap` stored: the loop goes by the most marks that a
+// lane has, so it does no more than that (reading each column again in it cost a wait a round: 200000 rows of 1026 classes, 20 alternatives: 151 us, 139 now).
+template <typename K>
+__device__ __forceinline__ int list_marked(uint32_t bits, bool narrow, const Cols& cols, int lane, K* cand, int cap) {
+  int n = 0;
   if (const u64 mask = __ballot(narrow)) {
-    const int at = place(mask);
-    if (narrow && at < cap) cand[at] = WaveKey<T>::make(xn, cols.wide - c0 + lane, c0);
+    const int at = lanes_below(mask);
+    if (narrow && at < cap) cand[at] = (K)(cols.wide - cols.c0 + lane);
+    n = __builtin_popcountll(mask);
   }
   for (u64 mask = __ballot(bits != 0); mask; mask = __ballot(bits != 0)) {
-    const int at = place(mask);
+    const int at = n + lanes_below(mask);
+    n += __builtin_popcountll(mask);
     if (bits) {
-      const int e = __builtin_clz(bits), c = (e >> 3) * 512 + lane * 8 + (e & 7);
+      const int e = __builtin_clz(bits);
       bits &= ~(0x80000000u >> e);
-      if (at < cap) cand[at] = WaveKey<T>::make((float)row[c0 + c], c, c0);
+      if (at < cap) cand[at] = (K)((e >> 3) * 512 + lane * 8 + (e & 7));
     }
   }
+  return n;
 }
 // columns equal to thr, lowest classes first, become keys from place n on, up to `end`; returns n + ties
 template <typename T, int NV>
@@ -277,13 +279,18 @@ __device__ __forceinline__ int wave_top(const float (&x)[NV][8], float xn, const
   } else {                // of 8 columns: with 64 groups the least of them would have to do
     thr = group_threshold<T, NV>(g, k, true);
   }
-  int n = 0;
-  auto next = [&](u64 mask) { const int at = n + lanes_below(mask); n += __builtin_popcountll(mask); return at; };
-  collect<T>(reached<false, NV>(x, thr, cols.steps), xn >= thr, xn, row, cols, lane, cand, WAVE_CAND, next);
-  if (n > WAVE_CAND) {
+  int n = list_marked(reached<false, NV>(x, thr, cols.steps), xn >= thr, cols, lane, cand, WAVE_CAND);
+  const bool exact = n > WAVE_CAND;
+  if (exact) {
     thr = group_threshold<T, NV>(g, k, false);
-    n = 0;
-    collect<T>(reached<true, NV>(x, thr, cols.steps), xn > thr, xn, row, cols, lane, cand, WAVE_CAND, next);
+    n = list_marked(reached<true, NV>(x, thr, cols.steps), xn > thr, cols, lane, cand, WAVE_CAND);
+  }
+  wave_fence();
+  for (int s = lane; s < n; s += 64) {      // (a register cannot be indexed by a lane: their values are read again)
+    const int at = (int)cand[s];
+    cand[s] = WaveKey<T>::make((float)row[cols.c0 + at], at, cols.c0);
+  }
+  if (exact) {
     const int end = max(n, k);
     n = min(end, collect_ties<T, NV>(x, xn, thr, cols, lane, cand, n, end));
   }
@@ -650,13 +657,14 @@ __global__ __launch_bounds__(W * 64, 8) void token_logprobs_top_kernel(ScorePara
   if (wave == W - 1 && lane == 0) write_row(p, row, a, r.tok >= 0, r.xt);
 }
 
-// The same for rows of up to 8 units by one wave each, four rows a workgroup and no barrier: all 512 groups are in its registers, so the
-// threshold is exact at once (rows of 8194 classes, 25000 of them, 20 alternatives: 135 us, 197 with a workgroup each).  Where the
-// candidates do not fit (values that repeat, or a row whose largest ones crowd into few groups): the k-th largest column itself,
-// searched by counting over the row, the fewer than k columns above it, and the lowest classes at it.
-template <typename T>
+// The same for rows of up to UNITS units by one wave each, four rows a workgroup and no barrier: all groups are in its registers, so the
+// threshold is exact at once (rows of 8194 classes, 25000 of them, 20 alternatives: 112 us, 197 with a workgroup each; of 32768, 6250:
+// 92, 104; 8 units with the registers of 16: 117).  Where the candidates do not fit (values that repeat, or a row whose largest ones
+// crowd into few groups): the k-th largest column itself, searched by counting over the row, the fewer than k columns above it, and
+// the lowest classes at it.
+template <typename T, int UNITS>
 __global__ __launch_bounds__(256) void token_logprobs_top_wave_kernel(ScoreParams p) {
-  constexpr int UNITS = 8, CAND = 320, LIST = 128;
+  constexpr int CAND = 320, LIST = 128;
   __shared__ __attribute__((aligned(16))) u64 sm_cand[4][CAND + 4];
   __shared__ int sm_list[4][LIST];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -699,14 +707,19 @@ __global__ __launch_bounds__(256) void token_logprobs_top_wave_kernel(ScoreParam
   wave_fence();
   // v: the lane's 8 columns from c on; test(v) of them become keys
   auto push = [&](const float (&v)[8], int c, auto test) {
+    uint32_t bits = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const bool in = test(v[j]);
-      const u64 mask = __ballot(in);
-      if (mask) {
-        const int at = n + lanes_below(mask);
-        if (in && at < CAND) cand[at] = top_key(v[j], c + j);
-        n += __builtin_popcountll(mask);
+    for (int j = 0; j < 8; ++j) bits |= test(v[j]) ? 1u << j : 0u;
+    for (u64 mask = __ballot(bits != 0); mask; mask = __ballot(bits != 0)) {
+      const int at = n + lanes_below(mask);
+      n += __builtin_popcountll(mask);
+      if (bits) {
+        const int e = __builtin_ctz(bits);
+        bits &= bits - 1;
+        float x = v[0];
+#pragma unroll
+        for (int j = 1; j < 8; ++j) x = e == j ? v[j] : x;
+        if (at < CAND) cand[at] = top_key(x, c + e);
       }
     }
   };
@@ -734,7 +747,7 @@ __global__ __launch_bounds__(256) void token_logprobs_top_wave_kernel(ScoreParam
     float v[8];
     uint32_t t = 0;
     for (uint32_t bit = 0x80000000u; bit >> LowBits<T>::n; bit >>= 1) {
-      float cnt = 0.f;                        // (whole numbers up to 16384)
+      float cnt = 0.f;                        // (whole numbers up to 32832)
       for (int c0 = 0; c0 < p.C; c0 += 512) {
         eight(c0 + lane * 8, p.C, v);
 #pragma unroll
@@ -1182,7 +1195,7 @@ static int launch_score(const ScoreParams& p, hipStream_t st) {
   const char* what = "token_logprobs_fwd";
   const int64_t grid = cdiv((int64_t)p.R * p.units, 4);
   int rc = need_grid(what, grid);
-  if (!rc && p.k && p.units > 8) rc = need_grid(what, p.R, p.units <= 64 ? 256 : 1024);
+  if (!rc && p.k && p.units > 16) rc = need_grid(what, p.R, p.units <= 64 ? 256 : 1024);
   if (rc) return rc;
   if (p.units == 1) {
     const size_t lds = p.k ? 4 * WAVE_TOP_LDS * sizeof(typename WaveKey<T>::type) : 0;
@@ -1194,7 +1207,8 @@ static int launch_score(const ScoreParams& p, hipStream_t st) {
   rc = check_launch(what);
   if (rc) return rc;
   if (p.k == 0) token_logprobs_join_kernel<T><<<(unsigned)cdiv(p.R, 4), 256, 0, st>>>(p);
-  else if (p.units <= 8) token_logprobs_top_wave_kernel<T><<<(unsigned)cdiv(p.R, 4), 256, 0, st>>>(p);   // up to 16448 classes
+  else if (p.units <= 8) token_logprobs_top_wave_kernel<T, 8><<<(unsigned)cdiv(p.R, 4), 256, 0, st>>>(p);   // up to 16448 classes
+  else if (p.units <= 16) token_logprobs_top_wave_kernel<T, 16><<<(unsigned)cdiv(p.R, 4), 256, 0, st>>>(p);   // up to 32832
   else if (p.units <= 64) token_logprobs_top_kernel<T, 4, 16><<<p.R, 256, 0, st>>>(p);     // up to 131136
   else token_logprobs_top_kernel<T, 16, 32><<<p.R, 1024, 0, st>>>(p);                      // up to TTTS_SCORE_MAX_CLASSES
   return check_launch("token_logprobs_fwd join");

@@ -915,15 +915,29 @@ __device__ __forceinline__ void finish_distill(const DistillParams& p, int64_t r
     p.stats[3 * row + 2] = none || !p.tail ? 0.f : zl / zr;
   }
 }
+// A column's value as it was loaded: nothing is done to it, and so not waited for, before it is used.
+template <typename T> struct Later {
+  uint32_t bits = 0;
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (sizeof(T) == 4) bits = *reinterpret_cast<const uint32_t*>(p);
+    else bits = *reinterpret_cast<const uint16_t*>(p);
+  }
+  __device__ __forceinline__ float value() const {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(T, bits);
+    else return (float)__builtin_bit_cast(T, (uint16_t)bits);
+  }
+};
 template <typename T>
-__device__ __forceinline__ void listed_logits(const T* row, const Listed& L, int K, T (&xl)[2]) {   // (some column's for an empty entry)
+__device__ __forceinline__ void listed_logits(const T* row, const Listed& L, int K, Later<T> (&xl)[2]) {   // (some column's for an empty entry)
 #pragma unroll
-  for (int h = 0; h < 2; ++h) xl[h] = h * 64 < K ? row[max(L.id[h], 0)] : T(0.f);
+  for (int h = 0; h < 2; ++h)
+    if (h * 64 < K) xl[h].load(row + max(L.id[h], 0));
 }
 
 // as token_logprobs_fwd_kernel; with tail each wave marks the listed classes of its columns in a bit map of its own
 template <typename T, bool LONG, int NV>
 __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillParams p) {
+  __builtin_assume(p.K > 0);   // (no branch around a list's loads, and so no wait behind each)
   __shared__ uint32_t marks[4][(WAVE_COLS + NARROW) / 32];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t id = (int64_t)blockIdx.x * 4 + wave;
@@ -939,7 +953,7 @@ __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillParams p) {
   load_raw(raw, lr, cols.c0, cols.wide, lane);
   const T narrow = cols.load_narrow(lr, p.C - 1, lane);
   Listed L;
-  T xl[2] = {T(0.f), T(0.f)};
+  Later<T> xl[2];
   if (!LONG || p.tail) list_classes(L, list, p.K, p.C, lane);
   if (!LONG) listed_logits(lr, L, p.K, xl);
   uint32_t* mark = marks[wave];
@@ -996,11 +1010,12 @@ __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillParams p) {
   const float f = __builtin_amdgcn_exp2f(-ex.delta);
   zr = sum_wave(zr) * f;
   if (p.tail) zl = sum_wave(zl) * f;
-  if (!LONG) finish_distill(p, row, L, (float)xl[0], (float)xl[1], m, zl, zr, lane);
+  if (!LONG) finish_distill(p, row, L, xl[0].value(), xl[1].value(), m, zl, zr, lane);
   else if (lane == 0) p.part[id] = make_float4(m, zl, zr, 0.f);
 }
 template <typename T>
 __global__ __launch_bounds__(256) void distill_join_kernel(DistillParams p) {   // a wave per row
+  __builtin_assume(p.K > 0);
   const int lane = threadIdx.x & 63;
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= p.R) return;
@@ -1010,7 +1025,7 @@ __global__ __launch_bounds__(256) void distill_join_kernel(DistillParams p) {   
   if (lane >= p.units) first = make_float4(-FMAX, 0.f, 0.f, 0.f);
   Listed L;
   list_classes(L, list, p.K, p.C, lane);
-  T xl[2];
+  Later<T> xl[2];
   listed_logits((const T*)p.logits + row * p.ldl, L, p.K, xl);
   list_weights(L, list, p.K, p.inv_t, p.tail);
   float m = first.x, zl = 0.f, zr = 0.f;
@@ -1022,7 +1037,7 @@ __global__ __launch_bounds__(256) void distill_join_kernel(DistillParams p) {   
     zl = fmaf(s.y, f, zl);
     zr = fmaf(s.z, f, zr);
   }
-  finish_distill(p, row, L, (float)xl[0], (float)xl[1], m, sum_wave(zl), sum_wave(zr), lane);
+  finish_distill(p, row, L, xl[0].value(), xl[1].value(), m, sum_wave(zl), sum_wave(zr), lane);
 }
 
 struct DistillGradParams {
@@ -1042,6 +1057,7 @@ struct DistillGradParams {
 // name one class find out by leaving their number at its place in LDS: each then writes the sum of their p, in the list's order.
 template <typename T, int NV>
 __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillGradParams p) {
+  __builtin_assume(p.K > 0);
   __shared__ uint8_t tags[4][WAVE_COLS + NARROW];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t unit = (int64_t)blockIdx.x * 4 + wave;
@@ -1061,14 +1077,13 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillGradParams p) {
   Listed L;
   list_classes(L, list, p.K, p.C, lane);
   bool here[2];
-  T xl[2], old[2];
+  Later<T> xl[2], old[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     here[h] = L.id[h] >= c0 && L.id[h] < cend;
-    xl[h] = old[h] = T(0.f);
     if (h * 64 < p.K) {
-      xl[h] = lr[here[h] ? L.id[h] : 0];
-      if (p.accumulate) old[h] = dr[here[h] ? L.id[h] : 0];
+      xl[h].load(lr + (here[h] ? L.id[h] : 0));
+      if (p.accumulate) old[h].load(dr + (here[h] ? L.id[h] : 0));
     }
   }
   const float m = p.stats[3 * row], logz = p.stats[3 * row + 1], w = p.stats[3 * row + 2], g = p.g_loss[row] * p.inv_t;
@@ -1134,8 +1149,8 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillGradParams p) {
 #pragma unroll
   for (int h = 0; h < 2; ++h)
     if (here[h]) {
-      const float q = __builtin_amdgcn_exp2f(((float)xl[h] - m) * c - log2z);
-      dr[L.id[h]] = (T)((float)old[h] + fmaf(q, on, -L.p[h]) * g);
+      const float q = __builtin_amdgcn_exp2f((xl[h].value() - m) * c - log2z);
+      dr[L.id[h]] = (T)(old[h].value() + fmaf(q, on, -L.p[h]) * g);
     }
 }
 

@@ -67,6 +67,11 @@ __device__ __forceinline__ void store8(T* p, int n, const float (&v)[8]) {
 template <typename T, int NV> struct Raw { typename Eight<T>::type v[NV]; };
 template <typename T, int NV>
 __device__ __forceinline__ void load_raw(Raw<T, NV>& r, const T* row, int c0, int cend, int lane) {
+  if (c0 + NV * 512 <= cend) {   // (all of them: one address for the wave)
+#pragma unroll
+    for (int i = 0; i < NV; ++i) r.v[i] = *reinterpret_cast<const typename Eight<T>::type*>(row + c0 + (unsigned)(i * 512 + lane * 8));
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = c0 + i * 512 + lane * 8;
@@ -104,10 +109,11 @@ struct Exponent {
     delta = plain ? fmaf(m, c, -mc) : 0.f;
   }
 };
-// (n / d, n % d) of a piece's number: in 32 bits where it fits (a 64-bit division costs as much as the piece's work)
+// (n / d, n % d) of the number of a launch's wave or thread, which fits 32 bits
 __device__ __forceinline__ void split_id(int64_t n, int d, int64_t& q, int& r) {
-  if ((uint64_t)n >> 32) { q = n / d; r = (int)(n % d); }
-  else { q = (uint32_t)n / (uint32_t)d; r = (int)((uint32_t)n % (uint32_t)d); }
+  const uint32_t whole = (uint32_t)n / (uint32_t)d;
+  q = whole;
+  r = (int)((uint32_t)n - whole * (uint32_t)d);
 }
 
 __device__ __forceinline__ void wave_fence() {   // LDS written by this wave's lanes is read by its other lanes

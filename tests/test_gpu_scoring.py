@@ -212,6 +212,32 @@ def test_alternatives_crowd_into_few_parts_of_a_row(dtype, C, every, top_k):
     assert torch.equal(r.top_idx.cpu(), want)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("C,offset", [(600, 1), (1088, 3), (1089, 0), (2112, 1), (2113, 0), (2200, 5), (4600, 0), (16448, 1), (16449, 0), (32832, 0),
+                                      (32833, 2), (131136, 0), (131137, 1)])
+def test_alternatives_where_the_layout_of_a_row_changes(dtype, C, offset):
+    """Widths around one wave's columns, the narrow rest, units of three steps, and the kernels' limits: the best classes are put
+    at the first and last columns and around every multiple of 512 and of 2048."""
+    from ttts_amd import ops
+    R = 3
+    g = torch.Generator().manual_seed(C)
+    x = torch.randn(R, C + offset, generator=g)
+    marks = sorted({c for m in (0, C) for c in range(m - 3, m + 3)} | {m + d for m in range(512, C, 512 if C < 6000 else 2048) for d in (-1, 0)})
+    marks = [c for c in marks if 0 <= c < C]
+    pick = torch.tensor(marks)[torch.randperm(len(marks), generator=g)[:40]]
+    x[:, pick + offset] += 20.0
+    x = x.to(dtype).cuda()[:, offset:]
+    tok = pick[:R].clone().cuda()
+    r = ops.token_logprobs_fwd(x, tok, top_k=64)
+    y = x.float().cpu()
+    assert torch.equal(r.top_idx.cpu(), torch.sort(y, dim=1, descending=True, stable=True).indices[:, :64])
+    lp = torch.log_softmax(y.double(), dim=1)
+    bound = _r(C) + 4 * U * y.abs().max().item()
+    assert (r.logp.cpu().double() - lp.gather(1, tok.cpu()[:, None])[:, 0]).abs().max().item() <= bound
+    # log Z - s / z: the one as above, the other's sums off by r of themselves each, |s / z| = log Z - H <= log C
+    assert (r.entropy.cpu().double() + (lp.exp() * lp).sum(dim=1)).abs().max().item() <= bound * (1 + 2 * math.log(C))
+
+
 def test_logits_far_from_zero():
     """The statistics hand the maximum and log Z on apart: rows around 4096 lose nothing of their gradient."""
     from ttts_amd import ops

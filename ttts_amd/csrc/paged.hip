@@ -370,7 +370,7 @@ template <typename T, int DH, int NW>
 static int launch_paged_waves(const PagedParams& p, int64_t grid, hipStream_t st) {
   static OnceFlag once;
   const int lds = NW * (p.group < 16 ? p.group : 16) * (DH + 2) * 4;
-  if (lds_opt_in(once, (const void*)attn_paged_decode_kernel<T, DH, NW>, NW * 16 * (DH + 2) * 4) != hipSuccess)
+  if (lds > 64 * 1024 && lds_opt_in(once, (const void*)attn_paged_decode_kernel<T, DH, NW>, NW * 16 * (DH + 2) * 4) != hipSuccess)
     return fail(TTTS_EHIP, "attn_paged_decode: LDS opt-in failed");
   attn_paged_decode_kernel<T, DH, NW><<<(unsigned)grid, NW * 64, lds, st>>>(p);
   return check_launch("attn_paged_decode");

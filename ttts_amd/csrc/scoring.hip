@@ -15,7 +15,7 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f, FMAX = 3
 // ---- one wave = up to 2048 columns of a row, held in registers as fp32 -------------------------------------------------
 // A row is read ONCE: maximum, sums, and the alternatives' threshold all come from the registers.  Rows up to 2048 columns take one wave;
 // longer ones a wave per 2048 columns, each on its own (a workgroup per row whose waves meet at barriers read 2.1 - 2.5 TB/s where
-// these read 4.4), and a second kernel that joins a row's parts.  A lane holds 8 neighbouring columns per load (16 or 32 bytes,
+// these read 5.4), and a second kernel that joins a row's parts.  A lane holds 8 neighbouring columns per load (16 or 32 bytes,
 // at whatever alignment the row has; only the row's last columns are read one by one), 64 lanes 512 neighbouring ones: x[i][j] is
 // column c0 + 512 i + 8 lane + j.  A rest of up to 64 columns behind the last whole 512 -- a codebook and its few special classes --
 // is one more column a lane (`narrow`) instead of a step of eight.  NV: the steps of 512 that a kernel is compiled for; rows up to 1088

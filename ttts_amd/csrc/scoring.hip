@@ -379,56 +379,6 @@ __device__ __forceinline__ void write_top(const ScoreParams& p, int64_t row, int
   p.top_logp[row * p.k + r] = have ? (unord((uint32_t)(key >> 32)) - a.m) * p.inv_t - __builtin_amdgcn_logf(a.z) * LN2 : nan ? a.z : -INFINITY;
 }
 
-// One wave per row (LONG false), or per unit of up to 2048 columns of a row.  (Waves that went through several of them, the next one's loads under this
-// one's arithmetic, were slower at every grid: 118 - 125 us instead of 109 for logits of 2048 x 100003 with 64 alternatives.)
-template <typename T, bool LONG, int NV>
-__global__ __launch_bounds__(256) void token_logprobs_fwd_kernel(ScoreParams p) {
-  extern __shared__ __attribute__((aligned(16))) unsigned char score_lds[];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t id = (int64_t)blockIdx.x * 4 + wave;
-  int64_t row = id;
-  int unit = 0;
-  if (LONG) split_id(id, p.units, row, unit);
-  if (row >= p.R) return;
-  const T* lr = (const T*)p.logits + row * p.ldl;
-  const Cols cols(unit * p.unit_cols, unit == p.units - 1 ? p.C : (unit + 1) * p.unit_cols);
-  float x[NV][8], vmax[NV];
-  int64_t tok = -1;
-  float xt = 0.f, xn;
-  {
-    Raw<T, NV> raw;
-    if (!LONG) tok = p.tokens[row];
-    load_raw(raw, lr, cols.c0, cols.wide, lane);
-    const T narrow = cols.load_narrow(lr, p.C - 1, lane);
-    const bool given = tok >= 0 && tok < p.C;
-    const T at_tok = LONG ? T(0.f) : lr[given ? tok : 0];   // (its latency runs beside the row's)
-    expand(raw, lr, cols.c0, cols.wide, lane, x);
-    xn = cols.narrow_value(narrow, p.C, lane);
-    xt = given ? (float)at_tok : 0.f;
-  }
-  float lmax = xn;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    vmax[i] = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) vmax[i] = max_med(vmax[i], x[i][j]);
-    lmax = max_med(lmax, vmax[i]);
-  }
-  if (!LONG) vmax[0] = max_med(vmax[0], xn);
-  lmax = max_med(lmax, -INFINITY);                         // (xn may be NaN)
-  const RowSums a = wave_sums(x, xn, cols, lmax, p.inv_t * LOG2E);
-  if constexpr (LONG) {
-    if (lane == 0) p.part[id] = make_float4(a.m, a.z, a.s, 0.f);
-    if (p.k) ((T*)p.part_max)[id * 64 + lane] = (T)group_max(vmax, xn, lane);
-    return;
-  }
-  if (lane == 0) write_row(p, row, a, tok >= 0 && tok < p.C, xt);
-  if (p.k) {
-    const int have = wave_top<T, NV>(x, xn, vmax, lr, cols, p.k, lane, reinterpret_cast<typename WaveKey<T>::type*>(score_lds) + wave * WAVE_TOP_LDS, [&](int r, u64 key) { write_top(p, row, r, key, a); });
-    if (lane >= have && lane < p.k) write_top(p, row, lane, 0, a);
-  }
-}
-
 // A long row's sums, by one wave, from its units' parts; every lane gets them.  What it takes from memory is asked for first, and by every
 // lane, so that its way is short when it is needed.
 struct LongRow { float4 first; int tok; float xt; };   // tok: -1 if none is given
@@ -441,8 +391,7 @@ __device__ __forceinline__ LongRow load_long_row(const ScoreParams& p, int64_t r
   r.xt = (float)((const T*)p.logits)[row * p.ldl + max(r.tok, 0)];
   return r;
 }
-__device__ __forceinline__ RowSums join_sums(const ScoreParams& p, int64_t row, const LongRow& r, int lane) {
-  const float4* part = p.part + row * p.units;
+__device__ __forceinline__ RowSums join_sums(const ScoreParams& p, const float4* part, const LongRow& r, int lane) {
   const float c = p.inv_t * LOG2E;
   float m = r.first.x;
   for (int u = lane + 64; u < p.units; u += 64) m = fmaxf(m, part[u].x);
@@ -456,13 +405,202 @@ __device__ __forceinline__ RowSums join_sums(const ScoreParams& p, int64_t row, 
   a.s = sum_wave(a.s);
   return a;
 }
+// Alternatives of a row of up to UNITS units by one wave: v are the maxima of all its groups, so the threshold is exact at once.  Where the
+// candidates do not fit (values that repeat, or a row whose largest ones crowd into few groups): the k-th largest column itself,
+// searched by counting over the row, the fewer than k columns above it, and the lowest classes at it.
+constexpr int ROW_CAND = 320, ROW_LIST = 128;
+template <typename T, int UNITS>
+__device__ __forceinline__ void row_top(const ScoreParams& p, int64_t row, const T* lr, const float (&v)[UNITS], const RowSums& a, u64* cand, int* list,
+                                        int lane) {
+  const int k = p.k;
+  uint32_t g[UNITS], lo, hi;
+  float most = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < UNITS; ++i) {
+    g[i] = ord(v[i]);
+    most = max_med(most, v[i]);
+  }
+  lane_bounds(most, lo, hi);
+  float thr = group_threshold<T, UNITS>(g, k, true, lo, hi);
+  int n = 0, listed = 0;
+  {
+    const uint32_t tb = ord(thr);
+#pragma unroll
+    for (int i = 0; i < UNITS; ++i) {
+      const u64 mask = __ballot(g[i] >= tb);
+      if (mask) {
+        const int at = listed + lanes_below(mask);
+        if (g[i] >= tb && at < ROW_LIST) list[at] = i * 64 + lane;
+        listed += __builtin_popcountll(mask);
+      }
+    }
+  }
+  wave_fence();
+  // v: the lane's 8 columns from c on; test(v) of them become keys
+  auto push = [&](const float (&v)[8], int c, auto test) {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) bits |= test(v[j]) ? 1u << j : 0u;
+    for (u64 mask = __ballot(bits != 0); mask; mask = __ballot(bits != 0)) {
+      const int at = n + lanes_below(mask);
+      n += __builtin_popcountll(mask);
+      if (bits) {
+        const int e = __builtin_ctz(bits);
+        bits &= bits - 1;
+        float x = v[0];
+#pragma unroll
+        for (int j = 1; j < 8; ++j) x = e == j ? v[j] : x;
+        if (at < ROW_CAND) cand[at] = top_key(x, c + e);
+      }
+    }
+  };
+  auto eight = [&](int c, int end, float (&v)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = -INFINITY;
+    if (c < end) load8<T>(lr + c, end - c, v);
+  };
+  bool full = listed > ROW_LIST;
+  if (!full) {
+    for (int s = 0; s < listed * (STEPS + 1); s += 64) {
+      const int task = s + lane, i = task % (STEPS + 1), id = task < listed * (STEPS + 1) ? list[task / (STEPS + 1)] : 0;
+      int c = (id >> 6) * p.unit_cols + (id & 3) * 512 + (id & 60) * 8 + i * 8, end = (id & 3) * 512 < p.unit_cols ? p.narrow_at : 0;
+      if (i == STEPS) {                              // the unit's narrow columns
+        c = p.narrow_at + (id & 63);
+        end = (id >> 6) == p.units - 1 ? min(p.C, c + 1) : 0;
+      }
+      float v[8];
+      eight(c, task < listed * (STEPS + 1) ? end : 0, v);
+      push(v, c, [&](float x) { return x >= thr; });
+    }
+    full = n > ROW_CAND;
+  }
+  if (full) {
+    float v[8];
+    uint32_t t = 0;
+    for (uint32_t bit = 0x80000000u; bit >> LowBits<T>::n; bit >>= 1) {
+      float cnt = 0.f;                        // (whole numbers up to 32832)
+      for (int c0 = 0; c0 < p.C; c0 += 512) {
+        eight(c0 + lane * 8, p.C, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) cnt += ord(v[j]) >= (t | bit) && v[j] == v[j] ? 1.f : 0.f;
+      }
+      if (sum_wave(cnt) >= (float)k) t |= bit;
+    }
+    thr = threshold_of<T>(t);
+    n = 0;
+    for (int c0 = 0; c0 < p.C; c0 += 512) {
+      eight(c0 + lane * 8, p.C, v);
+      push(v, c0 + lane * 8, [&](float x) { return x > thr; });
+    }
+    for (int c0 = 0; c0 < p.C && n < k; c0 += 512) {
+      eight(c0 + lane * 8, p.C, v);
+      int mine = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) mine += v[j] == thr;
+      int upto = mine;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(upto, o, 64);
+        if (lane >= o) upto += u;
+      }
+      int at = n + upto - mine;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (v[j] == thr) {
+          if (at < k) cand[at] = top_key(v[j], c0 + lane * 8 + j);
+          ++at;
+        }
+      n = min(k, n + __shfl(upto, 63, 64));
+    }
+    n = min(n, k);
+  }
+  if (lane < 4) cand[n + lane] = 0;
+  wave_fence();
+  rank_keys(cand, n, k, lane, 64, [&](int r, u64 key) { write_top(p, row, r, key, a); });
+  if (lane >= n && lane < k) write_top(p, row, lane, 0, a);
+}
+
+// One wave per row (ONE), or per unit of up to 2048 columns of a row: with a workgroup for a row (ROW), whose waves meet once and the first ends
+// the row, or on their own (PART), with a second kernel that does.  A workgroup a row saves the parts' way through memory and a launch:
+// 25000 fp32 rows of 4096 classes, 20 alternatives: 78 us, 105 in two kernels; 3125 of 32768: 80, 89.  Of 16-bit types, half the bytes for
+// the same arithmetic, only up to four waves: 25000 rows of 8194: 87, 107; but 10240 of 20000: 112, 96 (ten waves start where
+// ten have ended).  (Waves that went through several units, the next one's loads under this one's arithmetic, were slower at every grid:
+// 118 - 125 us instead of 109 for logits of 2048 x 100003 with 64 alternatives.)
+enum Kind { ONE, ROW, PART };
+template <typename T> struct RowUnits { static constexpr int n = sizeof(T) == 4 ? 16 : 4; };
+template <typename T, Kind KIND, int NV, int UNITS = 1>
+__global__ __launch_bounds__(KIND == ROW ? UNITS * 64 : 256, 8) void token_logprobs_fwd_kernel(ScoreParams p) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char score_lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t id = (int64_t)blockIdx.x * 4 + wave;
+  int64_t row = KIND == ROW ? blockIdx.x : id;
+  int unit = KIND == ROW ? wave : 0;
+  if (KIND == PART) split_id(id, p.units, row, unit);
+  if (row >= p.R) return;
+  const T* lr = (const T*)p.logits + row * p.ldl;
+  const Cols cols(unit * p.unit_cols, unit == p.units - 1 ? p.C : (unit + 1) * p.unit_cols);
+  float x[NV][8], vmax[NV];
+  int64_t tok = -1;
+  float xt = 0.f, xn;
+  {
+    Raw<T, NV> raw;
+    if (KIND != PART && unit == 0) tok = p.tokens[row];
+    load_raw(raw, lr, cols.c0, cols.wide, lane);
+    const T narrow = cols.load_narrow(lr, p.C - 1, lane);
+    const bool given = tok >= 0 && tok < p.C;
+    const T at_tok = KIND == PART ? T(0.f) : lr[given ? tok : 0];   // (its latency runs beside the row's)
+    expand(raw, lr, cols.c0, cols.wide, lane, x);
+    xn = cols.narrow_value(narrow, p.C, lane);
+    xt = given ? (float)at_tok : 0.f;
+  }
+  float lmax = xn;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    vmax[i] = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) vmax[i] = max_med(vmax[i], x[i][j]);
+    lmax = max_med(lmax, vmax[i]);
+  }
+  if (KIND == ONE) vmax[0] = max_med(vmax[0], xn);
+  lmax = max_med(lmax, -INFINITY);                         // (xn may be NaN)
+  const RowSums a = wave_sums(x, xn, cols, lmax, p.inv_t * LOG2E);
+  if constexpr (KIND == PART) {
+    if (lane == 0) p.part[id] = make_float4(a.m, a.z, a.s, 0.f);
+    if (p.k) ((T*)p.part_max)[id * 64 + lane] = (T)group_max(vmax, xn, lane);
+  } else if constexpr (KIND == ROW) {
+    __shared__ float4 sm_part[UNITS];
+    __shared__ float sm_max[UNITS][64];
+    __shared__ __attribute__((aligned(16))) u64 sm_cand[ROW_CAND + 4];
+    __shared__ int sm_list[ROW_LIST];
+    if (lane == 0) sm_part[unit] = make_float4(a.m, a.z, a.s, 0.f);
+    if (p.k) sm_max[unit][lane] = group_max(vmax, xn, lane);
+    __syncthreads();
+    if (unit) return;
+    const LongRow r = {sm_part[min(lane, p.units - 1)], tok >= 0 && tok < p.C ? (int)tok : -1, xt};
+    const RowSums all = join_sums(p, sm_part, r, lane);
+    if (lane == 0) write_row(p, row, all, r.tok >= 0, r.xt);
+    if (p.k) {
+      float v[UNITS];
+#pragma unroll
+      for (int i = 0; i < UNITS; ++i) v[i] = i < p.units ? sm_max[i][lane] : -INFINITY;
+      row_top<T, UNITS>(p, row, lr, v, all, sm_cand, sm_list, lane);
+    }
+  } else {
+    if (lane == 0) write_row(p, row, a, tok >= 0 && tok < p.C, xt);
+    if (p.k) {
+      const int have = wave_top<T, NV>(x, xn, vmax, lr, cols, p.k, lane, reinterpret_cast<typename WaveKey<T>::type*>(score_lds) + wave * WAVE_TOP_LDS, [&](int r, u64 key) { write_top(p, row, r, key, a); });
+      if (lane >= have && lane < p.k) write_top(p, row, lane, 0, a);
+    }
+  }
+}
+
 template <typename T>
 __global__ __launch_bounds__(256) void token_logprobs_join_kernel(ScoreParams p) {   // no alternatives: a wave per row
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= p.R) return;
   const int lane = threadIdx.x & 63;
   const LongRow r = load_long_row<T>(p, row, lane);
-  const RowSums a = join_sums(p, row, r, lane);
+  const RowSums a = join_sums(p, p.part + row * p.units, r, lane);
   if (lane == 0) write_row(p, row, a, r.tok >= 0, r.xt);
 }
 
@@ -524,7 +662,7 @@ __global__ __launch_bounds__(W * 64, 8) void token_logprobs_top_kernel(ScorePara
           ++at;
         }
       if (wave == W - 1 && round == 0) {
-        const RowSums a = join_sums(p, row, r, lane);
+        const RowSums a = join_sums(p, p.part + row * p.units, r, lane);
         if (lane == 0) sm_row = a;
       }
       __syncthreads();
@@ -663,136 +801,26 @@ __global__ __launch_bounds__(W * 64, 8) void token_logprobs_top_kernel(ScorePara
   if (wave == W - 1 && lane == 0) write_row(p, row, a, r.tok >= 0, r.xt);
 }
 
-// The same for rows of up to UNITS units by one wave each, four rows a workgroup and no barrier: all groups are in its registers, so the
-// threshold is exact at once (rows of 8194 classes, 25000 of them, 20 alternatives: 112 us, 197 with a workgroup each; of 32768, 6250:
-// 92, 104; 8 units with the registers of 16: 117).  Where the candidates do not fit (values that repeat, or a row whose largest ones
-// crowd into few groups): the k-th largest column itself, searched by counting over the row, the fewer than k columns above it, and
-// the lowest classes at it.
+// A wave per row of up to UNITS units, four rows a workgroup and no barrier (6250 rows of 32768 classes, 20 alternatives: 92 us, 104 with a
+// workgroup each; 8 units with the registers of 16 cost a tenth more).
 template <typename T, int UNITS>
 __global__ __launch_bounds__(256) void token_logprobs_top_wave_kernel(ScoreParams p) {
-  constexpr int CAND = 320, LIST = 128;
-  __shared__ __attribute__((aligned(16))) u64 sm_cand[4][CAND + 4];
-  __shared__ int sm_list[4][LIST];
+  __shared__ __attribute__((aligned(16))) u64 sm_cand[4][ROW_CAND + 4];
+  __shared__ int sm_list[4][ROW_LIST];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t row = (int64_t)blockIdx.x * 4 + wave;
   if (row >= p.R) return;
-  const T* lr = (const T*)p.logits + row * p.ldl;
   const T* gm = (const T*)p.part_max + row * p.units * 64;
-  u64* cand = sm_cand[wave];
-  int* list = sm_list[wave];
-  const int k = p.k;
   T raw[UNITS];
 #pragma unroll
   for (int i = 0; i < UNITS; ++i) raw[i] = gm[min(i, p.units - 1) * 64 + lane];
   const LongRow r = load_long_row<T>(p, row, lane);
-  uint32_t g[UNITS], lo, hi;
-  float most = -INFINITY;
+  float v[UNITS];
 #pragma unroll
-  for (int i = 0; i < UNITS; ++i) {
-    const float v = i < p.units ? (float)raw[i] : -INFINITY;
-    g[i] = ord(v);
-    most = max_med(most, v);
-  }
-  const RowSums a = join_sums(p, row, r, lane);
+  for (int i = 0; i < UNITS; ++i) v[i] = i < p.units ? (float)raw[i] : -INFINITY;
+  const RowSums a = join_sums(p, p.part + row * p.units, r, lane);
   if (lane == 0) write_row(p, row, a, r.tok >= 0, r.xt);
-  lane_bounds(most, lo, hi);
-  float thr = group_threshold<T, UNITS>(g, k, true, lo, hi);
-  int n = 0, listed = 0;
-  {
-    const uint32_t tb = ord(thr);
-#pragma unroll
-    for (int i = 0; i < UNITS; ++i) {
-      const u64 mask = __ballot(g[i] >= tb);
-      if (mask) {
-        const int at = listed + lanes_below(mask);
-        if (g[i] >= tb && at < LIST) list[at] = i * 64 + lane;
-        listed += __builtin_popcountll(mask);
-      }
-    }
-  }
-  wave_fence();
-  // v: the lane's 8 columns from c on; test(v) of them become keys
-  auto push = [&](const float (&v)[8], int c, auto test) {
-    uint32_t bits = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) bits |= test(v[j]) ? 1u << j : 0u;
-    for (u64 mask = __ballot(bits != 0); mask; mask = __ballot(bits != 0)) {
-      const int at = n + lanes_below(mask);
-      n += __builtin_popcountll(mask);
-      if (bits) {
-        const int e = __builtin_ctz(bits);
-        bits &= bits - 1;
-        float x = v[0];
-#pragma unroll
-        for (int j = 1; j < 8; ++j) x = e == j ? v[j] : x;
-        if (at < CAND) cand[at] = top_key(x, c + e);
-      }
-    }
-  };
-  auto eight = [&](int c, int end, float (&v)[8]) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = -INFINITY;
-    if (c < end) load8<T>(lr + c, end - c, v);
-  };
-  bool full = listed > LIST;
-  if (!full) {
-    for (int s = 0; s < listed * (STEPS + 1); s += 64) {
-      const int task = s + lane, i = task % (STEPS + 1), id = task < listed * (STEPS + 1) ? list[task / (STEPS + 1)] : 0;
-      int c = (id >> 6) * p.unit_cols + (id & 3) * 512 + (id & 60) * 8 + i * 8, end = (id & 3) * 512 < p.unit_cols ? p.narrow_at : 0;
-      if (i == STEPS) {                              // the unit's narrow columns
-        c = p.narrow_at + (id & 63);
-        end = (id >> 6) == p.units - 1 ? min(p.C, c + 1) : 0;
-      }
-      float v[8];
-      eight(c, task < listed * (STEPS + 1) ? end : 0, v);
-      push(v, c, [&](float x) { return x >= thr; });
-    }
-    full = n > CAND;
-  }
-  if (full) {
-    float v[8];
-    uint32_t t = 0;
-    for (uint32_t bit = 0x80000000u; bit >> LowBits<T>::n; bit >>= 1) {
-      float cnt = 0.f;                        // (whole numbers up to 32832)
-      for (int c0 = 0; c0 < p.C; c0 += 512) {
-        eight(c0 + lane * 8, p.C, v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) cnt += ord(v[j]) >= (t | bit) && v[j] == v[j] ? 1.f : 0.f;
-      }
-      if (sum_wave(cnt) >= (float)k) t |= bit;
-    }
-    thr = threshold_of<T>(t);
-    n = 0;
-    for (int c0 = 0; c0 < p.C; c0 += 512) {
-      eight(c0 + lane * 8, p.C, v);
-      push(v, c0 + lane * 8, [&](float x) { return x > thr; });
-    }
-    for (int c0 = 0; c0 < p.C && n < k; c0 += 512) {
-      eight(c0 + lane * 8, p.C, v);
-      int mine = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) mine += v[j] == thr;
-      int upto = mine;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int u = __shfl_up(upto, o, 64);
-        if (lane >= o) upto += u;
-      }
-      int at = n + upto - mine;
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (v[j] == thr) {
-          if (at < k) cand[at] = top_key(v[j], c0 + lane * 8 + j);
-          ++at;
-        }
-      n = min(k, n + __shfl(upto, 63, 64));
-    }
-    n = min(n, k);
-  }
-  if (lane < 4) cand[n + lane] = 0;
-  wave_fence();
-  rank_keys(cand, n, k, lane, 64, [&](int r, u64 key) { write_top(p, row, r, key, a); });
-  if (lane >= n && lane < k) write_top(p, row, lane, 0, a);
+  row_top<T, UNITS>(p, row, (const T*)p.logits + row * p.ldl, v, a, sm_cand[wave], sm_list[wave], lane);
 }
 
 // ---- gradient of the log-probabilities: one thread per 8 columns, everything of the row is known -------------------------
@@ -941,27 +969,44 @@ __device__ __forceinline__ void listed_logits(const T* row, const Listed& L, int
 }
 
 // as token_logprobs_fwd_kernel; with tail each wave marks the listed classes of its columns in a bit map of its own
-template <typename T, bool LONG, int NV>
-__global__ __launch_bounds__(256) void distill_fwd_kernel(DistillParams p) {
+// a row's sums, by one wave, from its units' parts; first: that of unit `lane`, or the last
+__device__ __forceinline__ void join_parts(const DistillParams& p, const float4* part, float4 first, float& m, float& zl, float& zr, int lane) {
+  if (lane >= p.units) first = make_float4(-FMAX, 0.f, 0.f, 0.f);
+  m = first.x;
+  for (int u = lane + 64; u < p.units; u += 64) m = fmaxf(m, part[u].x);
+  m = max_wave(m);
+  zl = zr = 0.f;
+  for (int u = lane; u < p.units; u += 64) {
+    const float4 s = u < 64 ? first : part[u];
+    const float f = __builtin_amdgcn_exp2f((s.x - m) * p.inv_t * LOG2E);
+    zl = fmaf(s.y, f, zl);
+    zr = fmaf(s.z, f, zr);
+  }
+  zl = sum_wave(zl);
+  zr = sum_wave(zr);
+}
+template <typename T, Kind KIND, int NV, int UNITS = 4>
+__global__ __launch_bounds__(KIND == ROW ? UNITS * 64 : 256, 8) void distill_fwd_kernel(DistillParams p) {
   __builtin_assume(p.K > 0);   // (no branch around a list's loads, and so no wait behind each)
-  __shared__ uint32_t marks[4][(WAVE_COLS + NARROW) / 32];
+  __shared__ uint32_t marks[UNITS][(WAVE_COLS + NARROW) / 32];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t id = (int64_t)blockIdx.x * 4 + wave;
-  int64_t row = id;
-  int unit = 0;
-  if (LONG) split_id(id, p.units, row, unit);
+  int64_t row = KIND == ROW ? blockIdx.x : id;
+  int unit = KIND == ROW ? wave : 0;
+  if (KIND == PART) split_id(id, p.units, row, unit);
   if (row >= p.R) return;
   const T* lr = (const T*)p.logits + row * p.ldl;
   const Cols cols(unit * p.unit_cols, unit == p.units - 1 ? p.C : (unit + 1) * p.unit_cols);
+  const bool ends = KIND != PART && unit == 0;   // this wave has the row's last word
   ListLoads list;
-  if (!LONG || p.tail) list = load_list(p.idx + row * p.K, p.tlogp + row * p.K, p.K, lane);
+  if (ends || p.tail) list = load_list(p.idx + row * p.K, p.tlogp + row * p.K, p.K, lane);
   Raw<T, NV> raw;
   load_raw(raw, lr, cols.c0, cols.wide, lane);
   const T narrow = cols.load_narrow(lr, p.C - 1, lane);
   Listed L;
   Later<T> xl[2];
-  if (!LONG || p.tail) list_classes(L, list, p.K, p.C, lane);
-  if (!LONG) listed_logits(lr, L, p.K, xl);
+  if (ends || p.tail) list_classes(L, list, p.K, p.C, lane);
+  if (ends) listed_logits(lr, L, p.K, xl);
   uint32_t* mark = marks[wave];
   if (p.tail) {
     mark[lane] = 0;
@@ -974,7 +1019,7 @@ __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillParams p) {
     }
     wave_fence();
   }
-  if (!LONG) list_weights(L, list, p.K, p.inv_t, p.tail);
+  if (ends) list_weights(L, list, p.K, p.inv_t, p.tail);
   const float xn = cols.narrow_value(narrow, p.C, lane);
   float x[NV][8], m = fmaxf(xn, -FMAX);
   expand(raw, lr, cols.c0, cols.wide, lane, x);
@@ -1016,8 +1061,18 @@ __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillParams p) {
   const float f = __builtin_amdgcn_exp2f(-ex.delta);
   zr = sum_wave(zr) * f;
   if (p.tail) zl = sum_wave(zl) * f;
-  if (!LONG) finish_distill(p, row, L, xl[0].value(), xl[1].value(), m, zl, zr, lane);
-  else if (lane == 0) p.part[id] = make_float4(m, zl, zr, 0.f);
+  if constexpr (KIND == PART) {
+    if (lane == 0) p.part[id] = make_float4(m, zl, zr, 0.f);
+  } else {
+    if constexpr (KIND == ROW) {
+      __shared__ float4 sm_part[UNITS];
+      if (lane == 0) sm_part[unit] = make_float4(m, zl, zr, 0.f);
+      __syncthreads();
+      if (unit) return;
+      join_parts(p, sm_part, sm_part[min(lane, p.units - 1)], m, zl, zr, lane);
+    }
+    finish_distill(p, row, L, xl[0].value(), xl[1].value(), m, zl, zr, lane);
+  }
 }
 template <typename T>
 __global__ __launch_bounds__(256) void distill_join_kernel(DistillParams p) {   // a wave per row
@@ -1027,23 +1082,15 @@ __global__ __launch_bounds__(256) void distill_join_kernel(DistillParams p) {   
   if (row >= p.R) return;
   const float4* part = p.part + row * p.units;
   const ListLoads list = load_list(p.idx + row * p.K, p.tlogp + row * p.K, p.K, lane);
-  float4 first = part[min(lane, p.units - 1)];
-  if (lane >= p.units) first = make_float4(-FMAX, 0.f, 0.f, 0.f);
+  const float4 first = part[min(lane, p.units - 1)];
   Listed L;
   list_classes(L, list, p.K, p.C, lane);
   Later<T> xl[2];
   listed_logits((const T*)p.logits + row * p.ldl, L, p.K, xl);
   list_weights(L, list, p.K, p.inv_t, p.tail);
-  float m = first.x, zl = 0.f, zr = 0.f;
-  for (int u = lane + 64; u < p.units; u += 64) m = fmaxf(m, part[u].x);
-  m = max_wave(m);
-  for (int u = lane; u < p.units; u += 64) {
-    const float4 s = u < 64 ? first : part[u];
-    const float f = __builtin_amdgcn_exp2f((s.x - m) * p.inv_t * LOG2E);
-    zl = fmaf(s.y, f, zl);
-    zr = fmaf(s.z, f, zr);
-  }
-  finish_distill(p, row, L, xl[0].value(), xl[1].value(), m, sum_wave(zl), sum_wave(zr), lane);
+  float m, zl, zr;
+  join_parts(p, part, first, m, zl, zr, lane);
+  finish_distill(p, row, L, xl[0].value(), xl[1].value(), m, zl, zr, lane);
 }
 
 struct DistillGradParams {
@@ -1208,7 +1255,7 @@ static Units split_columns(int n) {
 
 extern "C" int64_t ttts_token_logprobs_workspace_bytes(int32_t R, int32_t C, int32_t top_k) {
   const int units = C > 0 ? split_columns(C).units : 1;
-  return R > 0 && units > 1 ? (int64_t)R * units * (16 + (top_k > 0 ? 256 : 0)) : 0;
+  return R > 0 && units > RowUnits<bf16>::n ? (int64_t)R * units * (16 + (top_k > 0 ? 256 : 0)) : 0;
 }
 
 template <typename T>
@@ -1220,16 +1267,28 @@ static int launch_score(const ScoreParams& p, hipStream_t st) {
   if (rc) return rc;
   if (p.units == 1) {
     const size_t lds = p.k ? 4 * WAVE_TOP_LDS * sizeof(typename WaveKey<T>::type) : 0;
-    if (p.narrow_at <= 1024) token_logprobs_fwd_kernel<T, false, 2><<<(unsigned)grid, 256, lds, st>>>(p);
-    else token_logprobs_fwd_kernel<T, false, STEPS><<<(unsigned)grid, 256, lds, st>>>(p);
+    if (p.narrow_at <= 1024) token_logprobs_fwd_kernel<T, ONE, 2><<<(unsigned)grid, 256, lds, st>>>(p);
+    else token_logprobs_fwd_kernel<T, ONE, STEPS><<<(unsigned)grid, 256, lds, st>>>(p);
     return check_launch(what);
   }
-  token_logprobs_fwd_kernel<T, true, STEPS><<<(unsigned)grid, 256, 0, st>>>(p);
+  if (p.units <= RowUnits<T>::n) {
+    if (p.units <= 4) token_logprobs_fwd_kernel<T, ROW, STEPS, 4><<<(unsigned)p.R, p.units * 64, 0, st>>>(p);              // up to 8256 classes
+    else if constexpr (RowUnits<T>::n > 4) {
+      if (p.units <= 8) token_logprobs_fwd_kernel<T, ROW, STEPS, 8><<<(unsigned)p.R, p.units * 64, 0, st>>>(p);            // up to 16448
+      else token_logprobs_fwd_kernel<T, ROW, STEPS, RowUnits<T>::n><<<(unsigned)p.R, p.units * 64, 0, st>>>(p);            // up to 32832
+    }
+    return check_launch(what);
+  }
+  token_logprobs_fwd_kernel<T, PART, STEPS><<<(unsigned)grid, 256, 0, st>>>(p);
   rc = check_launch(what);
   if (rc) return rc;
   if (p.k == 0) token_logprobs_join_kernel<T><<<(unsigned)cdiv(p.R, 4), 256, 0, st>>>(p);
-  else if (p.units <= 8) token_logprobs_top_wave_kernel<T, 8><<<(unsigned)cdiv(p.R, 4), 256, 0, st>>>(p);   // up to 16448 classes
-  else if (p.units <= 16) token_logprobs_top_wave_kernel<T, 16><<<(unsigned)cdiv(p.R, 4), 256, 0, st>>>(p);   // up to 32832
+  else if (p.units <= 16) {
+    if constexpr (RowUnits<T>::n < 16) {
+      if (p.units <= 8) token_logprobs_top_wave_kernel<T, 8><<<(unsigned)cdiv(p.R, 4), 256, 0, st>>>(p);
+      else token_logprobs_top_wave_kernel<T, 16><<<(unsigned)cdiv(p.R, 4), 256, 0, st>>>(p);
+    }
+  }
   else if (p.units <= 64) token_logprobs_top_kernel<T, 4, 16><<<p.R, 256, 0, st>>>(p);     // up to 131136
   else token_logprobs_top_kernel<T, 16, 32><<<p.R, 1024, 0, st>>>(p);                      // up to TTTS_SCORE_MAX_CLASSES
   return check_launch("token_logprobs_fwd join");
@@ -1271,7 +1330,7 @@ extern "C" int ttts_token_logprobs_bwd(const void* logits, int32_t dtype, int64_
 
 extern "C" int64_t ttts_distill_workspace_bytes(int32_t R, int32_t C) {
   const int units = C > 0 ? split_columns(C).units : 1;
-  return R > 0 && units > 1 ? (int64_t)R * units * 16 : 0;
+  return R > 0 && units > RowUnits<bf16>::n ? (int64_t)R * units * 16 : 0;
 }
 
 template <typename T>
@@ -1281,11 +1340,16 @@ static int launch_distill(const DistillParams& p, hipStream_t st) {
   int rc = need_grid(what, grid);
   if (rc) return rc;
   if (p.units == 1) {
-    if (split_columns(p.C).narrow_at <= 1024) distill_fwd_kernel<T, false, 2><<<(unsigned)grid, 256, 0, st>>>(p);
-    else distill_fwd_kernel<T, false, STEPS><<<(unsigned)grid, 256, 0, st>>>(p);
+    if (split_columns(p.C).narrow_at <= 1024) distill_fwd_kernel<T, ONE, 2><<<(unsigned)grid, 256, 0, st>>>(p);
+    else distill_fwd_kernel<T, ONE, STEPS><<<(unsigned)grid, 256, 0, st>>>(p);
     return check_launch(what);
   }
-  distill_fwd_kernel<T, true, STEPS><<<(unsigned)grid, 256, 0, st>>>(p);
+  if (p.units <= RowUnits<T>::n) {
+    if (p.units <= 4) distill_fwd_kernel<T, ROW, STEPS, 4><<<(unsigned)p.R, p.units * 64, 0, st>>>(p);
+    else if constexpr (RowUnits<T>::n > 4) distill_fwd_kernel<T, ROW, STEPS, RowUnits<T>::n><<<(unsigned)p.R, p.units * 64, 0, st>>>(p);
+    return check_launch(what);
+  }
+  distill_fwd_kernel<T, PART, STEPS><<<(unsigned)grid, 256, 0, st>>>(p);
   rc = check_launch(what);
   if (rc) return rc;
   distill_join_kernel<T><<<(unsigned)cdiv(p.R, 4), 256, 0, st>>>(p);

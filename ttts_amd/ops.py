@@ -942,9 +942,9 @@ def _grad_rows(dlogits, logits, what):
     return dlogits, ldd
 
 
-def _workspace(nbytes, device):
+def _workspace(nbytes, like):
     """Scratch of one call: allocated on the current stream (a captured call gets it from its graph's own pool)."""
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None
+    return like.new_empty(nbytes, dtype=torch.uint8)
 
 
 TokenLogprobs = collections.namedtuple("TokenLogprobs", ["logp", "entropy", "top_logp", "top_idx", "stats"])
@@ -965,15 +965,15 @@ def token_logprobs_fwd(logits, tokens, C=None, top_k=0, temperature=1.0):
         with torch.cuda.device(other):
             return token_logprobs_fwd(logits, tokens, C, top_k, temperature)
     stats = logits.new_empty(R, 2, dtype=torch.float32)          # (the others from it: the cheapest way to a tensor, and there are five)
-    r = TokenLogprobs(stats.new_empty(R), stats.new_empty(R), stats.new_empty(R, k) if k > 0 else None,
-                      tokens.new_empty(R, k) if k > 0 else None, stats)
+    logp, entropy = stats.new_empty(R), stats.new_empty(R)
+    top_logp, top_idx = (stats.new_empty(R, k), tokens.new_empty(R, k)) if k > 0 else (None, None)
     n = lib.ttts_token_logprobs_workspace_bytes(R, C, k)
-    ws = _workspace(n, logits.device)
-    rc = lib.ttts_token_logprobs_fwd(_a(logits), code, ld, _a(tokens), _a(r.logp), _a(r.entropy), _a(r.stats), _a(r.top_logp),
-                                     _a(r.top_idx), R, C, k, float(temperature), _a(ws), n, _raw_stream())
+    ws = _workspace(n, logits) if n else None
+    rc = lib.ttts_token_logprobs_fwd(logits.data_ptr(), code, ld, tokens.data_ptr(), logp.data_ptr(), entropy.data_ptr(), stats.data_ptr(),
+                                     _a(top_logp), _a(top_idx), R, C, k, float(temperature), _a(ws), n, _raw_stream())
     if rc:
         check(rc, what)
-    return r
+    return TokenLogprobs(logp, entropy, top_logp, top_idx, stats)
 
 
 def token_logprobs_bwd(logits, tokens, stats, entropy, g_logp, g_entropy=None, C=None, temperature=1.0, dlogits=None):
@@ -989,8 +989,8 @@ def token_logprobs_bwd(logits, tokens, stats, entropy, g_logp, g_entropy=None, C
         with torch.cuda.device(other):
             return token_logprobs_bwd(logits, tokens, stats, entropy, g_logp, g_entropy, C, temperature, dlogits)
     dlogits, ldd = _grad_rows(dlogits, logits, what)
-    rc = lib.ttts_token_logprobs_bwd(_a(logits), code, ld, _a(tokens), _a(stats), _a(entropy), _a(g_logp), _a(g_entropy),
-                                     _a(dlogits), ldd, R, C, logits.shape[1], float(temperature), _raw_stream())
+    rc = lib.ttts_token_logprobs_bwd(logits.data_ptr(), code, ld, tokens.data_ptr(), stats.data_ptr(), _a(entropy), _a(g_logp), _a(g_entropy),
+                                     dlogits.data_ptr(), ldd, R, C, logits.shape[1], float(temperature), _raw_stream())
     if rc:
         check(rc, what)
     return dlogits
@@ -1010,9 +1010,9 @@ def distill_fwd(logits, teacher_idx, teacher_logp, C=None, temperature=1.0, tail
             return distill_fwd(logits, teacher_idx, teacher_logp, C, temperature, tail)
     loss, stats = teacher_logp.new_empty(R), teacher_logp.new_empty(R, 3)
     n = lib.ttts_distill_workspace_bytes(R, C)
-    ws = _workspace(n, logits.device)
-    rc = lib.ttts_distill_fwd(_a(logits), code, ld, _a(teacher_idx), _a(teacher_logp), _a(loss), _a(stats), R, C, K,
-                              float(temperature), int(bool(tail)), _a(ws), n, _raw_stream())
+    ws = _workspace(n, logits) if n else None
+    rc = lib.ttts_distill_fwd(logits.data_ptr(), code, ld, teacher_idx.data_ptr(), teacher_logp.data_ptr(), loss.data_ptr(), stats.data_ptr(), R, C, K,
+                              float(temperature), bool(tail), _a(ws), n, _raw_stream())
     if rc:
         check(rc, what)
     return loss, stats
@@ -1040,8 +1040,8 @@ def distill_bwd(logits, teacher_idx, teacher_logp, stats, g_loss, C=None, temper
         with torch.cuda.device(other):
             return distill_bwd(logits, teacher_idx, teacher_logp, stats, g_loss, C, temperature, tail, dlogits, accumulate)
     dlogits, ldd = _grad_rows(dlogits, logits, what)
-    rc = lib.ttts_distill_bwd(_a(logits), code, ld, _a(teacher_idx), _a(teacher_logp), _a(stats), _a(g_loss), _a(dlogits), ldd, R, C,
-                                    logits.shape[1], K, float(temperature), int(bool(tail)), int(bool(accumulate)), _raw_stream())
+    rc = lib.ttts_distill_bwd(logits.data_ptr(), code, ld, teacher_idx.data_ptr(), teacher_logp.data_ptr(), stats.data_ptr(), g_loss.data_ptr(),
+                              dlogits.data_ptr(), ldd, R, C, logits.shape[1], K, float(temperature), bool(tail), bool(accumulate), _raw_stream())
     if rc:
         check(rc, what)
     return dlogits
@@ -1049,11 +1049,12 @@ def distill_bwd(logits, teacher_idx, teacher_logp, stats, g_loss, C=None, temper
 
 # ---- paged key / value cache (csrc/paged.hip) -----------------------------------------------------------------------------
 def _pages(k_pages, v_pages, what):
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or not (k_pages.is_contiguous() and v_pages.is_contiguous()):
+    shape, dtype = k_pages.shape, k_pages.dtype
+    if len(shape) != 4 or shape != v_pages.shape or not (k_pages.is_contiguous() and v_pages.is_contiguous()):
         raise TttsError("%s: k_pages / v_pages must be contiguous [pages, heads, page size, head_dim] tensors of one shape" % what)
-    if k_pages.dtype not in (torch.bfloat16, torch.float16) or v_pages.dtype != k_pages.dtype:
-        raise TttsError("%s: the cache must be bfloat16 or float16, got %s / %s" % (what, k_pages.dtype, v_pages.dtype))
-    return _DTYPE_CODES[k_pages.dtype]
+    if (dtype is not torch.bfloat16 and dtype is not torch.float16) or v_pages.dtype is not dtype:
+        raise TttsError("%s: the cache must be bfloat16 or float16, got %s / %s" % (what, dtype, v_pages.dtype))
+    return _DTYPE_CODES[dtype], dtype, shape
 
 
 def _heads(t, dtype, shape, what, name):
@@ -1071,18 +1072,17 @@ def kv_page_write(k, v, k_pages, v_pages, slots):
     size, head_dim], bf16 or fp16.  slots int64 [N]; one outside the cache (-1: a padding row) writes nothing.  The slots of a call
     differ from each other, and k / v share no memory with the pages."""
     what, lib = "kv_page_write", _l.get()
-    code = _pages(k_pages, v_pages, what)
-    P, H, page, dh = k_pages.shape
+    code, dtype, (P, H, page, dh) = _pages(k_pages, v_pages, what)
     N = slots.shape[0] if slots.dim() == 1 else -1
     _vec(slots, torch.int64, (N,), what, "slots")
-    ksn, ksh = _heads(k, k_pages.dtype, (N, H, dh), what, "k")
-    vsn, vsh = _heads(v, k_pages.dtype, (N, H, dh), what, "v")
+    ksn, ksh = _heads(k, dtype, (N, H, dh), what, "k")
+    vsn, vsh = _heads(v, dtype, (N, H, dh), what, "v")
     other = _on(what, k, v, k_pages, v_pages, slots)
     if other is not None:
         with torch.cuda.device(other):
             return kv_page_write(k, v, k_pages, v_pages, slots)
-    rc = lib.ttts_kv_page_write(_a(k), _a(v), ksn, ksh, vsn, vsh, _a(k_pages), _a(v_pages),
-                                      _a(slots), code, N, H, dh, page, P, _raw_stream())
+    rc = lib.ttts_kv_page_write(k.data_ptr(), v.data_ptr(), ksn, ksh, vsn, vsh, k_pages.data_ptr(), v_pages.data_ptr(),
+                                slots.data_ptr(), code, N, H, dh, page, P, _raw_stream())
     if rc:
         check(rc, what)
 
@@ -1093,12 +1093,11 @@ def attn_paged_decode(q, k_pages, v_pages, block_table, seq_lens, scale, out=Non
     keys, the new token's among them.  Returns (out [M, H, head_dim] of q's type, lse f32 [M, H]).  A sequence without keys gets 0 and
     -inf; keys of a table entry outside the cache are left out.  A slice block_table[:, :n] bounds the lengths to n pages."""
     what, lib = "attn_paged_decode", _l.get()
-    code = _pages(k_pages, v_pages, what)
-    P, Hkv, page, dh = k_pages.shape
+    code, dtype, (P, Hkv, page, dh) = _pages(k_pages, v_pages, what)
     if q.dim() != 3 or block_table.dim() != 2 or block_table.dtype != torch.int32:
         raise TttsError("%s: q must be [M, H, head_dim], block_table int32 [M, width]" % what)
-    M, H = q.shape[:2]
-    qsm, qsh = _heads(q, k_pages.dtype, (M, H, dh), what, "q")
+    M, H, _ = q.shape
+    qsm, qsh = _heads(q, dtype, (M, H, dh), what, "q")
     _vec(seq_lens, torch.int32, (M,), what, "seq_lens")
     ts, tm, width = _rows(block_table, what, "block_table")
     if tm != M:
@@ -1109,14 +1108,16 @@ def attn_paged_decode(q, k_pages, v_pages, block_table, seq_lens, scale, out=Non
             return attn_paged_decode(q, k_pages, v_pages, block_table, seq_lens, scale, out)
     if out is None:
         out = q.new_empty(M, H, dh)
-    osm, osh = _heads(out, q.dtype, (M, H, dh), what, "out")
-    if (H > 1 and osh < dh) or (M > 1 and osm < dh) or (H > 1 and M > 1 and max(osm, osh) < min(osm, osh) * ((M if osm < osh else H) - 1) + dh):
-        raise TttsError("%s: rows of out overlap (strides %s)" % (what, out.stride()))
+        osm, osh = H * dh, dh
+    else:
+        osm, osh = _heads(out, dtype, (M, H, dh), what, "out")
+        if (H > 1 and osh < dh) or (M > 1 and osm < dh) or (H > 1 and M > 1 and max(osm, osh) < min(osm, osh) * ((M if osm < osh else H) - 1) + dh):
+            raise TttsError("%s: rows of out overlap (strides %s)" % (what, out.stride()))
     lse = q.new_empty(M, H, dtype=torch.float32)
     n = lib.ttts_attn_paged_decode_workspace_bytes(M, H, Hkv, dh, page, width)
-    ws = _workspace(n, q.device)
-    rc = lib.ttts_attn_paged_decode(_a(q), qsm, qsh, _a(k_pages), _a(v_pages), _a(block_table), ts, _a(seq_lens),
-                                    _a(out), osm, osh, _a(lse), code, M, H, Hkv, dh, page, P, width,
+    ws = _workspace(n, q) if n else None
+    rc = lib.ttts_attn_paged_decode(q.data_ptr(), qsm, qsh, k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), ts, seq_lens.data_ptr(),
+                                    out.data_ptr(), osm, osh, lse.data_ptr(), code, M, H, Hkv, dh, page, P, width,
                                     float(scale), _a(ws), n, _raw_stream())
     if rc:
         check(rc, what)

@@ -910,7 +910,7 @@ __device__ __forceinline__ void list_weights(Listed& L, const ListLoads& r, int 
       L.logp[h] = (t[h] - m) * inv_t;
       L.p[h] = L.id[h] >= 0 ? __expf(L.logp[h]) : 0.f;
     }
-  const float z = sum_wave(L.p[0] + L.p[1]), over = 1.f / z, logz = __logf(z);
+  const float z = sum_wave(L.p[0] + L.p[1]), over = __builtin_amdgcn_rcpf(z), logz = __builtin_amdgcn_logf(z) * LN2;   // (one step each; z is at least 1)
 #pragma unroll
   for (int h = 0; h < 2; ++h)
     if (h * 64 < K) {
@@ -932,7 +932,7 @@ struct DistillParams {
 // by one wave: the row's loss from its sums (listed and other classes apart with tail, else all in zr) and the listed classes' logits
 __device__ __forceinline__ void finish_distill(const DistillParams& p, int64_t row, const Listed& L, float x0, float x1, float m, float zl, float zr,
                                                int lane) {
-  const float z = zl + zr, logz = __logf(z);
+  const float z = zl + zr, logz = __builtin_amdgcn_logf(z) * LN2;
   float loss = 0.f;
 #pragma unroll
   for (int h = 0; h < 2; ++h)

@@ -480,8 +480,8 @@ int ttts_distill_bwd(const void* logits, int32_t dtype, int64_t ldl, const int64
  *    int32 [M, width] (row pitch table_stride): pages of sequence m in order; seq_lens int32 [M]: its keys, the new token's among
  *    them (write it first).  out [M, H, head_dim] = softmax(scale q K^T) V over keys 0 .. seq_lens[m] - 1, lse f32 [M, H] =
  *    log sum exp(scaled scores).  A length beyond width * page ends there; keys of a table entry outside [0, P) are left out;
- *    without keys (length <= 0) out is 0 and lse -inf.  fp32 softmax and sums; the weights are rounded to the cache's type (fp16: as
- *    2^15 times themselves) for the product with V.  workspace: ttts_attn_paged_decode_workspace_bytes (16-byte aligned), the call's own until it has run. */
+ *    without keys (length <= 0) out is 0 and lse -inf.  fp32 softmax and sums; a weight enters the product with V as the sum of two
+ *    numbers of the cache's type (fp16: of 2^15 times itself), so that only the result is rounded to it.  workspace: ttts_attn_paged_decode_workspace_bytes (16-byte aligned), the call's own until it has run. */
 int ttts_kv_page_write(const void* k, const void* v, int64_t k_stride_n, int64_t k_stride_h, int64_t v_stride_n,
                        int64_t v_stride_h, void* k_pages, void* v_pages, const int64_t* slots, int32_t dtype, int32_t N,
                        int32_t Hkv, int32_t head_dim, int32_t page, int32_t P, void* stream);

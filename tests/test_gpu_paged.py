@@ -362,3 +362,62 @@ def test_attn_paged_decode_out_must_not_overlap():
     across = torch.zeros(4, 2, 40, dtype=torch.bfloat16).cuda()[..., :32].transpose(0, 1)   # heads first in memory, with a pitch
     got, _ = ops.attn_paged_decode(*args, out=across)
     assert got is across and torch.equal(across, want)
+
+
+def _vectorised(q, kp, vp, table, lens, scale):
+    """(out, sum p |v|, lse, size of the scores' error) in 64 bits on the GPU, one sequence and cached head at a time."""
+    M, H, dh = q.shape
+    Hkv, page = kp.shape[1], kp.shape[2]
+    group = H // Hkv
+    out, mag = torch.zeros(2, M, H, dh, dtype=torch.float64, device="cuda")
+    S = torch.zeros(M, H, dtype=torch.float64, device="cuda")
+    for m, n in enumerate(lens):
+        ids = table[m, :-(-n // page)].long().cuda()
+        for h in range(Hkv if n else 0):
+            k, v = (t[ids, h].reshape(-1, dh)[:n].double() for t in (kp, vp))
+            heads = slice(h * group, (h + 1) * group)
+            qs = q[m, heads].double()
+            w = torch.softmax(qs @ k.t() * scale, dim=1)
+            out[m, heads], mag[m, heads] = w @ v, w @ v.abs()
+            S[m, heads] = (qs.abs() @ k.abs().t()).amax(dim=1) * abs(scale) * (dh + 8) * U
+    return out, mag, S
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dh,Hkv,group,page,lens", [
+    (64, 8, 1, 16, [613]), (64, 2, 3, 16, [2404, 0, 17, 900, 1]), (128, 2, 8, 64, [9001, 300]), (32, 1, 20, 32, [1500, 31]),
+    (64, 4, 4, 16, list(range(2, 34))),
+    (128, 8, 5, 32, [40 + 29 * i for i in range(70)])])
+def test_attn_paged_decode_weights_are_not_rounded_to_the_cache_type(dtype, dh, Hkv, group, page, lens):
+    """A weight enters the product with V in two parts of the cache's type, so the result has one rounding to that type, its own.  The first
+    part is at most three half steps below the weight (3 e of it), the second off by e of that: 3 e^2 of the weight, doubled here."""
+    from ttts_amd import ops
+    table, P, _ = _tables(lens, page, 11)
+    kp, vp = _cache(P, Hkv, page, dh, dtype, 12)
+    q = (torch.randn(len(lens), Hkv * group, dh, generator=_gen(13)) * 1.5).to(dtype).cuda()
+    scale = dh ** -0.5
+    got, _ = ops.attn_paged_decode(q, kp, vp, table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), scale)
+    out, mag, S = _vectorised(q, kp, vp, table, lens, scale)
+    e = torch.finfo(dtype).eps / 2
+    r = (max(lens) / 64 + 32) * U
+    inner = (6 * e * e + 4 * (S[..., None] + r)) * mag + torch.finfo(dtype).tiny
+    off = (got.double() - out).abs() - e * (out.abs() + inner) - inner
+    assert off.max().item() <= 0, off.max().item()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_attn_paged_decode_infinite_values(dtype):
+    """A value of +inf among the keys of a sequence makes its column inf, as the definition does; the other columns stay."""
+    from ttts_amd import ops
+    lens = [1, 40, 900]
+    table, P, _ = _tables(lens, 16, 14)
+    kp, vp = _cache(P, 1, 16, 64, dtype, 15)
+    for m in range(3):
+        vp[int(table[m, 0]), 0, 0, 5 + m] = math.inf
+    q = torch.randn(3, 2, 64, generator=_gen(16)).to(dtype).cuda() * 0.5
+    got, _ = ops.attn_paged_decode(q, kp, vp, table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), 0.125)
+    for m in range(3):
+        assert (got[m, :, 5 + m] == math.inf).all(), m
+    others = torch.ones(3, 64, dtype=torch.bool)
+    others[torch.arange(3), torch.arange(3) + 5] = False
+    assert torch.isfinite(got.cpu()[others[:, None].expand(3, 2, 64)]).all()

@@ -69,15 +69,29 @@ __device__ __forceinline__ int ordered_sequence(const int32_t* lens, int M, int 
   return 0;   // (not reached: every sequence has a level)
 }
 
+// A weight e in [0, 1] enters the product with V as two numbers of the cache's type, hi + lo = weight e: with hi alone, rounded, the outputs' error
+// was 17 % larger in bf16 (0.0019 of their size against 0.0016) than their own rounding makes it.  hi lies half a step to one and a
+// half below the weight, so lo is above zero wherever hi is: an infinite value stays infinite.
 template <typename T> struct Frag;
 template <> struct Frag<bf16> {
   static constexpr float weight = 1.f;
   static __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ void split(float e, bf16& hi, bf16& lo) {
+    const uint32_t h = __builtin_elementwise_sub_sat(__builtin_bit_cast(uint32_t, e), 0x8000u) & 0xffff0000u;
+    hi = __builtin_bit_cast(bf16, (uint16_t)(h >> 16));
+    lo = (bf16)(e - __builtin_bit_cast(float, h));
+  }
 };
 template <> struct Frag<_Float16> {
   static constexpr float weight = 32768.f;   // a weight of one enters the product as this: fp16 then holds them down to 2^-39 of the
-                                             // largest, 2^-29 in full (thousands of keys 2^-25 below it are part of the result)
+                                             // largest (thousands of keys 2^-25 below it are part of the result)
   static __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ void split(float e, _Float16& hi, _Float16& lo) {
+    e *= weight;
+    const float below = __builtin_bit_cast(float, __builtin_elementwise_sub_sat(__builtin_bit_cast(uint32_t, e), 0x1000u));
+    hi = (_Float16)__builtin_amdgcn_cvt_pkrtz(below, below)[0];   // (towards zero)
+    lo = (_Float16)(e - (float)hi);
+  }
 };
 // One workgroup = one chunk of keys of one (sequence, key / value head, 16 query rows); its waves take the chunk's 32-key tiles in turn,
 // each with a running maximum, sum and accumulator of its own, joined through LDS at the end.
@@ -185,19 +199,23 @@ __global__ __launch_bounds__(NW * 64) void attn_paged_decode_kernel(PagedParams 
         for (int r = 0; r < W; ++r) acc[r] *= a;
         mx = mn;
       }
-      T8 pf;                       // the weights enter the product in the cache's type; their sum is of the unrounded ones
+      T8 hi, lo;                   // the weights in two parts of the cache's type; their sum is of the weights themselves
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float e = __builtin_amdgcn_exp2f(s[j] - mx);
         l += e;
-        pf[j] = (T)(e * Frag<T>::weight);
+        T a, b;
+        Frag<T>::split(e, a, b);
+        hi[j] = a;
+        lo[j] = b;
       }
 #pragma unroll
       for (int r = 0; r < W; ++r) {
         T8 a;
 #pragma unroll
         for (int j = 0; j < 8; ++j) a[j] = vf[j][r];
-        acc[r] = Frag<T>::mfma(a, pf, acc[r]);
+        acc[r] = Frag<T>::mfma(a, lo, acc[r]);
+        acc[r] = Frag<T>::mfma(a, hi, acc[r]);
       }
       if (more) load_v(next);
       cur = next;

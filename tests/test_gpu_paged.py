@@ -421,3 +421,44 @@ def test_attn_paged_decode_infinite_values(dtype):
     others = torch.ones(3, 64, dtype=torch.bool)
     others[torch.arange(3), torch.arange(3) + 5] = False
     assert torch.isfinite(got.cpu()[others[:, None].expand(3, 2, 64)]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Hkv", [1, 7])
+def test_attn_paged_decode_longest_sequences(dtype, Hkv):
+    """More than 2048 * 4096 keys, by a table that repeats a few pages: about 2000 parts, as many as there may be.  The last page
+    is its own, and two keys of it hold a good part of the first queries' weight."""
+    from ttts_amd import ops
+    page, dh, pool = 1024, 32, 24
+    width = 2048 * 4096 // page + 300
+    g = _gen(Hkv)
+    kp, vp = _cache(pool + 1, Hkv, page, dh, dtype, 21)
+    table = torch.randint(0, pool, (1, width), generator=g, dtype=torch.int32)
+    n = width * page - 100
+    table[0, -1] = pool
+    q = torch.randn(1, 2 * Hkv, dh, generator=g).to(dtype).cuda()
+    scale = dh ** -0.5
+    times = torch.bincount(table[0, :-1].long(), minlength=pool).double().cuda()
+    vp[pool, :, :page - 100] = 3.0
+    for key in (0, page - 101):
+        kp[pool, :, key] = 0.0
+        for h in range(Hkv):       # a key along each head's first query: its score is log(keys) and a little
+            a = q[0, 2 * h].float()
+            kp[pool, h, key] = (a * (15.6 / scale / (a @ a))).to(dtype)
+    got, lse = ops.attn_paged_decode(q, kp, vp, table.cuda(), torch.tensor([n], dtype=torch.int32).cuda(), scale)
+    e = torch.finfo(dtype).eps / 2
+    r = (32 * 8 + 2048 / 8 + 32) * U          # a lane's share of a part, a thread's share of the parts, and the rest
+    for h in range(2 * Hkv):
+        k, v = kp[:, h // 2].double(), vp[:, h // 2].double()
+        z = k @ q[0, h].double() * scale
+        z[pool, page - 100:] = -math.inf
+        w = torch.exp(z - z.max()) * torch.cat([times, times.new_ones(1)])[:, None]
+        L = w.sum()
+        ref, mag = ((w / L)[..., None] * v).sum(dim=(0, 1)), ((w / L)[..., None] * v.abs()).sum(dim=(0, 1))
+        S = (k.abs() @ q[0, h].double().abs()).max() * scale * (dh + 8) * U
+        bound = e * ref.abs() + (1 + e) * (6 * e * e + 4 * (S + r)) * mag + torch.finfo(dtype).tiny
+        assert ((got[0, h].double() - ref).abs() <= bound).all(), h
+        want = z.max() + L.log()
+        assert (lse[0, h].double() - want).abs() <= 2 * S + r + 4 * U * want.abs(), h
+        if h % 2 == 0:
+            assert 0.1 < (w[pool].sum() / L).item()

@@ -133,3 +133,14 @@ def test_more_than_one_launch_holds(lib):
     _refused(lib, "ttts_distill_bwd", DBWD, "one launch", R=big)
     _refused(lib, "ttts_kv_page_write", WRITE, "one launch", N=big, H=64, ksn=4096, vsn=4096)
     _refused(lib, "ttts_attn_paged_decode", ATT, "one launch", M=big, width=4)
+
+
+@pytest.mark.parametrize("units", range(1, 10))
+def test_a_split_sequence_has_no_more_parts_than_its_join_holds(lib, units):
+    """The parts of the longest tables (2^30 keys), read off the workspace: the join keeps the weights of 2048 of them."""
+    for M, Hkv in {(units, 1), (1, units)}:
+        for log_page in (4, 7, 10):
+            for keys in [1 << n for n in range(12, 31)] + [2048 * 4096 + 1024, 5 * 10 ** 7, 10 ** 9]:
+                width = keys >> log_page
+                n = lib.ttts_attn_paged_decode_workspace_bytes(M, Hkv, Hkv, 32, 1 << log_page, width)
+                assert n // (M * Hkv * (32 + 2) * 4) <= 2048, (M, Hkv, keys)

@@ -260,7 +260,7 @@ __global__ __launch_bounds__(NW * 64) void attn_paged_decode_kernel(PagedParams 
 // The chunks of a split sequence: one workgroup per (sequence, query head).  Every chunk's weight 2^(m - M), a chunk per thread, and DH / 4
 // lanes per chunk that add up the weighted parts; the first 8 parts of a thread are on their way before the weights (and the
 // length) are known, so it takes one round of loads up to 8 * 1024 / DH chunks.
-constexpr int PAGED_MAX_CHUNKS = 2048;
+constexpr int PAGED_MAX_CHUNKS = 2048;   // whose weights a workgroup holds; paged_split makes no more
 template <typename T, int DH>
 __global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedParams p) {
   constexpr int LPC = DH / 4, G = 256 / LPC, AHEAD = 8;
@@ -324,6 +324,7 @@ __global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedParams p) {
 //  * beyond that into 1024 keys or more, about 1024 workgroups (4 sequences of 130000 keys: 178 us, 188 with 2048), or about 2048
 //    where a sequence gets few chunks, and chunks of at most 4096 keys while there are under 16384 of them: the lengths may be
 //    anything up to the longest, and a workgroup's chunk is what the others wait for.
+// No sequence gets more than PAGED_MAX_CHUNKS, the join's room (fewer than 8 units with tables of more than 8388608 keys would).
 struct PagedSplit { int chunk, chunks, waves; };
 static PagedSplit paged_split(int64_t units, int64_t longest) {
   auto least = [](int64_t a, int64_t b) { return a < b ? a : b; };
@@ -335,7 +336,7 @@ static PagedSplit paged_split(int64_t units, int64_t longest) {
     int64_t wide = cdiv(1024, units);
     if (wide < 8) wide = cdiv(2048, units);
     n = most(least(cdiv(longest, 1024), wide), least(cdiv(longest, 256), 256 / units));
-    n = most(n, least(cdiv(longest, 4096), 16384 / units));
+    n = least(most(n, least(cdiv(longest, 4096), 16384 / units)), PAGED_MAX_CHUNKS);
   }
   s.waves = many && n == 1 ? 4 : 8;
   const int64_t c = cdiv(cdiv(longest, n), 32 * s.waves) * 32 * s.waves;
@@ -424,6 +425,7 @@ extern "C" int ttts_attn_paged_decode(const void* q, int64_t q_stride_m, int64_t
   const int64_t units = M * (int64_t)Hkv * p.tiles;
   const PagedSplit sp = paged_split(units, (int64_t)width * page);
   p.chunk = sp.chunk; p.chunks = sp.chunks;
+  TTTS_REQUIRE(p.chunks <= PAGED_MAX_CHUNKS, "attn_paged_decode: %d parts of a sequence, more than the join holds", p.chunks);
   p.ordered = units >= 512 && M <= PAGED_ORDERED;
   const int64_t grid = units * p.chunks, rows = (int64_t)M * H, need = paged_bytes(M, H, head_dim, p.chunks);
   TTTS_REQUIRE(one_launch(grid, sp.waves * 64) && one_launch(rows, 256), "attn_paged_decode: more work than one launch holds (M %d, H %d)", M, H);

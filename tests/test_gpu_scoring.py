@@ -496,3 +496,19 @@ def test_refusals_on_the_gpu():
         with pytest.raises(TttsError):
             f()
             pytest.fail("refusal %d did not come" % n)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("C", [40, 1026, 8200, 40000])
+def test_distill_rows_with_nan_and_no_entries(C, dtype):
+    """With the mass that the list leaves out, a row without entries compares all of it: NaN or +inf among its classes shows in its loss."""
+    from ttts_amd import ops
+    x = _logits(4, C, C, dtype, 5)
+    x[1, C // 2], x[2, C - 1] = math.nan, math.inf
+    idx, t = torch.full((4, 3), -1).cuda(), torch.zeros(4, 3).cuda()
+    loss, stats = ops.distill_fwd(x, idx, t, tail=True)
+    d = ops.distill_bwd(x, idx, t, stats, torch.ones(4, device="cuda"), tail=True)
+    for r in (1, 2):
+        assert torch.isnan(loss[r]) and torch.isnan(d[r]).any(), r
+    for r in (0, 3):                                      # the whole mass on all classes: log 1 - log 1
+        assert loss[r].abs().item() <= 4 * U and d[r].float().abs().max().item() <= 4 * _r(C), r

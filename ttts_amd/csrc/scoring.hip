@@ -941,7 +941,7 @@ __device__ __forceinline__ void finish_distill(const DistillParams& p, int64_t r
   if (lane == 0) {
     const float left = 1.f - L.mass;
     // log of the student's rest = -log(1 + listed / others): the difference of two log-sums would lose it where little is listed
-    if (p.tail && left > 0.f && zr > 0.f) loss += left * (log1pf(-L.mass) + log1pf(zl / zr));
+    if (p.tail && left > 0.f && zr != 0.f) loss += left * (log1pf(-L.mass) + log1pf(zl / zr));
     const bool none = z == 0.f;
     p.row_loss[row] = none ? 0.f : loss;
     p.stats[3 * row] = none ? -INFINITY : m;

@@ -458,7 +458,10 @@ int ttts_token_logprobs_bwd(const void* logits, int32_t dtype, int64_t ldl, cons
  *           left = max(0, 1 - sum p);  row_loss += left (log left - log q_rest), q_rest = the student's mass on the classes that
  *           the list does not name (summed as such, not as 1 - the rest).  Without such a class the term is left out.
  *   A class named twice counts with both of its p.  A row without entries has loss 0 with tail 0; a row whose student classes are
- *   all -inf has loss 0 and no gradient.  stats f32 [R, 3] for the backward: (max, log Z, Z of the named classes over Z of the others).
+ *   all -inf has loss 0 and no gradient.  stats f32 [R, 3] for the backward: (max, log Z, Z of the named classes over Z of the others);
+ *   with tail 1, where the named classes lie more than 32 bits above the others, (the others' max, -2 - log of their Z, log-sum-exp of the
+ *   named classes in the logits' unit), the second below -1.  Maximum and sum of the others are their own, so the term keeps its value
+ *   and its gradient however far below the named classes they lie.
  * bwd: dlogits = g_loss[r] d row_loss / d logits:  g / temperature [q (sum p + left) - p - left q / q_rest (classes not named)];
  *   written over Cd columns as above, or with accumulate 1 added to what is there (columns 0 .. C - 1, one rounding of the sum). */
 int64_t ttts_distill_workspace_bytes(int32_t R, int32_t C);

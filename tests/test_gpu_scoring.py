@@ -512,3 +512,110 @@ def test_distill_rows_with_nan_and_no_entries(C, dtype):
         assert torch.isnan(loss[r]) and torch.isnan(d[r]).any(), r
     for r in (0, 3):                                      # the whole mass on all classes: log 1 - log 1
         assert loss[r].abs().item() <= 4 * U and d[r].float().abs().max().item() <= 4 * _r(C), r
+
+
+GAPS = [20.0, 23.0, 60.0, 80.0, 87.0, 90.0, 105.0, 200.0, 1000.0, -90.0, -1000.0]
+
+
+def _apart(x, idx, C, T, dtype):
+    """Rows of x changed in place so that the named classes lie by GAPS (in logits / T) above the others, and then: a finite mask over the others, the
+    lowest value over the others, over all but one of them, and over all but a few others of which some are at -inf."""
+    n = len(GAPS)
+    for r in range(len(x)):
+        named = idx[r][(idx[r] >= 0) & (idx[r] < C)].unique()
+        rest = torch.ones(C, dtype=torch.bool)
+        rest[named] = False
+        if not rest.any():
+            continue
+        if r < n:
+            x[r, :C] = (x[r, :C].float() / 6 * min(T, 1.0)).to(dtype)
+            x[r, named] = (x[r, named].float() + GAPS[r] * T).to(dtype)
+        else:
+            x[r, :C][rest.cuda()] = -1e4 if r == n else LOWEST[dtype]
+            if r == n + 2:
+                x[r, int(rest.nonzero()[0])] = 1.0
+            if r == n + 3:
+                x[r, int(rest.nonzero()[-1])] = -math.inf
+                x[r, int(rest.nonzero()[len(rest.nonzero()) // 2])] = -math.inf
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("C,offset", [(9, 0), (1026, 0), (2000, 1), (2049, 0), (8195, 1), (20000, 0), (40001, 0)])
+@pytest.mark.parametrize("K,T", [(1, 1.0), (5, 0.1), (64, 1.0), (100, 2.0)])
+def test_distill_where_named_and_other_classes_lie_far_apart(C, offset, dtype, K, T):
+    """The mass that the list leaves out is compared with the other classes' however far they lie below the named ones (or above): their
+    maximum and sum are their own.  The named classes' log-sum-exp b is one fp32 number where they lie far above: their share is off
+    by the rounding of b / T."""
+    from ttts_amd import ops
+    R = len(GAPS) + 4
+    x = _logits(R, C, C + offset, dtype, C + K, offset)
+    idx, t = _teacher(R, C, K, T, True, C + 3 * K, empty=0.1 if K > 1 else 0.0, repeat=K > 4)
+    if K == 1:
+        t = torch.log(torch.linspace(0.05, 0.95, R)).view(R, 1)
+    _apart(x, idx, C, T, dtype)
+    g = torch.randn(R, generator=_gen(9))
+    loss, stats = ops.distill_fwd(x, idx.cuda(), t.cuda(), C=C, temperature=T, tail=True)
+    d = ops.distill_bwd(x, idx.cuda(), t.cuda(), stats, g.cuda(), C=C, temperature=T, tail=True)
+    there = (idx >= 0) & (idx < C)
+    at = idx.clamp(0, C - 1)
+    z = x[:, :C].double().cpu() / T
+    named = torch.zeros(R, C, dtype=torch.float64).scatter_add_(1, at, there.double()) > 0
+    lp = torch.where(there, t, 0.0).double()
+    p = torch.where(there, lp.exp(), 0.0)
+    mass = p.sum(dim=1)
+    left = (1 - mass).clamp(min=0)
+    zr = z.masked_fill(named, -math.inf)
+    top = z.amax(dim=1, keepdim=True)
+    logz = (z - top).exp().sum(dim=1, keepdim=True).log()
+    held = (zr > -math.inf).any(dim=1) & (left > 0)
+    left = torch.where(held, left, 0.0)
+    top_r = zr.amax(dim=1, keepdim=True).clamp(min=-1e300)
+    logz_r = (zr - top_r).exp().sum(dim=1, keepdim=True).log()
+    y = z - top - logz
+    log_r = torch.where(zr > -math.inf, zr - top_r - logz_r, -math.inf)
+    rest = torch.where(held, (top_r - top + logz_r - logz)[:, 0], 0.0)      # log of the student's share of the others
+    terms = torch.where(p > 0, p * (lp - y.gather(1, at)), 0.0)
+    safe = torch.where(held, left, 1.0)
+    ref = terms.sum(dim=1) + left * (safe.log() - rest)
+    logs = torch.where(p > 0, p * (lp.abs() + y.gather(1, at).abs()), 0.0).sum(dim=1)
+    l_off = (K / 2 + 8) * U * (1 + mass)
+    bound = (_r(C) + 16 * U) * (mass + logs + left * (1 + rest.abs())) + (K + 8) * U * logs + l_off * (safe.log().abs() + rest.abs() + 1) + 8 * U
+    _inside(loss, ref.float().double(), bound, "row_loss")
+    q, r = y.exp(), log_r.exp()
+    target = torch.zeros(R, C, dtype=torch.float64).scatter_add_(1, at, p)
+    grad = (q * (mass + left)[:, None] - target - left[:, None] * r) * (g.double() / T)[:, None]
+    # exponents: of a named class |log q| and, far above the others, b / T (rounded once, and once more taken off); of another |log r| and the
+    # distance that still counts as near (32 bits: 22.2)
+    b = z.masked_fill(~named, -math.inf).amax(dim=1, keepdim=True).clamp(min=-1e300).abs() + 8
+    far = ((top - top_r) > 22)
+    span = torch.where(named, y.abs() + torch.where(far, b, 0.0), torch.minimum(log_r.abs() + 23, y.abs() + 23)).nan_to_num(posinf=0.0)
+    size = q * (mass + left)[:, None] + target + left[:, None] * r
+    err = (l_off * held)[:, None] * (q + r)
+    gb = g.double().abs()[:, None] / T
+    bound = gb * (size * (4 * _r(C) + (K + 16) * U + 8 * U * (span + 1)) + 2 * err) + _half_step(grad, dtype) + 1e-37
+    _inside(d[:, :C], grad, bound, "dlogits")
+    base = torch.randn(x.shape, generator=_gen(4)).to(dtype).cuda()
+    acc = ops.distill_bwd(x, idx.cuda(), t.cuda(), stats, g.cuda(), C=C, temperature=T, tail=True, dlogits=base.clone(), accumulate=True)
+    want = base[:, :C].double().cpu() + grad
+    _inside(acc[:, :C], want, bound + _half_step(want, dtype) + 2 * U * want.abs(), "accumulated dlogits")
+    assert ops.distill_bwd(x, idx.cuda(), t.cuda(), stats, g.cuda(), C=C, temperature=T, tail=True, dlogits=x) is x and torch.equal(x[:, :C], d[:, :C])
+
+
+@pytest.mark.parametrize("gap", [30.0, 100.0, 500.0])
+def test_distill_gradient_far_apart_agrees_with_differences(gap):
+    """As test_gradients_agree_with_differences, the named classes `gap` above the others: the forward's error grows with the loss, left * gap."""
+    from ttts_amd import ops
+    R, C, h, K = 6, 1500, 2.0 ** -5, 8
+    x = _logits(R, C, C, torch.float32, 22, std=1.0)
+    idx, t = _teacher(R, C, K, 1.0, True, 6, empty=0.0)
+    for r in range(R):
+        x[r, idx[r]] += gap
+    v = torch.rand(R, C, generator=_gen(3)).cuda() * 2 - 1
+    idx, t = idx.cuda(), t.cuda()
+    f = lambda z: ops.distill_fwd(z, idx, t, tail=True)[0].double()  # noqa: E731
+    _, stats = ops.distill_fwd(x, idx, t, tail=True)
+    d = ops.distill_bwd(x, idx, t, stats, torch.ones(R, device="cuda"), tail=True)
+    num = (f(x + h * v) - f(x - h * v)) / (2 * h)
+    B = (_r(C) + (K + 24) * U) * (gap + 12)
+    # x +- h v are rounded: each class by U (gap + 8), which moves the loss by at most that much twice over
+    assert ((d.double() * v.double()).sum(dim=1) - num).abs().max().item() <= (B + 2 * U * (gap + 8)) / h + h * h / 6 * 12

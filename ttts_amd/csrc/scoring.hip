@@ -925,28 +925,51 @@ struct DistillParams {
   const int64_t* idx;
   const float* tlogp;
   float *row_loss, *stats;
-  float4* part;        // long rows: [R, units] (m, z of the listed classes, z of the others, -) of each wave's columns
+  float4* part;        // long rows: [R, units] DistillSums of each wave's columns
   int R, C, K, tail, units, unit_cols;
   float inv_t;
 };
-// by one wave: the row's loss from its sums (listed and other classes apart with tail, else all in zr) and the listed classes' logits
-__device__ __forceinline__ void finish_distill(const DistillParams& p, int64_t row, const Listed& L, float x0, float x1, float m, float zl, float zr,
+// Maximum and sum of e^((x - maximum) / T) of the classes that the list names and of the others (without tail: all are others), each of its own: with
+// the row's maximum for both, others 87 nats below a named class had the sum 0 and were as good as not there.
+// None: -FMAX and 0; whatever there is has a sum of at least about 1.
+struct DistillSums { float ml, zl, mr, zr; };
+// Statistics of the tail form, [m, n, w] a row: (max, log Z, Z of the named classes over Z of the others), infinite w where there are no others.
+// Where the named classes lie more than FAR bits above the others, every class but them would be lost in the first two: then (max of the
+// others, FAR_MARK - log of their Z, log-sum-exp of the named classes in the logits' unit), known by n < -1 (log Z is at least 0).
+constexpr float FAR = 32.f, FAR_MARK = -2.f;
+// by one wave: the row's loss from its sums and the listed classes' logits
+__device__ __forceinline__ void finish_distill(const DistillParams& p, int64_t row, const Listed& L, float x0, float x1, const DistillSums& a,
                                                int lane) {
-  const float z = zl + zr, logz = __builtin_amdgcn_logf(z) * LN2;
+  const float c = p.inv_t * LOG2E, m = fmaxf(a.ml, a.mr);
+  float z = a.zr;
+  if (p.tail) z = fmaf(a.zl, __builtin_amdgcn_exp2f((a.ml - m) * c), a.zr * __builtin_amdgcn_exp2f((a.mr - m) * c));
+  const float logz = __builtin_amdgcn_logf(z) * LN2;
   float loss = 0.f;
 #pragma unroll
   for (int h = 0; h < 2; ++h)
     if (h * 64 < p.K && L.p[h] != 0.f) loss += L.p[h] * (L.logp[h] - (((h ? x1 : x0) - m) * p.inv_t - logz));
   loss = sum_wave(loss);
   if (lane == 0) {
-    const float left = 1.f - L.mass;
-    // log of the student's rest = -log(1 + listed / others): the difference of two log-sums would lose it where little is listed
-    if (p.tail && left > 0.f && zr != 0.f) loss += left * (log1pf(-L.mass) + log1pf(zl / zr));
     const bool none = z == 0.f;
+    float s0 = m, s1 = logz, s2 = 0.f;
+    if (p.tail) {
+      const float left = 1.f - L.mass, gap = (a.ml - a.mr) * c;
+      const bool far = gap > FAR && a.zr != 0.f;
+      const float ratio = a.zl / a.zr * __builtin_amdgcn_exp2f(fminf(gap, FAR));
+      // log of the student's rest = -log(1 + listed / others): the difference of two log-sums would lose it where little is listed
+      if (left > 0.f && a.zr != 0.f)
+        loss += left * (log1pf(-L.mass) + (far ? (a.ml - a.mr) * p.inv_t + __builtin_amdgcn_logf(a.zl / a.zr) * LN2 : log1pf(ratio)));
+      s2 = a.zr == 0.f ? INFINITY : ratio;
+      if (far && z == z) {
+        s0 = a.mr;
+        s1 = FAR_MARK - __builtin_amdgcn_logf(a.zr) * LN2;
+        s2 = a.ml + __builtin_amdgcn_logf(a.zl) * LN2 / p.inv_t;
+      }
+    }
     p.row_loss[row] = none ? 0.f : loss;
-    p.stats[3 * row] = none ? -INFINITY : m;
-    p.stats[3 * row + 1] = none ? -INFINITY : logz;
-    p.stats[3 * row + 2] = none || !p.tail ? 0.f : zl / zr;
+    p.stats[3 * row] = none ? -INFINITY : s0;
+    p.stats[3 * row + 1] = none ? -INFINITY : s1;
+    p.stats[3 * row + 2] = none ? 0.f : s2;
   }
 }
 // A column's value as it was loaded: nothing is done to it, and so not waited for, before it is used.
@@ -968,23 +991,29 @@ __device__ __forceinline__ void listed_logits(const T* row, const Listed& L, int
     if (h * 64 < K) xl[h].load(row + max(L.id[h], 0));
 }
 
-// as token_logprobs_fwd_kernel; with tail each wave marks the listed classes of its columns in a bit map of its own
+__device__ __forceinline__ float4 as_part(const DistillSums& a) { return make_float4(a.ml, a.zl, a.mr, a.zr); }
 // a row's sums, by one wave, from its units' parts; first: that of unit `lane`, or the last
-__device__ __forceinline__ void join_parts(const DistillParams& p, const float4* part, float4 first, float& m, float& zl, float& zr, int lane) {
-  if (lane >= p.units) first = make_float4(-FMAX, 0.f, 0.f, 0.f);
-  m = first.x;
-  for (int u = lane + 64; u < p.units; u += 64) m = fmaxf(m, part[u].x);
-  m = max_wave(m);
-  zl = zr = 0.f;
+__device__ __forceinline__ DistillSums join_parts(const DistillParams& p, const float4* part, float4 first, int lane) {
+  if (lane >= p.units) first = make_float4(-FMAX, 0.f, -FMAX, 0.f);
+  DistillSums a = {first.x, 0.f, first.z, 0.f};
+  for (int u = lane + 64; u < p.units; u += 64) {
+    a.ml = fmaxf(a.ml, part[u].x);
+    a.mr = fmaxf(a.mr, part[u].z);
+  }
+  a.mr = max_wave(a.mr);
+  if (p.tail) a.ml = max_wave(a.ml);
+  const float c = p.inv_t * LOG2E;
   for (int u = lane; u < p.units; u += 64) {
     const float4 s = u < 64 ? first : part[u];
-    const float f = __builtin_amdgcn_exp2f((s.x - m) * p.inv_t * LOG2E);
-    zl = fmaf(s.y, f, zl);
-    zr = fmaf(s.z, f, zr);
+    if (p.tail) a.zl = fmaf(s.y, __builtin_amdgcn_exp2f((s.x - a.ml) * c), a.zl);
+    a.zr = fmaf(s.w, __builtin_amdgcn_exp2f((s.z - a.mr) * c), a.zr);
   }
-  zl = sum_wave(zl);
-  zr = sum_wave(zr);
+  if (p.tail) a.zl = sum_wave(a.zl);
+  a.zr = sum_wave(a.zr);
+  return a;
 }
+template <bool TAIL> struct Form { static constexpr bool value = TAIL; };
+// as token_logprobs_fwd_kernel; with tail each wave marks the listed classes of its columns in a bit map of its own
 template <typename T, Kind KIND, int NV, int UNITS = 4>
 __global__ __launch_bounds__(KIND == ROW ? UNITS * 64 : 256, 8) void distill_fwd_kernel(DistillParams p) {
   __builtin_assume(p.K > 0);   // (no branch around a list's loads, and so no wait behind each)
@@ -1021,57 +1050,81 @@ __global__ __launch_bounds__(KIND == ROW ? UNITS * 64 : 256, 8) void distill_fwd
   }
   if (ends) list_weights(L, list, p.K, p.inv_t, p.tail);
   const float xn = cols.narrow_value(narrow, p.C, lane);
-  float x[NV][8], m = fmaxf(xn, -FMAX);
+  float x[NV][8];
   expand(raw, lr, cols.c0, cols.wide, lane, x);
+  DistillSums a = {-FMAX, 0.f, -FMAX, 0.f};
+  const float c = p.inv_t * LOG2E;
+  auto sums = [&](auto form) {
+    constexpr bool TAIL = decltype(form)::value;
+    uint32_t hits[NV];     // the listed ones of a lane's columns, a bit each
+    bool hit_n = false;
+    if constexpr (TAIL) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) m = max_med(m, x[i][j]);
-  m = max_wave(m);
-  const Exponent ex(m, p.inv_t * LOG2E);
-  float zl = 0.f, zr = 0.f;
-  auto add_up = [&](auto exponent) {
+      for (int i = 0; i < NV; ++i) hits[i] = i < cols.steps ? reinterpret_cast<const uint8_t*>(mark)[i * 64 + lane] : 0u;
+      const int at = cols.steps * 512 + lane;
+      hit_n = cols.narrow() && (mark[at >> 5] >> (at & 31)) & 1u;
+      if (hit_n) a.ml = fmaxf(xn, -FMAX);
+    }
+    if (!hit_n) a.mr = fmaxf(xn, -FMAX);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      if (i >= cols.steps) break;
-      const uint32_t bits = p.tail ? reinterpret_cast<const uint8_t*>(mark)[i * 64 + lane] : 0u;
-      if (p.tail && __any(bits != 0)) {
+      if (TAIL && __any(hits[i] != 0)) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float e = __builtin_amdgcn_exp2f(exponent(x[i][j]));
-          const bool hit = (bits >> j) & 1u;
-          zl += hit ? e : 0.f;
-          zr += hit ? 0.f : e;
+          const bool hit = (hits[i] >> j) & 1u;
+          a.ml = max_med(a.ml, hit ? x[i][j] : -FMAX);
+          a.mr = max_med(a.mr, hit ? -FMAX : x[i][j]);
         }
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) zr += __builtin_amdgcn_exp2f(exponent(x[i][j]));
+        for (int j = 0; j < 8; ++j) a.mr = max_med(a.mr, x[i][j]);
       }
     }
-    if (cols.narrow()) {
-      const float e = __builtin_amdgcn_exp2f(exponent(xn));
-      const int at = cols.steps * 512 + lane;
-      const bool hit = p.tail && (mark[at >> 5] >> (at & 31)) & 1u;
-      zl += hit ? e : 0.f;
-      zr += hit ? 0.f : e;
-    }
+    a.mr = max_wave(a.mr);
+    if (TAIL) a.ml = max_wave(a.ml);
+    const Exponent er(a.mr, c), el(a.ml == -FMAX ? a.mr : a.ml, c);   // (without a listed class: nothing is taken from it)
+    const bool plain = er.plain && (!TAIL || el.plain);
+    auto add_up = [&](auto exponent) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        if (i >= cols.steps) break;
+        if (TAIL && __any(hits[i] != 0)) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const bool hit = (hits[i] >> j) & 1u;
+            const float e = __builtin_amdgcn_exp2f(exponent(x[i][j], hit));
+            a.zl += hit ? e : 0.f;
+            a.zr += hit ? 0.f : e;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) a.zr += __builtin_amdgcn_exp2f(exponent(x[i][j], false));
+        }
+      }
+      if (cols.narrow()) {
+        const float e = __builtin_amdgcn_exp2f(exponent(xn, hit_n));
+        a.zl += hit_n ? e : 0.f;
+        a.zr += hit_n ? 0.f : e;
+      }
+    };
+    if (plain) add_up([&](float v, bool hit) { return fmaf(v, c, hit ? -el.mc : -er.mc); });
+    else add_up([&](float v, bool hit) { return (v - (hit ? el.m : er.m)) * c; });
+    a.zr = sum_wave(a.zr) * (plain ? __builtin_amdgcn_exp2f(-er.delta) : 1.f);
+    if (TAIL) a.zl = sum_wave(a.zl) * (plain ? __builtin_amdgcn_exp2f(-el.delta) : 1.f);
   };
-  if (ex.plain) add_up([&](float v) { return fmaf(v, ex.c, -ex.mc); });
-  else add_up([&](float v) { return (v - ex.m) * ex.c; });
-  const float f = __builtin_amdgcn_exp2f(-ex.delta);
-  zr = sum_wave(zr) * f;
-  if (p.tail) zl = sum_wave(zl) * f;
+  if (p.tail) sums(Form<true>{});
+  else sums(Form<false>{});
   if constexpr (KIND == PART) {
-    if (lane == 0) p.part[id] = make_float4(m, zl, zr, 0.f);
+    if (lane == 0) p.part[id] = as_part(a);
   } else {
     if constexpr (KIND == ROW) {
       __shared__ float4 sm_part[UNITS];
-      if (lane == 0) sm_part[unit] = make_float4(m, zl, zr, 0.f);
+      if (lane == 0) sm_part[unit] = as_part(a);
       __syncthreads();
       if (unit) return;
-      join_parts(p, sm_part, sm_part[min(lane, p.units - 1)], m, zl, zr, lane);
+      a = join_parts(p, sm_part, sm_part[min(lane, p.units - 1)], lane);
     }
-    finish_distill(p, row, L, xl[0].value(), xl[1].value(), m, zl, zr, lane);
+    finish_distill(p, row, L, xl[0].value(), xl[1].value(), a, lane);
   }
 }
 template <typename T>
@@ -1088,9 +1141,7 @@ __global__ __launch_bounds__(256) void distill_join_kernel(DistillParams p) {   
   Later<T> xl[2];
   listed_logits((const T*)p.logits + row * p.ldl, L, p.K, xl);
   list_weights(L, list, p.K, p.inv_t, p.tail);
-  float m, zl, zr;
-  join_parts(p, part, first, m, zl, zr, lane);
-  finish_distill(p, row, L, xl[0].value(), xl[1].value(), m, zl, zr, lane);
+  finish_distill(p, row, L, xl[0].value(), xl[1].value(), join_parts(p, part, first, lane), lane);
 }
 
 struct DistillGradParams {
@@ -1104,7 +1155,9 @@ struct DistillGradParams {
 };
 // A wave on its own takes up to 2048 columns of a row.  With q = softmax(y) and w = (listed / other mass of the student),
 //   d / dy = q (mass - left w) on the classes that the list does not name (left: the mass it leaves out; 0 without tail)
-//          = q (mass + left) - p on those it names:
+//          = q (mass + left) - p on those it names;
+// where the named classes lie far above the others (finish_distill), with r = softmax of the others alone and s their share of the student's
+// mass, q = s r of the former, and so d / dy = r ((mass + left) s - left):
 // one exponential a class by the first form, then the few named ones again by the second, each by the lane that holds its entry (whose
 // logit, and what is accumulated to, is fetched beside the row; a wave's own stores to one address stay in order).  Entries that
 // name one class find out by leaving their number at its place in LDS: each then writes the sum of their p, in the list's order.
@@ -1166,8 +1219,10 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillGradParams p) {
   const bool held = p.tail && w < INFINITY;          // other classes than the listed ones hold something
   const float left = held ? fmaxf(1.f - L.mass, 0.f) : 0.f;
   const bool none = m == -INFINITY;                  // every class at -inf: no gradient
-  const float on = L.mass + left, off = (left > 0.f ? L.mass - left * w : L.mass) * g;
-  const float c = p.inv_t * LOG2E, log2z = logz * LOG2E;
+  const bool far = p.tail && !none && logz < -1.f;   // (uniform)
+  const float on = L.mass + left, c = p.inv_t * LOG2E, log2z = (far ? FAR_MARK - logz : logz) * LOG2E;
+  const float named_m = far ? w : m, named_log2z = far ? 0.f : log2z;
+  const float off = (far ? on * __builtin_amdgcn_exp2f((m - w) * c + log2z) - left : left > 0.f ? L.mass - left * w : L.mass) * g;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int first = c0 + i * 512 + lane * 8;
@@ -1202,7 +1257,7 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillGradParams p) {
 #pragma unroll
   for (int h = 0; h < 2; ++h)
     if (here[h]) {
-      const float q = __builtin_amdgcn_exp2f((xl[h].value() - m) * c - log2z);
+      const float q = __builtin_amdgcn_exp2f((xl[h].value() - named_m) * c - named_log2z);
       dr[L.id[h]] = (T)(old[h].value() + fmaf(q, on, -L.p[h]) * g);
     }
 }

@@ -619,3 +619,18 @@ def test_distill_gradient_far_apart_agrees_with_differences(gap):
     B = (_r(C) + (K + 24) * U) * (gap + 12)
     # x +- h v are rounded: each class by U (gap + 8), which moves the loss by at most that much twice over
     assert ((d.double() * v.double()).sum(dim=1) - num).abs().max().item() <= (B + 2 * U * (gap + 8)) / h + h * h / 6 * 12
+
+
+@pytest.mark.parametrize("T", [4.3e-39, 1.5e-38, 3.0e38])
+def test_temperatures_at_the_ends_of_the_range(T):
+    """The least temperature makes the best class certain (ties share), the largest makes all alike."""
+    from ttts_amd import ops
+    x = _logits(4, 700, 700, torch.float32, 31)
+    best = x.argmax(dim=1)
+    x[3, (best[3] + 1) % 700] = x[3, best[3]]
+    r = ops.token_logprobs_fwd(x, best, top_k=2, temperature=T)
+    want = [0.0, 0.0, 0.0, math.log(2.0)] if T < 1 else [math.log(700.0)] * 4
+    for n in range(4):
+        assert abs(r.logp[n].item() + want[n]) <= 4 * _r(700) and abs(r.entropy[n].item() - want[n]) <= 24 * _r(700), n
+    loss, _ = ops.distill_fwd(x, best[:, None].contiguous(), torch.zeros(4, 1, device="cuda"), temperature=T)
+    assert (loss.cpu().double() - torch.tensor(want, dtype=torch.float64)).abs().max().item() <= 4 * _r(700)

@@ -144,3 +144,12 @@ def test_a_split_sequence_has_no_more_parts_than_its_join_holds(lib, units):
                 width = keys >> log_page
                 n = lib.ttts_attn_paged_decode_workspace_bytes(M, Hkv, Hkv, 32, 1 << log_page, width)
                 assert n // (M * Hkv * (32 + 2) * 4) <= 2048, (M, Hkv, keys)
+
+
+@pytest.mark.parametrize("fn,good", [("ttts_token_logprobs_fwd", FWD), ("ttts_token_logprobs_bwd", BWD), ("ttts_distill_fwd", DFWD),
+                                     ("ttts_distill_bwd", DBWD)])
+def test_temperatures_whose_reciprocal_in_bits_overflows(lib, fn, good):
+    """1 / temperature times log2 e is the exponents' factor: where that is not finite every exponent of a row's maximum would be NaN."""
+    for T in (3.4e-39, 4.0e-39, 4.2e-39):
+        _refused(lib, fn, good, "temperature", temperature=T)
+    assert _call(lib, fn, good, R=0, temperature=5.0e-39) == 0

@@ -1279,7 +1279,8 @@ static int check_logits(const char* what, const void* logits, int32_t dtype, int
   TTTS_REQUIRE(dtype == TTTS_DTYPE_F32 || dtype == TTTS_DTYPE_BF16 || dtype == TTTS_DTYPE_F16, "%s: unknown type code %d", what, (int)dtype);
   TTTS_REQUIRE(R >= 0 && C > 0 && C <= TTTS_SCORE_MAX_CLASSES && ldl >= C, "%s: need R >= 0, 0 < C <= %d, ldl >= C (R %d, C %d, ldl %lld)", what,
                TTTS_SCORE_MAX_CLASSES, R, C, (long long)ldl);
-  TTTS_REQUIRE(temperature > 0.f && temperature <= 3.0e38f && 1.0f / temperature <= 3.0e38f, "%s: the temperature must be positive and finite", what);
+  TTTS_REQUIRE(temperature >= TTTS_SCORE_MIN_TEMPERATURE && temperature <= TTTS_SCORE_MAX_TEMPERATURE,
+               "%s: the temperature must be positive and finite, and log2 e over it finite in fp32", what);
   TTTS_REQUIRE(R == 0 || logits, "%s: null pointer", what);
   const uintptr_t es = dtype == TTTS_DTYPE_F32 ? 4 : 2;
   TTTS_REQUIRE(reinterpret_cast<uintptr_t>(logits) % es == 0, "%s: logits are not aligned to their type", what);

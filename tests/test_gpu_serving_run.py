@@ -185,3 +185,18 @@ def test_teacher_arguments_are_checked_before_the_step():
     assert math.isfinite(eng.distill_loss.item())
     eng.train_step(tokens)
     assert eng.distill_loss is None                      # no loss of an earlier step's teacher
+
+
+@pytest.mark.parametrize("temperature", [1e-39, 4.2e-39, 3.2e38, math.nan])
+def test_teacher_temperatures_are_checked_before_the_step(temperature):
+    """A temperature that the distillation refuses is refused with the tokens, not in the middle of the backward."""
+    from ttts_amd.gpt.model import prepare_tokens
+    from ttts_amd.lib import TttsError
+    cfg, (teacher, student), batch = _models()
+    r = teacher.score(*batch, top_k=5)
+    eng = student.engine
+    before = eng.params.clone()
+    with pytest.raises(TttsError, match="set_teacher"):
+        eng.train_step([t.cuda() for t in prepare_tokens(teacher.cfg, *batch)],
+                       teacher=dict(teacher_idx=r.top_idx, teacher_logp=r.top_logp, temperature=temperature))
+    assert eng._teacher is None and torch.equal(eng.params, before) and not eng.grads.any()

@@ -23,7 +23,8 @@ import os
 import torch
 
 from .. import ops
-from ..lib import DISTILL_MAX_K, EPI_DGELU_BF16, EPI_GELU_BF16, EPI_RESID_ADD_F32, EPI_STORE_BF16, TttsError
+from ..lib import (DISTILL_MAX_K, EPI_DGELU_BF16, EPI_GELU_BF16, EPI_RESID_ADD_F32, EPI_STORE_BF16, SCORE_MAX_TEMPERATURE,
+                   SCORE_MIN_TEMPERATURE, TttsError)
 
 DEFAULTS = dict(layers=8, model_dim=512, heads=8, max_text_tokens=120, max_mel_tokens=250,
                 max_conditioning_inputs=1, mel_length_compression=1024, number_text_tokens=256,
@@ -732,8 +733,8 @@ class GptEngine:
             if t.dtype != dtype or t.device != self.params.device:
                 raise TttsError("set_teacher: need int64 indices and float32 log-probabilities on %s, got %s on %s"
                                 % (self.params.device, t.dtype, t.device))
-        if not 0 < teacher_idx.shape[2] <= DISTILL_MAX_K or not 0.0 < float(temperature) < float("inf"):
-            raise TttsError("set_teacher: need 1 .. %d entries and a positive temperature (got %d, %s)"
+        if not 0 < teacher_idx.shape[2] <= DISTILL_MAX_K or not SCORE_MIN_TEMPERATURE <= float(temperature) <= SCORE_MAX_TEMPERATURE:
+            raise TttsError("set_teacher: need 1 .. %d entries and a positive, finite temperature (got %d, %s)"
                             % (DISTILL_MAX_K, teacher_idx.shape[2], temperature))
         rows = B * Tm
         g_rows = torch.full((rows,), float(weight) / rows, dtype=torch.float32, device=self.device)

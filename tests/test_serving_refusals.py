@@ -153,3 +153,10 @@ def test_temperatures_whose_reciprocal_in_bits_overflows(lib, fn, good):
     for T in (3.4e-39, 4.0e-39, 4.2e-39):
         _refused(lib, fn, good, "temperature", temperature=T)
     assert _call(lib, fn, good, R=0, temperature=5.0e-39) == 0
+
+
+@pytest.mark.parametrize("scale", [2.4e38, -2.4e38, 3.4e38])
+def test_scales_that_overflow_in_bits(lib, scale):
+    """scale times log2 e multiplies the scores: infinite, a score of 0 would be NaN."""
+    _refused(lib, "ttts_attn_paged_decode", ATT, "scale", scale=scale)
+    assert _call(lib, "ttts_attn_paged_decode", ATT, M=0, scale=2.3e38 if scale > 0 else -2.3e38) == 0

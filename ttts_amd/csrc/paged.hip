@@ -412,7 +412,8 @@ extern "C" int ttts_attn_paged_decode(const void* q, int64_t q_stride_m, int64_t
   TTTS_REQUIRE(M >= 0 && H > 0 && H % Hkv == 0, "attn_paged_decode: need M >= 0 and H %% Hkv == 0 (M %d, H %d, Hkv %d)", M, H, Hkv);
   TTTS_REQUIRE(width > 0 && table_stride >= width && (int64_t)width * page <= 0x40000000,
                "attn_paged_decode: bad block table (width %d, row pitch %lld, at most 2^30 keys)", width, (long long)table_stride);
-  TTTS_REQUIRE(scale - scale == 0.f, "attn_paged_decode: the scale must be finite");
+  const float scale_log2 = scale * 1.4426950408889634f;
+  TTTS_REQUIRE(scale_log2 - scale_log2 == 0.f, "attn_paged_decode: the scale must be finite, times log2 e too");
   if (M == 0) return TTTS_OK;
   TTTS_REQUIRE(q && k_pages && v_pages && block_table && seq_lens && out && lse, "attn_paged_decode: null pointer");
   TTTS_REQUIRE(aligned16(q) && aligned16(k_pages) && aligned16(v_pages) && aligned16(out), "attn_paged_decode: 16-byte aligned bases are needed");
@@ -421,7 +422,7 @@ extern "C" int ttts_attn_paged_decode(const void* q, int64_t q_stride_m, int64_t
   p.q = q; p.kp = k_pages; p.vp = v_pages; p.out = out; p.lse = lse; p.table = block_table; p.lens = seq_lens;
   p.qs_m = q_stride_m; p.qs_h = q_stride_h; p.os_m = o_stride_m; p.os_h = o_stride_h; p.ts_m = table_stride;
   p.M = M; p.H = H; p.Hkv = Hkv; p.group = H / Hkv; p.tiles = (int)paged_tiles(H, Hkv); p.page_shift = __builtin_ctz(page); p.P = P; p.width = width;
-  p.scale_log2 = scale * 1.4426950408889634f;
+  p.scale_log2 = scale_log2;
   const int64_t units = M * (int64_t)Hkv * p.tiles;
   const PagedSplit sp = paged_split(units, (int64_t)width * page);
   p.chunk = sp.chunk; p.chunks = sp.chunks;

@@ -433,6 +433,7 @@ enum { TTTS_DTYPE_F32 = 0, TTTS_DTYPE_BF16 = 1, TTTS_DTYPE_F16 = 2 };
 #define TTTS_SCORE_MAX_CLASSES 1048576
 #define TTTS_SCORE_MAX_TOP 64
 #define TTTS_DISTILL_MAX_K 128
+#define TTTS_SCORE_F32_NO_WORKSPACE 32832     /* fp32 rows of up to so many classes need no workspace, whatever the queries below say */
 #define TTTS_SCORE_MIN_TEMPERATURE 4.3e-39f   /* log2 e / temperature is finite from 4.24e-39 on */
 #define TTTS_SCORE_MAX_TEMPERATURE 3.0e38f
 /* fwd: logp[r] = log softmax(y)[tokens[r]] (0 where tokens[r] is outside [0, C): the row has no token); entropy[r] = -sum p log p;

@@ -634,3 +634,35 @@ def test_temperatures_at_the_ends_of_the_range(T):
         assert abs(r.logp[n].item() + want[n]) <= 4 * _r(700) and abs(r.entropy[n].item() - want[n]) <= 24 * _r(700), n
     loss, _ = ops.distill_fwd(x, best[:, None].contiguous(), torch.zeros(4, 1, device="cuda"), temperature=T)
     assert (loss.cpu().double() - torch.tensor(want, dtype=torch.float64)).abs().max().item() <= 4 * _r(700)
+
+
+@pytest.mark.parametrize("dtype,C,used", [(torch.float32, 8256, False), (torch.float32, 8257, False), (torch.float32, 20000, False), (torch.float32, 32832, False),
+                                          (torch.float32, 32833, True), (torch.bfloat16, 8256, False), (torch.bfloat16, 8257, True)])
+def test_scratch_is_taken_where_it_is_used(dtype, C, used, monkeypatch):
+    """Rows that one workgroup ends take none, and the C entries do not ask for any there."""
+    from ttts_amd import lib as l
+    from ttts_amd import ops
+    taken = []
+    real = ops._workspace
+    monkeypatch.setattr(ops, "_workspace", lambda n, like: (taken.append(n), real(n, like))[1])
+    x = _logits(3, C, C, dtype, 8)
+    tokens = torch.tensor([0, C - 1, -1]).cuda()
+    idx, t = (z.cuda() for z in _teacher(3, C, 7, 1.0, True, 3))
+    r = ops.token_logprobs_fwd(x, tokens, top_k=9)
+    loss, stats = ops.distill_fwd(x, idx, t, tail=True)
+    assert len(taken) == (2 if used else 0)
+    logp, _, tl, ti, _, _ = _ref_logprobs(x, tokens, C, 9, 1.0)
+    assert torch.equal(r.top_idx.cpu(), ti)
+    _inside(r.logp, logp, _r(C) + 4 * U * logp.abs(), "logp")
+    outs = [torch.empty_like(z) for z in (r.logp, r.entropy, r.stats, r.top_logp, r.top_idx, loss, stats)]
+    p = [z.data_ptr() for z in outs]
+    code = l.DTYPE_F32 if dtype == torch.float32 else l.DTYPE_BF16
+    stream = torch.cuda.current_stream().cuda_stream
+    rc = [l.get().ttts_token_logprobs_fwd(x.data_ptr(), code, C, tokens.data_ptr(), p[0], p[1], p[2], p[3], p[4], 3, C, 9, 1.0, None, 0, stream),
+          l.get().ttts_distill_fwd(x.data_ptr(), code, C, idx.data_ptr(), t.data_ptr(), p[5], p[6], 3, C, 7, 1.0, 1, None, 0, stream)]
+    if used:
+        assert rc == [-1, -1] and "workspace" in l.get().ttts_last_error().decode()
+    else:
+        assert rc == [0, 0]
+        for a, b in zip(outs, (r.logp, r.entropy, r.stats, r.top_logp, r.top_idx, loss, stats)):
+            assert torch.equal(a, b)

@@ -1309,6 +1309,10 @@ static Units split_columns(int n) {
   return u;
 }
 
+// rows of the type whose units are the waves of one workgroup need no scratch (the queries do not know the type: 16 bits)
+static_assert(RowUnits<float>::n * WAVE_COLS + NARROW == TTTS_SCORE_F32_NO_WORKSPACE, "its meaning");
+static bool no_scratch(int32_t dtype, int32_t C) { return dtype == TTTS_DTYPE_F32 && C <= TTTS_SCORE_F32_NO_WORKSPACE; }
+
 extern "C" int64_t ttts_token_logprobs_workspace_bytes(int32_t R, int32_t C, int32_t top_k) {
   const int units = C > 0 ? split_columns(C).units : 1;
   return R > 0 && units > RowUnits<bf16>::n ? (int64_t)R * units * (16 + (top_k > 0 ? 256 : 0)) : 0;
@@ -1358,7 +1362,7 @@ extern "C" int ttts_token_logprobs_fwd(const void* logits, int32_t dtype, int64_
   TTTS_REQUIRE(top_k >= 0 && top_k <= TTTS_SCORE_MAX_TOP, "token_logprobs_fwd: need 0 <= top_k <= %d", TTTS_SCORE_MAX_TOP);
   if (R == 0) return TTTS_OK;
   TTTS_REQUIRE(tokens && logp && entropy && stats && (top_k == 0 || (top_logp && top_idx)), "token_logprobs_fwd: null pointer");
-  rc = need_workspace("token_logprobs_fwd", ttts_token_logprobs_workspace_bytes(R, C, top_k), workspace, workspace_bytes);
+  rc = need_workspace("token_logprobs_fwd", no_scratch(dtype, C) ? 0 : ttts_token_logprobs_workspace_bytes(R, C, top_k), workspace, workspace_bytes);
   if (rc) return rc;
   const Units u = split_columns(C);
   ScoreParams p{logits, ldl, tokens, logp, entropy, stats, top_logp, top_idx, (float4*)workspace, nullptr, R, C, top_k, u.units, u.cols, u.narrow_at, 1.0f / temperature};
@@ -1420,7 +1424,7 @@ extern "C" int ttts_distill_fwd(const void* logits, int32_t dtype, int64_t ldl, 
   TTTS_REQUIRE(K > 0 && K <= TTTS_DISTILL_MAX_K, "distill_fwd: need 0 < K <= %d", TTTS_DISTILL_MAX_K);
   if (R == 0) return TTTS_OK;
   TTTS_REQUIRE(teacher_idx && teacher_logp && row_loss && stats, "distill_fwd: null pointer");
-  rc = need_workspace("distill_fwd", ttts_distill_workspace_bytes(R, C), workspace, workspace_bytes);
+  rc = need_workspace("distill_fwd", no_scratch(dtype, C) ? 0 : ttts_distill_workspace_bytes(R, C), workspace, workspace_bytes);
   if (rc) return rc;
   const Units u = split_columns(C);
   const DistillParams p{logits, ldl, teacher_idx, teacher_logp, row_loss, stats, (float4*)workspace, R, C, K, tail != 0, u.units, u.cols, 1.0f / temperature};

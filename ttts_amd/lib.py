@@ -27,6 +27,7 @@ EXTRA_FLAGS = {"attn_dh64.hip": ["-fno-honor-nans", "-fno-slp-vectorize"]}
 TTTS_OK = 0
 DTYPE_F32, DTYPE_BF16, DTYPE_F16 = range(3)
 SCORE_MAX_CLASSES, SCORE_MAX_TOP, DISTILL_MAX_K = 1 << 20, 64, 128
+SCORE_F32_NO_WORKSPACE = 32832
 SCORE_MIN_TEMPERATURE, SCORE_MAX_TEMPERATURE = 4.3e-39, 3.0e38
 EPI_STORE_BF16, EPI_GELU_BF16, EPI_RESID_ADD_F32, EPI_DGELU_BF16, EPI_STORE_F32 = range(5)
 

@@ -967,7 +967,7 @@ def token_logprobs_fwd(logits, tokens, C=None, top_k=0, temperature=1.0):
     stats = logits.new_empty(R, 2, dtype=torch.float32)          # (the others from it: the cheapest way to a tensor, and there are five)
     logp, entropy = stats.new_empty(R), stats.new_empty(R)
     top_logp, top_idx = (stats.new_empty(R, k), tokens.new_empty(R, k)) if k > 0 else (None, None)
-    n = lib.ttts_token_logprobs_workspace_bytes(R, C, k)
+    n = 0 if C <= _l.SCORE_F32_NO_WORKSPACE and code == _l.DTYPE_F32 else lib.ttts_token_logprobs_workspace_bytes(R, C, k)
     ws = _workspace(n, logits) if n else None
     rc = lib.ttts_token_logprobs_fwd(logits.data_ptr(), code, ld, tokens.data_ptr(), logp.data_ptr(), entropy.data_ptr(), stats.data_ptr(),
                                      _a(top_logp), _a(top_idx), R, C, k, float(temperature), _a(ws), n, _raw_stream())
@@ -1009,7 +1009,7 @@ def distill_fwd(logits, teacher_idx, teacher_logp, C=None, temperature=1.0, tail
         with torch.cuda.device(other):
             return distill_fwd(logits, teacher_idx, teacher_logp, C, temperature, tail)
     loss, stats = teacher_logp.new_empty(R), teacher_logp.new_empty(R, 3)
-    n = lib.ttts_distill_workspace_bytes(R, C)
+    n = 0 if C <= _l.SCORE_F32_NO_WORKSPACE and code == _l.DTYPE_F32 else lib.ttts_distill_workspace_bytes(R, C)
     ws = _workspace(n, logits) if n else None
     rc = lib.ttts_distill_fwd(logits.data_ptr(), code, ld, teacher_idx.data_ptr(), teacher_logp.data_ptr(), loss.data_ptr(), stats.data_ptr(), R, C, K,
                               float(temperature), bool(tail), _a(ws), n, _raw_stream())

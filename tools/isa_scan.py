@@ -19,7 +19,8 @@ import sys
 import tempfile
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+sys.path.insert(0, ROOT)
+from ttts_amd import lib  # noqa: E402
 
 
 def cls(line):
@@ -71,9 +72,11 @@ def main():
     trace = args[args.index("--trace") + 1] if "--trace" in args else None
     with tempfile.TemporaryDirectory() as td:
         out = os.path.join(td, "k.s")
-        subprocess.run([HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-munsafe-fp-atomics -Xclang -target-feature -Xclang -packed-fp32-ops", "-I" + os.path.join(ROOT, "include"),
-                        "-I" + os.path.join(ROOT, "ttts_amd", "csrc"), "--cuda-device-only", "-S", "-o", out, src] + defs,
-                       check=True, stderr=subprocess.DEVNULL)
+        flags = [f for f in lib.FLAGS if f != "-fPIC"] + lib.EXTRA_FLAGS.get(os.path.basename(src), [])
+        r = subprocess.run([lib.HIPCC] + flags + ["-I" + os.path.join(ROOT, "include"), "-I" + lib.CSRC, "--cuda-device-only", "-S", "-o", out, src] + defs,
+                           capture_output=True, text=True)
+        if r.returncode != 0:
+            sys.exit("hipcc failed for %s:\n%s" % (src, r.stderr[-4000:]))
         asm = open(out).read()
     for name, lines in kernels(asm):
         for label, body in loops(lines):

@@ -540,7 +540,7 @@ def _apart(x, idx, C, T, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("C,offset", [(9, 0), (1026, 0), (2000, 1), (2049, 0), (8195, 1), (20000, 0), (40001, 0)])
+@pytest.mark.parametrize("C,offset", [(9, 0), (1026, 0), (2000, 1), (2049, 0), (8195, 1), (20000, 0), (40001, 0), (300007, 1)])
 @pytest.mark.parametrize("K,T", [(1, 1.0), (5, 0.1), (64, 1.0), (100, 2.0)])
 def test_distill_where_named_and_other_classes_lie_far_apart(C, offset, dtype, K, T):
     """The mass that the list leaves out is compared with the other classes' however far they lie below the named ones (or above): their

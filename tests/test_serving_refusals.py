@@ -160,3 +160,13 @@ def test_scales_that_overflow_in_bits(lib, scale):
     """scale times log2 e multiplies the scores: infinite, a score of 0 would be NaN."""
     _refused(lib, "ttts_attn_paged_decode", ATT, "scale", scale=scale)
     assert _call(lib, "ttts_attn_paged_decode", ATT, M=0, scale=2.3e38 if scale > 0 else -2.3e38) == 0
+
+
+def test_workspaces_that_are_needed_are_asked_for(lib):
+    """The three calls whose scratch is checked above do need some (more for more rows; the attention splits more sequences into fewer parts);
+    calls that one launch answers need none."""
+    for need in (lambda n: lib.ttts_token_logprobs_workspace_bytes(n, 300000, 3), lambda n: lib.ttts_distill_workspace_bytes(n, 300000)):
+        assert 0 < need(4) and need(8) == 2 * need(4)
+    assert lib.ttts_attn_paged_decode_workspace_bytes(4, 4, 2, 64, 16, ATT["width"]) > 0
+    assert lib.ttts_token_logprobs_workspace_bytes(4, 2048, 3) == lib.ttts_distill_workspace_bytes(4, 2048) == 0
+    assert lib.ttts_attn_paged_decode_workspace_bytes(4, 4, 2, 64, 16, 40) == 0

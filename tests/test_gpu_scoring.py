@@ -666,3 +666,17 @@ def test_scratch_is_taken_where_it_is_used(dtype, C, used, monkeypatch):
         assert rc == [0, 0]
         for a, b in zip(outs, (r.logp, r.entropy, r.stats, r.top_logp, r.top_idx, loss, stats)):
             assert torch.equal(a, b)
+
+
+def test_distill_lowest_values_at_a_temperature_of_their_size():
+    """Named classes at the lowest fp32 value, a temperature of 1e38 .. 3e38: they are e^-1 .. e^-4 of the others, not nothing."""
+    from ttts_amd import ops
+    x = _logits(3, 900, 900, torch.float32, 41)
+    idx = torch.tensor([[3, 500], [800, 801], [0, 899]])
+    for r in range(3):
+        x[r, idx[r]] = torch.finfo(torch.float32).min
+    t = torch.log(torch.tensor([[0.2, 0.3], [0.5, 0.1], [0.05, 0.6]]))
+    for T in (1e38, 3e38):
+        loss, stats = ops.distill_fwd(x, idx.cuda(), t.cuda(), temperature=T, tail=True)
+        ref = _ref_distill(x.double().cpu(), idx, t, 900, T, True)[0]
+        assert (loss.cpu().double() - ref).abs().max().item() <= 12 * _r(900), T

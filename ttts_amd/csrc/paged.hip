@@ -44,7 +44,8 @@ struct PagedParams {
 };
 
 // The i-th sequence of a batch by length, longest first, in 16 steps of length, for up to PAGED_ORDERED sequences: a batch that fills the card
-// several times over then ends with its short sequences (96 ragged ones up to 4096 keys: 160 -> 151 us; 64 up to 2404: 33.9 -> 29.6).
+// several times over then ends with its short sequences (96 ragged ones up to 4096 keys, 8 heads of 128: 147 -> 139 us a call; 64 up to 2404,
+// 8 heads of 64: 40.5 -> 39.2).
 // Every workgroup works it out for itself, from one load a lane and 64 sequences.
 constexpr int PAGED_ORDERED = 512;
 __device__ __forceinline__ int ordered_sequence(const int32_t* lens, int M, int i, int longest, int lane) {
@@ -101,7 +102,8 @@ template <> struct Frag<_Float16> {
 //                         weights are the B operand where they are, and a lane loads V rows 16 t + 4 g + r, DH / 16 neighbouring
 //                         columns each, which it re-pairs across rows in registers (product r of DH / 16 has rows d = (DH / 16) m + r).
 // The next tile's keys are loaded as soon as this one's have been multiplied, its values after the second product (held twice over,
-// 209 instead of 145 registers at 128 columns, they were no faster), the table entries another tile ahead.  The queries of a shared
+// 64 registers more at 128 columns, they were no faster), the table entries another tile ahead.  Both parts of the weights (Frag) cost
+// nothing that shows beside the loads: 175 us with them and without for 4 sequences of 130000 keys, 32 heads over 4 of 128.  The queries of a shared
 // head fill rows of the products that are there anyway, so a cached key is read once for up to 16 of them.
 template <typename T, int DH, int NW>
 __global__ __launch_bounds__(NW * 64) void attn_paged_decode_kernel(PagedParams p) {
@@ -318,7 +320,7 @@ __global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedParams p) {
 // units = workgroups of an unsplit call:
 //  * not at all up to 768 keys (three tiles for each of 8 waves): 613 keys of one sequence, 8 heads of 64: 6.0 us; split 6.4 - 7.0.
 //    Nor up to 4096 keys where the units alone give every CU two workgroups (of 4 waves then): 64 sequences up to 2404, 8 heads:
-//    40.7 us, 42.5 split; 96 up to 4096, 8 heads of 128: 148 us, 150 - 170 split in two to four (38.8 and 139 longest first).
+//    40.5 us, 42.9 split; 96 up to 4096, 8 heads of 128: 147 us, 153 split (39.2 and 139 unsplit and longest first).
 //  * into 256 keys, one tile a wave, while that gives the card's 256 CUs one workgroup each at most: 2404 keys of one sequence
 //    6.9 us, against 10.8 in chunks of 1024; more workgroups than CUs cost more than they give (20000 keys: 12.2 us, 14.2 with 512).
 //  * beyond that into 1024 keys or more, about 1024 workgroups (4 sequences of 130000 keys: 178 us, 188 with 2048), or about 2048

@@ -94,9 +94,6 @@ __device__ __forceinline__ void expand(const Raw<T, NV>& r, const T* row, int c0
   }
 }
 
-// max(a, b) without the two instructions that would first make signalling NaNs quiet; a NaN is passed over, as by fmaxf
-__device__ __forceinline__ float max_med(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); }
-
 // The exponent of a class from its row's (or wave's) maximum m >= -FMAX:  t = (x - m) c, in bits.  As fma(x, c, -m c) it is one
 // instruction and off by the one rounding of m c for the whole row, delta, which comes off the sums again; where m c is so large that
 // delta would matter (or not finite: a row of the type's lowest value) the difference is taken first.
@@ -349,10 +346,10 @@ __device__ __forceinline__ void add_sums(RowSums& a, float m, float z, float s, 
 __device__ __forceinline__ float group_max(const float (&v)[STEPS], float xn, int lane) {
   static_assert(STEPS == 4, "four lanes, four steps");
   const bool odd = lane & 1, high = lane & 2;
-  const float a = max_med(odd ? v[1] : v[0], dpp_mov<0xb1>(odd ? v[0] : v[1]));   // quad_perm 1, 0, 3, 2
-  const float b = max_med(odd ? v[3] : v[2], dpp_mov<0xb1>(odd ? v[2] : v[3]));
-  const float m = max_med(high ? b : a, dpp_mov<0x4e>(high ? a : b));             // quad_perm 2, 3, 0, 1
-  return max_med(max_med(m, xn), -INFINITY);
+  const float a = max_op(odd ? v[1] : v[0], dpp_mov<0xb1>(odd ? v[0] : v[1]));   // quad_perm 1, 0, 3, 2
+  const float b = max_op(odd ? v[3] : v[2], dpp_mov<0xb1>(odd ? v[2] : v[3]));
+  const float m = max_op(high ? b : a, dpp_mov<0x4e>(high ? a : b));             // quad_perm 2, 3, 0, 1
+  return max_op(max_op(m, xn), -INFINITY);
 }
 struct ScoreParams {
   const void* logits; int64_t ldl;
@@ -418,7 +415,7 @@ __device__ __forceinline__ void row_top(const ScoreParams& p, int64_t row, const
 #pragma unroll
   for (int i = 0; i < UNITS; ++i) {
     g[i] = ord(v[i]);
-    most = max_med(most, v[i]);
+    most = max_op(most, v[i]);
   }
   lane_bounds(most, lo, hi);
   float thr = group_threshold<T, UNITS>(g, k, true, lo, hi);
@@ -558,11 +555,11 @@ __global__ __launch_bounds__(KIND == ROW ? UNITS * 64 : 256, 8) void token_logpr
   for (int i = 0; i < NV; ++i) {
     vmax[i] = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) vmax[i] = max_med(vmax[i], x[i][j]);
-    lmax = max_med(lmax, vmax[i]);
+    for (int j = 0; j < 8; ++j) vmax[i] = max_op(vmax[i], x[i][j]);
+    lmax = max_op(lmax, vmax[i]);
   }
-  if (KIND == ONE) vmax[0] = max_med(vmax[0], xn);
-  lmax = max_med(lmax, -INFINITY);                         // (xn may be NaN)
+  if (KIND == ONE) vmax[0] = max_op(vmax[0], xn);
+  lmax = max_op(lmax, -INFINITY);                         // (xn may be NaN)
   const RowSums a = wave_sums(x, xn, cols, lmax, p.inv_t * LOG2E);
   if constexpr (KIND == PART) {
     if (lane == 0) p.part[id] = make_float4(a.m, a.z, a.s, 0.f);
@@ -640,8 +637,8 @@ __global__ __launch_bounds__(W * 64, 8) void token_logprobs_top_kernel(ScorePara
     for (int i = 0; i < SETS; ++i) {
       float set = v[i];
 #pragma unroll
-      for (int j = i + SETS; j < N; j += SETS) set = max_med(set, v[j]);
-      most = max_med(most, set);
+      for (int j = i + SETS; j < N; j += SETS) set = max_op(set, v[j]);
+      most = max_op(most, set);
       q[i] = ord(set);
     }
     lane_bounds(most, lo, hi);
@@ -1072,12 +1069,12 @@ __global__ __launch_bounds__(KIND == ROW ? UNITS * 64 : 256, 8) void distill_fwd
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const bool hit = (hits[i] >> j) & 1u;
-          a.ml = max_med(a.ml, hit ? x[i][j] : -FMAX);
-          a.mr = max_med(a.mr, hit ? -FMAX : x[i][j]);
+          a.ml = max_op(a.ml, hit ? x[i][j] : -FMAX);
+          a.mr = max_op(a.mr, hit ? -FMAX : x[i][j]);
         }
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) a.mr = max_med(a.mr, x[i][j]);
+        for (int j = 0; j < 8; ++j) a.mr = max_op(a.mr, x[i][j]);
       }
     }
     a.mr = max_wave(a.mr);
@@ -1110,7 +1107,10 @@ __global__ __launch_bounds__(KIND == ROW ? UNITS * 64 : 256, 8) void distill_fwd
     if (plain) add_up([&](float v, bool hit) { return fmaf(v, c, hit ? -el.mc : -er.mc); });
     else add_up([&](float v, bool hit) { return (v - (hit ? el.m : er.m)) * c; });
     a.zr = sum_wave(a.zr) * (plain ? __builtin_amdgcn_exp2f(-er.delta) : 1.f);
-    if (TAIL) a.zl = sum_wave(a.zl) * (plain ? __builtin_amdgcn_exp2f(-el.delta) : 1.f);
+    if (TAIL) {
+      a.zl = sum_wave(a.zl) * (plain ? __builtin_amdgcn_exp2f(-el.delta) : 1.f);
+      if (a.zl != 0.f) a.ml = el.m;
+    }
   };
   if (p.tail) sums(Form<true>{});
   else sums(Form<false>{});

@@ -680,3 +680,37 @@ def test_distill_lowest_values_at_a_temperature_of_their_size():
         loss, stats = ops.distill_fwd(x, idx.cuda(), t.cuda(), temperature=T, tail=True)
         ref = _ref_distill(x.double().cpu(), idx, t, 900, T, True)[0]
         assert (loss.cpu().double() - ref).abs().max().item() <= 12 * _r(900), T
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("C,offset", [(2, 0), (40, 1), (1026, 0), (1088, 0), (2112, 0), (5000, 1), (9152, 0), (20000, 0), (40001, 1), (150000, 0)])
+@pytest.mark.parametrize("T", [1.0, 0.7])
+def test_nearly_certain_classes_keep_their_bits(C, offset, dtype, T):
+    """The best class 5 to 60 nats ahead of the others: its log-probability, -log(1 + the others), and the entropy are good to a few steps
+    of THEMSELVES.  A term of the others is off by its exponent's roundings, 6 U of its distance and a few U; two best classes, and
+    four, share the rest."""
+    from ttts_amd import ops
+    gaps = [5.0, 7.0, 10.0, 14.0, 20.0, 40.0, 60.0]
+    R = 2 * len(gaps)
+    x = (_logits(R, C, C + offset, dtype, C, offset, std=0.5).float() * T).to(dtype)
+    best = torch.randint(0, C, (R,), generator=_gen(7))
+    for r in range(R):
+        x[r, best[r]] = x[r, :C].float().max().item() + (gaps[r % len(gaps)] + math.log(C)) * T
+        if r >= len(gaps):
+            for n in range(1, 2 if r % 2 else 4):
+                x[r, (best[r] + n * (C // 4 + 1)) % C] = x[r, best[r]]
+    r = ops.token_logprobs_fwd(x, best.cuda(), C=C, top_k=3, temperature=T)
+    z = x[:, :C].double().cpu() / T
+    d = z - z.amax(dim=1, keepdim=True)
+    ties = (d == 0).sum(dim=1)
+    rest = torch.where(d == 0, 0.0, d.exp()).sum(dim=1)
+    logz = torch.where(ties == 1, torch.log1p(rest), torch.log(ties + rest))
+    ent = logz - (d * d.exp()).sum(dim=1) / d.exp().sum(dim=1)
+    far = torch.where(d == 0, 0.0, d.abs()).amax(dim=1)
+    bound = (_r(C) + (6 * far + 20) * U)
+    _inside(r.logp, -logz, bound * logz, "logp")
+    _inside(r.entropy, ent, 2 * bound * ent, "entropy")
+    _inside(r.stats[:, 1], logz, bound * logz, "log Z")
+    first = torch.sort(z, dim=1, descending=True, stable=True)
+    assert torch.equal(r.top_idx[:, :min(3, C)].cpu(), first.indices[:, :3])
+    _inside(r.top_logp[:, 0], -logz, bound * logz, "top_logp")

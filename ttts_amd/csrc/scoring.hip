@@ -303,41 +303,66 @@ __device__ __forceinline__ int wave_top(const float (&x)[NV][8], float xn, const
   return min(n, k);
 }
 
-struct RowSums { float m, z, s; };   // maximum, sum e, sum e t (t in bits, from the maximum)
+// Maximum, excess = sum e - 1, sum e t (t in bits, from the maximum).  The 1 is the maximum's own, which is never added: the log-probability of a
+// class that is nearly certain, -log(1 + excess), and the row's entropy keep the bits that beside a 1 would be lost (an excess of 0.006 was off by
+// 2e-5 of itself; leaving the 1 out takes 46 of the 507 vector instructions a wave of two steps: 12816 rows of 1026 classes, 20
+// alternatives: 13.2 -> 14.2 us).  Without a class above -inf the excess is -1.
+struct RowSums {
+  float m, excess, s;
+  __device__ __forceinline__ float z() const { return 1.f + excess; }
+  __device__ __forceinline__ bool none() const { return excess < 0.f; }
+  __device__ __forceinline__ float log_z() const {   // log(1 + excess): by its series up to 1 / 16 (the rest 2^-27 of it)
+    const float x = excess;
+    const float series = x * fmaf(x, fmaf(x, fmaf(x, fmaf(x, fmaf(x, -1.f / 6, 1.f / 5), -1.f / 4), 1.f / 3), -1.f / 2), 1.f);
+    return x < 0.0625f ? series : __builtin_amdgcn_logf(z()) * LN2;
+  }
+};
 // of one wave's columns.  A class at -inf, or at the type's lowest value, has e = 0: e t must be 0, not NaN, so t is kept finite
-// there (a NaN passes through e).
+// there (a NaN passes through e).  vmax: the lanes' maxima of their 8 columns a step (vmax[0] may know the narrow one too).
 template <int NV>
-__device__ __forceinline__ RowSums wave_sums(const float (&x)[NV][8], float xn, const Cols& cols, float lmax, float c) {
+__device__ __forceinline__ RowSums wave_sums(const float (&x)[NV][8], float xn, const float (&vmax)[NV], const Cols& cols, float lmax, float c) {
   const int steps = cols.steps;
   RowSums a;
   a.m = max_wave(fmaxf(lmax, -FMAX));
-  a.z = a.s = 0.f;
+  a.excess = a.s = 0.f;
   const Exponent ex(a.m, c);
+  int most = 0;           // classes at the maximum: counted, not added (as 64 less those of a column that are not)
   auto add = [&](float t) {
     const float e = __builtin_amdgcn_exp2f(t);
-    a.z += e;
+    a.excess += e;
     a.s = fmaf(e, fmaxf(t, -200.f), a.s);
+  };
+  auto leave_out = [&](float& t, float v) {
+    const bool below = v != a.m;
+    most += 64 - __builtin_popcountll(__ballot(below));
+    t = below ? t : -INFINITY;
   };
   auto add_up = [&](auto exponent) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       if (i >= steps) break;
+      float t[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) add(exponent(x[i][j]));
+      for (int j = 0; j < 8; ++j) t[j] = exponent(x[i][j]);
+      if (__any(vmax[i] == a.m)) {        // (one step of the row's, as a rule)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) leave_out(t[j], x[i][j]);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) add(t[j]);
     }
-    if (cols.narrow()) add(exponent(xn));
+    if (cols.narrow()) {
+      float t = exponent(xn);
+      leave_out(t, xn);
+      add(t);
+    }
   };
   if (ex.plain) add_up([&](float v) { return fmaf(v, c, -ex.mc); });
   else add_up([&](float v) { return (v - a.m) * c; });
-  const float f = __builtin_amdgcn_exp2f(-ex.delta);
-  a.z = sum_wave(a.z) * f;
-  a.s = sum_wave(a.s) * f - ex.delta * a.z;
+  const float f = __builtin_amdgcn_exp2f(-ex.delta), below = sum_wave(a.excess) * f;
+  a.s = sum_wave(a.s) * f - ex.delta * below;
+  a.excess = below + (float)(most - 1) + (a.m - a.m);   // (NaN of an infinite maximum)
   return a;
-}
-__device__ __forceinline__ void add_sums(RowSums& a, float m, float z, float s, float c) {   // a.m is the row's maximum already
-  const float d = fmaxf((m - a.m) * c, -200.f), f = __builtin_amdgcn_exp2f(d);
-  a.z += z * f;
-  a.s += f * (s + z * d);
 }
 
 // Groups of a long row's unit, 64 of 32 neighbouring columns each: from the maxima of a lane's 8 columns a step (and its narrow column) lane
@@ -356,24 +381,23 @@ struct ScoreParams {
   const int64_t* tokens;
   float *logp, *entropy, *stats, *top_logp;
   int64_t* top_idx;
-  float4* part;          // long rows: [R, units] (m, z, s, -) of each wave's columns,
+  float4* part;          // long rows: [R, units] RowSums of each wave's columns,
   void* part_max;        // and with alternatives [R, units, 64] of the logits' type: the maximum of each group of columns (group_max)
   int R, C, k, units, unit_cols, narrow_at;   // the row's columns from narrow_at on are its last unit's narrow ones
   float inv_t;
 };
 
-__device__ __forceinline__ void write_row(const ScoreParams& p, int64_t row, const RowSums& a, bool given, float xt) {
-  const bool none = a.z == 0.f;   // every class at -inf
-  const float log2z = __builtin_amdgcn_logf(a.z);
+__device__ __forceinline__ void write_row(const ScoreParams& p, int64_t row, const RowSums& a, float logz, bool given, float xt) {
+  const bool none = a.none();   // every class at -inf
   p.stats[2 * row] = none ? -INFINITY : a.m;
-  p.stats[2 * row + 1] = none ? -INFINITY : log2z * LN2;
-  p.entropy[row] = none ? 0.f : (log2z - a.s / a.z) * LN2;
-  p.logp[row] = !given ? 0.f : none ? -INFINITY : (xt - a.m) * p.inv_t - log2z * LN2;
+  p.stats[2 * row + 1] = none ? -INFINITY : logz;
+  p.entropy[row] = none ? 0.f : logz - a.s / a.z() * LN2;
+  p.logp[row] = !given ? 0.f : none ? -INFINITY : (xt - a.m) * p.inv_t - logz;
 }
-__device__ __forceinline__ void write_top(const ScoreParams& p, int64_t row, int r, u64 key, const RowSums& a) {
-  const bool nan = a.z != a.z, have = key != 0 && !nan;
+__device__ __forceinline__ void write_top(const ScoreParams& p, int64_t row, int r, u64 key, const RowSums& a, float logz) {
+  const bool nan = a.excess != a.excess, have = key != 0 && !nan;
   p.top_idx[row * p.k + r] = have ? key_class(key) : -1;
-  p.top_logp[row * p.k + r] = have ? (unord((uint32_t)(key >> 32)) - a.m) * p.inv_t - __builtin_amdgcn_logf(a.z) * LN2 : nan ? a.z : -INFINITY;
+  p.top_logp[row * p.k + r] = have ? (unord((uint32_t)(key >> 32)) - a.m) * p.inv_t - logz : nan ? a.excess : -INFINITY;
 }
 
 // A long row's sums, by one wave, from its units' parts; every lane gets them.  What it takes from memory is asked for first, and by every
@@ -393,12 +417,17 @@ __device__ __forceinline__ RowSums join_sums(const ScoreParams& p, const float4*
   float m = r.first.x;
   for (int u = lane + 64; u < p.units; u += 64) m = fmaxf(m, part[u].x);
   RowSums a = {max_wave(m), 0.f, 0.f};
-  if (lane < p.units) add_sums(a, r.first.x, r.first.y, r.first.z, c);
-  for (int u = lane + 64; u < p.units; u += 64) {
-    const float4 s = part[u];
-    add_sums(a, s.x, s.y, s.z, c);
-  }
-  a.z = sum_wave(a.z);
+  float most = 0.f;       // parts at the maximum: their 1 is counted, not added
+  auto add = [&](const float4& u) {
+    const bool top = u.x == a.m;
+    const float d = fmaxf((u.x - a.m) * c, -200.f), f = __builtin_amdgcn_exp2f(d), z = 1.f + u.y;
+    most += top ? 1.f : 0.f;
+    a.excess += top ? u.y : z * f;
+    a.s += top ? u.z : f * (u.z + z * d);
+  };
+  if (lane < p.units) add(r.first);
+  for (int u = lane + 64; u < p.units; u += 64) add(part[u]);
+  a.excess = sum_wave(a.excess) + (sum_wave(most) - 1.f);
   a.s = sum_wave(a.s);
   return a;
 }
@@ -513,8 +542,9 @@ __device__ __forceinline__ void row_top(const ScoreParams& p, int64_t row, const
   }
   if (lane < 4) cand[n + lane] = 0;
   wave_fence();
-  rank_keys(cand, n, k, lane, 64, [&](int r, u64 key) { write_top(p, row, r, key, a); });
-  if (lane >= n && lane < k) write_top(p, row, lane, 0, a);
+  const float logz = a.log_z();
+  rank_keys(cand, n, k, lane, 64, [&](int r, u64 key) { write_top(p, row, r, key, a, logz); });
+  if (lane >= n && lane < k) write_top(p, row, lane, 0, a, logz);
 }
 
 // One wave per row (ONE), or per unit of up to 2048 columns of a row: with a workgroup for a row (ROW), whose waves meet once and the first ends
@@ -560,22 +590,22 @@ __global__ __launch_bounds__(KIND == ROW ? UNITS * 64 : 256, 8) void token_logpr
   }
   if (KIND == ONE) vmax[0] = max_op(vmax[0], xn);
   lmax = max_op(lmax, -INFINITY);                         // (xn may be NaN)
-  const RowSums a = wave_sums(x, xn, cols, lmax, p.inv_t * LOG2E);
+  const RowSums a = wave_sums(x, xn, vmax, cols, lmax, p.inv_t * LOG2E);
   if constexpr (KIND == PART) {
-    if (lane == 0) p.part[id] = make_float4(a.m, a.z, a.s, 0.f);
+    if (lane == 0) p.part[id] = make_float4(a.m, a.excess, a.s, 0.f);
     if (p.k) ((T*)p.part_max)[id * 64 + lane] = (T)group_max(vmax, xn, lane);
   } else if constexpr (KIND == ROW) {
     __shared__ float4 sm_part[UNITS];
     __shared__ float sm_max[UNITS][64];
     __shared__ __attribute__((aligned(16))) u64 sm_cand[ROW_CAND + 4];
     __shared__ int sm_list[ROW_LIST];
-    if (lane == 0) sm_part[unit] = make_float4(a.m, a.z, a.s, 0.f);
+    if (lane == 0) sm_part[unit] = make_float4(a.m, a.excess, a.s, 0.f);
     if (p.k) sm_max[unit][lane] = group_max(vmax, xn, lane);
     __syncthreads();
     if (unit) return;
     const LongRow r = {sm_part[min(lane, p.units - 1)], tok >= 0 && tok < p.C ? (int)tok : -1, xt};
     const RowSums all = join_sums(p, sm_part, r, lane);
-    if (lane == 0) write_row(p, row, all, r.tok >= 0, r.xt);
+    if (lane == 0) write_row(p, row, all, all.log_z(), r.tok >= 0, r.xt);
     if (p.k) {
       float v[UNITS];
 #pragma unroll
@@ -583,10 +613,11 @@ __global__ __launch_bounds__(KIND == ROW ? UNITS * 64 : 256, 8) void token_logpr
       row_top<T, UNITS>(p, row, lr, v, all, sm_cand, sm_list, lane);
     }
   } else {
-    if (lane == 0) write_row(p, row, a, tok >= 0 && tok < p.C, xt);
+    const float logz = a.log_z();
+    if (lane == 0) write_row(p, row, a, logz, tok >= 0 && tok < p.C, xt);
     if (p.k) {
-      const int have = wave_top<T, NV>(x, xn, vmax, lr, cols, p.k, lane, reinterpret_cast<typename WaveKey<T>::type*>(score_lds) + wave * WAVE_TOP_LDS, [&](int r, u64 key) { write_top(p, row, r, key, a); });
-      if (lane >= have && lane < p.k) write_top(p, row, lane, 0, a);
+      const int have = wave_top<T, NV>(x, xn, vmax, lr, cols, p.k, lane, reinterpret_cast<typename WaveKey<T>::type*>(score_lds) + wave * WAVE_TOP_LDS, [&](int r, u64 key) { write_top(p, row, r, key, a, logz); });
+      if (lane >= have && lane < p.k) write_top(p, row, lane, 0, a, logz);
     }
   }
 }
@@ -598,7 +629,7 @@ __global__ __launch_bounds__(256) void token_logprobs_join_kernel(ScoreParams p)
   const int lane = threadIdx.x & 63;
   const LongRow r = load_long_row<T>(p, row, lane);
   const RowSums a = join_sums(p, p.part + row * p.units, r, lane);
-  if (lane == 0) write_row(p, row, a, r.tok >= 0, r.xt);
+  if (lane == 0) write_row(p, row, a, a.log_z(), r.tok >= 0, r.xt);
 }
 
 // Alternatives of a long row: W waves, up to W * N * 64 groups of 32 columns.  A bound that k groups reach: the least of the waves' own
@@ -793,9 +824,10 @@ __global__ __launch_bounds__(W * 64, 8) void token_logprobs_top_kernel(ScorePara
   const RowSums a = sm_row;
   if (tid < 4) cand[n + tid] = 0;
   __syncthreads();
-  rank_keys(cand, n, k, tid, W * 64, [&](int r, u64 key) { write_top(p, row, r, key, a); });
-  for (int e = n + tid; e < k; e += W * 64) write_top(p, row, e, 0, a);
-  if (wave == W - 1 && lane == 0) write_row(p, row, a, r.tok >= 0, r.xt);
+  const float logz = a.log_z();
+  rank_keys(cand, n, k, tid, W * 64, [&](int r, u64 key) { write_top(p, row, r, key, a, logz); });
+  for (int e = n + tid; e < k; e += W * 64) write_top(p, row, e, 0, a, logz);
+  if (wave == W - 1 && lane == 0) write_row(p, row, a, a.log_z(), r.tok >= 0, r.xt);
 }
 
 // A wave per row of up to UNITS units, four rows a workgroup and no barrier (6250 rows of 32768 classes, 20 alternatives: 92 us, 104 with a
@@ -816,7 +848,7 @@ __global__ __launch_bounds__(256) void token_logprobs_top_wave_kernel(ScoreParam
 #pragma unroll
   for (int i = 0; i < UNITS; ++i) v[i] = i < p.units ? (float)raw[i] : -INFINITY;
   const RowSums a = join_sums(p, p.part + row * p.units, r, lane);
-  if (lane == 0) write_row(p, row, a, r.tok >= 0, r.xt);
+  if (lane == 0) write_row(p, row, a, a.log_z(), r.tok >= 0, r.xt);
   row_top<T, UNITS>(p, row, (const T*)p.logits + row * p.ldl, v, a, sm_cand[wave], sm_list[wave], lane);
 }
 
